@@ -1,0 +1,410 @@
+"""Timed cases of a paged key / value cache in 8 bits: the writer, the attention of single tokens, the reader, and the attention of prompts.
+
+A row is one token's key (or value) of one head, x of `hd` numbers: a = max |x| (2^-100 at least), scale = a / R, code = R x / a rounded to the
+cache's type, with R = 448 for e4m3 and 127 for int8.  It stands for code * scale.  Codes are [pages, heads, page, hd], scales float32 [pages, heads, page].
+
+* "write": queries, keys and values of new tokens come out of one projection; queries and keys may be normalised per head and are rotated by their
+  position, queries are returned in bf16, keys and values go into the cache.
+* "turn": the same for further turns of conversations, whose sequences are then read back whole, as attention over prompts does.
+* "read": sequences read back from their pages into dense bf16 pages of their own; rows behind a sequence's end are zero.
+* "decode": one query token for each sequence over all of its keys, the last `window` of them where that is not 0.
+* "prefill": causal attention of the last tokens of each sequence over all its keys.
+
+Head layouts are those of the presets in `zml_b200.models`.  Keys have channels of unequal size, as rotated keys have; block tables are
+shuffled.  The lengths of a batch are spread evenly over [shortest, longest] in a shuffled order that the case alone decides.
+"""
+from __future__ import annotations
+
+import math
+import random
+
+import torch
+
+own = False
+DEVICE = "cuda"
+RANGE = {"e4m3": 448.0, "int8": 127.0}
+DTYPE = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+EPS = 1e-6
+
+
+def _heads(hq, hkv, hd, cache, page=64):
+    return {"hq": hq, "hkv": hkv, "hd": hd, "cache": cache, "page": page}
+
+
+def _write(name, heads, batch, shortest, longest, past, norm=False, rot=None, layout=0, do="write"):
+    """[shortest, longest] new tokens of `batch` sequences that hold `past` tokens."""
+    return {"name": name, "do": do, **heads, "batch": batch, "shortest": shortest, "longest": longest, "past": past, "norm": norm,
+            "rot": rot or heads["hd"], "layout": layout}
+
+
+def _attend(name, do, heads, batch, shortest, longest, past=0, window=0):
+    """decode, read: sequences of [shortest, longest] tokens; prefill: as many new tokens behind `past` others."""
+    return {"name": name, "do": do, **heads, "batch": batch, "shortest": shortest, "longest": longest, "past": past, "window": window}
+
+
+def listed():
+    return [
+        # a decode step's new tokens of 32 users: launch and latency
+        _write("write-decode-32", _heads(32, 8, 128, "e4m3"), 32, 1, 1, 100),
+        # a batch of prompts, with norms of queries and keys: bandwidth
+        _write("write-prompts-8192", _heads(32, 4, 128, "e4m3"), 7, 128, 2212, 0, norm=True),
+        # further turns of three conversations, written and read back; heads of 256 of which a quarter turns
+        _write("turn-3-of-3000", _heads(16, 4, 256, "int8"), 3, 100, 401, 3000, norm=True, rot=64, do="turn"),
+        # what attention over a further turn reads back of three conversations
+        _attend("read-3-of-3300", "read", _heads(32, 8, 128, "e4m3"), 3, 3100, 3401),
+        # a long document and a batch of others, read back
+        _attend("read-documents", "read", _heads(32, 8, 64, "int8"), 6, 4001, 32768),
+        # one user, a short chat: latency
+        _attend("decode-1-of-512", "decode", _heads(32, 8, 64, "e4m3"), 1, 512, 512),
+        # 32 users of a service
+        _attend("decode-32-ragged", "decode", _heads(32, 8, 128, "int8"), 32, 128, 2048),
+        # heads of 256, few and long sequences
+        _attend("decode-6-long", "decode", _heads(16, 4, 256, "e4m3"), 6, 4000, 16000),
+        # 128 users, four key heads of eight queries each
+        _attend("decode-128-of-1024", "decode", _heads(32, 4, 128, "e4m3"), 128, 1024, 1024),
+        # one sequence as long as the model's positions reach
+        _attend("decode-1-of-131072", "decode", _heads(32, 8, 128, "e4m3"), 1, 131072, 131072),
+        # a further turn of three conversations
+        _attend("prefill-3-turns", "prefill", _heads(32, 8, 128, "e4m3"), 3, 100, 401, past=3000),
+        # prompts that were just written
+        _attend("prefill-4-of-2048", "prefill", _heads(32, 8, 128, "int8"), 4, 2048, 2048),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi))))))
+
+
+def draw(rng):
+    """Any of the above with other heads, lengths and page sizes, at most as much as the largest listed one of its kind."""
+    case = _drawn(rng)
+    del case["name"]
+    return case
+
+
+def _drawn(rng):
+    do = rng.choice(["write", "write", "turn", "read", "decode", "decode", "decode", "prefill"])
+    hd = rng.choice([64, 128, 128, 256])
+    hkv = rng.choice([1, 2, 3, 4, 5, 8, 8])
+    heads = _heads(hkv * rng.choice([1, 2, 3, 4, 4, 5, 7, 8, 8, 12, 16]), hkv, hd, "e4m3" if do == "write" else rng.choice(["e4m3", "int8"]),
+                   rng.choice([16, 32, 64, 64, 64, 128]))
+    width = hkv * hd
+    if do in ("write", "turn"):
+        room = 8192 * 36 * 128 // ((heads["hq"] + 2 * hkv) * hd)                 # new tokens
+        batch = _log_int(rng, 1, min(128, room))
+        longest = _log_int(rng, 1, max(1, room // batch))
+        past = _log_int(rng, 1, max(1, min(100000 if do == "write" else 16000, 10000 * 1024 // (batch * width)))) - 1
+        return _write("", heads, batch, _log_int(rng, max(1, longest // 16), longest), longest, past, rng.random() < 0.5,
+                      rng.choice([hd, hd, hd // 2, hd // 4, 24]), rng.choice([0, 0, 1]), do)
+    if do == "prefill":
+        batch = rng.choice([1, 1, 2, 3, 5, 8, 13])
+        total = _log_int(rng, batch, 8192)
+        longest = max(1, total // batch)
+        most = 4 * 32 * 128 * 2048 * 2048 // (batch * heads["hq"] * hd * longest)      # keys of a sequence
+        longest = min(longest, most)
+        past = _log_int(rng, 1, max(1, min(20000, most - longest + 1))) - 1
+        window = rng.choice([0, 0, 0, _log_int(rng, 1, longest + past)])
+        return _attend("", do, heads, batch, _log_int(rng, max(1, longest // 16), longest), longest, past, window)
+    room = (131072 * 1024 if do == "decode" else 110000 * 512) // width
+    batch = _log_int(rng, 1, 160)
+    longest = _log_int(rng, 1, max(1, min(131072, room // batch)))
+    window = rng.choice([0, 0, 0, _log_int(rng, 1, longest)]) if do == "decode" else 0
+    return _attend("", do, heads, batch, _log_int(rng, max(1, longest // 16), longest), longest, 0, window)
+
+
+# ------------------------------------------------------------------------------------------ sizes
+def _new(case):
+    """New tokens (write, turn, prefill) or all tokens (read, decode) of every sequence."""
+    n, lo, hi = case["batch"], case["shortest"], case["longest"]
+    out = [hi] if n == 1 else [lo + (hi - lo) * i // (n - 1) for i in range(n)]
+    random.Random(1000003 * n + 1009 * lo + hi).shuffle(out)
+    return out
+
+
+def _total(case):
+    return [n + case["past"] for n in _new(case)]
+
+
+def work(case):
+    hq, hkv, hd = case["hq"], case["hkv"], case["hd"]
+    new, total, window = _new(case), _total(case), case.get("window", 0)
+    row = 2 * hkv * (hd + 4)                                                     # a token's codes and scales
+    if case["do"] in ("write", "turn"):
+        n = sum(new)
+        data = n * (2 * (hq + 2 * hkv) * hd + 2 * hq * hd + row + 8)
+        flops = n * (10 * hq + 14 * hkv) * hd
+        if case["do"] == "turn":
+            data += (sum(total) - n) * row + sum(total) * 4 * hkv * hd           # what was just written need not be read again
+            flops += sum(total) * 2 * hkv * hd
+        return {"bytes": data, "flops": flops}
+    if case["do"] == "read":
+        return {"bytes": sum(total) * (row + 4 * hkv * hd), "flops": sum(total) * 2 * hkv * hd}
+    if case["do"] == "decode":
+        keys = sum(min(n, window) if window else n for n in total)
+        return {"bytes": keys * row + len(new) * 4 * hq * hd, "flops": keys * 4 * hq * hd}
+    seen = [min(t, n + window - 1) if window else t for n, t in zip(new, total)]      # keys that a sequence's new tokens see
+    pairs = sum((t - n) * n + n * (n + 1) // 2 if not window else sum(min(window, t - n + i + 1) for i in range(n)) for n, t in zip(new, total))
+    return {"bytes": sum(seen) * row + sum(new) * 4 * hq * hd, "flops": pairs * 4 * hq * hd}
+
+
+# ------------------------------------------------------------------------------------------ inputs
+def _cache(g, case, pages, spread):
+    """Codes and scales of rows N(0, spread) with channels of unequal size."""
+    shape = (pages, case["hkv"], case["page"], case["hd"])
+    channel = torch.empty((case["hkv"], 1, case["hd"]), device=DEVICE).normal_(0.0, 0.5, generator=g).exp_()
+    x = torch.empty(shape, device=DEVICE).normal_(0.0, spread, generator=g).mul_(channel)
+    a = x.abs().amax(-1)
+    x.mul_((RANGE[case["cache"]] / a)[..., None])
+    return (x.round_() if case["cache"] == "int8" else x.clamp_(-448.0, 448.0)).to(DTYPE[case["cache"]]), a / RANGE[case["cache"]]
+
+
+def prepare(case, seed):
+    g = torch.Generator(device=DEVICE).manual_seed(seed)
+    new, total, page = _new(case), _total(case), case["page"]
+    hq, hkv, hd = case["hq"], case["hkv"], case["hd"]
+    held = [-(-t // page) for t in total]                                        # pages of every sequence
+    pages = sum(held) + 1
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(seed)).tolist()
+    table = torch.zeros((len(held), max(held)), dtype=torch.int32)
+    at = 0
+    for i, n in enumerate(held):
+        table[i, :n] = torch.tensor(order[at:at + n], dtype=torch.int32)
+        at += n
+    state = {"case": case, "k": _cache(g, case, pages, 2.0), "v": _cache(g, case, pages, 1.0), "table": table.to(DEVICE),
+             "lens": torch.tensor(total, dtype=torch.int32, device=DEVICE), "pages": sum(held), "longest": max(total)}
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    if case["do"] in ("write", "turn"):
+        # the program's own plan of the step: positions, slots, and the model's frequencies and norm weights
+        pos = torch.cat([torch.arange(t - n, t) for n, t in zip(new, total)])
+        seq = torch.repeat_interleave(torch.arange(len(new)), torch.tensor(new))
+        slots = table[seq, pos // page] * page + pos % page
+        channel = torch.empty((1, (hq + 2 * hkv) * hd), device=DEVICE).normal_(0.0, 0.5, generator=g).exp_()
+        state["qkv"] = torch.empty((len(pos), (hq + 2 * hkv) * hd), device=DEVICE).normal_(generator=g).mul_(channel).bfloat16()
+        state["positions"], state["slots"] = pos.int().to(DEVICE), slots.int().to(DEVICE)
+        half = case["rot"] // 2
+        state["inv_freq"] = (500000.0 ** (-torch.arange(half, dtype=torch.float64) / half)).float().to(DEVICE)
+        weights = [torch.empty(hd, device=DEVICE).normal_(1.0, 0.1, generator=g).bfloat16() for _ in range(2)]
+        state["norms"] = weights if case["norm"] else [None, None]
+    elif case["do"] in ("decode", "prefill"):
+        rows = len(new) if case["do"] == "decode" else sum(new)
+        state["q"] = torch.empty((rows, hq, hd), device=DEVICE).normal_(generator=g).bfloat16()
+        state["starts"], state["most_new"] = torch.tensor(starts, dtype=torch.int32, device=DEVICE), max(new)
+    return state
+
+
+# ------------------------------------------------------------------------------------------ a pass
+def run(state):
+    if own:
+        return _own(state)
+    return {"write": _plain_write, "turn": _plain_turn, "read": _plain_read, "decode": _plain_decode, "prefill": _plain_prefill}[state["case"]["do"]](state)
+
+
+def _own(s):
+    from zml_b200 import ops
+    c = s["case"]
+    k, v = ops.QuantKV(*s["k"]), ops.QuantKV(*s["v"])
+    if c["do"] in ("write", "turn"):
+        q = ops.rope_kvwrite(s["qkv"], s["positions"], s["slots"], s["inv_freq"], k, v, c["hq"], c["hkv"], c["hd"], c["layout"], c["rot"],
+                             q_norm_w=s["norms"][0], k_norm_w=s["norms"][1], norm_eps=EPS)
+        if c["do"] == "write":
+            return {"q": q, "k": s["k"], "v": s["v"]}
+        kd, vd, _ = ops.paged_read(k, v, s["table"], s["lens"], num_pages=s["pages"])
+        return {"q": q, "k": kd, "v": vd}
+    if c["do"] == "read":
+        kd, vd, table = ops.paged_read(k, v, s["table"], s["lens"], num_pages=s["pages"])
+        return {"k": kd, "v": vd, "table": table}
+    if c["do"] == "decode":
+        return ops.paged_decode(s["q"], k, v, s["table"], s["lens"], window=c["window"], max_seq_len=s["longest"])
+    return ops.paged_prefill(s["q"], k, v, s["table"], s["lens"], s["starts"], window=c["window"], max_seq_len=s["longest"], kv_pages=s["pages"])
+
+
+# ------------------------------------------------------------------------------------------ plain form
+def _turned(s, x, weight):
+    """Norm and rotation of x [tokens, heads, hd] in 32 bits; the angles are formed in 64."""
+    c = s["case"]
+    if weight is not None:
+        x = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + EPS) * weight.float()
+    angle = s["positions"].double()[:, None] * s["inv_freq"].double()[None]
+    cos, sin = angle.cos().float()[:, None], angle.sin().float()[:, None]
+    half = c["rot"] // 2
+    i = torch.arange(half, device=x.device)
+    i, j = (2 * i, 2 * i + 1) if c["layout"] == 1 else (i, i + half)
+    u, v, y = x[..., i], x[..., j], x.clone()
+    y[..., i] = u * cos - v * sin
+    y[..., j] = v * cos + u * sin
+    return y
+
+
+def _plain_put(s, cache, x):
+    c = s["case"]
+    codes, scales = cache
+    a = x.abs().amax(-1).clamp_min(2.0 ** -100)
+    y = x * RANGE[c["cache"]] / a[..., None]
+    y = (y.round() if c["cache"] == "int8" else y.clamp(-448.0, 448.0)).to(DTYPE[c["cache"]])
+    page, row = s["slots"].long() // c["page"], s["slots"].long() % c["page"]
+    codes.view(torch.uint8)[page, :, row] = y.view(torch.uint8)
+    scales[page, :, row] = a / RANGE[c["cache"]]
+
+
+def _plain_write(s):
+    c = s["case"]
+    x = s["qkv"].float().reshape(-1, c["hq"] + 2 * c["hkv"], c["hd"])
+    q, k, v = x.split([c["hq"], c["hkv"], c["hkv"]], 1)
+    _plain_put(s, s["k"], _turned(s, k, s["norms"][1]))
+    _plain_put(s, s["v"], v)
+    return {"q": _turned(s, q, s["norms"][0]).bfloat16(), "k": s["k"], "v": s["v"]}
+
+
+def _plain_read(s):
+    c = s["case"]
+    page = c["page"]
+    held = (s["lens"].long() + page - 1) // page
+    first = held.cumsum(0) - held
+    seq = torch.repeat_interleave(torch.arange(c["batch"], device=DEVICE), held, output_size=s["pages"])
+    nth = torch.arange(s["pages"], device=DEVICE) - first[seq]
+    source = s["table"].long()[seq, nth]
+    valid = nth[:, None] * page + torch.arange(page, device=DEVICE)[None] < s["lens"][seq][:, None]
+    out = {n: (s[n][0].view(torch.uint8)[source].view(DTYPE[c["cache"]]).float() * s[n][1][source][..., None]).transpose(1, 2).masked_fill(
+        ~valid[:, :, None, None], 0.0).bfloat16() for n in ("k", "v")}
+    column = torch.arange(s["table"].shape[1], device=DEVICE)[None]
+    out["table"] = torch.where(column < held[:, None], first[:, None] + column, 0).int()
+    return out
+
+
+def _plain_turn(s):
+    q, dense = _plain_write(s)["q"], _plain_read(s)
+    return {"q": q, "k": dense["k"], "v": dense["v"]}
+
+
+def _gathered(s, cache):
+    """All sequences side by side: [batch, heads, longest, hd] in 32 bits."""
+    codes, scales = cache
+    t = s["table"].long()
+    x = codes.view(torch.uint8)[t].view(codes.dtype).float() * scales[t][..., None]
+    return x.transpose(1, 2).reshape(t.shape[0], x.shape[2], -1, x.shape[-1])[:, :, :s["longest"]]
+
+
+def _softmax_over(s, scores, k_pos, q_pos):
+    """Softmax over the keys that a query at q_pos sees; nothing where it sees none."""
+    window = s["case"]["window"]
+    seen = (k_pos <= q_pos) & (k_pos > q_pos - window) if window else k_pos <= q_pos
+    scores = scores.masked_fill(~seen, -math.inf)
+    top = scores.amax(-1, keepdim=True).clamp_min(-1e30)
+    p = torch.exp(scores - top)
+    return p / p.sum(-1, keepdim=True).clamp_min(1e-30)
+
+
+def _plain_decode(s):
+    c = s["case"]
+    b, hkv, hd = c["batch"], c["hkv"], c["hd"]
+    q = s["q"].float().reshape(b, hkv, -1, hd)
+    scores = q @ _gathered(s, s["k"]).transpose(-1, -2) / math.sqrt(hd)
+    p = _softmax_over(s, scores, torch.arange(s["longest"], device=DEVICE), s["lens"][:, None, None, None] - 1)
+    return (p @ _gathered(s, s["v"])).reshape(b, c["hq"], hd).bfloat16()
+
+
+def _plain_prefill(s):
+    c = s["case"]
+    b, hkv, hd, n = c["batch"], c["hkv"], c["hd"], s["most_new"]
+    first = s["starts"][:-1].long()
+    count = s["starts"][1:].long() - first
+    row = torch.arange(n, device=DEVICE)
+    at = (first[:, None] + row).clamp_max(s["q"].shape[0] - 1)
+    q = s["q"].float()[at].reshape(b, n, hkv, -1, hd).permute(0, 2, 3, 1, 4)         # [batch, heads, group, rows, hd]
+    scores = q @ _gathered(s, s["k"]).transpose(-1, -2)[:, :, None] / math.sqrt(hd)
+    q_pos = ((s["lens"] - count)[:, None] + row)[:, None, None, :, None]
+    p = _softmax_over(s, scores, torch.arange(s["longest"], device=DEVICE), q_pos)
+    o = (p @ _gathered(s, s["v"])[:, :, None]).permute(0, 3, 1, 2, 4).reshape(b, n, c["hq"], hd).bfloat16()
+    seq = torch.repeat_interleave(torch.arange(b, device=DEVICE), count, output_size=s["q"].shape[0])
+    return o[seq, torch.arange(s["q"].shape[0], device=DEVICE) - first[seq]]
+
+
+# ------------------------------------------------------------------------------------------ in 64 bits
+def _e4m3(y):
+    """The nearest value of e4m3, ties to the even one."""
+    _, e = torch.frexp(y)
+    step = torch.ldexp(torch.ones_like(y), (e - 1).clamp_min(-6) - 3)
+    return (torch.round(y / step) * step).clamp(-448.0, 448.0)
+
+
+def _rows64(state, name, i):
+    """Keys or values of sequence i, [tokens, heads, hd]."""
+    n = int(state["lens"][i])
+    codes, scales = state[name]
+    pages = state["table"][i, :-(-n // codes.shape[2])].long()
+    x = codes.view(torch.uint8)[pages].view(codes.dtype).double() * scales[pages].double().unsqueeze(-1)
+    return x.permute(0, 2, 1, 3).flatten(0, 1)[:n]
+
+
+def _written64(state):
+    """Rotated queries in 64 bits, and the cache with the new rows: codes (in 64 bits) and scales."""
+    c = state["case"]
+    hq, hkv, hd, half = c["hq"], c["hkv"], c["hd"], c["rot"] // 2
+    x = state["qkv"].double().unflatten(1, (hq + 2 * hkv, hd))
+    angle = torch.outer(state["positions"].double(), state["inv_freq"].double())
+    spin = torch.polar(torch.ones_like(angle), angle)[:, None]
+    parts = []
+    for lo, hi, w in ((0, hq, state["norms"][0]), (hq, hq + hkv, state["norms"][1])):
+        y = x[:, lo:hi].clone()
+        if w is not None:
+            y = y / (y.square().mean(-1, keepdim=True) + EPS).sqrt() * w.double()
+        re, im = (y[..., 0:2 * half:2], y[..., 1:2 * half:2]) if c["layout"] == 1 else (y[..., :half], y[..., half:2 * half])
+        z = torch.complex(re, im) * spin
+        if c["layout"] == 1:
+            y[..., 0:2 * half:2], y[..., 1:2 * half:2] = z.real, z.imag
+        else:
+            y[..., :half], y[..., half:2 * half] = z.real, z.imag
+        parts.append(y)
+    out, limit = {}, RANGE[c["cache"]]
+    for name, y in (("k", parts[1]), ("v", x[:, hq + hkv:])):
+        a = y.abs().amax(-1)
+        code = y * limit / a[..., None]
+        code = torch.round(code) if c["cache"] == "int8" else _e4m3(code)
+        codes, scales = state[name][0].to(torch.float64), state[name][1].double()
+        slot = state["slots"].long()
+        p, r = torch.div(slot, c["page"], rounding_mode="floor"), slot % c["page"]
+        codes[p, :, r], scales[p, :, r] = code, a / limit
+        out[name] = (codes, scales)
+    return parts[0], out
+
+
+def exact(case, seed):
+    state = prepare(case, seed)
+    hkv, hd, page = case["hkv"], case["hd"], case["page"]
+    if case["do"] in ("write", "turn"):
+        q, cache = _written64(state)
+        if case["do"] == "write":
+            return {"q": q, "k": cache["k"], "v": cache["v"]}
+    if case["do"] in ("read", "turn"):
+        out, table, at = {}, torch.zeros_like(state["table"]), 0
+        for i, n in enumerate(_total(case)):
+            m = -(-n // page)
+            table[i, :m] = torch.arange(at, at + m, dtype=torch.int32)
+            at += m
+        for name in ("k", "v"):
+            dense = torch.zeros((at, page, hkv, hd), dtype=torch.float64, device=DEVICE)
+            for i, n in enumerate(_total(case)):
+                pages = state["table"][i, :-(-n // page)].long()
+                if case["do"] == "turn":
+                    x = (cache[name][0][pages] * cache[name][1][pages].unsqueeze(-1)).permute(0, 2, 1, 3).flatten(0, 1)[:n]
+                else:
+                    x = _rows64(state, name, i)
+                dense.flatten(0, 1)[int(table[i, 0]) * page:][:n] = x
+            out[name] = dense
+        return {"q": q, **out} if case["do"] == "turn" else {**out, "table": table}
+    window, outs = case["window"], []
+    for i, (n, t) in enumerate(zip(_new(case), _total(case))):
+        rows = 1 if case["do"] == "decode" else n
+        first = i if case["do"] == "decode" else int(state["starts"][i])
+        q = state["q"][first:first + rows].double().unflatten(1, (hkv, -1))
+        k, v = _rows64(state, "k", i), _rows64(state, "v", i)
+        q_pos, k_pos = torch.arange(t - rows, t, device=DEVICE)[:, None], torch.arange(t, device=DEVICE)[None]
+        hidden = (k_pos > q_pos) | ((k_pos <= q_pos - window) if window else torch.zeros_like(k_pos > q_pos))
+        o = torch.empty((rows, hkv, case["hq"] // hkv, hd), dtype=torch.float64, device=DEVICE)
+        for h in range(hkv):
+            logits = torch.einsum("rgd,td->grt", q[:, h], k[:, h]) / math.sqrt(hd)
+            o[:, h] = torch.einsum("grt,td->rgd", logits.masked_fill_(hidden, -math.inf).softmax(-1), v[:, h])
+        outs.append(o.flatten(1, 2))
+    return torch.cat(outs)
