@@ -1,7 +1,8 @@
 """Timed cases of a paged key / value cache in 8 bits: the writer, the attention of single tokens, the reader, and the attention of prompts.
 
-A row is one token's key (or value) of one head, x of `hd` numbers: a = max |x| (2^-100 at least), scale = a / R, code = R x / a rounded to the
-cache's type, with R = 448 for e4m3 and 127 for int8.  It stands for code * scale.  Codes are [pages, heads, page, hd], scales float32 [pages, heads, page].
+A row is one token's key (or value) of one head, x of `hd` numbers.  Its scale is the smallest power of two 2^k with max |x| <= R 2^k, R = 448 for e4m3 and
+127 for int8, its codes are x / 2^k rounded to the cache's type, and it stands for codes * 2^k.  Codes are [pages, heads, page, hd]; the scales' exponents
+are held as bytes k + 127, [pages, heads, page].
 
 * "write": queries, keys and values of new tokens come out of one projection; queries and keys may be normalised per head and are rotated by their
   position, queries are returned in bf16, keys and values go into the cache.
@@ -22,7 +23,7 @@ import torch
 
 own = False
 DEVICE = "cuda"
-RANGE = {"e4m3": 448.0, "int8": 127.0}
+RANGE = {"e4m3": (8, 1.75), "int8": (6, 1.984375)}      # R = 2^e * m
 DTYPE = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
 EPS = 1e-6
 
@@ -128,7 +129,7 @@ def _total(case):
 def work(case):
     hq, hkv, hd = case["hq"], case["hkv"], case["hd"]
     new, total, window = _new(case), _total(case), case.get("window", 0)
-    row = 2 * hkv * (hd + 4)                                                     # a token's codes and scales
+    row = 2 * hkv * (hd + 1)                                                     # a token's codes and exponents
     if case["do"] in ("write", "turn"):
         n = sum(new)
         data = n * (2 * (hq + 2 * hkv) * hd + 2 * hq * hd + row + 8)
@@ -148,14 +149,28 @@ def work(case):
 
 
 # ------------------------------------------------------------------------------------------ inputs
+def _coded(case, x):
+    """Codes and exponents of the rows of x, in 32 bits."""
+    m, e = torch.frexp(x.abs().amax(-1))                                         # a = m 2^e, m in [0.5, 1)
+    k = e - 1 - RANGE[case["cache"]][0] + (2 * m > RANGE[case["cache"]][1])
+    y = x * _power(-k)[..., None]
+    return (y.round() if case["cache"] == "int8" else y).to(DTYPE[case["cache"]]), (k + 127).to(torch.uint8)
+
+
+def _power(k):
+    """2^k in 32 bits."""
+    return ((k.int() + 127) << 23).view(torch.float32)
+
+
+def _values(codes, exponents):
+    return codes.float() * _power(exponents.int() - 127)[..., None]
+
+
 def _cache(g, case, pages, spread):
-    """Codes and scales of rows N(0, spread) with channels of unequal size."""
+    """Codes and exponents of rows N(0, spread) with channels of unequal size."""
     shape = (pages, case["hkv"], case["page"], case["hd"])
     channel = torch.empty((case["hkv"], 1, case["hd"]), device=DEVICE).normal_(0.0, 0.5, generator=g).exp_()
-    x = torch.empty(shape, device=DEVICE).normal_(0.0, spread, generator=g).mul_(channel)
-    a = x.abs().amax(-1)
-    x.mul_((RANGE[case["cache"]] / a)[..., None])
-    return (x.round_() if case["cache"] == "int8" else x.clamp_(-448.0, 448.0)).to(DTYPE[case["cache"]]), a / RANGE[case["cache"]]
+    return _coded(case, torch.empty(shape, device=DEVICE).normal_(0.0, spread, generator=g).mul_(channel))
 
 
 def prepare(case, seed):
@@ -201,6 +216,11 @@ def run(state):
     return {"write": _plain_write, "turn": _plain_turn, "read": _plain_read, "decode": _plain_decode, "prefill": _plain_prefill}[state["case"]["do"]](state)
 
 
+def _held(s):
+    """The cache's buffers as what they stand for: codes, and bytes as powers of two."""
+    return {n: (s[n][0], s[n][1].view(torch.float8_e8m0fnu)) for n in ("k", "v")}
+
+
 def _own(s):
     from zml_b200 import ops
     c = s["case"]
@@ -209,7 +229,7 @@ def _own(s):
         q = ops.rope_kvwrite(s["qkv"], s["positions"], s["slots"], s["inv_freq"], k, v, c["hq"], c["hkv"], c["hd"], c["layout"], c["rot"],
                              q_norm_w=s["norms"][0], k_norm_w=s["norms"][1], norm_eps=EPS)
         if c["do"] == "write":
-            return {"q": q, "k": s["k"], "v": s["v"]}
+            return {"q": q, **_held(s)}
         kd, vd, _ = ops.paged_read(k, v, s["table"], s["lens"], num_pages=s["pages"])
         return {"q": q, "k": kd, "v": vd}
     if c["do"] == "read":
@@ -239,13 +259,10 @@ def _turned(s, x, weight):
 
 def _plain_put(s, cache, x):
     c = s["case"]
-    codes, scales = cache
-    a = x.abs().amax(-1).clamp_min(2.0 ** -100)
-    y = x * RANGE[c["cache"]] / a[..., None]
-    y = (y.round() if c["cache"] == "int8" else y.clamp(-448.0, 448.0)).to(DTYPE[c["cache"]])
+    codes, exponents = _coded(c, x)
     page, row = s["slots"].long() // c["page"], s["slots"].long() % c["page"]
-    codes.view(torch.uint8)[page, :, row] = y.view(torch.uint8)
-    scales[page, :, row] = a / RANGE[c["cache"]]
+    cache[0].view(torch.uint8)[page, :, row] = codes.view(torch.uint8)
+    cache[1][page, :, row] = exponents
 
 
 def _plain_write(s):
@@ -254,7 +271,7 @@ def _plain_write(s):
     q, k, v = x.split([c["hq"], c["hkv"], c["hkv"]], 1)
     _plain_put(s, s["k"], _turned(s, k, s["norms"][1]))
     _plain_put(s, s["v"], v)
-    return {"q": _turned(s, q, s["norms"][0]).bfloat16(), "k": s["k"], "v": s["v"]}
+    return {"q": _turned(s, q, s["norms"][0]).bfloat16(), **_held(s)}
 
 
 def _plain_read(s):
@@ -266,7 +283,7 @@ def _plain_read(s):
     nth = torch.arange(s["pages"], device=DEVICE) - first[seq]
     source = s["table"].long()[seq, nth]
     valid = nth[:, None] * page + torch.arange(page, device=DEVICE)[None] < s["lens"][seq][:, None]
-    out = {n: (s[n][0].view(torch.uint8)[source].view(DTYPE[c["cache"]]).float() * s[n][1][source][..., None]).transpose(1, 2).masked_fill(
+    out = {n: _values(s[n][0].view(torch.uint8)[source].view(DTYPE[c["cache"]]), s[n][1][source]).transpose(1, 2).masked_fill(
         ~valid[:, :, None, None], 0.0).bfloat16() for n in ("k", "v")}
     column = torch.arange(s["table"].shape[1], device=DEVICE)[None]
     out["table"] = torch.where(column < held[:, None], first[:, None] + column, 0).int()
@@ -280,9 +297,9 @@ def _plain_turn(s):
 
 def _gathered(s, cache):
     """All sequences side by side: [batch, heads, longest, hd] in 32 bits."""
-    codes, scales = cache
+    codes, exponents = cache
     t = s["table"].long()
-    x = codes.view(torch.uint8)[t].view(codes.dtype).float() * scales[t][..., None]
+    x = _values(codes.view(torch.uint8)[t].view(codes.dtype), exponents[t])
     return x.transpose(1, 2).reshape(t.shape[0], x.shape[2], -1, x.shape[-1])[:, :, :s["longest"]]
 
 
@@ -332,14 +349,14 @@ def _e4m3(y):
 def _rows64(state, name, i):
     """Keys or values of sequence i, [tokens, heads, hd]."""
     n = int(state["lens"][i])
-    codes, scales = state[name]
+    codes, exponents = state[name]
     pages = state["table"][i, :-(-n // codes.shape[2])].long()
-    x = codes.view(torch.uint8)[pages].view(codes.dtype).double() * scales[pages].double().unsqueeze(-1)
+    x = codes.view(torch.uint8)[pages].view(codes.dtype).double() * torch.exp2(exponents[pages].double() - 127.0).unsqueeze(-1)
     return x.permute(0, 2, 1, 3).flatten(0, 1)[:n]
 
 
 def _written64(state):
-    """Rotated queries in 64 bits, and the cache with the new rows: codes (in 64 bits) and scales."""
+    """Rotated queries in 64 bits, and the cache with the new rows: codes and powers of two."""
     c = state["case"]
     hq, hkv, hd, half = c["hq"], c["hkv"], c["hd"], c["rot"] // 2
     x = state["qkv"].double().unflatten(1, (hq + 2 * hkv, hd))
@@ -357,15 +374,15 @@ def _written64(state):
         else:
             y[..., :half], y[..., half:2 * half] = z.real, z.imag
         parts.append(y)
-    out, limit = {}, RANGE[c["cache"]]
+    out, limit = {}, 448.0 if c["cache"] == "e4m3" else 127.0
     for name, y in (("k", parts[1]), ("v", x[:, hq + hkv:])):
-        a = y.abs().amax(-1)
-        code = y * limit / a[..., None]
+        scale = torch.exp2(torch.ceil(torch.log2(y.abs().amax(-1) / limit)))
+        code = y / scale[..., None]
         code = torch.round(code) if c["cache"] == "int8" else _e4m3(code)
-        codes, scales = state[name][0].to(torch.float64), state[name][1].double()
+        codes, scales = state[name][0].to(torch.float64), torch.exp2(state[name][1].double() - 127.0)
         slot = state["slots"].long()
         p, r = torch.div(slot, c["page"], rounding_mode="floor"), slot % c["page"]
-        codes[p, :, r], scales[p, :, r] = code, a / limit
+        codes[p, :, r], scales[p, :, r] = code, scale
         out[name] = (codes, scales)
     return parts[0], out
 
