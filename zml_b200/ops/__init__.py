@@ -11,12 +11,13 @@ import math
 
 import torch
 
-from . import _lib, reference
+from . import _lib, kv8, reference
 from ._lib import CollectiveTimeout, KernelError, launch_count, raise_on_status  # noqa: F401
+from .kv8 import QuantKV, QuantKVCache, paged_read  # noqa: F401
 
 __all__ = [
     "gemm", "linear", "row_sumsq", "RowStats", "interleave_gate_up", "rmsnorm", "rope_kvwrite", "swiglu", "embedding", "argmax", "topk_sample",
-    "paged_prefill", "paged_decode", "decode_plan_splits", "KernelError", "launch_count",
+    "paged_prefill", "paged_decode", "paged_read", "QuantKV", "QuantKVCache", "decode_plan_splits", "KernelError", "launch_count",
     "raise_on_status",
 ]
 
@@ -224,9 +225,12 @@ def rope_kvwrite(qkv, positions, slot_mapping, inv_freq, k_cache, v_cache, hq: i
     """RoPE on q and k of the fused qkv activation and scatter of k, v into the paged cache.
 
     qkv [T, (hq + 2 hkv) * hd]; caches [pages, page_size, hkv, hd]; slot_mapping[t] =
-    page * page_size + offset (negative: padding token, nothing is written).
-    Returns q [T, hq, hd].
+    page * page_size + offset (negative: padding token, nothing is written).  With `QuantKV` caches k and v are written in 8 bits
+    (`ops.kv8`).  Returns q [T, hq, hd].
     """
+    if isinstance(k_cache, QuantKV) or isinstance(v_cache, QuantKV):
+        return kv8.rope_kvwrite(qkv, positions, slot_mapping, inv_freq, k_cache, v_cache, hq, hkv, hd, layout, rot_dim, attn_factor, q_norm_w, k_norm_w,
+                                norm_eps, norm_unit_offset, q_out)
     if not _cuda(qkv):
         return reference.rope_kvwrite(qkv, positions, slot_mapping, inv_freq, k_cache, v_cache, hq,
                                       hkv, hd, layout, rot_dim, attn_factor, q_norm_w, k_norm_w,
@@ -361,7 +365,11 @@ def paged_decode(q, k_cache, v_cache, block_table, seq_lens, scale: float | None
                  window: int = 0, num_splits: int | None = None, max_seq_len: int | None = None,
                  out=None, ext=None):
     """One query token per sequence against its paged KV.  q [B, hq, hd] -> [B, hq, hd].  `ext` (CUDA only, with `out`): a
-    `gqa.AttnExt`, see `ops.gqa`."""
+    `gqa.AttnExt`, see `ops.gqa`.  `QuantKV` caches are read in 8 bits (`ops.kv8`; they take no `ext`, and split the keys by themselves)."""
+    if isinstance(k_cache, QuantKV) or isinstance(v_cache, QuantKV):
+        if ext is not None:
+            raise ValueError("attention over a quantised cache has no extensions")
+        return kv8.paged_decode(q, k_cache, v_cache, block_table, seq_lens, scale, window, max_seq_len, out)
     if not _cuda(q):
         return reference.paged_decode(q, k_cache, v_cache, block_table, seq_lens, scale, window)
     _need_bf16(q, k_cache, v_cache)
@@ -420,14 +428,20 @@ def prefill_on_tc(q, k_cache, ext=None) -> bool:
 
 
 def paged_prefill(q, k_cache, v_cache, block_table, seq_lens, q_start, scale: float | None = None,
-                  window: int = 0, out=None, total_q_blocks: int | None = None, impl: str = "auto", ext=None, max_seq_len: int | None = None):
+                  window: int = 0, out=None, total_q_blocks: int | None = None, impl: str = "auto", ext=None, max_seq_len: int | None = None,
+                  kv_pages: int | None = None):
     """Varlen causal attention of new tokens against the paged KV (which already holds them).
 
     q [T, hq, hd]; q_start int32 [B+1] (device); seq_lens int32 [B] = keys per sequence.
     `max_seq_len`: keys of the longest sequence, where the caller knows it (else the block table's width); it chooses the kernel only.
     `impl`: "auto" (the tcgen05 kernel where it applies and is the faster one), "tc" (require it) or "mma" (the mma.sync kernel).  `ext` (CUDA
-    only, with `out`): a `gqa.AttnExt`, see `ops.gqa`.
+    only, with `out`): a `gqa.AttnExt`, see `ops.gqa`.  `QuantKV` caches are read back to bf16 first (`ops.kv8`; no `ext`); `kv_pages`: pages
+    that the sequences hold together, where the caller knows it, which sizes that workspace.
     """
+    if isinstance(k_cache, QuantKV) or isinstance(v_cache, QuantKV):
+        if ext is not None:
+            raise ValueError("attention over a quantised cache has no extensions")
+        return kv8.paged_prefill(q, k_cache, v_cache, block_table, seq_lens, q_start, scale, window, out, total_q_blocks, impl, max_seq_len, kv_pages)
     if not _cuda(q):
         return reference.paged_attention(q, k_cache, v_cache, block_table, seq_lens.tolist(),
                                          q_start.tolist(), scale, window)

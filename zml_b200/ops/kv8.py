@@ -1,0 +1,371 @@
+"""Paged key / value cache in 8 bits: the form of the cache, and the ops that write it, attend to it and read it back.
+
+A row is one token's key (or value) of one head, x of `hd` numbers.  Its scale is the smallest power of two 2^k with max |x| <= R 2^k, R = 448 for
+float8_e4m3fn and 127 for int8; its codes are x / 2^k rounded to the cache's type, and it stands for codes * 2^k, which are bf16 numbers: reading
+back is exact.  The scale is held as the byte k + 127.  A row that holds an infinity or a NaN has the byte 255 and codes of zero, and reads as
+NaN.  A row takes hd + 1 bytes where the bf16 cache has 2 hd.
+
+The ops of the bf16 cache take a `QuantKV` in the place of a cache tensor: `ops.rope_kvwrite`, `ops.paged_decode`, `ops.paged_prefill`;
+`ops.paged_read` reads sequences back to bf16.  `QuantKVCache` is the whole cache of a model, indexed as the engine's bf16 tensor is.
+(The reference's paged kernels take an fp8 cache with per-tensor scales, zml/attention/triton_attention.zig:308-315, which every call site
+turns off.)
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+_p, _i, _ll, _f = C.c_void_p, C.c_int, C.c_longlong, C.c_float
+_lib.register_signature("zb_kv8_write", _i, [_p] * 11 + [_ll] + [_i] * 7 + [_ll, _f, _f, _i, _i, _p])
+_lib.register_signature("zb_kv8_read", _i, [_p] * 9 + [_i] * 8 + [_p])
+_lib.register_signature("zb_kv8_decode_plan", _i, [_i] * 5 + [_p])
+_lib.register_signature("zb_kv8_decode", _i, [_p] * 8 + [_i] * 7 + [_ll, _f, _i, _i, _p, _i, _p])
+
+# names that the engine and the command line take -> type of the codes
+KV_DTYPES = {"fp8": torch.float8_e4m3fn, "int8": torch.int8}
+_RANGE = {torch.float8_e4m3fn: (8, 1.75), torch.int8: (6, 1.984375)}     # R = 2^e * m
+HEAD_DIMS = (64, 128, 256)
+MIN_EXPONENT, NAN_EXPONENT = 27, 255                                     # the smallest scale that is written is 2^-100
+
+
+class QuantKV:
+    """Keys or values of one layer: `codes` [pages, kv_heads, page_size, hd] (float8_e4m3fn or int8) and the scales' `exponents` uint8 [pages,
+    kv_heads, page_size].  A page of one head is contiguous."""
+    __slots__ = ("codes", "exponents")
+
+    def __init__(self, codes: torch.Tensor, exponents: torch.Tensor):
+        if codes.dtype not in _RANGE:
+            raise TypeError(f"a quantised cache holds float8_e4m3fn or int8 codes, got {codes.dtype}")
+        if exponents.dtype is not torch.uint8:
+            raise TypeError(f"the exponents of a quantised cache are uint8, got {exponents.dtype}")
+        if codes.dim() != 4 or exponents.shape != codes.shape[:3]:
+            raise ValueError(f"codes [pages, heads, page_size, hd] with exponents [pages, heads, page_size], got {tuple(codes.shape)} and "
+                             f"{tuple(exponents.shape)}")
+        if exponents.device != codes.device or not codes.is_contiguous() or not exponents.is_contiguous():
+            raise ValueError("codes and exponents are contiguous and on one device")
+        self.codes, self.exponents = codes, exponents
+
+    @staticmethod
+    def alloc(pages: int, kv_heads: int, page_size: int, hd: int, dtype=torch.float8_e4m3fn, device="cpu") -> "QuantKV":
+        """Zeros."""
+        return QuantKV(torch.zeros((pages, kv_heads, page_size, hd), dtype=dtype, device=device),
+                       torch.zeros((pages, kv_heads, page_size), dtype=torch.uint8, device=device))
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def page_size(self) -> int:
+        return self.codes.shape[2]
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        """What all rows stand for, in the layout of a bf16 cache: [pages, page_size, kv_heads, hd]."""
+        return _values(self.codes, self.exponents).transpose(1, 2).to(dtype)
+
+
+class QuantKVCache:
+    """Codes [layers, 2, pages, kv_heads, page_size, hd] and exponents of a whole model; `cache[layer, 0]` are the keys of a layer, `cache[layer, 1]`
+    its values, as `QuantKV`."""
+
+    def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, hd: int, dtype=torch.float8_e4m3fn, device="cpu"):
+        if dtype not in _RANGE:
+            raise TypeError(f"a quantised cache holds float8_e4m3fn or int8 codes, got {dtype}")
+        if hd not in HEAD_DIMS or page_size % 16 or page_size <= 0:
+            raise ValueError(f"a quantised cache has heads of {HEAD_DIMS} and pages of a multiple of 16 tokens, got {hd} and {page_size}")
+        self.codes = torch.zeros((layers, 2, pages, kv_heads, page_size, hd), dtype=dtype, device=device)
+        self.exponents = torch.zeros((layers, 2, pages, kv_heads, page_size), dtype=torch.uint8, device=device)
+        self._layers = [[QuantKV(self.codes[l, i], self.exponents[l, i]) for i in range(2)] for l in range(layers)]
+
+    def __getitem__(self, at) -> QuantKV:
+        layer, which = at
+        return self._layers[layer][which]
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.exponents.numel()
+
+
+def kv_dtype(name) -> torch.dtype:
+    """The code type that "fp8", "int8" or a torch dtype names."""
+    dt = KV_DTYPES.get(name, name)
+    if dt not in _RANGE:
+        raise ValueError(f"unknown cache type {name!r}; known: {', '.join(KV_DTYPES)}")
+    return dt
+
+
+def _power(exponents: torch.Tensor) -> torch.Tensor:
+    """The powers of two that exponent bytes stand for, NaN for 255."""
+    p = (exponents.int() << 23).view(torch.float32)
+    return torch.where(exponents == NAN_EXPONENT, float("nan"), p)
+
+
+def _values(codes, exponents) -> torch.Tensor:
+    return codes.float() * _power(exponents)[..., None]
+
+
+def quantize(x: torch.Tensor, dtype=torch.float8_e4m3fn):
+    """Rows x [..., hd] -> (codes, exponents [...]); the restatement of what the writing kernel does."""
+    e, m = _RANGE[dtype]
+    xf = x.float()
+    a = xf.abs().amax(-1)
+    ok = torch.isfinite(a)
+    frac, exp = torch.frexp(torch.where(ok, a, torch.ones_like(a)))          # a = frac 2^exp, frac in [0.5, 1)
+    byte = (exp - 1 - e + (2 * frac > m) + 127).clamp_min(MIN_EXPONENT)
+    y = torch.where(ok[..., None], xf * _power(254 - byte)[..., None], 0.0)
+    y = y.round() if dtype is torch.int8 else y
+    return y.to(dtype), torch.where(ok, byte, NAN_EXPONENT).to(torch.uint8)
+
+
+# ------------------------------------------------------------------ checks
+def _pair(k: QuantKV, v) -> None:
+    if not isinstance(v, QuantKV) or not isinstance(k, QuantKV):
+        raise TypeError("keys and values are both quantised or both not")
+    if k.codes.dtype is not v.codes.dtype or k.codes.shape != v.codes.shape or k.codes.device != v.codes.device:
+        raise ValueError("keys and values of one type, shape and device")
+    n = k.codes.shape
+    if n[3] not in HEAD_DIMS or n[2] % 16 or n[2] == 0 or n[0] == 0:
+        raise ValueError(f"a quantised cache has heads of {HEAD_DIMS} and pages of a multiple of 16 tokens, got {n[3]} and {n[2]}")
+    if (k.codes.data_ptr() | v.codes.data_ptr() | k.exponents.data_ptr() | v.exponents.data_ptr()) % 16:
+        raise ValueError("codes and exponents start on 16 bytes")
+    if n[0] * n[1] * n[2] >= 2 ** 31:
+        raise ValueError("a quantised cache of a layer has fewer than 2^31 rows")
+
+
+def _ints(device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t.dtype is not torch.int32 or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"{name}: contiguous int32 on {device}, got {t.dtype} on {t.device}")
+
+
+def _table(k: QuantKV, block_table, seq_lens) -> None:
+    _ints(k.codes.device, block_table=block_table, seq_lens=seq_lens)
+    if block_table.dim() != 2 or seq_lens.dim() != 1 or block_table.shape[0] != seq_lens.shape[0]:
+        raise ValueError(f"block_table [batch, pages] with seq_lens [batch], got {tuple(block_table.shape)} and {tuple(seq_lens.shape)}")
+
+
+def _queries(q, k: QuantKV, out) -> tuple[int, int, int]:
+    if q.dtype is not torch.bfloat16 or q.device != k.codes.device or q.dim() != 3:
+        raise TypeError(f"queries [rows, heads, hd] in bfloat16 on {k.codes.device}, got {q.dtype} {tuple(q.shape)} on {q.device}")
+    rows, hq, hd = q.shape
+    if hd != k.codes.shape[3] or hq % k.codes.shape[1] or hq == 0:
+        raise ValueError(f"{hq} query heads of {hd} do not go with {k.codes.shape[1]} key heads of {k.codes.shape[3]}")
+    if out is not None and (out.dtype is not torch.bfloat16 or out.shape != q.shape or out.device != q.device or not out.is_contiguous()):
+        raise ValueError("out: contiguous bfloat16 of the queries' shape")
+    return rows, hq, hd
+
+
+def _on(device):
+    """The device's kernels run with it as the current one."""
+    return torch.cuda.device(device)
+
+
+def _foreign(device) -> bool:
+    return torch.cuda.current_device() != device.index
+
+
+# ------------------------------------------------------------------ writer
+def rope_kvwrite(qkv, positions, slot_mapping, inv_freq, k: QuantKV, v: QuantKV, hq: int, hkv: int, hd: int, layout: int = 0,
+                 rot_dim: Optional[int] = None, attn_factor: float = 1.0, q_norm_w=None, k_norm_w=None, norm_eps: float = 1e-6,
+                 norm_unit_offset: bool = False, q_out=None):
+    """`ops.rope_kvwrite` on a quantised cache.  From the projection to the one rounding at the end all is 32 bits, and angles are formed in 64.
+    The slots of one call differ from one another."""
+    _pair(k, v)
+    pages, heads, page_size, head = k.codes.shape
+    t, rot = qkv.shape[0], hd if rot_dim is None else rot_dim
+    dev = k.codes.device
+    if qkv.dtype is not torch.bfloat16 or qkv.device != dev or qkv.dim() != 2 or qkv.stride(1) != 1:
+        raise TypeError(f"qkv [tokens, (hq + 2 hkv) hd] in bfloat16 on {dev}, got {qkv.dtype} {tuple(qkv.shape)} on {qkv.device}")
+    if (heads, head) != (hkv, hd) or qkv.shape[1] != (hq + 2 * hkv) * hd:
+        raise ValueError(f"a projection of {qkv.shape[1]} columns and a cache of {heads} heads of {head} for {hq} + 2 x {hkv} heads of {hd}")
+    if rot % 2 or not 0 <= rot <= hd or layout not in (0, 1, 2):
+        raise ValueError(f"rotation of {rot} of {hd} columns in layout {layout}")
+    _ints(dev, positions=positions, slot_mapping=slot_mapping)
+    if positions.shape != (t,) or slot_mapping.shape != (t,):
+        raise ValueError(f"{t} tokens with positions {tuple(positions.shape)} and slots {tuple(slot_mapping.shape)}")
+    if inv_freq.dtype is not torch.float32 or inv_freq.device != dev or inv_freq.numel() < rot // 2 or not inv_freq.is_contiguous():
+        raise ValueError(f"inv_freq: {rot // 2} contiguous float32 numbers on {dev}")
+    for w in (q_norm_w, k_norm_w):
+        if w is not None and (w.dtype is not torch.bfloat16 or w.shape != (hd,) or w.device != dev or not w.is_contiguous()):
+            raise ValueError(f"norm weights: {hd} contiguous bfloat16 numbers on {dev}")
+    if q_out is not None and (q_out.dtype is not torch.bfloat16 or q_out.shape != (t, hq, hd) or q_out.device != dev or not q_out.is_contiguous()):
+        raise ValueError(f"q_out: contiguous bfloat16 [{t}, {hq}, {hd}] on {dev}")
+    if not qkv.is_cuda:
+        q = _rope_kvwrite_cpu(qkv, positions, slot_mapping, inv_freq, k, v, hq, hkv, hd, layout, rot, attn_factor, q_norm_w, k_norm_w, norm_eps,
+                              norm_unit_offset)
+        return q if q_out is None else q_out.copy_(q)
+    if _foreign(dev):
+        with _on(dev):
+            return rope_kvwrite(qkv, positions, slot_mapping, inv_freq, k, v, hq, hkv, hd, layout, rot, attn_factor, q_norm_w, k_norm_w, norm_eps,
+                                norm_unit_offset, q_out)
+    if q_out is None:
+        q_out = torch.empty((t, hq, hd), dtype=torch.bfloat16, device=dev)
+    rc = _lib.lib().zb_kv8_write(
+        qkv.data_ptr(), q_out.data_ptr(), k.codes.data_ptr(), k.exponents.data_ptr(), v.codes.data_ptr(), v.exponents.data_ptr(), positions.data_ptr(),
+        slot_mapping.data_ptr(), inv_freq.data_ptr(), None if q_norm_w is None else q_norm_w.data_ptr(), None if k_norm_w is None else k_norm_w.data_ptr(),
+        qkv.stride(0), t, hq, hkv, hd, rot, layout, page_size, pages * page_size, attn_factor, norm_eps, norm_unit_offset,
+        k.codes.dtype is torch.int8, _lib.stream_ptr())
+    _lib.check(rc, "zb_kv8_write")
+    return q_out
+
+
+def _rope_kvwrite_cpu(qkv, positions, slot_mapping, inv_freq, k, v, hq, hkv, hd, layout, rot, attn_factor, q_norm_w, k_norm_w, norm_eps, norm_unit_offset):
+    t, half = qkv.shape[0], rot // 2
+    x = qkv.float().reshape(t, hq + 2 * hkv, hd)
+    angle = positions.double()[:, None] * inv_freq.double()[None, :half]
+    cos, sin = (angle.cos().float() * attn_factor)[:, None], (angle.sin().float() * attn_factor)[:, None]
+    i = torch.arange(half)
+    i, j = {0: (i, i + half), 1: (2 * i, 2 * i + 1), 2: (i, i + hd // 2)}[layout]
+
+    def turned(y, w):
+        if w is not None:
+            y = y * torch.rsqrt(y.pow(2).mean(-1, keepdim=True) + norm_eps) * (w.float() + (1.0 if norm_unit_offset else 0.0))
+        out = y.clone()
+        out[..., i] = y[..., i] * cos - y[..., j] * sin
+        out[..., j] = y[..., j] * cos + y[..., i] * sin
+        return out
+
+    slots = slot_mapping.long()
+    n = k.codes.shape[0] * k.page_size
+    if bool((slots >= n).any()):
+        raise IndexError(f"slot {int(slots.max())} of a cache of {n}")
+    at = slots >= 0
+    page, row = slots[at] // k.page_size, slots[at] % k.page_size
+    for cache, y in ((k, turned(x[:, hq:hq + hkv], k_norm_w)), (v, x[:, hq + hkv:])):
+        codes, exponents = quantize(y[at], cache.codes.dtype)
+        cache.codes.view(torch.uint8)[page, :, row] = codes.view(torch.uint8)
+        cache.exponents[page, :, row] = exponents
+    return turned(x[:, :hq], q_norm_w).to(qkv.dtype)
+
+
+# ------------------------------------------------------------------ reader
+def paged_read(k: QuantKV, v: QuantKV, block_table, seq_lens, num_pages: Optional[int] = None):
+    """Reads whole sequences back: (keys, values, table) with keys and values bfloat16 [num_pages, page_size, kv_heads, hd], the pages of sequence
+    after sequence, and the block table int32 [batch, pages] that finds them there (zeros behind a sequence's pages).  Rows behind a sequence's
+    end in its last page are zero.  `num_pages`: pages that the sequences hold together, where the caller knows it (else room for as many as
+    the block table has; those behind the last sequence are not written).  Fewer than they hold are read as far as they go, and reported (`raise_on_status`)."""
+    _pair(k, v)
+    _table(k, block_table, seq_lens)
+    pages, heads, page_size, hd = k.codes.shape
+    b, width = block_table.shape
+    dev = k.codes.device
+    n = b * width if num_pages is None else int(num_pages)
+    if n < 0:
+        raise ValueError(f"{n} pages")
+    if dev.type != "cuda":
+        return _paged_read_cpu(k, v, block_table, seq_lens, n)
+    if _foreign(dev):
+        with _on(dev):
+            return paged_read(k, v, block_table, seq_lens, num_pages)
+    out = torch.empty((2, n, page_size, heads, hd), dtype=torch.bfloat16, device=dev)
+    table = torch.empty((b, width), dtype=torch.int32, device=dev)
+    kd, vd = out.unbind(0)
+    rc = _lib.lib().zb_kv8_read(k.codes.data_ptr(), k.exponents.data_ptr(), v.codes.data_ptr(), v.exponents.data_ptr(), kd.data_ptr(), vd.data_ptr(),
+                                block_table.data_ptr(), seq_lens.data_ptr(), table.data_ptr(), b, heads, hd, page_size, width, pages, n,
+                                k.codes.dtype is torch.int8, _lib.stream_ptr())
+    _lib.check(rc, "zb_kv8_read")
+    return kd, vd, table
+
+
+def _paged_read_cpu(k, v, block_table, seq_lens, n):
+    pages, heads, page_size, hd = k.codes.shape
+    b, width = block_table.shape
+    out = torch.zeros((2, n, page_size, heads, hd), dtype=torch.bfloat16)
+    table = torch.zeros((b, width), dtype=torch.int32)
+    lens = seq_lens.clamp(0, width * page_size).tolist()
+    if sum(-(-x // page_size) for x in lens) > n:
+        raise ValueError(f"the sequences hold more than {n} pages")
+    at = 0
+    for i, length in enumerate(lens):
+        m = -(-length // page_size)
+        source = block_table[i, :m].long()
+        for to, cache in zip(out, (k, v)):
+            x = _values(cache.codes.view(torch.uint8)[source].view(cache.codes.dtype), cache.exponents[source])
+            to[at:at + m] = x.transpose(1, 2).to(torch.bfloat16)
+            to[at:at + m].reshape(m * page_size, heads, hd)[length:] = 0
+        table[i, :m] = torch.arange(at, at + m, dtype=torch.int32)
+        at += m
+    return out[0], out[1], table
+
+
+# ------------------------------------------------------------------ attention
+_PLANS: dict = {}
+
+
+def _plan(device, b, hq, hkv, hd, max_len) -> tuple[int, int]:
+    """(CTAs, numbers of the workspace) of a decode call: a function of its sizes."""
+    key = (device.index, b, hq, hkv, hd, -(-max_len // 64))
+    got = _PLANS.get(key)
+    if got is None:
+        n = C.c_longlong()
+        ctas = _lib.lib().zb_kv8_decode_plan(b, hq, hkv, hd, max_len, C.byref(n))
+        if ctas < 0:
+            _lib.check(ctas, "zb_kv8_decode_plan")
+        if len(_PLANS) >= 4096:
+            _PLANS.clear()
+        got = _PLANS[key] = (ctas, n.value)
+    return got
+
+
+def paged_decode(q, k: QuantKV, v: QuantKV, block_table, seq_lens, scale: Optional[float] = None, window: int = 0,
+                 max_seq_len: Optional[int] = None, out=None):
+    """`ops.paged_decode` on a quantised cache.  The keys are split over the GPU on the device, from the lengths there (`max_seq_len` bounds
+    the launch only); any number of query heads for a key head."""
+    _pair(k, v)
+    _table(k, block_table, seq_lens)
+    b, hq, hd = _queries(q, k, out)
+    pages, hkv, page_size, _ = k.codes.shape
+    width = block_table.shape[1]
+    if block_table.shape[0] != b:
+        raise ValueError(f"{b} queries for {block_table.shape[0]} sequences")
+    if not q.is_cuda:
+        from . import reference
+        a = reference.paged_decode(q.float(), k.dequantize(), v.dequantize(), block_table, seq_lens.clamp(0, width * page_size), scale, window).to(q.dtype)
+        return a if out is None else out.copy_(a)
+    dev = k.codes.device
+    if _foreign(dev):
+        with _on(dev):
+            return paged_decode(q, k, v, block_table, seq_lens, scale, window, max_seq_len, out)
+    if q.stride(2) != 1 or q.stride(1) != hd or (b > 1 and q.stride(0) % 4) or q.data_ptr() % 8:
+        q = q.contiguous() if not q.is_contiguous() else q.clone()           # the kernel reads 8 bytes of a row at a time
+    if out is None:
+        out = torch.empty((b, hq, hd), dtype=torch.bfloat16, device=dev)
+    most = width * page_size
+    ctas, numbers = _plan(dev, b, hq, hkv, hd, most if max_seq_len is None else min(max_seq_len, most))
+    work = torch.empty(numbers, dtype=torch.float32, device=dev)
+    rc = _lib.lib().zb_kv8_decode(
+        q.data_ptr(), k.codes.data_ptr(), k.exponents.data_ptr(), v.codes.data_ptr(), v.exponents.data_ptr(), out.data_ptr(), block_table.data_ptr(),
+        seq_lens.data_ptr(), b, hq, hkv, hd, page_size, width, pages, q.stride(0), 1.0 / math.sqrt(hd) if scale is None else scale, window,
+        k.codes.dtype is torch.int8, work.data_ptr(), ctas, _lib.stream_ptr())
+    _lib.check(rc, "zb_kv8_decode")
+    return out
+
+
+def paged_prefill(q, k: QuantKV, v: QuantKV, block_table, seq_lens, q_start, scale: Optional[float] = None, window: int = 0, out=None,
+                  total_q_blocks: Optional[int] = None, impl: str = "auto", max_seq_len: Optional[int] = None, kv_pages: Optional[int] = None):
+    """`ops.paged_prefill` on a quantised cache: the sequences are read back to bf16 (`paged_read`; `kv_pages` is its `num_pages`), and the bf16
+    kernels attend to that.  Prompts are bound by their products: reading back moves 6 bytes a key, head and column once, where every query of
+    the group makes 4 operations of them; the workspace lives as long as the call."""
+    _pair(k, v)
+    _table(k, block_table, seq_lens)
+    _queries(q, k, out)
+    _ints(k.codes.device, q_start=q_start)
+    from . import paged_prefill as bf16_prefill
+    dev = k.codes.device
+    if dev.type == "cuda" and _foreign(dev):
+        with _on(dev):
+            return paged_prefill(q, k, v, block_table, seq_lens, q_start, scale, window, out, total_q_blocks, impl, max_seq_len, kv_pages)
+    b, width = block_table.shape
+    if kv_pages is None and max_seq_len is not None:
+        kv_pages = b * min(width, -(-max_seq_len // k.page_size))
+    kd, vd, table = paged_read(k, v, block_table, seq_lens, kv_pages)
+    a = bf16_prefill(q, kd, vd, table, seq_lens, q_start, scale, window, out=out, total_q_blocks=total_q_blocks, impl=impl, max_seq_len=max_seq_len)
+    return a if out is None or a is out else out.copy_(a)
