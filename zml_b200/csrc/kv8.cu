@@ -316,91 +316,110 @@ void launch_write_hd(const Kv8WriteParams& p, bool int8, dim3 grid, int threads,
 
 extern "C" {
 
-// Codes and exponents are contiguous and start on 16 bytes; negative slots write nothing.
-int zb_kv8_write(const void* qkv, void* q_out, void* k_codes, void* k_exps, void* v_codes, void* v_exps, const int32_t* positions,
-                 const int32_t* slot_mapping, const float* inv_freq, const void* q_norm_w, const void* k_norm_w, long long qkv_stride, int tokens,
-                 int hq, int hkv, int hd, int rot_dim, int layout, int page_size, long long num_slots, float attn_factor, float norm_eps,
-                 int norm_unit_offset, int int8, void* stream) {
-  if (tokens <= 0) return 0;
+// The arguments of a call, as the caller packs them (ops/kv8.py).
+struct ZbKv8Write {
+  const void* qkv;
+  void* q_out;
+  void *k_codes, *k_exps, *v_codes, *v_exps;       // contiguous, on 16 bytes
+  const int32_t* positions;
+  const int32_t* slot_mapping;                     // negative: the token's keys and values are not written
+  const float* inv_freq;
+  const void *q_norm_w, *k_norm_w;                 // or null
+  void* stream;
+  long long qkv_stride, num_slots;
+  int tokens, hq, hkv, hd, rot_dim, layout, page_size, norm_unit_offset, int8;
+  float attn_factor, norm_eps;
+};
+struct ZbKv8Read {
+  const void *k_codes, *k_exps, *v_codes, *v_exps;
+  void *k_out, *v_out;                             // out_pages pages; a batch that needs more is reported and read as far as they go
+  const int32_t* block_table;
+  const int32_t* seq_lens;
+  int32_t* out_table;
+  void* stream;
+  int batch, hkv, hd, page_size, max_pages, num_pages, out_pages, int8;
+};
+
+int zb_kv8_write(const ZbKv8Write* c) {
+  if (c->tokens <= 0) return 0;
+  const int hd = c->hd, rot_dim = c->rot_dim, layout = c->layout;
   if ((hd != 64 && hd != 128 && hd != 256) || rot_dim % 2 != 0 || rot_dim < 0 || rot_dim > hd || layout < 0 || layout > 2) return -42;
-  if (page_size <= 0 || num_slots > 0x7fffffffll) return -43;
+  if (c->page_size <= 0 || c->num_slots > 0x7fffffffll) return -43;
   ZbDeviceState* st = zb_device_state();
   if (!st) return -20;
   Kv8WriteParams p = {};
-  p.qkv = reinterpret_cast<const __nv_bfloat16*>(qkv);
-  p.q_out = reinterpret_cast<__nv_bfloat16*>(q_out);
-  p.k_codes = reinterpret_cast<uint8_t*>(k_codes);
-  p.v_codes = reinterpret_cast<uint8_t*>(v_codes);
-  p.k_exps = reinterpret_cast<uint8_t*>(k_exps);
-  p.v_exps = reinterpret_cast<uint8_t*>(v_exps);
-  p.positions = positions;
-  p.slot_mapping = slot_mapping;
-  p.inv_freq = inv_freq;
-  p.q_norm_w = reinterpret_cast<const __nv_bfloat16*>(q_norm_w);
-  p.k_norm_w = reinterpret_cast<const __nv_bfloat16*>(k_norm_w);
-  p.qkv_stride = qkv_stride;
-  p.num_slots = num_slots;
-  p.tokens = tokens;
-  p.hq = hq;
-  p.hkv = hkv;
+  p.qkv = reinterpret_cast<const __nv_bfloat16*>(c->qkv);
+  p.q_out = reinterpret_cast<__nv_bfloat16*>(c->q_out);
+  p.k_codes = reinterpret_cast<uint8_t*>(c->k_codes);
+  p.v_codes = reinterpret_cast<uint8_t*>(c->v_codes);
+  p.k_exps = reinterpret_cast<uint8_t*>(c->k_exps);
+  p.v_exps = reinterpret_cast<uint8_t*>(c->v_exps);
+  p.positions = c->positions;
+  p.slot_mapping = c->slot_mapping;
+  p.inv_freq = c->inv_freq;
+  p.q_norm_w = reinterpret_cast<const __nv_bfloat16*>(c->q_norm_w);
+  p.k_norm_w = reinterpret_cast<const __nv_bfloat16*>(c->k_norm_w);
+  p.qkv_stride = c->qkv_stride;
+  p.num_slots = c->num_slots;
+  p.tokens = c->tokens;
+  p.hq = c->hq;
+  p.hkv = c->hkv;
   p.hd = hd;
   p.rot_dim = rot_dim;
   p.layout = layout;
-  p.page_size = page_size;
-  p.attn_factor = attn_factor;
-  p.norm_eps = norm_eps;
-  p.norm_unit_offset = norm_unit_offset;
+  p.page_size = c->page_size;
+  p.attn_factor = c->attn_factor;
+  p.norm_eps = c->norm_eps;
+  p.norm_unit_offset = c->norm_unit_offset;
   p.status = st->status;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(c->stream);
   const auto at16 = [](const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; };
-  const bool aligned = qkv_stride % 8 == 0 && at16(qkv) && at16(q_out) && at16(q_norm_w) && at16(k_norm_w);
+  const bool aligned = c->qkv_stride % 8 == 0 && at16(c->qkv) && at16(c->q_out) && at16(c->q_norm_w) && at16(c->k_norm_w);
   if (aligned && (layout == 1 || (layout == 0 && rot_dim % 16 == 0))) {
-    const int units = (hq + 2 * hkv) * (hd / 16), parts = tokens <= 64 ? (units + 511) / 512 : 1;
+    const int units = (p.hq + 2 * p.hkv) * (hd / 16), parts = p.tokens <= 64 ? (units + 511) / 512 : 1;
     p.share = ((units + parts - 1) / parts + 31) / 32 * 32;
     const int threads = p.share < 512 ? p.share : 512;
-    if (layout == 0) launch_write_hd<0>(p, int8 != 0, dim3(tokens, parts), threads, s);
-    else launch_write_hd<1>(p, int8 != 0, dim3(tokens, parts), threads, s);
-  } else if (int8) {
-    zb_launch(zb_kv8_write_any_kernel<true>, dim3(tokens), dim3(256), 0, s, p);
+    if (layout == 0) launch_write_hd<0>(p, c->int8 != 0, dim3(p.tokens, parts), threads, s);
+    else launch_write_hd<1>(p, c->int8 != 0, dim3(p.tokens, parts), threads, s);
+  } else if (c->int8) {
+    zb_launch(zb_kv8_write_any_kernel<true>, dim3(p.tokens), dim3(256), 0, s, p);
   } else {
-    zb_launch(zb_kv8_write_any_kernel<false>, dim3(tokens), dim3(256), 0, s, p);
+    zb_launch(zb_kv8_write_any_kernel<false>, dim3(p.tokens), dim3(256), 0, s, p);
   }
   zb_count_launch(1);
   return static_cast<int>(cudaGetLastError());
 }
 
-// Outputs hold out_pages pages; a batch that needs more is reported in the status word and read as far as they go.
-int zb_kv8_read(const void* k_codes, const void* k_exps, const void* v_codes, const void* v_exps, void* k_out, void* v_out,
-                const int32_t* block_table, const int32_t* seq_lens, int32_t* out_table, int batch, int hkv, int hd, int page_size, int max_pages,
-                int num_pages, int out_pages, int int8, void* stream) {
-  if (batch <= 0) return 0;
-  if (hd != 64 && hd != 128 && hd != 256) return -42;
+int zb_kv8_read(const ZbKv8Read* c) {
+  if (c->batch <= 0) return 0;
+  if (c->hd != 64 && c->hd != 128 && c->hd != 256) return -42;
   ZbDeviceState* st = zb_device_state();
   if (!st) return -20;
   Kv8ReadParams p = {};
-  p.k_codes = reinterpret_cast<const uint8_t*>(k_codes);
-  p.v_codes = reinterpret_cast<const uint8_t*>(v_codes);
-  p.k_exps = reinterpret_cast<const uint8_t*>(k_exps);
-  p.v_exps = reinterpret_cast<const uint8_t*>(v_exps);
-  p.k_out = reinterpret_cast<__nv_bfloat16*>(k_out);
-  p.v_out = reinterpret_cast<__nv_bfloat16*>(v_out);
-  p.block_table = block_table;
-  p.seq_lens = seq_lens;
-  p.out_table = out_table;
-  p.batch = batch;
-  p.hkv = hkv;
-  p.page_size = page_size;
-  p.max_pages = max_pages;
-  p.num_pages = num_pages;
-  p.out_pages = out_pages;
+  p.k_codes = reinterpret_cast<const uint8_t*>(c->k_codes);
+  p.v_codes = reinterpret_cast<const uint8_t*>(c->v_codes);
+  p.k_exps = reinterpret_cast<const uint8_t*>(c->k_exps);
+  p.v_exps = reinterpret_cast<const uint8_t*>(c->v_exps);
+  p.k_out = reinterpret_cast<__nv_bfloat16*>(c->k_out);
+  p.v_out = reinterpret_cast<__nv_bfloat16*>(c->v_out);
+  p.block_table = c->block_table;
+  p.seq_lens = c->seq_lens;
+  p.out_table = c->out_table;
+  p.batch = c->batch;
+  p.hkv = c->hkv;
+  p.page_size = c->page_size;
+  p.max_pages = c->max_pages;
+  p.num_pages = c->num_pages;
+  p.out_pages = c->out_pages;
   p.status = st->status;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const long long items = static_cast<long long>(out_pages) * 2 * hkv;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(c->stream);
+  const long long items = static_cast<long long>(c->out_pages) * 2 * c->hkv;
   if (items > 0x7fffffffll) return -43;
   const int most = st->num_sms * 8;
   const dim3 grid(static_cast<unsigned>(items < 1 ? 1 : (items < most ? items : most)));
-  if (hd == 64) zb_launch(int8 ? zb_kv8_read_kernel<64, true> : zb_kv8_read_kernel<64, false>, grid, dim3(256), 0, s, p);
-  else if (hd == 128) zb_launch(int8 ? zb_kv8_read_kernel<128, true> : zb_kv8_read_kernel<128, false>, grid, dim3(256), 0, s, p);
+  const bool int8 = c->int8 != 0;
+  if (c->hd == 64) zb_launch(int8 ? zb_kv8_read_kernel<64, true> : zb_kv8_read_kernel<64, false>, grid, dim3(256), 0, s, p);
+  else if (c->hd == 128) zb_launch(int8 ? zb_kv8_read_kernel<128, true> : zb_kv8_read_kernel<128, false>, grid, dim3(256), 0, s, p);
   else zb_launch(int8 ? zb_kv8_read_kernel<256, true> : zb_kv8_read_kernel<256, false>, grid, dim3(256), 0, s, p);
   zb_count_launch(1);
   return static_cast<int>(cudaGetLastError());

@@ -12,8 +12,11 @@
 //   16-byte pieces of a row.  Rows are 128 bytes in shared memory (half a row of a head of 256, two rows of a head of 64) in the 128-byte swizzle of
 //   the tensor-map copy: the pieces that eight neighbouring lanes read lie in different banks.
 // * f16 holds neither every bf16 query nor every product p_j s_vj.  A query row is scaled by a power of two to a largest magnitude in
-//   [2^13, 2^14), exactly, and that power is taken out of its scores; s_vj is taken relative to the largest one so far, which rescales the
-//   accumulators like the maximum of the scores does.  What f16 drops lies 2^-25 below the largest weight.
+//   [2^13, 2^14), exactly, and that power is taken out of its scores; s_vj is taken relative to the largest one so far, and the weight times
+//   2^7: what f16 drops lies 2^-32 below.
+// * The reference that scores are taken from, and that of the values' scales, move only when a score exceeds its reference by 2^8 or a scale its own:
+//   the weights stay below 2^15, and a warp looks for that with one vote, where keeping the very maximum takes three shuffles a column
+//   and a multiplication of all accumulators nearly every time.
 // * All tiles of 64 keys of all (sequence, key head) pairs are one list, cut into equal parts, one for each CTA: whatever the mix of lengths,
 //   all SMs stream alike.  A CTA whose part ends inside a pair leaves its sums in the workspace, and a second kernel joins each such
 //   pair.  Lengths are read on the device, so a captured launch serves any of them; nothing outlives the two launches.
@@ -21,6 +24,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "host_api.h"
 #include "kv8.cuh"
@@ -32,6 +36,9 @@ namespace {
 constexpr uint32_t kKernelKv8Decode = 41;
 constexpr int kTile = 64;                       // keys
 constexpr int kMaxCtas = 384;                   // of the partition: what the joining kernel keeps weights for
+constexpr float kNoScore = -3.402823466e38f;    // the reference in front of the first key
+constexpr float kSlack = 8.f;                   // in units of log2: how far a score may exceed its reference
+constexpr uint32_t kLift = 7;                   // log2 of what weights are multiplied by
 
 struct Kv8DecodeParams {
   const __nv_bfloat16* q;
@@ -57,6 +64,21 @@ ZB_DEVICE void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uin
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+ZB_DEVICE uint4 lds128(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+ZB_DEVICE uint2 lds64(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+  return v;
+}
+ZB_DEVICE uint32_t lds8(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
 ZB_DEVICE uint32_t transpose8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -80,8 +102,16 @@ ZB_DEVICE Kv8Span kv8_span(const Kv8DecodeParams& p, int seq) {
   s.tiles = max(1, (s.len + kTile - 1) / kTile - s.tile0);
   return s;
 }
-// First position of CTA c's part of `total`.
-ZB_DEVICE int kv8_part(int total, int c, int ctas) { return static_cast<int>(static_cast<long long>(total) * c / ctas); }
+// The list of `total` tiles in equal parts: part c begins at begin(c), the first ones are one longer.
+struct Kv8Parts {
+  int each, longer;
+  ZB_DEVICE Kv8Parts(int total, int ctas) : each(total / ctas), longer(total - each * ctas) {}
+  ZB_DEVICE int begin(int c) const { return c * each + min(c, longer); }
+  ZB_DEVICE int of(int pos) const {                   // the part that holds a position
+    const int turn = longer * (each + 1);
+    return pos < turn ? pos / (each + 1) : longer + (pos - turn) / each;
+  }
+};
 
 // A CTA's walk over its part: segments of one pair each.  Every warp walks on its own.
 struct Kv8Walk {
@@ -94,8 +124,9 @@ ZB_DEVICE bool kv8_start(const Kv8DecodeParams& p, Kv8Walk& w) {
   const int pairs = p.hkv * p.blocks;
   const auto count = [&](int s) { return kv8_span(p, s).tiles * pairs; };
   const int total = kv8_total(p.batch, count);
-  w.at = kv8_part(total, blockIdx.x, p.ctas);
-  w.last = kv8_part(total, blockIdx.x + 1, p.ctas);
+  const Kv8Parts parts(total, p.ctas);
+  w.at = parts.begin(blockIdx.x);
+  w.last = parts.begin(blockIdx.x + 1);
   if (w.at >= w.last) return false;
   int before;
   kv8_locate(p.batch, w.at, count, w.seq, before);
@@ -136,7 +167,7 @@ __global__ void __launch_bounds__(160, Kv8Sizes<HD, NB>::kPerSm) zb_kv8_decode_k
   using Z = Kv8Sizes<HD, NB>;
   constexpr int kStages = Z::kStages, kRows = Z::kRows, kSteps = HD / 16, kSubs = HD > 128 ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* smem = smem_raw + ((1024u - (zb_smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* exps = smem + kStages * Z::kStageBytes;                                // [stage][keys, values][64]
   float* sums = reinterpret_cast<float*>(exps + kStages * 2 * kTile);             // [warp][row][kPitch]
   float* stats = sums + 4 * kRows * Z::kPitch;                                    // [warp][row][maximum, sum, scale of the values]
@@ -168,6 +199,7 @@ __global__ void __launch_bounds__(160, Kv8Sizes<HD, NB>::kPerSm) zb_kv8_decode_k
       const int kvh = w.pair / p.blocks;
       const int32_t* bt = p.block_table + static_cast<size_t>(w.seq) * p.max_pages;
       int pages = 0;                                 // of the 32 copies from a multiple of 32 on, one a lane
+      int off = (w.span.tile0 + w.begin) * kTile % p.page_size;
       for (int t = w.begin; t < w.end; ++t) {
         if (((t - w.begin) * per_tile & 31) == 0) {
           const int key = (w.span.tile0 + t) * kTile + lane * p.unit;
@@ -186,8 +218,10 @@ __global__ void __launch_bounds__(160, Kv8Sizes<HD, NB>::kPerSm) zb_kv8_decode_k
         uint8_t* ex = exps + stage * 2 * kTile;
         for (int c = 0; c < copies; ++c) {
           const int page = __shfl_sync(0xffffffffu, pages, ((t - w.begin) * per_tile + c) & 31);
+          const long long row = (static_cast<long long>(page) * p.hkv + kvh) * p.page_size + off;
+          off += p.unit;
+          if (off == p.page_size) off = 0;
           if (dead || lane != 0) continue;
-          const long long row = (static_cast<long long>(page) * p.hkv + kvh) * p.page_size + (key0 + c * p.unit) % p.page_size;
           const int y = static_cast<int>(HD == 64 ? row >> 1 : row);
           uint8_t* to = ks + c * p.unit * (HD > 128 ? 128 : HD);
 #pragma unroll
@@ -206,6 +240,26 @@ __global__ void __launch_bounds__(160, Kv8Sizes<HD, NB>::kPerSm) zb_kv8_decode_k
     } while (kv8_next(p, w));
   } else {
     const int g = lane >> 2, t4 = lane & 3;
+    // what this thread reads of a stage: keys g and g + 8 of the warp's 16 in S^T = K Q^T, values 2 t4, 2 t4 + 1 (and 8 further) in O^T = V^T P^T
+    uint32_t k_off[2], v_off[4];
+    if constexpr (HD == 64) {
+      const int r = warp * 16 + g;
+      k_off[0] = (r >> 1) * 128 + (((((r & 1) << 2) + t4) ^ ((r >> 1) & 7)) << 4);
+      k_off[1] = (k_off[0] ^ 64u) + 512u;
+      v_off[0] = Z::kTileBytes + (warp * 8 + t4) * 128 + (((g >> 1) ^ t4) << 4) + (g & 1) * 8;
+      v_off[1] = v_off[0] ^ 64u;
+      v_off[2] = v_off[1] + 512u;
+      v_off[3] = v_off[0] + 512u;
+    } else {
+      const int r = warp * 16 + g, q = warp * 16 + 2 * t4;
+      k_off[0] = r * 128 + (((2 * t4) ^ (r & 7)) << 4);
+      k_off[1] = k_off[0] + 1024u;
+      v_off[0] = Z::kTileBytes + q * 128 + ((g ^ (q & 7)) << 4);
+      v_off[1] = Z::kTileBytes + (q + 1) * 128 + ((g ^ ((q + 1) & 7)) << 4);
+      v_off[2] = v_off[0] + 1024u;
+      v_off[3] = v_off[1] + 1024u;
+    }
+    const uint32_t stages_at = zb_smem_u32(smem), exps_at = zb_smem_u32(exps) + warp * 16 + g;
     bool first_segment = true;
     do {
       const int kvh = w.pair / p.blocks, row0 = (w.pair - kvh * p.blocks) * kRows, rows = min(kRows, p.group - row0);
@@ -245,123 +299,134 @@ __global__ void __launch_bounds__(160, Kv8Sizes<HD, NB>::kPerSm) zb_kv8_decode_k
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) o[b][i][0] = o[b][i][1] = o[b][i][2] = o[b][i][3] = 0.f;
-      float m[NB][2], l[NB][2];
+      float m[NB][2], l[NB][2];                       // references, and the sums of this thread's keys
 #pragma unroll
-      for (int b = 0; b < NB; ++b) m[b][0] = m[b][1] = -INFINITY, l[b][0] = l[b][1] = 0.f;
-      uint32_t power = 1u;                            // exponent byte of the largest scale of a value so far
+      for (int b = 0; b < NB; ++b) m[b][0] = m[b][1] = kNoScore, l[b][0] = l[b][1] = 0.f;
+      uint32_t power = kLift + 1;                     // exponent byte that the values' scales are relative to
+      float unit = __uint_as_float((254u + kLift - power) << 23);
+
+      // 16 keys; !WHOLE: some of them lie behind the end or in front of the window
+      const auto block = [&](auto whole, uint32_t at, uint32_t ex, int key0) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        constexpr int kWords = HD == 64 ? 2 : 4;
+        uint4 kx[2][kSteps / 4];
+        uint32_t v[kSubs][4][kWords];
+#pragma unroll
+        for (int c = 0; c < kSteps / 4; ++c) {
+          kx[0][c] = lds128(at + (c >> 1) * kTile * 128 + (k_off[0] ^ ((c & 1) << 4)));
+          kx[1][c] = lds128(at + (c >> 1) * kTile * 128 + (k_off[1] ^ ((c & 1) << 4)));
+        }
+        const bool see0 = WHOLE || (key0 + g >= w.span.first && key0 + g < w.span.len);
+        const bool see1 = WHOLE || (key0 + g + 8 >= w.span.first && key0 + g + 8 < w.span.len);
+        const float ks0 = kv8_scale(lds8(ex)), ks1 = kv8_scale(lds8(ex + 8));
+        uint32_t ve0 = lds8(ex + kTile), ve1 = lds8(ex + kTile + 8);
+        if (!see0) ve0 = 0u;
+        if (!see1) ve1 = 0u;
+#pragma unroll
+        for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (HD == 64) {
+              const uint2 x = lds64(at + v_off[k]);
+              v[sub][k][0] = x.x, v[sub][k][1] = x.y;
+            } else {
+              const uint4 x = lds128(at + sub * kTile * 128 + v_off[k]);
+              v[sub][k][0] = x.x, v[sub][k][1] = x.y, v[sub][k][2] = x.z, v[sub][k][3] = x.w;
+            }
+            // codes of rows that nobody sees may be anything, e4m3's NaN, too
+            const int key = key0 + 2 * t4 + (k & 1) + (k >> 1) * 8;
+            if (!WHOLE && (key < w.span.first || key >= w.span.len)) {
+#pragma unroll
+              for (int i = 0; i < kWords; ++i) v[sub][k][i] = 0u;
+            }
+          }
+        float s[NB][4];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < kSteps / 4; ++c) {
+          const uint32_t wx[4] = {kx[0][c].x, kx[0][c].y, kx[0][c].z, kx[0][c].w}, wy[4] = {kx[1][c].x, kx[1][c].y, kx[1][c].z, kx[1][c].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t a0, a1, a2, a3;
+            kv8_to_half<INT8>(wx[i], a0, a2);
+            kv8_to_half<INT8>(wy[i], a1, a3);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) mma_f16(s[b], a0, a1, a2, a3, qf[b][c * 4 + i][0], qf[b][c * 4 + i][1]);
+          }
+        }
+        bool moves = max(ve0, ve1) > power;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            s[b][j] = see0 ? s[b][j] * (ks0 * factor[b][j]) : -INFINITY;
+            s[b][j + 2] = see1 ? s[b][j + 2] * (ks1 * factor[b][j]) : -INFINITY;
+            moves = moves || fmaxf(s[b][j], s[b][j + 2]) > m[b][j] + kSlack;
+          }
+        if (__any_sync(0xffffffffu, moves)) {
+          // a row that is NaN has the byte 255: its scale stays an infinity, and its codes of zero make a NaN of it
+          const uint32_t now = max(power, __reduce_max_sync(0xffffffffu, min(max(ve0, ve1), 253u)));
+          const float shrink = now - power > 126u ? 0.f : __uint_as_float((127u - (now - power)) << 23);
+          power = now;
+          unit = __uint_as_float((254u + kLift - now) << 23);
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float mx = fmaxf(s[b][j], s[b][j + 2]);
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16)), m[b][j]);
+              const float c = zb_ex2(m[b][j] - mx);
+              m[b][j] = mx;
+              l[b][j] *= c;
+#pragma unroll
+              for (int i = 0; i < kSteps; ++i) {
+                o[b][i][j] *= c * shrink;
+                o[b][i][j + 2] *= c * shrink;
+              }
+            }
+        }
+        const float vs0 = kv8_scale(ve0) * unit, vs1 = kv8_scale(ve1) * unit;
+        uint32_t pb[NB][2];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            s[b][j] = zb_ex2(s[b][j] - m[b][j]);
+            s[b][j + 2] = zb_ex2(s[b][j + 2] - m[b][j]);
+            l[b][j] += s[b][j] + s[b][j + 2];
+          }
+          pb[b][0] = transpose8(pack_half2(s[b][0] * vs0, s[b][1] * vs0));
+          pb[b][1] = transpose8(pack_half2(s[b][2] * vs1, s[b][3] * vs1));
+        }
+        // columns of a word: pairs of keys of each
+#pragma unroll
+        for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+          for (int i = 0; i < kWords; ++i) {
+            uint32_t a[4], c[4];
+            kv8_to_half<INT8>(__byte_perm(v[sub][0][i], v[sub][1][i], 0x5140), a[0], a[1]);
+            kv8_to_half<INT8>(__byte_perm(v[sub][2][i], v[sub][3][i], 0x5140), a[2], a[3]);
+            kv8_to_half<INT8>(__byte_perm(v[sub][0][i], v[sub][1][i], 0x7362), c[0], c[1]);
+            kv8_to_half<INT8>(__byte_perm(v[sub][2][i], v[sub][3][i], 0x7362), c[2], c[3]);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              mma_f16(o[b][sub * 8 + 2 * i], a[0], a[1], a[2], a[3], pb[b][0], pb[b][1]);
+              mma_f16(o[b][sub * 8 + 2 * i + 1], c[0], c[1], c[2], c[3], pb[b][0], pb[b][1]);
+            }
+          }
+      };
 
       for (int t = w.begin; t < w.end; ++t) {
         if (!dead) dead = !zb_mbar_wait(&full_bar[stage], phase, abort_flag);
         dead = __any_sync(0xffffffffu, dead);
         const int key0 = (w.span.tile0 + t) * kTile + warp * 16;
         if (!dead && key0 < w.span.len && key0 + 16 > w.span.first) {
-          const uint8_t* ks = smem + stage * Z::kStageBytes;
-          const uint8_t* vs = ks + Z::kTileBytes;
-          const uint8_t* ex = exps + stage * 2 * kTile + warp * 16;
-          const bool whole = key0 >= w.span.first && key0 + 16 <= w.span.len;
-          // S^T: keys g and g + 8 of the 16
-          float s[NB][4];
-#pragma unroll
-          for (int b = 0; b < NB; ++b) s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
-          const int r0 = warp * 16 + g, r1 = r0 + 8;
-#pragma unroll
-          for (int c = 0; c < kSteps / 4; ++c) {
-            uint4 x, y;
-            if constexpr (HD == 64) {
-              x = *reinterpret_cast<const uint4*>(ks + (r0 >> 1) * 128 + (((((r0 & 1) << 2) + t4) ^ ((r0 >> 1) & 7)) << 4));
-              y = *reinterpret_cast<const uint4*>(ks + (r1 >> 1) * 128 + (((((r1 & 1) << 2) + t4) ^ ((r1 >> 1) & 7)) << 4));
-            } else {
-              const int at = (c >> 1) * kTile * 128 + (((2 * t4 + (c & 1)) ^ (r0 & 7)) << 4);
-              x = *reinterpret_cast<const uint4*>(ks + at + r0 * 128);
-              y = *reinterpret_cast<const uint4*>(ks + at + r1 * 128);
-            }
-            const uint32_t wx[4] = {x.x, x.y, x.z, x.w}, wy[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t a0, a1, a2, a3;
-              kv8_to_half<INT8>(wx[i], a0, a2);
-              kv8_to_half<INT8>(wy[i], a1, a3);
-#pragma unroll
-              for (int b = 0; b < NB; ++b) mma_f16(s[b], a0, a1, a2, a3, qf[b][c * 4 + i][0], qf[b][c * 4 + i][1]);
-            }
-          }
-          const bool see0 = whole || (key0 + g >= w.span.first && key0 + g < w.span.len);
-          const bool see1 = whole || (key0 + g + 8 >= w.span.first && key0 + g + 8 < w.span.len);
-          const float ks0 = kv8_scale(ex[g]), ks1 = kv8_scale(ex[g + 8]);
-          const uint32_t ve0 = see0 ? ex[kTile + g] : 0u, ve1 = see1 ? ex[kTile + g + 8] : 0u;
-          // values' scales relative to the largest one so far; 255 (a row that is NaN) stays an infinity and its codes of zero make a NaN of it
-          const uint32_t now = max(power, __reduce_max_sync(0xffffffffu, min(max(ve0, ve1), 253u)));
-          const float shrink = power == now ? 1.f : (now - power > 126u ? 0.f : __uint_as_float((127u - (now - power)) << 23));
-          power = now;
-          const float unit = __uint_as_float((254u - now) << 23), vs0 = kv8_scale(ve0) * unit, vs1 = kv8_scale(ve1) * unit;
-          float corr[NB][2];
-          bool moved = shrink != 1.f;
-          uint32_t pb[NB][2];
-#pragma unroll
-          for (int b = 0; b < NB; ++b) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              s[b][j] = see0 ? s[b][j] * (ks0 * factor[b][j]) : -INFINITY;
-              s[b][j + 2] = see1 ? s[b][j + 2] * (ks1 * factor[b][j]) : -INFINITY;
-              float mx = fmaxf(s[b][j], s[b][j + 2]);
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              const float mnew = fmaxf(m[b][j], mx), use = mnew == -INFINITY ? 0.f : mnew;
-              const float c = exp2f(m[b][j] - use);
-              m[b][j] = mnew;
-              s[b][j] = exp2f(s[b][j] - use);
-              s[b][j + 2] = exp2f(s[b][j + 2] - use);
-              l[b][j] = l[b][j] * c + (s[b][j] + s[b][j + 2]);
-              corr[b][j] = c * shrink;
-              moved = moved || c != 1.f;
-            }
-            pb[b][0] = transpose8(pack_half2(see0 ? s[b][0] * vs0 : 0.f, see0 ? s[b][1] * vs0 : 0.f));
-            pb[b][1] = transpose8(pack_half2(see1 ? s[b][2] * vs1 : 0.f, see1 ? s[b][3] * vs1 : 0.f));
-          }
-          if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-              for (int i = 0; i < kSteps; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[b][i][j] *= corr[b][j & 1];
-          }
-          // O^T: keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9 of the 16; columns: piece g of each half row (HD 64: half a piece)
-#pragma unroll
-          for (int sub = 0; sub < kSubs; ++sub) {
-            uint32_t v[4][HD == 64 ? 2 : 4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int kk = 2 * t4 + (k & 1) + (k >> 1) * 8, r = warp * 16 + kk;
-              if constexpr (HD == 64) {
-                const uint2 x = *reinterpret_cast<const uint2*>(vs + (r >> 1) * 128 + (((((r & 1) << 2) + (g >> 1)) ^ ((r >> 1) & 7)) << 4) + (g & 1) * 8);
-                v[k][0] = x.x, v[k][1] = x.y;
-              } else {
-                const uint4 x = *reinterpret_cast<const uint4*>(vs + sub * kTile * 128 + r * 128 + ((g ^ (r & 7)) << 4));
-                v[k][0] = x.x, v[k][1] = x.y, v[k][2] = x.z, v[k][3] = x.w;
-              }
-              // codes of rows that nobody sees may be anything, e4m3's NaN, too
-              if (!whole && (key0 + kk < w.span.first || key0 + kk >= w.span.len)) {
-#pragma unroll
-                for (int i = 0; i < (HD == 64 ? 2 : 4); ++i) v[k][i] = 0u;
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < (HD == 64 ? 2 : 4); ++i) {
-              // pairs of keys of each of the word's four columns
-              uint32_t a[4], c[4];
-              kv8_to_half<INT8>(__byte_perm(v[0][i], v[1][i], 0x5140), a[0], a[1]);
-              kv8_to_half<INT8>(__byte_perm(v[2][i], v[3][i], 0x5140), a[2], a[3]);
-              kv8_to_half<INT8>(__byte_perm(v[0][i], v[1][i], 0x7362), c[0], c[1]);
-              kv8_to_half<INT8>(__byte_perm(v[2][i], v[3][i], 0x7362), c[2], c[3]);
-#pragma unroll
-              for (int b = 0; b < NB; ++b) {
-                mma_f16(o[b][sub * 8 + 2 * i], a[0], a[1], a[2], a[3], pb[b][0], pb[b][1]);
-                mma_f16(o[b][sub * 8 + 2 * i + 1], c[0], c[1], c[2], c[3], pb[b][0], pb[b][1]);
-              }
-            }
-          }
+          const uint32_t at = stages_at + stage * Z::kStageBytes, ex = exps_at + stage * 2 * kTile;
+          if (key0 >= w.span.first && key0 + 16 <= w.span.len) block(std::true_type(), at, ex, key0);
+          else block(std::false_type(), at, ex, key0);
         }
         __syncwarp();
         if (lane == 0) zb_mbar_arrive(&empty_bar[stage]);
@@ -372,7 +437,7 @@ __global__ void __launch_bounds__(160, Kv8Sizes<HD, NB>::kPerSm) zb_kv8_decode_k
       }
 
       // the four warps' sums of this segment
-      const float power_of = __uint_as_float(power << 23);
+      const float power_of = __uint_as_float((power - kLift) << 23);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -401,15 +466,14 @@ __global__ void __launch_bounds__(160, Kv8Sizes<HD, NB>::kPerSm) zb_kv8_decode_k
       const int slot = 2 * static_cast<int>(blockIdx.x) + (first_segment ? 0 : 1);
       for (int i = threadIdx.x; i < rows * (HD / 2); i += 128) {
         const int r = i / (HD / 2), col = 2 * (i - r * (HD / 2));
-        float top = -INFINITY;
+        float top = kNoScore;
 #pragma unroll
         for (int k = 0; k < 4; ++k) top = fmaxf(top, stats[(k * kRows + r) * 3]);
-        const float use = top == -INFINITY ? 0.f : top;
         float ax = 0.f, ay = 0.f, sum = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float* st = stats + (k * kRows + r) * 3;
-          const float f = exp2f(st[0] - use), fo = f * st[2];
+          const float f = zb_ex2(st[0] - top), fo = f * st[2];
           const float2 x = *reinterpret_cast<const float2*>(sums + (k * kRows + r) * Z::kPitch + col);
           ax += fo * x.x;
           ay += fo * x.y;
@@ -439,10 +503,10 @@ __global__ void __launch_bounds__(160, Kv8Sizes<HD, NB>::kPerSm) zb_kv8_decode_k
 }
 
 // Joins the pairs that several CTAs have a part of.  CTA c looks at the pair at the beginning of part c + 1; the first one to meet a pair there
-// joins it, a row of queries for eight or 16 of its 32 warps at a time.
+// joins it, a row of queries in each warp, or in each of two where rows are eight.
 template <int HD, int NB>
-__global__ void __launch_bounds__(1024) zb_kv8_join_kernel(const Kv8DecodeParams p) {
-  constexpr int kRows = 8 * NB, kGroups = 32 / kRows, kCols = HD / 32;
+__global__ void __launch_bounds__(512) zb_kv8_join_kernel(const Kv8DecodeParams p) {
+  constexpr int kRows = 8 * NB, kGroups = 16 / kRows, kCols = HD / 32;
   __shared__ float weight[kRows][kMaxCtas];
   __shared__ float sums[kRows];
   __shared__ float parts[kGroups][kRows][HD];
@@ -452,37 +516,30 @@ __global__ void __launch_bounds__(1024) zb_kv8_join_kernel(const Kv8DecodeParams
   const int pairs = p.hkv * p.blocks;
   const auto count = [&](int s) { return kv8_span(p, s).tiles * pairs; };
   const int total = kv8_total(p.batch, count);
-  const int c = static_cast<int>(blockIdx.x), at = kv8_part(total, c + 1, p.ctas), start = kv8_part(total, c, p.ctas);
+  const Kv8Parts list(total, p.ctas);
+  const int c = static_cast<int>(blockIdx.x), at = list.begin(c + 1), start = list.begin(c);
   if (at >= total || at == start) return;
   int seq, before;
   kv8_locate(p.batch, at, count, seq, before);
-  const int tiles = kv8_span(p, seq).tiles, pair = (at - before) / tiles, pair0 = before + pair * tiles, pair1 = pair0 + tiles;
+  const int tiles = kv8_span(p, seq).tiles, pair = (at - before) / tiles, pair0 = before + pair * tiles;
   if (at == pair0 || start > pair0) return;           // nothing is cut here, or the pair has been met before
-  const int end = static_cast<int>((static_cast<long long>(pair1) * p.ctas - 1) / total);      // the last part that begins in front of pair1
-  const int n = end - c + 1;
+  const int n = list.of(pair0 + tiles - 1) - c + 1;   // parts c .. c + n - 1, none of them empty
   const int kvh = pair / p.blocks, row0 = (pair - kvh * p.blocks) * kRows, rows = min(kRows, p.group - row0);
-  const auto slot_of = [&](int i) {                   // -1: an empty part
-    const int x = kv8_part(total, c + i, p.ctas);
-    return x == kv8_part(total, c + i + 1, p.ctas) ? -1 : 2 * (c + i) + (x >= pair0 ? 0 : 1);
-  };
+  // the pair is the last segment of part c, unless that begins with it, and the first one of the others
+  const int slot0 = 2 * c + (start >= pair0 ? 0 : 1);
+  const auto slot_of = [&](int i) { return i == 0 ? slot0 : 2 * (c + i); };
   if (part == 0 && row < rows) {
-    float top = -INFINITY;
+    float top = kNoScore, sum = 0.f;
     for (int i = lane; i < n; i += 32) {
-      const int s = slot_of(i);
-      const float m = s < 0 ? -INFINITY : p.part_ml[static_cast<size_t>(s) * kRows + row].x;
-      weight[row][i] = m;
-      top = fmaxf(top, m);
+      const float2 ml = p.part_ml[static_cast<size_t>(slot_of(i)) * kRows + row];
+      weight[row][i] = ml.x;
+      const float up = fmaxf(top, ml.x);
+      sum = sum * zb_ex2(top - up) + ml.y * zb_ex2(ml.x - up);
+      top = up;
     }
-    top = zb_warp_max(top);
-    const float use = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    for (int i = lane; i < n; i += 32) {
-      const int s = slot_of(i);
-      const float f = exp2f(weight[row][i] - use);
-      weight[row][i] = f;
-      if (s >= 0) sum += f * p.part_ml[static_cast<size_t>(s) * kRows + row].y;
-    }
-    sum = zb_warp_sum(sum);
+    const float all = zb_warp_max(top);
+    sum = zb_warp_sum(sum * zb_ex2(top - all));
+    for (int i = lane; i < n; i += 32) weight[row][i] = zb_ex2(weight[row][i] - all);
     if (lane == 0) sums[row] = sum;
   }
   __syncthreads();
@@ -492,10 +549,8 @@ __global__ void __launch_bounds__(1024) zb_kv8_join_kernel(const Kv8DecodeParams
   if (row < rows) {
 #pragma unroll 4
     for (int i = part; i < n; i += kGroups) {
-      const int s = slot_of(i);
-      if (s < 0) continue;
       const float f = weight[row][i];
-      const float* src = p.part_o + (static_cast<size_t>(s) * kRows + row) * HD;
+      const float* src = p.part_o + (static_cast<size_t>(slot_of(i)) * kRows + row) * HD;
 #pragma unroll
       for (int j = 0; j < kCols; ++j) acc[j] += f * src[lane + 32 * j];
     }
@@ -503,7 +558,7 @@ __global__ void __launch_bounds__(1024) zb_kv8_join_kernel(const Kv8DecodeParams
 #pragma unroll
   for (int j = 0; j < kCols; ++j) parts[part][row][lane + 32 * j] = acc[j];
   __syncthreads();
-  for (int i = threadIdx.x; i < rows * HD; i += 1024) {
+  for (int i = threadIdx.x; i < rows * HD; i += 512) {
     const int r = i / HD, col = i - r * HD;
     float x = 0.f;
 #pragma unroll
@@ -526,7 +581,7 @@ int launch_decode(const Kv8DecodeParams& p, const void* k_codes, const void* v_c
   cudaError_t e = zb_launch(zb_kv8_decode_kernel<HD, NB, INT8>, dim3(p.ctas), dim3(160), Z::kSmem, stream, tk, tv, p);
   zb_count_launch(1);
   if (e == cudaSuccess && p.ctas > 1) {
-    e = zb_launch(zb_kv8_join_kernel<HD, NB>, dim3(p.ctas - 1), dim3(1024), 0, stream, p);
+    e = zb_launch(zb_kv8_join_kernel<HD, NB>, dim3(p.ctas - 1), dim3(512), 0, stream, p);
     zb_count_launch(1);
   }
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
@@ -560,55 +615,68 @@ int zb_kv8_decode_plan(int batch, int hq, int hkv, int hd, int max_len, long lon
   return ctas;
 }
 
-// q [batch, hq, hd] with q_stride elements between rows, which start on 8 bytes; out [batch, hq, hd]; codes and exponents start on 16 bytes;
-// `work`: the numbers that the plan of `ctas` CTAs asked for.
-int zb_kv8_decode(const void* q, const void* k_codes, const void* k_exps, const void* v_codes, const void* v_exps, void* out,
-                  const int32_t* block_table, const int32_t* seq_lens, int batch, int hq, int hkv, int hd, int page_size, int max_pages,
-                  int num_pages, long long q_stride, float scale, int window, int int8, float* work, int ctas, void* stream) {
-  if (batch <= 0) return 0;
+// The arguments of a call, as the caller packs them (ops/kv8.py).
+struct ZbKv8Decode {
+  const void* q;                                   // [batch, hq, hd], rows on 8 bytes
+  const void *k_codes, *k_exps, *v_codes, *v_exps;  // contiguous, on 16 bytes
+  void* out;                                       // [batch, hq, hd], contiguous
+  const int32_t* block_table;
+  const int32_t* seq_lens;
+  float* work;                                     // the numbers that the plan of `ctas` CTAs asked for
+  void* stream;
+  long long q_stride;
+  int batch, hq, hkv, hd, page_size, max_pages, num_pages, window, int8, ctas;
+  float scale;
+};
+
+int zb_kv8_decode(const ZbKv8Decode* c) {
+  const int hq = c->hq, hkv = c->hkv, hd = c->hd, page_size = c->page_size;
+  if (c->batch <= 0) return 0;
   if (hkv <= 0 || hq <= 0 || hq % hkv != 0 || (hd != 64 && hd != 128 && hd != 256)) return -30;
-  if (page_size <= 0 || page_size % 16 != 0 || num_pages <= 0 || static_cast<long long>(num_pages) * hkv * page_size > 0x7fffffffll ||
-      static_cast<long long>(max_pages) * page_size > 0x7fffff00ll)
+  if (page_size <= 0 || page_size % 16 != 0 || c->num_pages <= 0 || static_cast<long long>(c->num_pages) * hkv * page_size > 0x7fffffffll ||
+      static_cast<long long>(c->max_pages) * page_size > 0x7fffff00ll)
     return -31;
-  if (ctas < 1 || ctas > kMaxCtas) return -33;
+  if (c->ctas < 1 || c->ctas > kMaxCtas) return -33;
   ZbDeviceState* st = zb_device_state();
   if (!st) return -20;
   const int rows = rows_of(hd, hq / hkv);
   Kv8DecodeParams p = {};
-  p.q = reinterpret_cast<const __nv_bfloat16*>(q);
-  p.k_exps = reinterpret_cast<const uint8_t*>(k_exps);
-  p.v_exps = reinterpret_cast<const uint8_t*>(v_exps);
-  p.out = reinterpret_cast<__nv_bfloat16*>(out);
-  p.block_table = block_table;
-  p.seq_lens = seq_lens;
-  p.part_o = work;
-  p.part_ml = reinterpret_cast<float2*>(work + 2ll * ctas * rows * hd);
-  p.q_stride = q_stride;
-  p.batch = batch;
+  p.q = reinterpret_cast<const __nv_bfloat16*>(c->q);
+  p.k_exps = reinterpret_cast<const uint8_t*>(c->k_exps);
+  p.v_exps = reinterpret_cast<const uint8_t*>(c->v_exps);
+  p.out = reinterpret_cast<__nv_bfloat16*>(c->out);
+  p.block_table = c->block_table;
+  p.seq_lens = c->seq_lens;
+  p.part_o = c->work;
+  p.part_ml = reinterpret_cast<float2*>(c->work + 2ll * c->ctas * rows * hd);
+  p.q_stride = c->q_stride;
+  p.batch = c->batch;
   p.hkv = hkv;
   p.group = hq / hkv;
   p.blocks = (p.group + rows - 1) / rows;
   p.page_size = page_size;
-  p.max_pages = max_pages;
-  p.num_pages = num_pages;
-  p.window = window;
+  p.max_pages = c->max_pages;
+  p.num_pages = c->num_pages;
+  p.window = c->window;
   p.unit = 16;
   while (p.unit < kTile && page_size % (2 * p.unit) == 0) p.unit *= 2;
-  p.ctas = ctas;
-  p.scale_log2 = scale * 1.4426950408889634f;
+  p.ctas = c->ctas;
+  p.scale_log2 = c->scale * 1.4426950408889634f;
   p.status = st->status;
-  if (static_cast<long long>(batch) * hkv * p.blocks * std::max<long long>(1, (static_cast<long long>(max_pages) * page_size + kTile - 1) / kTile) > 0x3fffffffll)
+  if (static_cast<long long>(c->batch) * hkv * p.blocks * std::max<long long>(1, (static_cast<long long>(c->max_pages) * page_size + kTile - 1) / kTile) > 0x3fffffffll)
     return -34;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(c->stream);
+  const void *k = c->k_codes, *v = c->v_codes;
+  const bool int8 = c->int8 != 0;
   if (hd == 64) {
-    if (rows == 8) return int8 ? launch_decode<64, 1, true>(p, k_codes, v_codes, s) : launch_decode<64, 1, false>(p, k_codes, v_codes, s);
-    return int8 ? launch_decode<64, 2, true>(p, k_codes, v_codes, s) : launch_decode<64, 2, false>(p, k_codes, v_codes, s);
+    if (rows == 8) return int8 ? launch_decode<64, 1, true>(p, k, v, s) : launch_decode<64, 1, false>(p, k, v, s);
+    return int8 ? launch_decode<64, 2, true>(p, k, v, s) : launch_decode<64, 2, false>(p, k, v, s);
   }
   if (hd == 128) {
-    if (rows == 8) return int8 ? launch_decode<128, 1, true>(p, k_codes, v_codes, s) : launch_decode<128, 1, false>(p, k_codes, v_codes, s);
-    return int8 ? launch_decode<128, 2, true>(p, k_codes, v_codes, s) : launch_decode<128, 2, false>(p, k_codes, v_codes, s);
+    if (rows == 8) return int8 ? launch_decode<128, 1, true>(p, k, v, s) : launch_decode<128, 1, false>(p, k, v, s);
+    return int8 ? launch_decode<128, 2, true>(p, k, v, s) : launch_decode<128, 2, false>(p, k, v, s);
   }
-  return int8 ? launch_decode<256, 1, true>(p, k_codes, v_codes, s) : launch_decode<256, 1, false>(p, k_codes, v_codes, s);
+  return int8 ? launch_decode<256, 1, true>(p, k, v, s) : launch_decode<256, 1, false>(p, k, v, s);
 }
 
 }  // extern "C"

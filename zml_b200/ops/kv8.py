@@ -14,17 +14,21 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from typing import Optional
 
 import torch
 
 from . import _lib
 
-_p, _i, _ll, _f = C.c_void_p, C.c_int, C.c_longlong, C.c_float
-_lib.register_signature("zb_kv8_write", _i, [_p] * 11 + [_ll] + [_i] * 7 + [_ll, _f, _f, _i, _i, _p])
-_lib.register_signature("zb_kv8_read", _i, [_p] * 9 + [_i] * 8 + [_p])
-_lib.register_signature("zb_kv8_decode_plan", _i, [_i] * 5 + [_p])
-_lib.register_signature("zb_kv8_decode", _i, [_p] * 8 + [_i] * 7 + [_ll, _f, _i, _i, _p, _i, _p])
+# a call's arguments travel as one packed struct: ZbKv8Write, ZbKv8Read (csrc/kv8.cu), ZbKv8Decode (csrc/kv8_attention.cu).  ctypes takes 2.6 us to
+# convert 22 arguments one by one, packing takes 0.6
+for _name in ("zb_kv8_write", "zb_kv8_read", "zb_kv8_decode"):
+    _lib.register_signature(_name, C.c_int, [C.c_void_p])
+_lib.register_signature("zb_kv8_decode_plan", C.c_int, [C.c_int] * 5 + [C.c_void_p])
+_WRITE = struct.Struct("12P 2q 9i 2f").pack
+_READ = struct.Struct("10P 8i").pack
+_DECODE = struct.Struct("10P q 10i f").pack
 
 # names that the engine and the command line take -> type of the codes
 KV_DTYPES = {"fp8": torch.float8_e4m3fn, "int8": torch.int8}
@@ -36,19 +40,24 @@ MIN_EXPONENT, NAN_EXPONENT = 27, 255                                     # the s
 class QuantKV:
     """Keys or values of one layer: `codes` [pages, kv_heads, page_size, hd] (float8_e4m3fn or int8) and the scales' `exponents` uint8 [pages,
     kv_heads, page_size].  A page of one head is contiguous."""
-    __slots__ = ("codes", "exponents")
+    __slots__ = ("_codes", "_exponents", "_shape", "_index")
 
     def __init__(self, codes: torch.Tensor, exponents: torch.Tensor):
         if codes.dtype not in _RANGE:
             raise TypeError(f"a quantised cache holds float8_e4m3fn or int8 codes, got {codes.dtype}")
         if exponents.dtype is not torch.uint8:
             raise TypeError(f"the exponents of a quantised cache are uint8, got {exponents.dtype}")
-        if codes.dim() != 4 or exponents.shape != codes.shape[:3]:
-            raise ValueError(f"codes [pages, heads, page_size, hd] with exponents [pages, heads, page_size], got {tuple(codes.shape)} and "
+        shape = codes.shape
+        if len(shape) != 4 or exponents.shape != shape[:3]:
+            raise ValueError(f"codes [pages, heads, page_size, hd] with exponents [pages, heads, page_size], got {tuple(shape)} and "
                              f"{tuple(exponents.shape)}")
-        if exponents.device != codes.device or not codes.is_contiguous() or not exponents.is_contiguous():
+        self._index = codes.get_device()
+        if exponents.get_device() != self._index or not codes.is_contiguous() or not exponents.is_contiguous():
             raise ValueError("codes and exponents are contiguous and on one device")
-        self.codes, self.exponents = codes, exponents
+        self._codes, self._exponents, self._shape = codes, exponents, shape
+
+    codes = property(lambda self: self._codes)
+    exponents = property(lambda self: self._exponents)
 
     @staticmethod
     def alloc(pages: int, kv_heads: int, page_size: int, hd: int, dtype=torch.float8_e4m3fn, device="cpu") -> "QuantKV":
@@ -126,50 +135,50 @@ def quantize(x: torch.Tensor, dtype=torch.float8_e4m3fn):
 
 
 # ------------------------------------------------------------------ checks
-def _pair(k: QuantKV, v) -> None:
-    if not isinstance(v, QuantKV) or not isinstance(k, QuantKV):
+def _pair(k, v) -> tuple[int, int, int, int]:
+    """The common shape of keys and values that the kernels take."""
+    if type(k) is not QuantKV or type(v) is not QuantKV:
         raise TypeError("keys and values are both quantised or both not")
-    if k.codes.dtype is not v.codes.dtype or k.codes.shape != v.codes.shape or k.codes.device != v.codes.device:
+    kc, vc, n = k._codes, v._codes, k._shape
+    if kc.dtype is not vc.dtype or n != v._shape or k._index != v._index:
         raise ValueError("keys and values of one type, shape and device")
-    n = k.codes.shape
-    if n[3] not in HEAD_DIMS or n[2] % 16 or n[2] == 0 or n[0] == 0:
-        raise ValueError(f"a quantised cache has heads of {HEAD_DIMS} and pages of a multiple of 16 tokens, got {n[3]} and {n[2]}")
-    if (k.codes.data_ptr() | v.codes.data_ptr() | k.exponents.data_ptr() | v.exponents.data_ptr()) % 16:
+    pages, heads, page_size, hd = n
+    if hd not in HEAD_DIMS or page_size % 16 or page_size == 0 or pages == 0 or heads == 0:
+        raise ValueError(f"a quantised cache has heads of {HEAD_DIMS} and pages of a multiple of 16 tokens, got {tuple(n)}")
+    if (kc.data_ptr() | vc.data_ptr() | k._exponents.data_ptr() | v._exponents.data_ptr()) % 16:
         raise ValueError("codes and exponents start on 16 bytes")
-    if n[0] * n[1] * n[2] >= 2 ** 31:
+    if pages * heads * page_size >= 2 ** 31:
         raise ValueError("a quantised cache of a layer has fewer than 2^31 rows")
+    return n
 
 
-def _ints(device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t.dtype is not torch.int32 or not t.is_contiguous() or t.device != device:
-            raise ValueError(f"{name}: contiguous int32 on {device}, got {t.dtype} on {t.device}")
+def _ints(index: int, name: str, t) -> None:
+    if t.dtype is not torch.int32 or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous int32 on the cache's device, got {t.dtype} on {t.device}")
 
 
-def _table(k: QuantKV, block_table, seq_lens) -> None:
-    _ints(k.codes.device, block_table=block_table, seq_lens=seq_lens)
-    if block_table.dim() != 2 or seq_lens.dim() != 1 or block_table.shape[0] != seq_lens.shape[0]:
-        raise ValueError(f"block_table [batch, pages] with seq_lens [batch], got {tuple(block_table.shape)} and {tuple(seq_lens.shape)}")
+def _table(k: QuantKV, block_table, seq_lens) -> tuple[int, int]:
+    _ints(k._index, "block_table", block_table)
+    _ints(k._index, "seq_lens", seq_lens)
+    shape = block_table.shape
+    if len(shape) != 2 or seq_lens.shape != shape[:1]:
+        raise ValueError(f"block_table [batch, pages] with seq_lens [batch], got {tuple(shape)} and {tuple(seq_lens.shape)}")
+    return shape
 
 
 def _queries(q, k: QuantKV, out) -> tuple[int, int, int]:
-    if q.dtype is not torch.bfloat16 or q.device != k.codes.device or q.dim() != 3:
-        raise TypeError(f"queries [rows, heads, hd] in bfloat16 on {k.codes.device}, got {q.dtype} {tuple(q.shape)} on {q.device}")
-    rows, hq, hd = q.shape
-    if hd != k.codes.shape[3] or hq % k.codes.shape[1] or hq == 0:
-        raise ValueError(f"{hq} query heads of {hd} do not go with {k.codes.shape[1]} key heads of {k.codes.shape[3]}")
-    if out is not None and (out.dtype is not torch.bfloat16 or out.shape != q.shape or out.device != q.device or not out.is_contiguous()):
+    shape = q.shape
+    if q.dtype is not torch.bfloat16 or q.get_device() != k._index or len(shape) != 3:
+        raise TypeError(f"queries [rows, heads, hd] in bfloat16 on {k.device}, got {q.dtype} {tuple(shape)} on {q.device}")
+    if shape[2] != k._shape[3] or shape[1] % k._shape[1] or shape[1] == 0:
+        raise ValueError(f"{shape[1]} query heads of {shape[2]} do not go with {k._shape[1]} key heads of {k._shape[3]}")
+    if out is not None and (out.dtype is not torch.bfloat16 or out.shape != shape or out.get_device() != k._index or not out.is_contiguous()):
         raise ValueError("out: contiguous bfloat16 of the queries' shape")
-    return rows, hq, hd
+    return shape
 
 
-def _on(device):
-    """The device's kernels run with it as the current one."""
-    return torch.cuda.device(device)
-
-
-def _foreign(device) -> bool:
-    return torch.cuda.current_device() != device.index
+_current = getattr(torch._C, "_cuda_getDevice", None)                     # absent in builds of torch without CUDA
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 # ------------------------------------------------------------------ writer
@@ -178,42 +187,44 @@ def rope_kvwrite(qkv, positions, slot_mapping, inv_freq, k: QuantKV, v: QuantKV,
                  norm_unit_offset: bool = False, q_out=None):
     """`ops.rope_kvwrite` on a quantised cache.  From the projection to the one rounding at the end all is 32 bits, and angles are formed in 64.
     The slots of one call differ from one another."""
-    _pair(k, v)
-    pages, heads, page_size, head = k.codes.shape
-    t, rot = qkv.shape[0], hd if rot_dim is None else rot_dim
-    dev = k.codes.device
-    if qkv.dtype is not torch.bfloat16 or qkv.device != dev or qkv.dim() != 2 or qkv.stride(1) != 1:
-        raise TypeError(f"qkv [tokens, (hq + 2 hkv) hd] in bfloat16 on {dev}, got {qkv.dtype} {tuple(qkv.shape)} on {qkv.device}")
-    if (heads, head) != (hkv, hd) or qkv.shape[1] != (hq + 2 * hkv) * hd:
-        raise ValueError(f"a projection of {qkv.shape[1]} columns and a cache of {heads} heads of {head} for {hq} + 2 x {hkv} heads of {hd}")
+    pages, heads, page_size, head = _pair(k, v)
+    t, columns = qkv.shape
+    rot, index = hd if rot_dim is None else rot_dim, k._index
+    if qkv.dtype is not torch.bfloat16 or qkv.get_device() != index or qkv.stride()[1] != 1:
+        raise TypeError(f"qkv [tokens, (hq + 2 hkv) hd] in bfloat16 on {k.device}, got {qkv.dtype} {tuple(qkv.shape)} on {qkv.device}")
+    if heads != hkv or head != hd or hq <= 0 or columns != (hq + 2 * hkv) * hd:
+        raise ValueError(f"a projection of {columns} columns and a cache of {heads} heads of {head} for {hq} + 2 x {hkv} heads of {hd}")
     if rot % 2 or not 0 <= rot <= hd or layout not in (0, 1, 2):
         raise ValueError(f"rotation of {rot} of {hd} columns in layout {layout}")
-    _ints(dev, positions=positions, slot_mapping=slot_mapping)
+    _ints(index, "positions", positions)
+    _ints(index, "slot_mapping", slot_mapping)
     if positions.shape != (t,) or slot_mapping.shape != (t,):
         raise ValueError(f"{t} tokens with positions {tuple(positions.shape)} and slots {tuple(slot_mapping.shape)}")
-    if inv_freq.dtype is not torch.float32 or inv_freq.device != dev or inv_freq.numel() < rot // 2 or not inv_freq.is_contiguous():
-        raise ValueError(f"inv_freq: {rot // 2} contiguous float32 numbers on {dev}")
+    if inv_freq.dtype is not torch.float32 or inv_freq.get_device() != index or inv_freq.numel() < rot // 2 or not inv_freq.is_contiguous():
+        raise ValueError(f"inv_freq: {rot // 2} contiguous float32 numbers on {k.device}")
     for w in (q_norm_w, k_norm_w):
-        if w is not None and (w.dtype is not torch.bfloat16 or w.shape != (hd,) or w.device != dev or not w.is_contiguous()):
-            raise ValueError(f"norm weights: {hd} contiguous bfloat16 numbers on {dev}")
-    if q_out is not None and (q_out.dtype is not torch.bfloat16 or q_out.shape != (t, hq, hd) or q_out.device != dev or not q_out.is_contiguous()):
-        raise ValueError(f"q_out: contiguous bfloat16 [{t}, {hq}, {hd}] on {dev}")
-    if not qkv.is_cuda:
+        if w is not None and (w.dtype is not torch.bfloat16 or w.shape != (hd,) or w.get_device() != index or not w.is_contiguous()):
+            raise ValueError(f"norm weights: {hd} contiguous bfloat16 numbers on {k.device}")
+    if q_out is not None and (q_out.dtype is not torch.bfloat16 or q_out.shape != (t, hq, hd) or q_out.get_device() != index or not q_out.is_contiguous()):
+        raise ValueError(f"q_out: contiguous bfloat16 [{t}, {hq}, {hd}] on {k.device}")
+    if index < 0:
         q = _rope_kvwrite_cpu(qkv, positions, slot_mapping, inv_freq, k, v, hq, hkv, hd, layout, rot, attn_factor, q_norm_w, k_norm_w, norm_eps,
                               norm_unit_offset)
         return q if q_out is None else q_out.copy_(q)
-    if _foreign(dev):
-        with _on(dev):
+    if _current() != index:
+        with torch.cuda.device(index):
             return rope_kvwrite(qkv, positions, slot_mapping, inv_freq, k, v, hq, hkv, hd, layout, rot, attn_factor, q_norm_w, k_norm_w, norm_eps,
                                 norm_unit_offset, q_out)
     if q_out is None:
-        q_out = torch.empty((t, hq, hd), dtype=torch.bfloat16, device=dev)
-    rc = _lib.lib().zb_kv8_write(
-        qkv.data_ptr(), q_out.data_ptr(), k.codes.data_ptr(), k.exponents.data_ptr(), v.codes.data_ptr(), v.exponents.data_ptr(), positions.data_ptr(),
-        slot_mapping.data_ptr(), inv_freq.data_ptr(), None if q_norm_w is None else q_norm_w.data_ptr(), None if k_norm_w is None else k_norm_w.data_ptr(),
-        qkv.stride(0), t, hq, hkv, hd, rot, layout, page_size, pages * page_size, attn_factor, norm_eps, norm_unit_offset,
-        k.codes.dtype is torch.int8, _lib.stream_ptr())
-    _lib.check(rc, "zb_kv8_write")
+        q_out = qkv.new_empty((t, hq, hd))
+    kc = k._codes
+    rc = _lib.lib().zb_kv8_write(_WRITE(
+        qkv.data_ptr(), q_out.data_ptr(), kc.data_ptr(), k._exponents.data_ptr(), v._codes.data_ptr(), v._exponents.data_ptr(), positions.data_ptr(),
+        slot_mapping.data_ptr(), inv_freq.data_ptr(), 0 if q_norm_w is None else q_norm_w.data_ptr(), 0 if k_norm_w is None else k_norm_w.data_ptr(),
+        _stream(index), qkv.stride()[0], pages * page_size, t, hq, hkv, hd, rot, layout, page_size, bool(norm_unit_offset),
+        kc.dtype is torch.int8, attn_factor, norm_eps))
+    if rc:
+        _lib.check(rc, "zb_kv8_write")
     return q_out
 
 
@@ -252,26 +263,26 @@ def paged_read(k: QuantKV, v: QuantKV, block_table, seq_lens, num_pages: Optiona
     after sequence, and the block table int32 [batch, pages] that finds them there (zeros behind a sequence's pages).  Rows behind a sequence's
     end in its last page are zero.  `num_pages`: pages that the sequences hold together, where the caller knows it (else room for as many as
     the block table has; those behind the last sequence are not written).  Fewer than they hold are read as far as they go, and reported (`raise_on_status`)."""
-    _pair(k, v)
-    _table(k, block_table, seq_lens)
-    pages, heads, page_size, hd = k.codes.shape
-    b, width = block_table.shape
-    dev = k.codes.device
+    pages, heads, page_size, hd = _pair(k, v)
+    b, width = _table(k, block_table, seq_lens)
+    index = k._index
     n = b * width if num_pages is None else int(num_pages)
     if n < 0:
         raise ValueError(f"{n} pages")
-    if dev.type != "cuda":
+    if index < 0:
         return _paged_read_cpu(k, v, block_table, seq_lens, n)
-    if _foreign(dev):
-        with _on(dev):
+    if _current() != index:
+        with torch.cuda.device(index):
             return paged_read(k, v, block_table, seq_lens, num_pages)
-    out = torch.empty((2, n, page_size, heads, hd), dtype=torch.bfloat16, device=dev)
-    table = torch.empty((b, width), dtype=torch.int32, device=dev)
-    kd, vd = out.unbind(0)
-    rc = _lib.lib().zb_kv8_read(k.codes.data_ptr(), k.exponents.data_ptr(), v.codes.data_ptr(), v.exponents.data_ptr(), kd.data_ptr(), vd.data_ptr(),
-                                block_table.data_ptr(), seq_lens.data_ptr(), table.data_ptr(), b, heads, hd, page_size, width, pages, n,
-                                k.codes.dtype is torch.int8, _lib.stream_ptr())
-    _lib.check(rc, "zb_kv8_read")
+    kd = block_table.new_empty((n, page_size, heads, hd), dtype=torch.bfloat16)
+    vd = torch.empty_like(kd)
+    table = torch.empty_like(block_table)
+    kc = k._codes
+    rc = _lib.lib().zb_kv8_read(_READ(
+        kc.data_ptr(), k._exponents.data_ptr(), v._codes.data_ptr(), v._exponents.data_ptr(), kd.data_ptr(), vd.data_ptr(), block_table.data_ptr(),
+        seq_lens.data_ptr(), table.data_ptr(), _stream(index), b, heads, hd, page_size, width, pages, n, kc.dtype is torch.int8))
+    if rc:
+        _lib.check(rc, "zb_kv8_read")
     return kd, vd, table
 
 
@@ -300,9 +311,9 @@ def _paged_read_cpu(k, v, block_table, seq_lens, n):
 _PLANS: dict = {}
 
 
-def _plan(device, b, hq, hkv, hd, max_len) -> tuple[int, int]:
+def _plan(index, b, hq, hkv, hd, max_len) -> tuple[int, int]:
     """(CTAs, numbers of the workspace) of a decode call: a function of its sizes."""
-    key = (device.index, b, hq, hkv, hd, -(-max_len // 64))
+    key = (index, b, hq, hkv, hd, -(-max_len // 64))
     got = _PLANS.get(key)
     if got is None:
         n = C.c_longlong()
@@ -319,33 +330,35 @@ def paged_decode(q, k: QuantKV, v: QuantKV, block_table, seq_lens, scale: Option
                  max_seq_len: Optional[int] = None, out=None):
     """`ops.paged_decode` on a quantised cache.  The keys are split over the GPU on the device, from the lengths there (`max_seq_len` bounds
     the launch only); any number of query heads for a key head."""
-    _pair(k, v)
-    _table(k, block_table, seq_lens)
+    pages, hkv, page_size, _ = _pair(k, v)
+    sequences, width = _table(k, block_table, seq_lens)
     b, hq, hd = _queries(q, k, out)
-    pages, hkv, page_size, _ = k.codes.shape
-    width = block_table.shape[1]
-    if block_table.shape[0] != b:
-        raise ValueError(f"{b} queries for {block_table.shape[0]} sequences")
-    if not q.is_cuda:
+    index = k._index
+    if sequences != b:
+        raise ValueError(f"{b} queries for {sequences} sequences")
+    if index < 0:
         from . import reference
         a = reference.paged_decode(q.float(), k.dequantize(), v.dequantize(), block_table, seq_lens.clamp(0, width * page_size), scale, window).to(q.dtype)
         return a if out is None else out.copy_(a)
-    dev = k.codes.device
-    if _foreign(dev):
-        with _on(dev):
+    if _current() != index:
+        with torch.cuda.device(index):
             return paged_decode(q, k, v, block_table, seq_lens, scale, window, max_seq_len, out)
-    if q.stride(2) != 1 or q.stride(1) != hd or (b > 1 and q.stride(0) % 4) or q.data_ptr() % 8:
-        q = q.contiguous() if not q.is_contiguous() else q.clone()           # the kernel reads 8 bytes of a row at a time
+    s0, s1, s2 = q.stride()
+    if s2 != 1 or s1 != hd or s0 % 4 or q.data_ptr() % 8:
+        q = q.clone(memory_format=torch.contiguous_format)                   # the kernel reads 8 bytes of a row at a time
+        s0 = hq * hd
     if out is None:
-        out = torch.empty((b, hq, hd), dtype=torch.bfloat16, device=dev)
+        out = q.new_empty((b, hq, hd))
     most = width * page_size
-    ctas, numbers = _plan(dev, b, hq, hkv, hd, most if max_seq_len is None else min(max_seq_len, most))
-    work = torch.empty(numbers, dtype=torch.float32, device=dev)
-    rc = _lib.lib().zb_kv8_decode(
-        q.data_ptr(), k.codes.data_ptr(), k.exponents.data_ptr(), v.codes.data_ptr(), v.exponents.data_ptr(), out.data_ptr(), block_table.data_ptr(),
-        seq_lens.data_ptr(), b, hq, hkv, hd, page_size, width, pages, q.stride(0), 1.0 / math.sqrt(hd) if scale is None else scale, window,
-        k.codes.dtype is torch.int8, work.data_ptr(), ctas, _lib.stream_ptr())
-    _lib.check(rc, "zb_kv8_decode")
+    ctas, numbers = _plan(index, b, hq, hkv, hd, most if max_seq_len is None else min(max_seq_len, most))
+    work = q.new_empty((numbers,), dtype=torch.float32)
+    kc = k._codes
+    rc = _lib.lib().zb_kv8_decode(_DECODE(
+        q.data_ptr(), kc.data_ptr(), k._exponents.data_ptr(), v._codes.data_ptr(), v._exponents.data_ptr(), out.data_ptr(), block_table.data_ptr(),
+        seq_lens.data_ptr(), work.data_ptr(), _stream(index), s0, b, hq, hkv, hd, page_size, width, pages, window, kc.dtype is torch.int8, ctas,
+        1.0 / math.sqrt(hd) if scale is None else scale))
+    if rc:
+        _lib.check(rc, "zb_kv8_decode")
     return out
 
 
@@ -354,18 +367,18 @@ def paged_prefill(q, k: QuantKV, v: QuantKV, block_table, seq_lens, q_start, sca
     """`ops.paged_prefill` on a quantised cache: the sequences are read back to bf16 (`paged_read`; `kv_pages` is its `num_pages`), and the bf16
     kernels attend to that.  Prompts are bound by their products: reading back moves 6 bytes a key, head and column once, where every query of
     the group makes 4 operations of them; the workspace lives as long as the call."""
-    _pair(k, v)
-    _table(k, block_table, seq_lens)
+    page_size = _pair(k, v)[2]
+    b, width = _table(k, block_table, seq_lens)
     _queries(q, k, out)
-    _ints(k.codes.device, q_start=q_start)
+    _ints(k._index, "q_start", q_start)
+    if q_start.shape != (b + 1,):
+        raise ValueError(f"q_start has one number more than the {b} sequences, got {tuple(q_start.shape)}")
     from . import paged_prefill as bf16_prefill
-    dev = k.codes.device
-    if dev.type == "cuda" and _foreign(dev):
-        with _on(dev):
+    if k._index >= 0 and _current() != k._index:
+        with torch.cuda.device(k._index):
             return paged_prefill(q, k, v, block_table, seq_lens, q_start, scale, window, out, total_q_blocks, impl, max_seq_len, kv_pages)
-    b, width = block_table.shape
     if kv_pages is None and max_seq_len is not None:
-        kv_pages = b * min(width, -(-max_seq_len // k.page_size))
+        kv_pages = b * min(width, -(-max_seq_len // page_size))
     kd, vd, table = paged_read(k, v, block_table, seq_lens, kv_pages)
     a = bf16_prefill(q, kd, vd, table, seq_lens, q_start, scale, window, out=out, total_q_blocks=total_q_blocks, impl=impl, max_seq_len=max_seq_len)
     return a if out is None or a is out else out.copy_(a)
