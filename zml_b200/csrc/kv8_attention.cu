@@ -5,63 +5,89 @@
 // for a key's codes ck, cv and scales s_k, s_v: the scales multiply scores and probabilities, so codes go to the tensor core as they are
 // (e4m3 and int8 are subsets of f16) and a key costs its 2 (HD + 1) bytes and nothing else.
 //
-// * The products are S^T = K Q^T and O^T = V^T P^T (mma.sync m16n8k16, f16 inputs, fp32 sums): 16 keys, then 16 columns, are the rows, and
-//   eight query heads of one key head the columns.  Groups of up to eight heads, which is nearly all there are, fill the columns instead of
-//   half of 16 rows, and the accumulators of a head of 128 are 32 registers.  P^T reaches its operand layout by two transposes of 8 x 8.
-// * The contraction may take the columns of a head in any order and the output columns may lie anywhere, so every thread reads its operands as whole
-//   16-byte pieces of a row.  Rows are 128 bytes in shared memory (half a row of a head of 256, two rows of a head of 64) in the 128-byte swizzle of
-//   the tensor-map copy: the pieces that eight neighbouring lanes read lie in different banks.
-// * f16 holds neither every bf16 query nor every product p_j s_vj.  A query row is scaled by a power of two to a largest magnitude in
-//   [2^13, 2^14), exactly, and that power is taken out of its scores; s_vj is taken relative to the largest one so far, and the weight times
-//   2^7: what f16 drops lies 2^-32 below.
+// * The products are S^T = K Q^T and O^T = V^T P^T (mma.sync): keys, then columns, are the 16 rows and eight query heads of one key head the columns.
+//   Groups of up to eight heads, which is nearly all there are, fill the columns instead of half of 16 rows, and the accumulators of a head of
+//   128 are 32 registers.  P^T reaches its operand layout by transposes of 8 x 8.
+// * e4m3 and int8 are subsets of f16: codes are converted two at a time and multiplied by m16n8k16 with fp32 sums.  (m16n8k32 of e4m3 is made of
+//   the same conversions and products on this GPU, and more of them.)  A query row is scaled by a power of two to a largest magnitude in [2^13,
+//   2^14), exactly, and that power is taken out of its scores.  int8 has a product of its own for S^T, m16n8k32 with int32 sums, without
+//   conversions: the query is 256 times one int8 number and another (the largest of a row in [2^14, 2^15), half a unit is lost).
+// * f16 does not hold every product p_j s_vj: s_vj is taken relative to the largest one so far, which rescales the accumulators like the reference
+//   of the scores does, and the weight times 2^7: what f16 drops lies 2^-32 below.
+// * The contraction may take the columns of a head in any order, the output columns may lie anywhere, and so may the keys in the rows, so every
+//   thread reads its operands as whole 16-byte pieces of a row and the exponents of its four keys as one word.  Rows are 128 bytes in shared memory
+//   (half a row of a head of 256, two rows of a head of 64) in the 128-byte swizzle of the tensor-map copy; kv8_key says which key lies in
+//   which row, so that the pieces that eight neighbouring lanes read lie in different banks, in both products.
 // * The reference that scores are taken from, and that of the values' scales, move only when a score exceeds its reference by 2^8 or a scale its own:
 //   the weights stay below 2^15, and a warp looks for that with one vote, where keeping the very maximum takes three shuffles a column
 //   and a multiplication of all accumulators nearly every time.
-// * All tiles of 64 keys of all (sequence, key head) pairs are one list, cut into equal parts, one for each CTA: whatever the mix of lengths,
-//   all SMs stream alike.  A CTA whose part ends inside a pair leaves its sums in the workspace, and a second kernel joins each such
-//   pair.  Lengths are read on the device, so a captured launch serves any of them; nothing outlives the two launches.
-// * Four warps take 16 keys of a tile each; a fifth one feeds the ring of tiles, page numbers fetched 32 at a time.
-#include <cuda.h>
-
+// * Every warp has a ring of tiles of 32 keys of its own and waits for nobody while it streams; the sums of a CTA's four warps (two, for heads of 256)
+//   meet in shared memory in the end.  (One ring for eight warps, fed by tensor-map copies: 130 clocks an SM for each of a tile's four copies, and
+//   2 us at each end of a pair in which the SM's memory stood still.  CTAs that walk over equal parts of a list of all tiles: even, but nearly every
+//   pair is cut, and a CTA that joins one or begins another stands still for 3 us.  128 x 1024 keys of 4 heads: 39 and 36 us, now 28.)
+// * A CTA takes a chunk of a (sequence, key head) pair.  The lengths on the device decide how long chunks are, so that a captured launch serves any
+//   of them: the smallest length that leaves no more chunks than the GPU holds CTAs, an even share where there are more pairs than that.  Chunks of a
+//   cut pair leave their sums in the workspace, and the last one to finish, which a ticket of the pair tells, joins them.
+//   CLUSTER, for work that would leave a warp only a tile or two: a cluster of up to 16 CTAs takes a pair, and the sums of the CTAs meet through
+//   distributed shared memory: no ticket, no workspace.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "host_api.h"
 #include "kv8.cuh"
 
-int zb_make_tmap_u8_2d_ex(CUtensorMap* out, const void* base, long long rows, long long row_bytes, int box_bytes, int box_rows, int swizzle128);
-
 namespace {
 
 constexpr uint32_t kKernelKv8Decode = 41;
-constexpr int kTile = 64;                       // keys
-constexpr int kMaxCtas = 384;                   // of the partition: what the joining kernel keeps weights for
+constexpr int kTile = 32;                       // keys
+constexpr int kMaxBatch = 8192;                 // sequences whose lengths a CTA looks at: beyond, pairs are not cut
+constexpr int kMinChunk = 8;                    // tiles: two for each warp
 constexpr float kNoScore = -3.402823466e38f;    // the reference in front of the first key
 constexpr float kSlack = 8.f;                   // in units of log2: how far a score may exceed its reference
 constexpr uint32_t kLift = 7;                   // log2 of what weights are multiplied by
 
 struct Kv8DecodeParams {
   const __nv_bfloat16* q;
+  const uint8_t* k_codes;
+  const uint8_t* v_codes;
   const uint8_t* k_exps;
   const uint8_t* v_exps;
   __nv_bfloat16* out;
   const int32_t* block_table;
   const int32_t* seq_lens;
-  float* part_o;               // [2 * ctas][rows][HD]: a CTA's first and its last pair
-  float2* part_ml;             // [2 * ctas][rows]: maximum and sum
+  float* part_o;               // [slots][rows][HD]: the sums of a cut pair's chunk
+  float2* part_ml;             // [slots][rows]: reference and sum
+  uint32_t* tickets;           // [pairs], zero between launches
   long long q_stride;
-  int batch, hkv, group, blocks;      // blocks: of `rows` query heads in a group
+  int batch, hkv, group, blocks, rows;      // blocks: of `rows` query heads (the last one of fewer) in a group
   int page_size, max_pages, num_pages, window;
-  int unit;                    // keys of one copy: the largest power of two up to 64 that divides a page
-  int ctas;
+  int parts;                   // CTAs that the GPU holds; CLUSTER: CTAs of a cluster
   float scale_log2;
   ZbStatus* status;
 };
 
 ZB_DEVICE void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The first product of a sum.
+ZB_DEVICE void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+ZB_DEVICE void mma_int8_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+}
+ZB_DEVICE void mma_int8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 ZB_DEVICE uint4 lds128(uint32_t at) {
@@ -74,11 +100,33 @@ ZB_DEVICE uint2 lds64(uint32_t at) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
   return v;
 }
-ZB_DEVICE uint32_t lds8(uint32_t at) {
+ZB_DEVICE uint32_t lds32(uint32_t at) {
   uint32_t v;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
   return v;
 }
+
+// Key (of a warp's 32) in row `g` of the idx-th group of eight rows.  Four keys of a thread are neighbours, one word of exponents; in the low bits,
+// rows g = 2 i and 2 i + 1 differ so that their pieces of S^T's operand lie in different halves of the banks, and rows g = 2 t (or 2 t + 1) over
+// t so that eight lanes of O^T's operand meet eight banks.
+template <int HD>
+ZB_DEVICE int kv8_key(int g, int idx) {
+  if constexpr (HD == 64) return 4 * ((g & 4) | ((((g >> 2) ^ g) & 1) << 1) | ((g >> 1) & 1)) + idx;
+  else return 4 * (g ^ ((g >> 1) & 1)) + (idx ^ (2 * (g >> 2)));
+}
+// What the idx-th key's offset in a swizzled tile differs from the first one's by.
+template <int HD>
+ZB_DEVICE constexpr uint32_t kv8_step(int idx) {
+  return HD == 64 ? ((idx >> 1) * 144) ^ ((idx & 1) * 64) : idx * 144;
+}
+// Offset of 16-byte piece c of key r in a tile.
+template <int HD>
+ZB_DEVICE uint32_t kv8_at(int r, int c) {
+  if constexpr (HD == 64) return (r >> 1) * 128 + (((((r & 1) << 2) + c) ^ ((r >> 1) & 7)) << 4);
+  else return r * 128 + ((c ^ (r & 7)) << 4);
+}
+// The scale (its bits) of byte i of a word of exponents.
+ZB_DEVICE uint32_t kv8_scale_of(uint32_t word, int i) { return (i < 3 ? word << (23 - 8 * i) : word >> 1) & 0x7f800000u; }
 ZB_DEVICE uint32_t transpose8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -88,7 +136,29 @@ ZB_DEVICE uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-ZB_DEVICE void consumer_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+ZB_DEVICE void copy16(uint32_t to, const void* from, bool some) {      // zeros where not
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(some ? 16u : 0u) : "memory");
+}
+ZB_DEVICE float2 load_peer2(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
+}
+ZB_DEVICE float4 load_peer4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+ZB_DEVICE void store32(float* to, const float (&x)[8]) {      // on 32 bytes
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]),
+               "f"(x[7])
+               : "memory");
+}
+ZB_DEVICE void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+ZB_DEVICE void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
 // Tiles of a sequence that its query sees, one where it sees none (the pair's output has to be written).
 struct Kv8Span {
@@ -102,168 +172,168 @@ ZB_DEVICE Kv8Span kv8_span(const Kv8DecodeParams& p, int seq) {
   s.tiles = max(1, (s.len + kTile - 1) / kTile - s.tile0);
   return s;
 }
-// The list of `total` tiles in equal parts: part c begins at begin(c), the first ones are one longer.
-struct Kv8Parts {
-  int each, longer;
-  ZB_DEVICE Kv8Parts(int total, int ctas) : each(total / ctas), longer(total - each * ctas) {}
-  ZB_DEVICE int begin(int c) const { return c * each + min(c, longer); }
-  ZB_DEVICE int of(int pos) const {                   // the part that holds a position
-    const int turn = longer * (each + 1);
-    return pos < turn ? pos / (each + 1) : longer + (pos - turn) / each;
-  }
-};
-
-// A CTA's walk over its part: segments of one pair each.  Every warp walks on its own.
-struct Kv8Walk {
+// What a CTA does: tiles [begin, end) of a pair, chunk `nth` of `chunks`.
+struct Kv8Work {
   Kv8Span span;
-  int seq, pair, begin, end;         // pair of the sequence, tiles [begin, end) of it
-  int at, last;                      // positions in the list
+  int seq, pair;                     // pair of the sequence
+  int begin, end, nth, chunks;
+  int slot;                          // of the pair's first chunk, where there are several
 };
-ZB_DEVICE void kv8_segment(Kv8Walk& w) { w.end = min(w.span.tiles, w.begin + (w.last - w.at)); }
-ZB_DEVICE bool kv8_start(const Kv8DecodeParams& p, Kv8Walk& w) {
-  const int pairs = p.hkv * p.blocks;
-  const auto count = [&](int s) { return kv8_span(p, s).tiles * pairs; };
-  const int total = kv8_total(p.batch, count);
-  const Kv8Parts parts(total, p.ctas);
-  w.at = parts.begin(blockIdx.x);
-  w.last = parts.begin(blockIdx.x + 1);
-  if (w.at >= w.last) return false;
-  int before;
-  kv8_locate(p.batch, w.at, count, w.seq, before);
-  w.span = kv8_span(p, w.seq);
-  w.pair = (w.at - before) / w.span.tiles;
-  w.begin = (w.at - before) - w.pair * w.span.tiles;
-  kv8_segment(w);
-  return true;
+ZB_DEVICE void kv8_cut(Kv8Work& w) {
+  const int each = w.span.tiles / w.chunks, longer = w.span.tiles - each * w.chunks;
+  w.begin = w.nth * each + min(w.nth, longer);
+  w.end = w.begin + each + (w.nth < longer ? 1 : 0);
 }
-ZB_DEVICE bool kv8_next(const Kv8DecodeParams& p, Kv8Walk& w) {
-  w.at += w.end - w.begin;
-  if (w.at >= w.last) return false;
-  w.begin = 0;
-  if (++w.pair == p.hkv * p.blocks) {
-    w.pair = 0;
-    w.span = kv8_span(p, ++w.seq);
+// false: there are fewer chunks.  `tiles`: shared memory for a number of each sequence.
+ZB_DEVICE bool kv8_work(const Kv8DecodeParams& p, Kv8Work& w, int* tiles) {
+  const int pairs = p.hkv * p.blocks;
+  for (int s = threadIdx.x; s < p.batch; s += blockDim.x) tiles[s] = kv8_span(p, s).tiles;
+  __syncthreads();
+  const int total = kv8_total(p.batch, [&](int s) { return tiles[s]; });
+  int length = 0, chunks = 0;
+  float each = 0.f;
+  // tiles / length, rounded up: the product of the reciprocal is off by less than one, and corrected
+  const auto chunks_of = [&](int s) {
+    int n = static_cast<int>(static_cast<float>(tiles[s]) * each);
+    n += n * length < tiles[s] ? 1 : 0;
+    n += n * length < tiles[s] ? 1 : 0;
+    return (n - 1) * length >= tiles[s] ? n - 1 : n;
+  };
+  const auto cut_by = [&](int n) {
+    length = max(kMinChunk, n);
+    each = 1.f / static_cast<float>(length);
+    chunks = kv8_total(p.batch, chunks_of) * pairs;
+  };
+  if (p.batch * pairs > p.parts) {
+    cut_by(static_cast<int>(static_cast<float>(total) * static_cast<float>(pairs) / static_cast<float>(p.parts)) + 1);
+  } else {
+    // Rounding up adds half a chunk a sequence on average, and less than a whole one: the length for the former if that fits, else for more
+    const int room = p.parts / pairs;                  // chunks of all sequences, at least one each
+    for (int more = 2 * p.batch; more <= 4 * p.batch; more += p.batch) {
+      const int left = 4 * room - more;
+      cut_by(left > 0 ? static_cast<int>(4.f * static_cast<float>(total) / static_cast<float>(left)) + 1 : total);
+      if (chunks <= p.parts) break;
+    }
   }
-  kv8_segment(w);
+  const int at = blockIdx.x;
+  if (at >= chunks) return false;
+  int before;
+  kv8_locate(p.batch, at, [&](int s) { return chunks_of(s) * pairs; }, w.seq, before);
+  w.span = kv8_span(p, w.seq);
+  w.chunks = chunks_of(w.seq);
+  w.pair = (at - before) / w.chunks;
+  w.nth = (at - before) - w.pair * w.chunks;
+  w.slot = 0;
+  if (w.chunks > 1)
+    w.slot = kv8_total(w.seq, [&](int s) {
+      const int n = chunks_of(s);
+      return n > 1 ? n * pairs : 0;
+    }) + w.pair * w.chunks;
+  kv8_cut(w);
+  __syncthreads();                                     // the rings lie over the numbers
   return true;
 }
 
 template <int HD, int NB>
 struct Kv8Sizes {
-  static constexpr int kRows = 8 * NB;                              // query heads of a pair
   static constexpr int kTileBytes = kTile * HD;
   static constexpr int kStageBytes = 2 * kTileBytes;
-  static constexpr int kStages = HD == 64 ? 9 : (HD == 128 ? (NB == 1 ? 5 : 4) : 5);
-  static constexpr int kPitch = HD + 4;                             // floats of a row of the four warps' sums
-  static constexpr int kExpBytes = kStages * 2 * kTile;
-  static constexpr int kMergeBytes = 4 * kRows * kPitch * 4 + 4 * kRows * 3 * 4;
-  static constexpr int kSmem = 1024 + kStages * kStageBytes + kExpBytes + kMergeBytes + 2 * kStages * 8 + 16;
-  static constexpr int kPerSm = kSmem <= 113 * 1024 ? 2 : 1;
+  static constexpr int kStages = HD == 64 ? 6 : 3;
+  static constexpr int kWarps = HD == 256 ? 2 : 4, kCtas = HD == 128 && NB == 2 ? 1 : 2;       // of a CTA, and CTAs on an SM
+  static constexpr int kWarpBytes = kStages * kStageBytes;
+  static constexpr int kPitch = HD + 4;                             // floats of a row of sums
+  static constexpr int kSums = (kWarps / 2) * 8 * NB * kPitch;      // half of the warps leave theirs, the others add to them
+  static constexpr int kSmem = kWarps * (kWarpBytes + kStages * 2 * kTile) + kSums * 4 + (kWarps + 1) * 8 * NB * 8 + 1024;
+  static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
-template <int HD, int NB, bool INT8>
-__global__ void __launch_bounds__(160, Kv8Sizes<HD, NB>::kPerSm) zb_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
-                                                            const Kv8DecodeParams p) {
+template <int HD, int NB, bool INT8, bool CLUSTER>
+__global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB>::kWarps, Kv8Sizes<HD, NB>::kCtas) zb_kv8_decode_kernel(const Kv8DecodeParams p) {
   using Z = Kv8Sizes<HD, NB>;
-  constexpr int kStages = Z::kStages, kRows = Z::kRows, kSteps = HD / 16, kSubs = HD > 128 ? 2 : 1;
+  constexpr int kStages = Z::kStages, kWarps = Z::kWarps, kRows = 8 * NB, kSteps = HD / 16, kSubs = HD > 128 ? 2 : 1, kPieces = HD / 64;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024u - (zb_smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t* exps = smem + kStages * Z::kStageBytes;                                // [stage][keys, values][64]
-  float* sums = reinterpret_cast<float*>(exps + kStages * 2 * kTile);             // [warp][row][kPitch]
-  float* stats = sums + 4 * kRows * Z::kPitch;                                    // [warp][row][maximum, sum, scale of the values]
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(stats + 4 * kRows * 3);
-  uint64_t* empty_bar = full_bar + kStages;
-  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(empty_bar + kStages);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      zb_mbar_init(&full_bar[s], 1);
-      zb_mbar_init(&empty_bar[s], 4);
-    }
-    *abort_flag = 0u;
-    zb_mbar_fence_init();
-    zb_tma_prefetch_desc(&tmap_k);
-    zb_tma_prefetch_desc(&tmap_v);
-  }
-  __syncthreads();
   zb_pdl_launch();
   zb_pdl_wait();
-  Kv8Walk w;
-  if (!kv8_start(p, w)) return;
-  uint32_t stage = 0, phase = 0;
-  bool dead = false;                                 // a wait ran out: the walk goes on without waiting, so that all meet at the barriers
+  uint8_t* const smem = smem_raw + ((1024u - (zb_smem_u32(smem_raw) & 1023u)) & 1023u);
+  Kv8Work w;
+  if constexpr (CLUSTER) {
+    const int index = blockIdx.x / p.parts, pairs = p.hkv * p.blocks;
+    w.seq = index / pairs;
+    w.pair = index - w.seq * pairs;
+    w.span = kv8_span(p, w.seq);
+    w.nth = blockIdx.x - index * p.parts;
+    w.chunks = p.parts;
+    w.slot = 0;
+    kv8_cut(w);
+  } else {
+    if (!kv8_work(p, w, reinterpret_cast<int*>(smem))) return;
+  }
+  const uint32_t smem_at = zb_smem_u32(smem), stages_at = smem_at + warp * Z::kWarpBytes;
+  const uint32_t exps_at = smem_at + kWarps * Z::kWarpBytes + warp * kStages * 2 * kTile;
+  float* const sums = reinterpret_cast<float*>(smem + kWarps * (Z::kWarpBytes + kStages * 2 * kTile));      // [half of the warps][row][kPitch]
+  float* const stats = sums + Z::kSums;                                                                     // [warp, all][row][reference, sum]
 
-  if (warp == 4) {
-    const int per_tile = kTile / p.unit;
-    do {
-      const int kvh = w.pair / p.blocks;
-      const int32_t* bt = p.block_table + static_cast<size_t>(w.seq) * p.max_pages;
-      int pages = 0;                                 // of the 32 copies from a multiple of 32 on, one a lane
-      int off = (w.span.tile0 + w.begin) * kTile % p.page_size;
-      for (int t = w.begin; t < w.end; ++t) {
-        if (((t - w.begin) * per_tile & 31) == 0) {
-          const int key = (w.span.tile0 + t) * kTile + lane * p.unit;
-          pages = key < w.span.len ? bt[key / p.page_size] : 0;
-          if (static_cast<uint32_t>(pages) >= static_cast<uint32_t>(p.num_pages)) {
-            if ((w.span.tile0 + w.end) * kTile > key) zb_record_error(p.status, ZB_ERR_BOUNDS, kKernelKv8Decode, 1u, static_cast<uint32_t>(pages));
-            pages = 0;
-          }
+  // copies run kStages - 1 tiles ahead
+  const int kvh = w.pair / p.blocks, row0 = (w.pair - kvh * p.blocks) * kRows, rows = min(kRows, p.group - row0);
+  const int32_t* const bt = p.block_table + static_cast<size_t>(w.seq) * p.max_pages;
+  int f_tile = w.begin + warp, f_nth = 0, f_stage = 0, f_pages = 0;
+  const int line = lane >> 3, in_line = lane & 7;      // a lane copies 16 bytes of each of four lines of 128 bytes
+  const uint32_t copy_to = HD == 256 ? (line & 1) * kTile * 128 + (line >> 1) * 128 + ((in_line ^ (line >> 1)) << 4) : line * 128 + ((in_line ^ line) << 4);
+  const auto fetch = [&]() {
+    if (f_tile < w.end) {
+      const int nth = f_nth & 15;
+      if (nth == 0) {                                  // pages of the next 16 tiles, 16 keys a lane
+        const int tile = f_tile + (lane >> 1) * kWarps, key = (w.span.tile0 + tile) * kTile + (lane & 1) * 16;
+        const bool some = tile < w.end && key < w.span.len && key + 16 > w.span.first;
+        f_pages = some ? bt[key / p.page_size] : 0;
+        if (static_cast<uint32_t>(f_pages) >= static_cast<uint32_t>(p.num_pages)) {
+          zb_record_error(p.status, ZB_ERR_BOUNDS, kKernelKv8Decode, 1u, static_cast<uint32_t>(f_pages));
+          f_pages = 0;
         }
-        if (!dead) dead = !zb_mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag);
-        dead = __any_sync(0xffffffffu, dead);
-        const int key0 = (w.span.tile0 + t) * kTile;
-        const int copies = min(per_tile, (max(w.span.len - key0, 0) + p.unit - 1) / p.unit);
-        if (!dead && lane == 0) zb_mbar_expect_tx(&full_bar[stage], copies * p.unit * 2 * (HD + 1));
-        uint8_t* ks = smem + stage * Z::kStageBytes;
-        uint8_t* ex = exps + stage * 2 * kTile;
-        for (int c = 0; c < copies; ++c) {
-          const int page = __shfl_sync(0xffffffffu, pages, ((t - w.begin) * per_tile + c) & 31);
-          const long long row = (static_cast<long long>(page) * p.hkv + kvh) * p.page_size + off;
-          off += p.unit;
-          if (off == p.page_size) off = 0;
-          if (dead || lane != 0) continue;
-          const int y = static_cast<int>(HD == 64 ? row >> 1 : row);
-          uint8_t* to = ks + c * p.unit * (HD > 128 ? 128 : HD);
+        // from here on: the row of the group's first key, in units of 16 rows
+        f_pages = ((f_pages * p.hkv + kvh) * p.page_size + key % p.page_size) >> 4;
+        if (!some) f_pages = -1;
+      }
+      const int unit0 = __shfl_sync(0xffffffffu, f_pages, 2 * nth), unit1 = __shfl_sync(0xffffffffu, f_pages, 2 * nth + 1);
+      const uint32_t to = stages_at + f_stage * Z::kStageBytes;
+      constexpr int kCopies = kTile * HD / 512;
 #pragma unroll
-          for (int sub = 0; sub < kSubs; ++sub) {
-            zb_tma_load_2d(to + sub * kTile * 128, &tmap_k, &full_bar[stage], sub * 128, y);
-            zb_tma_load_2d(to + Z::kTileBytes + sub * kTile * 128, &tmap_v, &full_bar[stage], sub * 128, y);
-          }
-          zb_bulk_load(ex + c * p.unit, p.k_exps + row, p.unit, &full_bar[stage]);
-          zb_bulk_load(ex + kTile + c * p.unit, p.v_exps + row, p.unit, &full_bar[stage]);
-        }
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1u;
+      for (int half = 0; half < 2; ++half) {
+        const int unit = half ? unit1 : unit0;
+        const size_t from = static_cast<size_t>(max(unit, 0)) * (16 * HD) + lane * 16;
+#pragma unroll
+        for (int i = 0; i < kCopies / 2; ++i) {
+          const int n = half * (kCopies / 2) + i;
+          const uint32_t at = HD == 256 ? n * 256 + (copy_to ^ (((2 * n) & 7) << 4)) : n * 512 + (copy_to ^ ((n & 1) << 6));
+          copy16(to + at, p.k_codes + from + i * 512, unit >= 0);
+          copy16(to + Z::kTileBytes + at, p.v_codes + from + i * 512, unit >= 0);
         }
       }
-    } while (kv8_next(p, w));
-  } else {
-    const int g = lane >> 2, t4 = lane & 3;
-    // what this thread reads of a stage: keys g and g + 8 of the warp's 16 in S^T = K Q^T, values 2 t4, 2 t4 + 1 (and 8 further) in O^T = V^T P^T
-    uint32_t k_off[2], v_off[4];
-    if constexpr (HD == 64) {
-      const int r = warp * 16 + g;
-      k_off[0] = (r >> 1) * 128 + (((((r & 1) << 2) + t4) ^ ((r >> 1) & 7)) << 4);
-      k_off[1] = (k_off[0] ^ 64u) + 512u;
-      v_off[0] = Z::kTileBytes + (warp * 8 + t4) * 128 + (((g >> 1) ^ t4) << 4) + (g & 1) * 8;
-      v_off[1] = v_off[0] ^ 64u;
-      v_off[2] = v_off[1] + 512u;
-      v_off[3] = v_off[0] + 512u;
-    } else {
-      const int r = warp * 16 + g, q = warp * 16 + 2 * t4;
-      k_off[0] = r * 128 + (((2 * t4) ^ (r & 7)) << 4);
-      k_off[1] = k_off[0] + 1024u;
-      v_off[0] = Z::kTileBytes + q * 128 + ((g ^ (q & 7)) << 4);
-      v_off[1] = Z::kTileBytes + (q + 1) * 128 + ((g ^ ((q + 1) & 7)) << 4);
-      v_off[2] = v_off[0] + 1024u;
-      v_off[3] = v_off[1] + 1024u;
+      if (lane < 4) {                                  // exponents: keys, values of the first 16, of the others
+        const int unit = (lane >> 1) ? unit1 : unit0;
+        copy16(exps_at + f_stage * 2 * kTile + (lane & 1) * kTile + (lane >> 1) * 16, ((lane & 1) ? p.v_exps : p.k_exps) + static_cast<size_t>(max(unit, 0)) * 16, unit >= 0);
+      }
+      if (++f_stage == kStages) f_stage = 0;
+      ++f_nth;
+      f_tile += kWarps;
     }
-    const uint32_t stages_at = zb_smem_u32(smem), exps_at = zb_smem_u32(exps) + warp * 16 + g;
-    bool first_segment = true;
-    do {
-      const int kvh = w.pair / p.blocks, row0 = (w.pair - kvh * p.blocks) * kRows, rows = min(kRows, p.group - row0);
-      // queries, scaled to f16, and what a score has to be multiplied by (columns 2 t4, 2 t4 + 1 of each block of eight)
+    copies_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch();
+
+  const int g = lane >> 2, t4 = lane & 3;
+  // what this thread reads of a stage: keys of row g in S^T = K Q^T, of rows 2 t4 and 2 t4 + 1 in O^T = V^T P^T, and the exponents of the former
+  const uint32_t ex_off = kv8_key<HD>(g, 0) & ~3;
+  const uint32_t k_off = kv8_at<HD>(kv8_key<HD>(g, 0), t4);
+  const uint32_t v_off0 = Z::kTileBytes + kv8_at<HD>(kv8_key<HD>(2 * t4, 0), HD == 64 ? g >> 1 : g) + (HD == 64 ? (g & 1) * 8 : 0);
+  const uint32_t v_off1 = Z::kTileBytes + kv8_at<HD>(kv8_key<HD>(2 * t4 + 1, 0), HD == 64 ? g >> 1 : g) + (HD == 64 ? (g & 1) * 8 : 0);
+  const uint32_t turn = HD != 64 && g >= 4 ? 0x1032 : 0x3210;      // kv8_key's order of the four
+  int stage = 0;
+  {
+      // queries (e4m3: f16, two registers for 16 columns; int8: both parts of 32 columns), and what a score has to be multiplied by (columns 2 t4,
+      // 2 t4 + 1 of each block of eight)
       uint32_t qf[NB][kSteps][2];
       float factor[NB][2];
 #pragma unroll
@@ -273,23 +343,35 @@ __global__ void __launch_bounds__(160, Kv8Sizes<HD, NB>::kPerSm) zb_kv8_decode_k
         uint2 raw[kSteps];
         uint32_t top = 0u;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          // 16-byte piece of the row that step s belongs to, and its four columns in there
-          const int piece = HD == 64 ? t4 : (s >> 3) * 8 + 2 * t4 + ((s >> 2) & 1);
-          raw[s] = *reinterpret_cast<const uint2*>(src + piece * 16 + (s & 3) * 4);
-          if (r >= rows) raw[s] = make_uint2(0u, 0u);
-          const uint32_t x = raw[s].x & 0x7fff7fffu, y = raw[s].y & 0x7fff7fffu;
+        for (int i = 0; i < kSteps; ++i) {
+          raw[i] = *reinterpret_cast<const uint2*>(src + (t4 + 4 * (i >> 2)) * 16 + (i & 3) * 4);
+          if (r >= rows) raw[i] = make_uint2(0u, 0u);
+          const uint32_t x = raw[i].x & 0x7fff7fffu, y = raw[i].y & 0x7fff7fffu;
           top = max(max(top, max(x >> 16, x & 0xffffu)), max(y >> 16, y & 0xffffu));
         }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = min(max(267 - static_cast<int>(top >> 7), 1), 253);             // exponent of 2^13 / 2^floor(log2 top)
-        const float up = __uint_as_float(static_cast<uint32_t>(e) << 23), down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+        const int e = min(max((INT8 ? 268 : 267) - static_cast<int>(top >> 7), 1), 253);      // exponent of 2^14 or 2^13 over 2^floor(log2 top)
+        const float up = __uint_as_float(static_cast<uint32_t>(e) << 23);
+        const float down = __uint_as_float(top >= 0x7f80u ? 0x7fffffffu : static_cast<uint32_t>(254 - e) << 23);      // no numbers, no scores
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          const float2 x = zb_unpack_bf16x2(raw[s].x), y = zb_unpack_bf16x2(raw[s].y);
-          qf[b][s][0] = pack_half2(x.x * up, x.y * up);
-          qf[b][s][1] = pack_half2(y.x * up, y.y * up);
+        for (int i = 0; i < kSteps; ++i) {
+          const float2 x = zb_unpack_bf16x2(raw[i].x), y = zb_unpack_bf16x2(raw[i].y);
+          if constexpr (INT8) {
+            const float f[4] = {x.x * up, x.y * up, y.x * up, y.y * up};
+            uint32_t hi = 0u, lo = 0u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int n = min(max(__float2int_rn(f[j]), -32639), 32639), h = (n + 128) >> 8;
+              hi |= (static_cast<uint32_t>(h) & 255u) << (8 * j);
+              lo |= (static_cast<uint32_t>(n) & 255u) << (8 * j);
+            }
+            qf[b][i & ~1][i & 1] = hi;
+            qf[b][i | 1][i & 1] = lo;
+          } else {
+            qf[b][i][0] = pack_half2(x.x * up, x.y * up);
+            qf[b][i][1] = pack_half2(y.x * up, y.y * up);
+          }
         }
         factor[b][0] = __shfl_sync(0xffffffffu, down, 8 * t4) * p.scale_log2;
         factor[b][1] = __shfl_sync(0xffffffffu, down, 8 * t4 + 4) * p.scale_log2;
@@ -302,79 +384,158 @@ __global__ void __launch_bounds__(160, Kv8Sizes<HD, NB>::kPerSm) zb_kv8_decode_k
       float m[NB][2], l[NB][2];                       // references, and the sums of this thread's keys
 #pragma unroll
       for (int b = 0; b < NB; ++b) m[b][0] = m[b][1] = kNoScore, l[b][0] = l[b][1] = 0.f;
-      uint32_t power = kLift + 1;                     // exponent byte that the values' scales are relative to
-      float unit = __uint_as_float((254u + kLift - power) << 23);
+      uint32_t power = (kLift + 1) << 23;              // what the values' scales are relative to, as bits
+      float unit = __uint_as_float(((254u + kLift) << 23) - power);
 
-      // 16 keys; !WHOLE: some of them lie behind the end or in front of the window
-      const auto block = [&](auto whole, uint32_t at, uint32_t ex, int key0) {
-        constexpr bool WHOLE = decltype(whole)::value;
-        constexpr int kWords = HD == 64 ? 2 : 4;
-        uint4 kx[2][kSteps / 4];
-        uint32_t v[kSubs][4][kWords];
+      // A tile's work is S^T = K Q^T (products), the weights (weigh), and O^T += V^T P^T (multiply).  The last one runs beside the next tile's first:
+      // neither waits for the other, and a tile's conversions fill the time of the other's products.  The tile's values wait in registers (HD 256:
+      // there are none left; their stage is kept).
+      constexpr int kWords = HD == 64 ? 2 : 4;
+      constexpr bool KEEP = HD <= 128;
+      uint32_t v[KEEP ? kSubs : 1][2][4][kWords], pb[NB][4];
+      float s[NB][2][4];
 #pragma unroll
-        for (int c = 0; c < kSteps / 4; ++c) {
-          kx[0][c] = lds128(at + (c >> 1) * kTile * 128 + (k_off[0] ^ ((c & 1) << 4)));
-          kx[1][c] = lds128(at + (c >> 1) * kTile * 128 + (k_off[1] ^ ((c & 1) << 4)));
-        }
-        const bool see0 = WHOLE || (key0 + g >= w.span.first && key0 + g < w.span.len);
-        const bool see1 = WHOLE || (key0 + g + 8 >= w.span.first && key0 + g + 8 < w.span.len);
-        const float ks0 = kv8_scale(lds8(ex)), ks1 = kv8_scale(lds8(ex + 8));
-        uint32_t ve0 = lds8(ex + kTile), ve1 = lds8(ex + kTile + 8);
-        if (!see0) ve0 = 0u;
-        if (!see1) ve1 = 0u;
+      for (int i = 0; i < 8 * kWords * (KEEP ? kSubs : 1); ++i) v[i / (8 * kWords)][(i / (4 * kWords)) & 1][(i / kWords) & 3][i % kWords] = 0u;
 #pragma unroll
-        for (int sub = 0; sub < kSubs; ++sub)
+      for (int b = 0; b < NB; ++b) pb[b][0] = pb[b][1] = pb[b][2] = pb[b][3] = 0u;
+
+      const auto products = [&](uint32_t at) {
+        const uint32_t k_at = at + k_off;
+        int n[INT8 ? NB : 1][2][2][4];                 // int8: the products of the two parts of a query
+        float f[INT8 ? 1 : NB][2][2][4];               // e4m3: two sums, so that no product waits for the one before it
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if constexpr (HD == 64) {
-              const uint2 x = lds64(at + v_off[k]);
-              v[sub][k][0] = x.x, v[sub][k][1] = x.y;
+        for (int c = 0; c < kPieces; ++c) {
+          uint4 x[4];                                  // piece c of four keys
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = lds128(((k_at ^ kv8_step<HD>(i)) ^ ((c & 1) << 6)) + (c >> 1) * kTile * 128);
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+            const uint32_t y[4] = {x[2 * mt].x, x[2 * mt].y, x[2 * mt].z, x[2 * mt].w}, z[4] = {x[2 * mt + 1].x, x[2 * mt + 1].y, x[2 * mt + 1].z, x[2 * mt + 1].w};
+            if constexpr (INT8) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                  for (int part = 0; part < 2; ++part) {
+                    const uint32_t b0 = qf[b][4 * c + 2 * h + part][0], b1 = qf[b][4 * c + 2 * h + part][1];
+                    if (c + h == 0) mma_int8_first(n[b][mt][part], y[2 * h], z[2 * h], y[2 * h + 1], z[2 * h + 1], b0, b1);
+                    else mma_int8(n[b][mt][part], y[2 * h], z[2 * h], y[2 * h + 1], z[2 * h + 1], b0, b1);
+                  }
             } else {
-              const uint4 x = lds128(at + sub * kTile * 128 + v_off[k]);
-              v[sub][k][0] = x.x, v[sub][k][1] = x.y, v[sub][k][2] = x.z, v[sub][k][3] = x.w;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                uint32_t a0, a1, a2, a3;
+                kv8_to_half<false>(y[i], a0, a2);
+                kv8_to_half<false>(z[i], a1, a3);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                  if (c == 0 && i < 2) mma_f16_first(f[b][mt][i], a0, a1, a2, a3, qf[b][i][0], qf[b][i][1]);
+                  else mma_f16(f[b][mt][i & 1], a0, a1, a2, a3, qf[b][4 * c + i][0], qf[b][4 * c + i][1]);
+                }
+              }
             }
-            // codes of rows that nobody sees may be anything, e4m3's NaN, too
-            const int key = key0 + 2 * t4 + (k & 1) + (k >> 1) * 8;
-            if (!WHOLE && (key < w.span.first || key >= w.span.len)) {
-#pragma unroll
-              for (int i = 0; i < kWords; ++i) v[sub][k][i] = 0u;
-            }
-          }
-        float s[NB][4];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
-#pragma unroll
-        for (int c = 0; c < kSteps / 4; ++c) {
-          const uint32_t wx[4] = {kx[0][c].x, kx[0][c].y, kx[0][c].z, kx[0][c].w}, wy[4] = {kx[1][c].x, kx[1][c].y, kx[1][c].z, kx[1][c].w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t a0, a1, a2, a3;
-            kv8_to_half<INT8>(wx[i], a0, a2);
-            kv8_to_half<INT8>(wy[i], a1, a3);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) mma_f16(s[b], a0, a1, a2, a3, qf[b][c * 4 + i][0], qf[b][c * 4 + i][1]);
           }
         }
-        bool moves = max(ve0, ve1) > power;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            s[b][j] = see0 ? s[b][j] * (ks0 * factor[b][j]) : -INFINITY;
-            s[b][j + 2] = see1 ? s[b][j + 2] * (ks1 * factor[b][j]) : -INFINITY;
-            moves = moves || fmaxf(s[b][j], s[b][j + 2]) > m[b][j] + kSlack;
+          for (int i = 0; i < 8; ++i) {
+            if constexpr (INT8) s[b][i >> 2][i & 3] = fmaf(256.f, static_cast<float>(n[b][i >> 2][0][i & 3]), static_cast<float>(n[b][i >> 2][1][i & 3]));
+            else s[b][i >> 2][i & 3] = f[b][i >> 2][0][i & 3] + f[b][i >> 2][1][i & 3];
           }
+      };
+
+      // values of half `mt` of the tile's keys, columns of half `sub` of a head of 256: keys of rows 2 t4, 2 t4 + 1, and the same eight rows further
+      const auto read = [&](uint32_t at, int key0, int sub, int mt, uint32_t (&x)[4][kWords]) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int idx = 2 * mt + (k >> 1);
+          const uint32_t from = ((at + ((k & 1) ? v_off1 : v_off0)) ^ kv8_step<HD>(idx)) + sub * kTile * 128;
+          if constexpr (HD == 64) {
+            const uint2 y = lds64(from);
+            x[k][0] = y.x, x[k][1] = y.y;
+          } else {
+            const uint4 y = lds128(from);
+            x[k][0] = y.x, x[k][1] = y.y, x[k][2] = y.z, x[k][3] = y.w;
+          }
+          // codes of rows that nobody sees may be anything, e4m3's NaN, too
+          const int key = key0 + kv8_key<HD>(2 * t4 + (k & 1), idx);
+          if (key0 >= 0 && (key < w.span.first || key >= w.span.len)) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) x[k][i] = 0u;
+          }
+        }
+      };
+      const auto multiply = [&](int sub, int mt, const uint32_t (&x)[4][kWords]) {
+        // columns of a word: pairs of keys of each
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+          uint32_t a[4], c[4];
+          kv8_to_half<INT8>(__byte_perm(x[0][i], x[1][i], 0x5140), a[0], a[1]);
+          kv8_to_half<INT8>(__byte_perm(x[2][i], x[3][i], 0x5140), a[2], a[3]);
+          kv8_to_half<INT8>(__byte_perm(x[0][i], x[1][i], 0x7362), c[0], c[1]);
+          kv8_to_half<INT8>(__byte_perm(x[2][i], x[3][i], 0x7362), c[2], c[3]);
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            mma_f16(o[b][sub * 8 + 2 * i], a[0], a[1], a[2], a[3], pb[b][2 * mt], pb[b][2 * mt + 1]);
+            mma_f16(o[b][sub * 8 + 2 * i + 1], c[0], c[1], c[2], c[3], pb[b][2 * mt], pb[b][2 * mt + 1]);
+          }
+        }
+      };
+      const auto multiply_all = [&]() {
+        if constexpr (KEEP) {
+#pragma unroll
+          for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) multiply(sub, mt, v[sub][mt]);
+        }
+      };
+
+      // !WHOLE: some of the 32 keys lie behind the end or in front of the window
+      const auto weigh = [&](auto whole, uint32_t at, uint32_t ex, int key0) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        const uint32_t k_exps = __byte_perm(lds32(ex), 0u, turn), v_exps = __byte_perm(lds32(ex + kTile), 0u, turn);
+        if constexpr (KEEP) {
+#pragma unroll
+          for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) read(at, WHOLE ? -1 : key0, sub, mt, v[sub][mt]);
+        }
+        bool see[4];
+        uint32_t ve[4];                                // scales of the values, as bits: larger ones are larger numbers
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = key0 + kv8_key<HD>(g, i);
+          see[i] = WHOLE || (key >= w.span.first && key < w.span.len);
+          ve[i] = see[i] ? kv8_scale_of(v_exps, i) : 0u;
+        }
+        const uint32_t ve_most = max(max(ve[0], ve[1]), max(ve[2], ve[3]));
+        bool moves = ve_most > power;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float& x = s[b][i >> 1][(i & 1) * 2 + j];
+              x = see[i] ? x * (__uint_as_float(kv8_scale_of(k_exps, i)) * factor[b][j]) : -INFINITY;
+            }
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) moves = moves || fmaxf(fmaxf(s[b][0][j], s[b][0][j + 2]), fmaxf(s[b][1][j], s[b][1][j + 2])) > m[b][j] + kSlack;
         if (__any_sync(0xffffffffu, moves)) {
           // a row that is NaN has the byte 255: its scale stays an infinity, and its codes of zero make a NaN of it
-          const uint32_t now = max(power, __reduce_max_sync(0xffffffffu, min(max(ve0, ve1), 253u)));
-          const float shrink = now - power > 126u ? 0.f : __uint_as_float((127u - (now - power)) << 23);
+          const uint32_t now = max(power, __reduce_max_sync(0xffffffffu, min(ve_most, 253u << 23))), grown = (now - power) >> 23;
+          const float shrink = grown > 126u ? 0.f : __uint_as_float((127u - grown) << 23);
           power = now;
-          unit = __uint_as_float((254u + kLift - now) << 23);
+          unit = __uint_as_float(((254u + kLift) << 23) - now);
 #pragma unroll
           for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              float mx = fmaxf(s[b][j], s[b][j + 2]);
+              float mx = fmaxf(fmaxf(s[b][0][j], s[b][0][j + 2]), fmaxf(s[b][1][j], s[b][1][j + 2]));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16)), m[b][j]);
@@ -388,231 +549,281 @@ __global__ void __launch_bounds__(160, Kv8Sizes<HD, NB>::kPerSm) zb_kv8_decode_k
               }
             }
         }
-        const float vs0 = kv8_scale(ve0) * unit, vs1 = kv8_scale(ve1) * unit;
-        uint32_t pb[NB][2];
+        float vs[4];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
+        for (int i = 0; i < 4; ++i) vs[i] = __uint_as_float(ve[i]) * unit;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            s[b][j] = zb_ex2(s[b][j] - m[b][j]);
-            s[b][j + 2] = zb_ex2(s[b][j + 2] - m[b][j]);
-            l[b][j] += s[b][j] + s[b][j + 2];
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p0 = zb_ex2(s[b][i >> 1][(i & 1) * 2] - m[b][0]), p1 = zb_ex2(s[b][i >> 1][(i & 1) * 2 + 1] - m[b][1]);
+            l[b][0] += p0;
+            l[b][1] += p1;
+            pb[b][i] = transpose8(pack_half2(p0 * vs[i], p1 * vs[i]));
           }
-          pb[b][0] = transpose8(pack_half2(s[b][0] * vs0, s[b][1] * vs0));
-          pb[b][1] = transpose8(pack_half2(s[b][2] * vs1, s[b][3] * vs1));
-        }
-        // columns of a word: pairs of keys of each
+        if constexpr (!KEEP) {
 #pragma unroll
-        for (int sub = 0; sub < kSubs; ++sub)
+          for (int sub = 0; sub < kSubs; ++sub)
 #pragma unroll
-          for (int i = 0; i < kWords; ++i) {
-            uint32_t a[4], c[4];
-            kv8_to_half<INT8>(__byte_perm(v[sub][0][i], v[sub][1][i], 0x5140), a[0], a[1]);
-            kv8_to_half<INT8>(__byte_perm(v[sub][2][i], v[sub][3][i], 0x5140), a[2], a[3]);
-            kv8_to_half<INT8>(__byte_perm(v[sub][0][i], v[sub][1][i], 0x7362), c[0], c[1]);
-            kv8_to_half<INT8>(__byte_perm(v[sub][2][i], v[sub][3][i], 0x7362), c[2], c[3]);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-              mma_f16(o[b][sub * 8 + 2 * i], a[0], a[1], a[2], a[3], pb[b][0], pb[b][1]);
-              mma_f16(o[b][sub * 8 + 2 * i + 1], c[0], c[1], c[2], c[3], pb[b][0], pb[b][1]);
+            for (int mt = 0; mt < 2; ++mt) {
+              uint32_t x[4][kWords];
+              read(at, WHOLE ? -1 : key0, sub, mt, x);
+              multiply(sub, mt, x);
             }
-          }
+        }
       };
 
-      for (int t = w.begin; t < w.end; ++t) {
-        if (!dead) dead = !zb_mbar_wait(&full_bar[stage], phase, abort_flag);
-        dead = __any_sync(0xffffffffu, dead);
-        const int key0 = (w.span.tile0 + t) * kTile + warp * 16;
-        if (!dead && key0 < w.span.len && key0 + 16 > w.span.first) {
-          const uint32_t at = stages_at + stage * Z::kStageBytes, ex = exps_at + stage * 2 * kTile;
-          if (key0 >= w.span.first && key0 + 16 <= w.span.len) block(std::true_type(), at, ex, key0);
-          else block(std::false_type(), at, ex, key0);
+      for (int t = w.begin + warp; t < w.end; t += kWarps) {
+        copies_wait<kStages - 2>();
+        __syncwarp();                                  // everybody's copies of this tile have landed, and the last tile has been read
+        fetch();
+        const int key0 = (w.span.tile0 + t) * kTile;
+        const uint32_t at = stages_at + stage * Z::kStageBytes, ex = exps_at + stage * 2 * kTile + ex_off;
+        if (w.span.len > 0) {
+          products(at);
+          multiply_all();
+          if (key0 >= w.span.first && key0 + kTile <= w.span.len) weigh(std::true_type(), at, ex, key0);
+          else weigh(std::false_type(), at, ex, key0);
         }
-        __syncwarp();
-        if (lane == 0) zb_mbar_arrive(&empty_bar[stage]);
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
+        if (++stage == kStages) stage = 0;
       }
+      multiply_all();
 
-      // the four warps' sums of this segment
-      const float power_of = __uint_as_float((power - kLift) << 23);
+      // The CTA's sums: the warps' references, then half of the warps leave their sums, the others add theirs.  A thread's columns of a row are
+      // neighbours, eight of them (HD 64), or 16 of each 128.
+      const int out_row = w.seq * p.hkv * p.group + kvh * p.group + row0;
+      constexpr int kPitch = Z::kPitch, kHalf = kWarps / 2, kFours = HD / 4;
+      const float power_of = __uint_as_float(power - (kLift << 23));
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float x = l[b][j];
-          x += __shfl_xor_sync(0xffffffffu, x, 4);
-          x += __shfl_xor_sync(0xffffffffu, x, 8);
-          x += __shfl_xor_sync(0xffffffffu, x, 16);
-          const int r = b * 8 + 2 * t4 + j;
-          if (g == 0) {
-            float* st = stats + (warp * kRows + r) * 3;
-            st[0] = m[b][j];
-            st[1] = x;
-            st[2] = power_of;
-          }
-          float* dst = sums + (warp * kRows + r) * Z::kPitch;
+          float sum = l[b][j];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          if (g == 0) *reinterpret_cast<float2*>(stats + (warp * kRows + b * 8 + 2 * t4 + j) * 2) = make_float2(m[b][j], sum);
+        }
+      __syncthreads();
 #pragma unroll
-          for (int i = 0; i < kSteps; ++i) {
-            const int col = HD == 64 ? g * 8 + 2 * i : (i >> 3) * 128 + g * 16 + 2 * (i & 7);
-            *reinterpret_cast<float2*>(dst + col) = make_float2(o[b][i][j], o[b][i][j + 2]);
+      for (int turns = 0; turns < 2; ++turns) {
+        if ((warp >= kHalf) == (turns == 0)) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int r = b * 8 + 2 * t4 + j;
+              if (r >= rows) continue;
+              float top = kNoScore;
+#pragma unroll
+              for (int k = 0; k < kWarps; ++k) top = fmaxf(top, stats[(k * kRows + r) * 2]);
+              const float by = zb_ex2(m[b][j] - top) * power_of;
+#pragma unroll
+              for (int i = 0; i < kSteps; i += 2) {
+                const int col = HD == 64 ? g * 8 + 2 * i : (i >> 3) * 128 + g * 16 + 2 * (i & 7);
+                float4* dst = reinterpret_cast<float4*>(sums + ((turns == 0 ? warp - kHalf : warp) * kRows + r) * kPitch + col);
+                float4 x = make_float4(o[b][i][j] * by, o[b][i][j + 2] * by, o[b][i + 1][j] * by, o[b][i + 1][j + 2] * by);
+                if (turns == 1) {
+                  const float4 y = *dst;
+                  x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+                }
+                *dst = x;
+              }
+            }
+        }
+        __syncthreads();
+      }
+      // the CTA's sums of a row and four columns
+      const auto sum_of = [&](int r, int col, float& top, float& sum) {
+        top = kNoScore, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) top = fmaxf(top, stats[(k * kRows + r) * 2]);
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) {
+          const float2 st = *reinterpret_cast<const float2*>(stats + (k * kRows + r) * 2);
+          sum += zb_ex2(st.x - top) * st.y;
+        }
+        float4 x = *reinterpret_cast<const float4*>(sums + r * kPitch + col);
+#pragma unroll
+        for (int k = 1; k < kHalf; ++k) {
+          const float4 y = *reinterpret_cast<const float4*>(sums + (k * kRows + r) * kPitch + col);
+          x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+        }
+        return x;
+      };
+      const auto put = [&](int r, int col, const float4& x, float sum) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;              // a row that sees nothing is zero
+        *reinterpret_cast<uint2*>(p.out + static_cast<size_t>(out_row + r) * HD + col) = make_uint2(zb_pack_bf16x2(x.x * inv, x.y * inv), zb_pack_bf16x2(x.z * inv, x.w * inv));
+      };
+      if constexpr (CLUSTER) {
+        const bool alone = w.chunks == 1;
+        for (int i = threadIdx.x; i < rows * kFours; i += 32 * kWarps) {
+          const int r = i / kFours, col = 4 * (i - r * kFours);
+          float top, sum;
+          const float4 x = sum_of(r, col, top, sum);
+          if (alone) {
+            put(r, col, x, sum);
+          } else {
+            *reinterpret_cast<float4*>(sums + r * kPitch + col) = x;
+            if (col == 0) *reinterpret_cast<float2*>(stats + (kWarps * kRows + r) * 2) = make_float2(top, sum);
           }
+        }
+        if (alone) return;
+        // those of the cluster's CTAs, each of which finishes a share of the columns
+        __syncwarp();
+        zb_cluster_arrive();
+        zb_cluster_wait();
+        const uint32_t sums_at = zb_smem_u32(sums), stats_at = zb_smem_u32(stats + kWarps * kRows * 2);
+        for (int i = w.nth + p.parts * threadIdx.x; i < rows * kFours; i += p.parts * 32 * kWarps) {
+          const int r = i / kFours, col = 4 * (i - r * kFours);
+          float top = kNoScore, sum = 0.f;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int c0 = 0; c0 < p.parts; c0 += 8) {
+            float2 st[8];
+            float4 x[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              if (c0 + c >= p.parts) continue;
+              st[c] = load_peer2(zb_mapa(stats_at + r * 8, c0 + c));
+              x[c] = load_peer4(zb_mapa(sums_at + (r * kPitch + col) * 4, c0 + c));
+            }
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              if (c0 + c >= p.parts) continue;
+              const float up = fmaxf(top, st[c].x), was = zb_ex2(top - up), by = zb_ex2(st[c].x - up);
+              acc.x = acc.x * was + by * x[c].x, acc.y = acc.y * was + by * x[c].y, acc.z = acc.z * was + by * x[c].z, acc.w = acc.w * was + by * x[c].w;
+              sum = sum * was + by * st[c].y;
+              top = up;
+            }
+          }
+          put(r, col, acc, sum);
+        }
+        __syncwarp();
+        zb_cluster_arrive();                           // nobody leaves while another one reads its shared memory
+        zb_cluster_wait();
+        return;
+      } else {
+        const bool complete = w.chunks == 1;
+        const auto slot_at = [&](int nth, int r) { return static_cast<size_t>(w.slot + nth) * p.rows + r; };
+        for (int i = threadIdx.x; i < rows * kFours; i += 32 * kWarps) {
+          const int r = i / kFours, col = 4 * (i - r * kFours);
+          float top, sum;
+          const float4 x = sum_of(r, col, top, sum);
+          if (complete) {
+            put(r, col, x, sum);
+          } else {
+            *reinterpret_cast<float4*>(p.part_o + slot_at(w.nth, r) * HD + col) = x;
+            if (col == 0) p.part_ml[slot_at(w.nth, r)] = make_float2(top, sum);
+          }
+        }
+        if (complete) return;
+        __shared__ uint32_t drawn;
+        __syncthreads();                               // all of the CTA's sums are written
+        if (threadIdx.x == 0) {
+          __threadfence();
+          uint32_t* ticket = p.tickets + static_cast<size_t>(w.seq) * p.hkv * p.blocks + w.pair;
+          drawn = atomicAdd(ticket, 1u);
+          if (drawn == static_cast<uint32_t>(w.chunks - 1)) *ticket = 0u;      // for the next launch
+          __threadfence();
+        }
+        __syncthreads();
+        if (drawn != static_cast<uint32_t>(w.chunks - 1)) return;
+        // a warp for each row: the weights of 32 chunks at a time, one a lane, and the sums of 16
+        for (int r = warp; r < rows; r += kWarps) {
+          float top = kNoScore, sum = 0.f;
+          float acc[HD / 32];
+#pragma unroll
+          for (int j = 0; j < HD / 32; ++j) acc[j] = 0.f;
+          for (int i0 = 0; i0 < w.chunks; i0 += 32) {
+            constexpr int kOnce = HD == 256 ? 8 : 16;
+            const int most = min(32, w.chunks - i0);
+            const float2 ml = lane < most ? __ldcg(&p.part_ml[slot_at(i0 + lane, r)]) : make_float2(kNoScore, 0.f);
+            float x[kOnce][HD / 32];
+            const auto load = [&](int i1) {
+#pragma unroll
+              for (int i = 0; i < kOnce; ++i)
+#pragma unroll
+                for (int j = 0; j < HD / 32; ++j) x[i][j] = i1 + i < most ? __ldcg(p.part_o + slot_at(i0 + i1 + i, r) * HD + lane + 32 * j) : 0.f;
+            };
+            load(0);
+            const float up = fmaxf(top, zb_warp_max(ml.x)), was = zb_ex2(top - up), f = zb_ex2(ml.x - up);
+            top = up;
+            sum = sum * was + zb_warp_sum(f * ml.y);
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j) acc[j] *= was;
+            for (int i1 = 0; i1 < most; i1 += kOnce) {
+              if (i1 > 0) load(i1);
+#pragma unroll
+              for (int i = 0; i < kOnce; ++i) {
+                const float by = __shfl_sync(0xffffffffu, f, (i1 + i) & 31);
+#pragma unroll
+                for (int j = 0; j < HD / 32; ++j) acc[j] += by * x[i][j];
+              }
+            }
+          }
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+          for (int j = 0; j < HD / 32; ++j) p.out[static_cast<size_t>(out_row + r) * HD + lane + 32 * j] = __float2bfloat16(acc[j] * inv);
         }
       }
-      consumer_barrier();
-      const bool complete = w.begin == 0 && w.end == w.span.tiles;
-      const int slot = 2 * static_cast<int>(blockIdx.x) + (first_segment ? 0 : 1);
-      for (int i = threadIdx.x; i < rows * (HD / 2); i += 128) {
-        const int r = i / (HD / 2), col = 2 * (i - r * (HD / 2));
-        float top = kNoScore;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) top = fmaxf(top, stats[(k * kRows + r) * 3]);
-        float ax = 0.f, ay = 0.f, sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float* st = stats + (k * kRows + r) * 3;
-          const float f = zb_ex2(st[0] - top), fo = f * st[2];
-          const float2 x = *reinterpret_cast<const float2*>(sums + (k * kRows + r) * Z::kPitch + col);
-          ax += fo * x.x;
-          ay += fo * x.y;
-          sum += f * st[1];
-        }
-        if (complete) {
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;            // a row that sees nothing is zero
-          *reinterpret_cast<uint32_t*>(p.out + (static_cast<size_t>(w.seq) * p.hkv * p.group + kvh * p.group + row0 + r) * HD + col) =
-              zb_pack_bf16x2(ax * inv, ay * inv);
-        } else {
-          *reinterpret_cast<float2*>(p.part_o + (static_cast<size_t>(slot) * kRows + r) * HD + col) = make_float2(ax, ay);
-          if (col == 0) p.part_ml[static_cast<size_t>(slot) * kRows + r] = make_float2(top, sum);
-        }
-      }
-      consumer_barrier();                             // the sums may be overwritten
-      first_segment = false;
-    } while (kv8_next(p, w));
-  }
-  __syncthreads();
-  if (*abort_flag != 0u) {
-    if (threadIdx.x == 0) zb_record_error(p.status, ZB_ERR_MBAR_TIMEOUT, kKernelKv8Decode, 1u, blockIdx.x);
-    // copies that may still be in flight must land before the shared memory is reused
-    const uint64_t t0 = zb_globaltimer();
-    while (zb_globaltimer() - t0 < 200000ull) {
-    }
   }
 }
 
-// Joins the pairs that several CTAs have a part of.  CTA c looks at the pair at the beginning of part c + 1; the first one to meet a pair there
-// joins it, a row of queries in each warp, or in each of two where rows are eight.
-template <int HD, int NB>
-__global__ void __launch_bounds__(512) zb_kv8_join_kernel(const Kv8DecodeParams p) {
-  constexpr int kRows = 8 * NB, kGroups = 16 / kRows, kCols = HD / 32;
-  __shared__ float weight[kRows][kMaxCtas];
-  __shared__ float sums[kRows];
-  __shared__ float parts[kGroups][kRows][HD];
-  zb_pdl_launch();
-  zb_pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = warp % kRows, part = warp / kRows;
-  const int pairs = p.hkv * p.blocks;
-  const auto count = [&](int s) { return kv8_span(p, s).tiles * pairs; };
-  const int total = kv8_total(p.batch, count);
-  const Kv8Parts list(total, p.ctas);
-  const int c = static_cast<int>(blockIdx.x), at = list.begin(c + 1), start = list.begin(c);
-  if (at >= total || at == start) return;
-  int seq, before;
-  kv8_locate(p.batch, at, count, seq, before);
-  const int tiles = kv8_span(p, seq).tiles, pair = (at - before) / tiles, pair0 = before + pair * tiles;
-  if (at == pair0 || start > pair0) return;           // nothing is cut here, or the pair has been met before
-  const int n = list.of(pair0 + tiles - 1) - c + 1;   // parts c .. c + n - 1, none of them empty
-  const int kvh = pair / p.blocks, row0 = (pair - kvh * p.blocks) * kRows, rows = min(kRows, p.group - row0);
-  // the pair is the last segment of part c, unless that begins with it, and the first one of the others
-  const int slot0 = 2 * c + (start >= pair0 ? 0 : 1);
-  const auto slot_of = [&](int i) { return i == 0 ? slot0 : 2 * (c + i); };
-  if (part == 0 && row < rows) {
-    float top = kNoScore, sum = 0.f;
-    for (int i = lane; i < n; i += 32) {
-      const float2 ml = p.part_ml[static_cast<size_t>(slot_of(i)) * kRows + row];
-      weight[row][i] = ml.x;
-      const float up = fmaxf(top, ml.x);
-      sum = sum * zb_ex2(top - up) + ml.y * zb_ex2(ml.x - up);
-      top = up;
-    }
-    const float all = zb_warp_max(top);
-    sum = zb_warp_sum(sum * zb_ex2(top - all));
-    for (int i = lane; i < n; i += 32) weight[row][i] = zb_ex2(weight[row][i] - all);
-    if (lane == 0) sums[row] = sum;
-  }
-  __syncthreads();
-  float acc[kCols];
-#pragma unroll
-  for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
-  if (row < rows) {
-#pragma unroll 4
-    for (int i = part; i < n; i += kGroups) {
-      const float f = weight[row][i];
-      const float* src = p.part_o + (static_cast<size_t>(slot_of(i)) * kRows + row) * HD;
-#pragma unroll
-      for (int j = 0; j < kCols; ++j) acc[j] += f * src[lane + 32 * j];
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < kCols; ++j) parts[part][row][lane + 32 * j] = acc[j];
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows * HD; i += 512) {
-    const int r = i / HD, col = i - r * HD;
-    float x = 0.f;
-#pragma unroll
-    for (int k = 0; k < kGroups; ++k) x += parts[k][r][col];
-    p.out[(static_cast<size_t>(seq) * p.hkv * p.group + kvh * p.group + row0 + r) * HD + col] = __float2bfloat16(sums[r] == 0.f ? 0.f : x / sums[r]);
-  }
-}
-
-template <int HD, int NB, bool INT8>
-int launch_decode(const Kv8DecodeParams& p, const void* k_codes, const void* v_codes, cudaStream_t stream) {
+template <int HD, int NB, bool INT8, bool CLUSTER>
+int launch_decode(const Kv8DecodeParams& p, int pairs, cudaStream_t stream) {
   using Z = Kv8Sizes<HD, NB>;
+  const auto kernel = zb_kv8_decode_kernel<HD, NB, INT8, CLUSTER>;
   static bool configured[16] = {};
-  if (const int rc = zb_config_smem_once(zb_kv8_decode_kernel<HD, NB, INT8>, Z::kSmem, configured)) return rc;
-  const long long rows = static_cast<long long>(p.num_pages) * p.hkv * p.page_size;
-  const int box_rows = HD == 64 ? p.unit / 2 : p.unit;
-  CUtensorMap tk, tv;
-  const long long map_rows = HD == 64 ? rows / 2 : rows, map_bytes = HD == 64 ? 128 : HD;
-  if (const int rc = zb_make_tmap_u8_2d_ex(&tk, k_codes, map_rows, map_bytes, 128, box_rows, 1)) return rc;
-  if (const int rc = zb_make_tmap_u8_2d_ex(&tv, v_codes, map_rows, map_bytes, 128, box_rows, 1)) return rc;
-  cudaError_t e = zb_launch(zb_kv8_decode_kernel<HD, NB, INT8>, dim3(p.ctas), dim3(160), Z::kSmem, stream, tk, tv, p);
-  zb_count_launch(1);
-  if (e == cudaSuccess && p.ctas > 1) {
-    e = zb_launch(zb_kv8_join_kernel<HD, NB>, dim3(p.ctas - 1), dim3(512), 0, stream, p);
-    zb_count_launch(1);
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 16) return -21;
+  cudaError_t e = cudaSuccess;
+  if (!configured[dev]) {
+    e = zb_config_smem(kernel, Z::kSmem);
+    if (CLUSTER && e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);      // 16 CTAs
+    if (e != cudaSuccess) return static_cast<int>(e);
+    configured[dev] = true;
   }
+  if (CLUSTER) e = zb_launch_cluster(kernel, dim3(static_cast<unsigned>(pairs * p.parts)), dim3(32 * Z::kWarps), Z::kSmem, stream, p.parts, p);
+  else e = zb_launch(kernel, dim3(static_cast<unsigned>(pairs <= p.parts ? p.parts : pairs + p.parts)), dim3(32 * Z::kWarps), Z::kSmem, stream, p);
+  zb_count_launch(1);
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
+template <int HD, int NB>
+int launch_decode(const Kv8DecodeParams& p, bool int8, bool cluster, int pairs, cudaStream_t stream) {
+  if (cluster) return int8 ? launch_decode<HD, NB, true, true>(p, pairs, stream) : launch_decode<HD, NB, false, true>(p, pairs, stream);
+  return int8 ? launch_decode<HD, NB, true, false>(p, pairs, stream) : launch_decode<HD, NB, false, false>(p, pairs, stream);
+}
+
+// Chunks of cut pairs: at most as many as there are CTAs, or, where there are more pairs, two for each even share that such a pair has.
+long long slots_of(int parts) { return 2ll * parts; }
 
 // Query heads of a pair: 16 where the group has more than eight (a head of 256 has registers for eight).
 int rows_of(int hd, int group) { return group > 8 && hd <= 128 ? 16 : 8; }
-int per_sm_of(int hd, int rows) {
-  if (hd == 64) return rows == 8 ? Kv8Sizes<64, 1>::kPerSm : Kv8Sizes<64, 2>::kPerSm;
-  if (hd == 128) return rows == 8 ? Kv8Sizes<128, 1>::kPerSm : Kv8Sizes<128, 2>::kPerSm;
-  return Kv8Sizes<256, 1>::kPerSm;
-}
-
 }  // namespace
 
 extern "C" {
 
-// CTAs of a call, and (in *floats) the fp32 numbers of its workspace.  max_len: keys of the longest sequence, or a bound of them: it bounds the
-// CTAs that have something to do, any number gives right results.
+// How a call is cut: CTAs of a cluster as a negative number, or the CTAs that share the chunks, and (in *floats) the fp32 numbers of its workspace, which
+// needs no particular contents.  max_len: keys of the longest sequence, or a bound of them; any number gives right results.
 int zb_kv8_decode_plan(int batch, int hq, int hkv, int hd, int max_len, long long* floats) {
   *floats = 0;
   if (batch <= 0) return 0;
-  if (hkv <= 0 || hq <= 0 || hq % hkv != 0 || (hd != 64 && hd != 128 && hd != 256)) return -30;
+  if (hkv <= 0 || hq <= 0 || hq % hkv != 0 || (hd != 64 && hd != 128 && hd != 256)) return INT_MIN;
   ZbDeviceState* st = zb_device_state();
-  if (!st) return -20;
-  const int rows = rows_of(hd, hq / hkv), blocks = (hq / hkv + rows - 1) / rows;
-  const long long tiles = static_cast<long long>(batch) * hkv * blocks * std::max(1, (max_len + kTile - 1) / kTile);
-  if (tiles > 0x3fffffffll) return -34;
-  const int ctas = static_cast<int>(std::min<long long>(tiles, std::min(kMaxCtas, st->num_sms * per_sm_of(hd, rows))));
-  *floats = 2ll * ctas * rows * (hd + 2);
-  return ctas;
+  if (!st) return INT_MIN;
+  const int block = rows_of(hd, hq / hkv), blocks = (hq / hkv + block - 1) / block, rows = std::min(hq / hkv, block), warps = hd == 256 ? 2 : 4;
+  const long long pairs = static_cast<long long>(batch) * hkv * blocks, longest = std::max(1, (max_len + kTile - 1) / kTile), tiles = pairs * longest;
+  if (tiles > 0x3fffffffll) return INT_MIN;
+  const int most = st->num_sms * (hd == 128 && block == 16 ? 1 : 2);
+  int size = 1;
+  while (size < 16 && size * warps < longest) size *= 2;
+  if (pairs * size <= most && size * warps * 2 >= longest) return -size;
+  // No sequence is long, and there is no room to cut one: a CTA for each pair, which need not look at the other lengths (128 x 1024 keys of 4
+  // heads: 28.5 us, 31.5 with that look)
+  if (batch > kMaxBatch || (2 * pairs > most && longest <= 64)) return -1;
+  const int parts = static_cast<int>(std::min<long long>(tiles, most));
+  *floats = slots_of(parts) * rows * (hd + 2);
+  return parts;
 }
 
 // The arguments of a call, as the caller packs them (ops/kv8.py).
@@ -622,10 +833,11 @@ struct ZbKv8Decode {
   void* out;                                       // [batch, hq, hd], contiguous
   const int32_t* block_table;
   const int32_t* seq_lens;
-  float* work;                                     // the numbers that the plan of `ctas` CTAs asked for
+  float* work;                                     // the numbers that the plan asked for
+  uint32_t* tickets;                               // [batch * hkv * blocks of queries] where the plan is a list: zero before the call, and after it
   void* stream;
   long long q_stride;
-  int batch, hq, hkv, hd, page_size, max_pages, num_pages, window, int8, ctas;
+  int batch, hq, hkv, hd, page_size, max_pages, num_pages, window, int8, parts;
   float scale;
 };
 
@@ -636,47 +848,46 @@ int zb_kv8_decode(const ZbKv8Decode* c) {
   if (page_size <= 0 || page_size % 16 != 0 || c->num_pages <= 0 || static_cast<long long>(c->num_pages) * hkv * page_size > 0x7fffffffll ||
       static_cast<long long>(c->max_pages) * page_size > 0x7fffff00ll)
     return -31;
-  if (c->ctas < 1 || c->ctas > kMaxCtas) return -33;
+  if (c->parts == 0 || c->parts < -16 || c->parts > 65536) return -33;
   ZbDeviceState* st = zb_device_state();
   if (!st) return -20;
-  const int rows = rows_of(hd, hq / hkv);
+  const int block = rows_of(hd, hq / hkv);
   Kv8DecodeParams p = {};
   p.q = reinterpret_cast<const __nv_bfloat16*>(c->q);
+  p.k_codes = reinterpret_cast<const uint8_t*>(c->k_codes);
+  p.v_codes = reinterpret_cast<const uint8_t*>(c->v_codes);
   p.k_exps = reinterpret_cast<const uint8_t*>(c->k_exps);
   p.v_exps = reinterpret_cast<const uint8_t*>(c->v_exps);
   p.out = reinterpret_cast<__nv_bfloat16*>(c->out);
   p.block_table = c->block_table;
   p.seq_lens = c->seq_lens;
-  p.part_o = c->work;
-  p.part_ml = reinterpret_cast<float2*>(c->work + 2ll * c->ctas * rows * hd);
-  p.q_stride = c->q_stride;
   p.batch = c->batch;
   p.hkv = hkv;
   p.group = hq / hkv;
-  p.blocks = (p.group + rows - 1) / rows;
+  p.blocks = (p.group + block - 1) / block;
+  p.rows = std::min(p.group, block);
+  const long long pairs = static_cast<long long>(c->batch) * hkv * p.blocks;
+  if (pairs > 0x3ffffff) return -34;
+  const bool cluster = c->parts < 0;
+  p.parts = cluster ? -c->parts : c->parts;
+  p.part_o = c->work;
+  p.part_ml = reinterpret_cast<float2*>(c->work + slots_of(c->parts) * p.rows * hd);
+  p.tickets = c->tickets;
+  if (!cluster && c->batch > kMaxBatch) return -33;
+  if (!cluster && (c->work == nullptr || c->tickets == nullptr)) return -33;
+  p.q_stride = c->q_stride;
   p.page_size = page_size;
   p.max_pages = c->max_pages;
   p.num_pages = c->num_pages;
   p.window = c->window;
-  p.unit = 16;
-  while (p.unit < kTile && page_size % (2 * p.unit) == 0) p.unit *= 2;
-  p.ctas = c->ctas;
   p.scale_log2 = c->scale * 1.4426950408889634f;
   p.status = st->status;
-  if (static_cast<long long>(c->batch) * hkv * p.blocks * std::max<long long>(1, (static_cast<long long>(c->max_pages) * page_size + kTile - 1) / kTile) > 0x3fffffffll)
-    return -34;
+  if (pairs * std::max<long long>(1, (static_cast<long long>(c->max_pages) * page_size + kTile - 1) / kTile) > 0x3fffffffll) return -34;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(c->stream);
-  const void *k = c->k_codes, *v = c->v_codes;
-  const bool int8 = c->int8 != 0;
-  if (hd == 64) {
-    if (rows == 8) return int8 ? launch_decode<64, 1, true>(p, k, v, s) : launch_decode<64, 1, false>(p, k, v, s);
-    return int8 ? launch_decode<64, 2, true>(p, k, v, s) : launch_decode<64, 2, false>(p, k, v, s);
-  }
-  if (hd == 128) {
-    if (rows == 8) return int8 ? launch_decode<128, 1, true>(p, k, v, s) : launch_decode<128, 1, false>(p, k, v, s);
-    return int8 ? launch_decode<128, 2, true>(p, k, v, s) : launch_decode<128, 2, false>(p, k, v, s);
-  }
-  return int8 ? launch_decode<256, 1, true>(p, k, v, s) : launch_decode<256, 1, false>(p, k, v, s);
+  const int n = static_cast<int>(pairs);
+  if (hd == 64) return block == 8 ? launch_decode<64, 1>(p, c->int8 != 0, cluster, n, s) : launch_decode<64, 2>(p, c->int8 != 0, cluster, n, s);
+  if (hd == 128) return block == 8 ? launch_decode<128, 1>(p, c->int8 != 0, cluster, n, s) : launch_decode<128, 2>(p, c->int8 != 0, cluster, n, s);
+  return launch_decode<256, 1>(p, c->int8 != 0, cluster, n, s);
 }
 
 }  // extern "C"

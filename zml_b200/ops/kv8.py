@@ -28,7 +28,7 @@ for _name in ("zb_kv8_write", "zb_kv8_read", "zb_kv8_decode"):
 _lib.register_signature("zb_kv8_decode_plan", C.c_int, [C.c_int] * 5 + [C.c_void_p])
 _WRITE = struct.Struct("12P 2q 9i 2f").pack
 _READ = struct.Struct("10P 8i").pack
-_DECODE = struct.Struct("10P q 10i f").pack
+_DECODE = struct.Struct("11P q 10i f").pack
 
 # names that the engine and the command line take -> type of the codes
 KV_DTYPES = {"fp8": torch.float8_e4m3fn, "int8": torch.int8}
@@ -179,6 +179,7 @@ def _queries(q, k: QuantKV, out) -> tuple[int, int, int]:
 
 _current = getattr(torch._C, "_cuda_getDevice", None)                     # absent in builds of torch without CUDA
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)
 
 
 # ------------------------------------------------------------------ writer
@@ -312,17 +313,33 @@ _PLANS: dict = {}
 
 
 def _plan(index, b, hq, hkv, hd, max_len) -> tuple[int, int]:
-    """(CTAs, numbers of the workspace) of a decode call: a function of its sizes."""
-    key = (index, b, hq, hkv, hd, -(-max_len // 64))
+    """(how a decode call is cut, numbers of its workspace): a function of its sizes."""
+    key = (index, b, hq, hkv, hd, -(-max_len // 32))
     got = _PLANS.get(key)
     if got is None:
         n = C.c_longlong()
-        ctas = _lib.lib().zb_kv8_decode_plan(b, hq, hkv, hd, max_len, C.byref(n))
-        if ctas < 0:
-            _lib.check(ctas, "zb_kv8_decode_plan")
+        parts = _lib.lib().zb_kv8_decode_plan(b, hq, hkv, hd, max_len, C.byref(n))
+        if parts == -2 ** 31:
+            raise _lib.KernelError(f"no plan for {b} sequences of up to {max_len} keys, {hq} / {hkv} heads of {hd}")
         if len(_PLANS) >= 4096:
             _PLANS.clear()
-        got = _PLANS[key] = (ctas, n.value)
+        got = _PLANS[key] = (parts, n.value)
+    return got
+
+
+_TICKETS: dict = {}
+
+
+def _tickets(q, index: int, stream: int, n: int):
+    """At least n zeros (int32) that no other call in flight uses; the kernel leaves zeros behind.  The calls of one stream follow one another and
+    share theirs; a captured call has its own, cleared by every replay, since graphs may be replayed on any streams."""
+    if _capturing():
+        return q.new_zeros((n,), dtype=torch.int32)
+    got = _TICKETS.get((index, stream))
+    if got is None or got.numel() < n:
+        if len(_TICKETS) >= 256:
+            _TICKETS.clear()
+        got = _TICKETS[(index, stream)] = q.new_zeros((max(n, 4096),), dtype=torch.int32)
     return got
 
 
@@ -350,12 +367,17 @@ def paged_decode(q, k: QuantKV, v: QuantKV, block_table, seq_lens, scale: Option
     if out is None:
         out = q.new_empty((b, hq, hd))
     most = width * page_size
-    ctas, numbers = _plan(index, b, hq, hkv, hd, most if max_seq_len is None else min(max_seq_len, most))
-    work = q.new_empty((numbers,), dtype=torch.float32)
+    parts, numbers = _plan(index, b, hq, hkv, hd, most if max_seq_len is None else min(max_seq_len, most))
+    stream = _stream(index)
+    work = tickets = 0
+    if numbers:                                                              # the parts of a list leave sums, and draw tickets
+        partial = q.new_empty((numbers,), dtype=torch.float32)
+        ticket = _tickets(q, index, stream, b * hq)
+        work, tickets = partial.data_ptr(), ticket.data_ptr()
     kc = k._codes
     rc = _lib.lib().zb_kv8_decode(_DECODE(
         q.data_ptr(), kc.data_ptr(), k._exponents.data_ptr(), v._codes.data_ptr(), v._exponents.data_ptr(), out.data_ptr(), block_table.data_ptr(),
-        seq_lens.data_ptr(), work.data_ptr(), _stream(index), s0, b, hq, hkv, hd, page_size, width, pages, window, kc.dtype is torch.int8, ctas,
+        seq_lens.data_ptr(), work, tickets, stream, s0, b, hq, hkv, hd, page_size, width, pages, window, kc.dtype is torch.int8, parts,
         1.0 / math.sqrt(hd) if scale is None else scale))
     if rc:
         _lib.check(rc, "zb_kv8_decode")
