@@ -7,6 +7,8 @@
 // Between the bf16 projection and the one rounding at the end (bf16 queries, codes) everything is fp32: a rounding to bf16 in between would put
 // three codes of a hundred into the neighbouring step.  Angles p * f are formed and reduced in fp64 (one per pair of columns and token, used
 // by all heads), so that far positions keep the digits that fp32 products lose (1e5 radians: 0.004).
+#include <algorithm>
+
 #include "host_api.h"
 #include "kv8.cuh"
 
@@ -72,104 +74,126 @@ ZB_DEVICE void kv8_unpack8(const uint4& u, float (&f)[8]) {
 }
 
 // Halves (LAYOUT 0, rot_dim a multiple of 16) or neighbours (LAYOUT 1) rotate into each other; rows start on 16 bytes.  A thread has two pieces of
-// eight columns of one head: the two that rotate into each other, or two neighbours.  The HD / 16 threads of a head lie in one warp and add up
-// its squares and its largest magnitude.  One CTA takes a token (few tokens of many heads: a part of its pieces).
+// eight columns of one head, the same of every token: the two that rotate into each other, or two neighbours.  The HD / 16 threads of a head lie in
+// one warp and add up its squares and its largest magnitude.  A CTA takes one token after the other (its threads a part of the pieces where those are more
+// than 512): the next projection is on its way while it works on this one, and its threads form the angles of kAhead tokens at once, one or
+// two each, so that they meet once in as many tokens.
+constexpr int kAhead = 4;
 template <int HD, int LAYOUT, bool INT8>
-__global__ void __launch_bounds__(512) zb_kv8_write_kernel(const Kv8WriteParams p) {
-  constexpr int kLanes = HD / 16;
-  __shared__ __align__(16) float sn[HD / 2], cs[HD / 2];
+__global__ void __launch_bounds__(512, 2) zb_kv8_write_kernel(const Kv8WriteParams p) {
+  constexpr int kLanes = HD / 16, kHalf = HD / 2;
+  // cosines and sines; angle i lies where a thread's eight are two pieces of 16 bytes, neighbouring threads' beside each other
+  __shared__ __align__(16) float cs[2][kAhead][kHalf], sn[2][kAhead][kHalf];
   zb_pdl_launch();
   zb_pdl_wait();
-  const int tok = blockIdx.x, half = p.rot_dim >> 1;
-  const int pos = p.positions[tok];
-  const long long slot = kv8_slot(p, tok);
-  const int from = static_cast<int>(blockIdx.y) * p.share, units = min(from + p.share, (p.hq + 2 * p.hkv) * kLanes);
-  const int rounded = from + ((units - from + 31) & ~31);      // a warp goes through the loop as a whole
-  bool first = true;
-  for (int u0 = from + threadIdx.x; u0 < rounded; u0 += blockDim.x) {
-    const bool in = u0 < units;
-    const int u = in ? u0 : units - 1, h = u / kLanes, j = u - h * kLanes;
-    const bool is_q = h < p.hq, turned = h < p.hq + p.hkv;
-    const bool turns = LAYOUT == 0 && turned && j < half / 8;
-    // 8-column pieces of the head
-    const int a0 = LAYOUT == 1 || !turned ? 2 * j : (turns ? j : half / 4 + 2 * (j - half / 8));
-    const int a1 = turns ? j + half / 8 : a0 + 1;
-    const uint4* src = reinterpret_cast<const uint4*>(p.qkv + static_cast<size_t>(tok) * p.qkv_stride + static_cast<size_t>(h) * HD);
-    const uint4 x0 = src[a0], x1 = src[a1];
-    if (first) {                                     // the angles, while the loads are on their way
-      first = false;
-      for (int i = threadIdx.x; i < half; i += blockDim.x) kv8_angle(pos, p.inv_freq[i], p.attn_factor, sn[i], cs[i]);
-      __syncthreads();
+  const int half = p.rot_dim >> 1;
+  const int units = (p.hq + 2 * p.hkv) * kLanes, u = min(static_cast<int>(blockIdx.y) * p.share + static_cast<int>(threadIdx.x), units - 1);
+  const bool in = static_cast<int>(threadIdx.x) < p.share && static_cast<int>(blockIdx.y) * p.share + static_cast<int>(threadIdx.x) < units;
+  const int h = u / kLanes, j = u - h * kLanes;
+  const bool is_q = h < p.hq, turned = h < p.hq + p.hkv, turns = turned && (LAYOUT == 1 || j < half / 8);
+  const int a0 = LAYOUT == 1 || !turned ? 2 * j : (turns ? j : half / 4 + 2 * (j - half / 8));
+  const int a1 = LAYOUT == 0 && turns ? j + half / 8 : a0 + 1;
+  const bool any_kv = __any_sync(0xffffffffu, !is_q);
+  const uint4* src = reinterpret_cast<const uint4*>(p.qkv + static_cast<size_t>(h) * HD);
+  const __nv_bfloat16* nw = !turned ? nullptr : (is_q ? p.q_norm_w : p.k_norm_w);
+  const bool normed = p.q_norm_w != nullptr || p.k_norm_w != nullptr;
+  uint4 w0 = make_uint4(0u, 0u, 0u, 0u), w1 = w0;
+  if (nw != nullptr) w0 = reinterpret_cast<const uint4*>(nw)[a0], w1 = reinterpret_cast<const uint4*>(nw)[a1];
+  const float one = p.norm_unit_offset ? 1.f : 0.f;
+  const int kvh = turned ? h - p.hq : h - p.hq - p.hkv;
+  uint8_t* const codes = turned ? p.k_codes : p.v_codes;
+  uint8_t* const exps = turned ? p.k_exps : p.v_exps;
+
+  const auto angles = [&](int from, int buf) {         // of the next kAhead tokens of this CTA
+    for (int i = threadIdx.x; i < kAhead * half; i += blockDim.x) {
+      const int k = i / half, n = i - k * half;
+      const long long tok = from + static_cast<long long>(k) * gridDim.x;
+      if (tok >= p.tokens) break;
+      const int at = ((n >> 2) & 1) * (kHalf / 2) + (n >> 3) * 4 + (n & 3);
+      kv8_angle(p.positions[tok], p.inv_freq[n], p.attn_factor, sn[buf][k][at], cs[buf][k][at]);
+    }
+  };
+  int tok = blockIdx.x, buf = 0, k = 0;
+  size_t row = static_cast<size_t>(tok) * p.qkv_stride / 8;
+  uint4 x0 = src[row + a0], x1 = src[row + a1];
+  long long slot = kv8_slot(p, tok);
+  angles(tok, 0);
+  __syncthreads();
+  while (true) {
+    const long long tok1 = static_cast<long long>(tok) + gridDim.x;
+    const bool more = tok1 < p.tokens;
+    uint4 y0 = x0, y1 = x1;
+    long long slot1 = slot;
+    if (more) {
+      row = static_cast<size_t>(tok1) * p.qkv_stride / 8;
+      y0 = src[row + a0], y1 = src[row + a1];
+      slot1 = kv8_slot(p, static_cast<int>(tok1));
+      if (k == 0 && tok + static_cast<long long>(kAhead) * gridDim.x < p.tokens) angles(tok + kAhead * static_cast<int>(gridDim.x), buf ^ 1);
     }
     float f0[8], f1[8];
     kv8_unpack8(x0, f0);
     kv8_unpack8(x1, f1);
-    const uint32_t group = ((1ull << kLanes) - 1ull) << ((threadIdx.x & 31) / kLanes * kLanes);
-    if (turned) {
-      const __nv_bfloat16* nw = is_q ? p.q_norm_w : p.k_norm_w;
+    if (normed) {
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss += f0[i] * f0[i] + f1[i] * f1[i];
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
       if (nw != nullptr) {
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss += f0[i] * f0[i] + f1[i] * f1[i];
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
-        const float inv = rsqrtf(ss / static_cast<float>(HD) + p.norm_eps), one = p.norm_unit_offset ? 1.f : 0.f;
+        const float inv = rsqrtf(ss / static_cast<float>(HD) + p.norm_eps);
         float g0[8], g1[8];
-        kv8_unpack8(reinterpret_cast<const uint4*>(nw)[a0], g0);
-        kv8_unpack8(reinterpret_cast<const uint4*>(nw)[a1], g1);
+        kv8_unpack8(w0, g0);
+        kv8_unpack8(w1, g1);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           f0[i] = f0[i] * inv * (g0[i] + one);
           f1[i] = f1[i] * inv * (g1[i] + one);
         }
       }
-      if (LAYOUT == 0) {
-        if (turns) {
+    }
+    if (turns) {
+      const float4 c0 = *reinterpret_cast<const float4*>(&cs[buf][k][4 * j]), c1 = *reinterpret_cast<const float4*>(&cs[buf][k][kHalf / 2 + 4 * j]);
+      const float4 s0 = *reinterpret_cast<const float4*>(&sn[buf][k][4 * j]), s1 = *reinterpret_cast<const float4*>(&sn[buf][k][kHalf / 2 + 4 * j]);
+      const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float c_ = cs[8 * j + i], s_ = sn[8 * j + i], x = f0[i], y = f1[i];
-            f0[i] = x * c_ - y * s_;
-            f1[i] = y * c_ + x * s_;
-          }
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int i0 = 8 * j + i, i1 = i0 + 4;
-          if (i0 < half) {
-            const float x = f0[2 * i], y = f0[2 * i + 1];
-            f0[2 * i] = x * cs[i0] - y * sn[i0];
-            f0[2 * i + 1] = y * cs[i0] + x * sn[i0];
-          }
-          if (i1 < half) {
-            const float x = f1[2 * i], y = f1[2 * i + 1];
-            f1[2 * i] = x * cs[i1] - y * sn[i1];
-            f1[2 * i + 1] = y * cs[i1] + x * sn[i1];
-          }
+      for (int i = 0; i < 8; ++i) {
+        float& x = LAYOUT == 0 ? f0[i] : (i < 4 ? f0[2 * i] : f1[2 * i - 8]);
+        float& y = LAYOUT == 0 ? f1[i] : (i < 4 ? f0[2 * i + 1] : f1[2 * i - 7]);
+        if (LAYOUT == 0 || 8 * j + i < half) {
+          const float a = x, b = y;
+          x = a * c[i] - b * s[i];
+          y = b * c[i] + a * s[i];
         }
       }
     }
-    if (is_q) {
-      if (!in) continue;
+    if (is_q && in) {
       uint4* dst = reinterpret_cast<uint4*>(p.q_out + (static_cast<size_t>(tok) * p.hq + h) * HD);
       dst[a0] = make_uint4(zb_pack_bf16x2(f0[0], f0[1]), zb_pack_bf16x2(f0[2], f0[3]), zb_pack_bf16x2(f0[4], f0[5]), zb_pack_bf16x2(f0[6], f0[7]));
       dst[a1] = make_uint4(zb_pack_bf16x2(f1[0], f1[1]), zb_pack_bf16x2(f1[2], f1[3]), zb_pack_bf16x2(f1[4], f1[5]), zb_pack_bf16x2(f1[6], f1[7]));
-      continue;
     }
-    uint32_t amax = 0u;
+    if (any_kv) {
+      uint32_t amax = 0u;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = max(amax, max(kv8_abs_bits(f0[i]), kv8_abs_bits(f1[i])));
+      for (int i = 0; i < 8; ++i) amax = max(amax, max(kv8_abs_bits(f0[i]), kv8_abs_bits(f1[i])));
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(group, amax, o));
-    if (!in || slot < 0) continue;
-    const uint32_t byte = kv8_exponent<INT8>(amax);
-    const float inv = kv8_inverse(byte);
-    const int kvh = turned ? h - p.hq : h - p.hq - p.hkv;
-    const size_t at = kv8_row_at(p, slot, kvh);
-    uint2* dst = reinterpret_cast<uint2*>((turned ? p.k_codes : p.v_codes) + at * HD);
-    dst[a0] = make_uint2(kv8_pack4<INT8>(inv, f0[0], f0[1], f0[2], f0[3]), kv8_pack4<INT8>(inv, f0[4], f0[5], f0[6], f0[7]));
-    dst[a1] = make_uint2(kv8_pack4<INT8>(inv, f1[0], f1[1], f1[2], f1[3]), kv8_pack4<INT8>(inv, f1[4], f1[5], f1[6], f1[7]));
-    if (j == 0) (turned ? p.k_exps : p.v_exps)[at] = static_cast<uint8_t>(byte);
+      for (int o = kLanes / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      if (!is_q && in && slot >= 0) {
+        const uint32_t byte = kv8_exponent<INT8>(amax);
+        const float inv = kv8_inverse(byte);
+        const size_t at = kv8_row_at(p, slot, kvh);
+        uint2* dst = reinterpret_cast<uint2*>(codes + at * HD);
+        dst[a0] = make_uint2(kv8_pack4<INT8>(inv, f0[0], f0[1], f0[2], f0[3]), kv8_pack4<INT8>(inv, f0[4], f0[5], f0[6], f0[7]));
+        dst[a1] = make_uint2(kv8_pack4<INT8>(inv, f1[0], f1[1], f1[2], f1[3]), kv8_pack4<INT8>(inv, f1[4], f1[5], f1[6], f1[7]));
+        if (j == 0) exps[at] = static_cast<uint8_t>(byte);
+      }
+    }
+    if (!more) return;
+    if (++k == kAhead) {
+      __syncthreads();                               // the next angles are there, and these have been read
+      k = 0;
+      buf ^= 1;
+    }
+    tok = static_cast<int>(tok1), x0 = y0, x1 = y1, slot = slot1;
   }
 }
 
@@ -248,15 +272,22 @@ struct Kv8ReadParams {
   ZbStatus* status;
 };
 
-// A CTA takes (page, keys or values, head) after (page, ...) of all pages that the sequences hold; the sum over the sequences' pages tells
-// which one a page belongs to.  A thread has eight codes of a row: 8 bytes in, 16 bytes out.
+ZB_DEVICE void kv8_store32(void* to, const uint32_t (&x)[8]) {      // on 32 bytes
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
+               : "memory");
+}
+
+// The work is a list: keys and values of every head of the first page that the sequences hold, of the second one, and so on; a CTA takes an equal,
+// contiguous part of it.  The sum over the sequences' pages tells which one a page belongs to, looked up where the page changes.  A thread has 16
+// codes of a row, 16 bytes in and 32 bytes out, of 64 rows or fewer at once, and asks for the next ones before it writes these.
 template <int HD, bool INT8>
-__global__ void __launch_bounds__(256) zb_kv8_read_kernel(const Kv8ReadParams p) {
-  constexpr int kPieces = HD / 8;
+__global__ void __launch_bounds__(256, 4) zb_kv8_read_kernel(const Kv8ReadParams p) {
+  constexpr int kPieces = HD / 16, kRows = 256 / kPieces, kOnce = 64 / kRows;      // rows of a pass, passes of 64 rows
   zb_pdl_launch();
   zb_pdl_wait();
-  const auto pages_of = [&](int s) { return (kv8_len(p.seq_lens, s, p.max_pages * p.page_size) + p.page_size - 1) / p.page_size; };
-  const int total = kv8_total(p.batch, pages_of), items = min(total, p.out_pages) * 2 * p.hkv;
+  const int most = p.max_pages * p.page_size;
+  const auto pages_of = [&](int s) { return (kv8_len(p.seq_lens, s, most) + p.page_size - 1) / p.page_size; };
+  const int total = kv8_total(p.batch, pages_of);
   if (total > p.out_pages && blockIdx.x == 0 && threadIdx.x == 0)
     zb_record_error(p.status, ZB_ERR_BOUNDS, kKernelKv8Read, 1u, static_cast<uint32_t>(total));
   for (int s = blockIdx.x; s < p.batch; s += gridDim.x) {
@@ -264,39 +295,77 @@ __global__ void __launch_bounds__(256) zb_kv8_read_kernel(const Kv8ReadParams p)
     for (int i = threadIdx.x; i < p.max_pages; i += blockDim.x)
       p.out_table[static_cast<size_t>(s) * p.max_pages + i] = i < n && first + i < p.out_pages ? first + i : 0;
   }
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    const int to = item / (2 * p.hkv), rest = item - to * 2 * p.hkv, kv = rest / p.hkv, head = rest - kv * p.hkv;
+  // 64 rows (or a page's rest) of a head at a time
+  const int blocks = (p.page_size + 63) / 64, per_page = 2 * p.hkv * blocks;
+  const long long items = static_cast<long long>(min(total, p.out_pages)) * per_page;
+  const long long first = items * blockIdx.x / gridDim.x, last = items * (blockIdx.x + 1) / gridDim.x;
+  if (first >= last) return;
+  int left = static_cast<int>(last - first);
+  int to = static_cast<int>(first / per_page), rest = static_cast<int>(first - static_cast<long long>(to) * per_page);
+  const int row0 = threadIdx.x / kPieces, piece = threadIdx.x % kPieces;
+  int page = 0, valid = 0;
+  const auto look = [&]() {
     int seq, before;
     kv8_locate(p.batch, to, pages_of, seq, before);
-    const int nth = to - before, valid = min(p.page_size, kv8_len(p.seq_lens, seq, p.max_pages * p.page_size) - nth * p.page_size);
-    int page = p.block_table[static_cast<size_t>(seq) * p.max_pages + nth];
+    const int nth = to - before;
+    valid = min(p.page_size, kv8_len(p.seq_lens, seq, most) - nth * p.page_size);
+    page = p.block_table[static_cast<size_t>(seq) * p.max_pages + nth];
     if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(p.num_pages)) {
       if (threadIdx.x == 0) zb_record_error(p.status, ZB_ERR_BOUNDS, kKernelKv8Read, 2u, static_cast<uint32_t>(page));
       page = 0;
     }
-    const size_t from = (static_cast<size_t>(page) * p.hkv + head) * p.page_size;
-    const uint2* src = reinterpret_cast<const uint2*>((kv ? p.v_codes : p.k_codes) + from * HD);
+  };
+  look();
+  struct Rows {
+    uint4 codes[kOnce];
+    uint32_t exps[kOnce];
+    __nv_bfloat16* to;
+    int rows;                                          // of the page behind this thread's first one
+  };
+  const auto load = [&](Rows& r) {
+    const int kv = rest / (p.hkv * blocks), in = rest - kv * p.hkv * blocks, head = in / blocks, at = (in - head * blocks) * 64 + row0;
+    const size_t from = (static_cast<size_t>(page) * p.hkv + head) * p.page_size + at;
+    const uint4* src = reinterpret_cast<const uint4*>((kv ? p.v_codes : p.k_codes) + from * HD) + piece;
     const uint8_t* ex = (kv ? p.v_exps : p.k_exps) + from;
-    __nv_bfloat16* dst = (kv ? p.v_out : p.k_out) + (static_cast<size_t>(to) * p.page_size * p.hkv + head) * HD;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < p.page_size * kPieces; i += 256) {
-      const int row = i / kPieces, piece = i - row * kPieces;
-      uint4 o = make_uint4(0u, 0u, 0u, 0u);
-      if (row < valid) {
-        const uint2 w = src[i];
-        const float s = kv8_scale(ex[row]);
-        uint32_t h[4], b[4];
-        kv8_to_half<INT8>(w.x, h[0], h[1]);
-        kv8_to_half<INT8>(w.y, h[2], h[3]);
+    r.to = (kv ? p.v_out : p.k_out) + ((static_cast<size_t>(to) * p.page_size + at) * p.hkv + head) * HD + piece * 16;
+    r.rows = min(p.page_size - at, 64 - row0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
-          b[e] = zb_pack_bf16x2(v.x * s, v.y * s);
-        }
-        o = make_uint4(b[0], b[1], b[2], b[3]);
-      }
-      *reinterpret_cast<uint4*>(dst + static_cast<size_t>(row) * p.hkv * HD + piece * 8) = o;
+    for (int i = 0; i < kOnce; ++i) {
+      const bool some = at + i * kRows < valid;
+      r.codes[i] = some ? __ldcs(src + i * kRows * kPieces) : make_uint4(0u, 0u, 0u, 0u);
+      r.exps[i] = some ? ex[i * kRows] : 0u;
     }
+  };
+  Rows r;
+  load(r);
+  while (true) {
+    Rows next = r;
+    if (--left > 0) {
+      if (++rest == per_page) {
+        rest = 0;
+        ++to;
+        look();
+      }
+      load(next);
+    }
+#pragma unroll
+    for (int i = 0; i < kOnce; ++i) {
+      if (i * kRows >= r.rows) continue;
+      const float s = kv8_scale(r.exps[i]);
+      const uint32_t w[4] = {r.codes[i].x, r.codes[i].y, r.codes[i].z, r.codes[i].w};
+      uint32_t o[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t lo, hi;
+        kv8_to_half<INT8>(w[e], lo, hi);
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        o[2 * e] = zb_pack_bf16x2(a.x * s, a.y * s);
+        o[2 * e + 1] = zb_pack_bf16x2(b.x * s, b.y * s);
+      }
+      kv8_store32(r.to + static_cast<size_t>(i) * kRows * p.hkv * HD, o);
+    }
+    if (left <= 0) return;
+    r = next;
   }
 }
 
@@ -376,11 +445,11 @@ int zb_kv8_write(const ZbKv8Write* c) {
   const auto at16 = [](const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; };
   const bool aligned = c->qkv_stride % 8 == 0 && at16(c->qkv) && at16(c->q_out) && at16(c->q_norm_w) && at16(c->k_norm_w);
   if (aligned && (layout == 1 || (layout == 0 && rot_dim % 16 == 0))) {
-    const int units = (p.hq + 2 * p.hkv) * (hd / 16), parts = p.tokens <= 64 ? (units + 511) / 512 : 1;
+    const int units = (p.hq + 2 * p.hkv) * (hd / 16), parts = (units + 511) / 512;
     p.share = ((units + parts - 1) / parts + 31) / 32 * 32;
-    const int threads = p.share < 512 ? p.share : 512;
-    if (layout == 0) launch_write_hd<0>(p, c->int8 != 0, dim3(p.tokens, parts), threads, s);
-    else launch_write_hd<1>(p, c->int8 != 0, dim3(p.tokens, parts), threads, s);
+    const int grid = std::max(1, std::min(p.tokens, st->num_sms * std::min(1024 / p.share, 4) / parts));
+    if (layout == 0) launch_write_hd<0>(p, c->int8 != 0, dim3(grid, parts), p.share, s);
+    else launch_write_hd<1>(p, c->int8 != 0, dim3(grid, parts), p.share, s);
   } else if (c->int8) {
     zb_launch(zb_kv8_write_any_kernel<true>, dim3(p.tokens), dim3(256), 0, s, p);
   } else {
@@ -413,10 +482,8 @@ int zb_kv8_read(const ZbKv8Read* c) {
   p.out_pages = c->out_pages;
   p.status = st->status;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(c->stream);
-  const long long items = static_cast<long long>(c->out_pages) * 2 * c->hkv;
-  if (items > 0x7fffffffll) return -43;
-  const int most = st->num_sms * 8;
-  const dim3 grid(static_cast<unsigned>(items < 1 ? 1 : (items < most ? items : most)));
+  const long long items = static_cast<long long>(c->out_pages) * 2 * c->hkv * ((c->page_size + 63) / 64);
+  const dim3 grid(static_cast<unsigned>(std::max(1ll, std::min(items, 4ll * st->num_sms))));
   const bool int8 = c->int8 != 0;
   if (c->hd == 64) zb_launch(int8 ? zb_kv8_read_kernel<64, true> : zb_kv8_read_kernel<64, false>, grid, dim3(256), 0, s, p);
   else if (c->hd == 128) zb_launch(int8 ? zb_kv8_read_kernel<128, true> : zb_kv8_read_kernel<128, false>, grid, dim3(256), 0, s, p);
