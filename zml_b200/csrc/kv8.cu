@@ -78,12 +78,36 @@ ZB_DEVICE void kv8_unpack8(const uint4& u, float (&f)[8]) {
 // one warp and add up its squares and its largest magnitude.  A CTA takes one token after the other (its threads a part of the pieces where those are more
 // than 512): the next projection is on its way while it works on this one, and its threads form the angles of kAhead tokens at once, one or
 // two each, so that they meet once in as many tokens.
+// Numbers go in packed pairs, which halves the arithmetic (the kernel is bound by its instructions as much as by memory).
 constexpr int kAhead = 4;
+ZB_DEVICE ZbF2 kv8_pair(uint32_t bf16x2) {
+  const float2 v = zb_unpack_bf16x2(bf16x2);
+  return zb_pack2(v.x, v.y);
+}
+ZB_DEVICE uint32_t kv8_bf16x2(ZbF2 v) {
+  float x, y;
+  zb_unpack2(v, x, y);
+  return zb_pack_bf16x2(x, y);
+}
+ZB_DEVICE uint32_t kv8_abs_max(uint32_t most, ZbF2 v) {
+  float x, y;
+  zb_unpack2(v, x, y);
+  return max(most, max(kv8_abs_bits(x), kv8_abs_bits(y)));
+}
+template <bool INT8>
+ZB_DEVICE uint32_t kv8_codes4(ZbF2 inv, ZbF2 a, ZbF2 b, bool finite) {
+  float x0, x1, x2, x3;
+  zb_unpack2(zb_mul2(a, inv), x0, x1);
+  zb_unpack2(zb_mul2(b, inv), x2, x3);
+  return finite ? kv8_pack4<INT8>(1.f, x0, x1, x2, x3) : 0u;
+}
+
 template <int HD, int LAYOUT, bool INT8>
 __global__ void __launch_bounds__(512, 2) zb_kv8_write_kernel(const Kv8WriteParams p) {
   constexpr int kLanes = HD / 16, kHalf = HD / 2;
   // cosines and sines; angle i lies where a thread's eight are two pieces of 16 bytes, neighbouring threads' beside each other
   __shared__ __align__(16) float cs[2][kAhead][kHalf], sn[2][kAhead][kHalf];
+  __shared__ __align__(16) float weights[2][HD];       // of queries' and keys' norms
   zb_pdl_launch();
   zb_pdl_wait();
   const int half = p.rot_dim >> 1;
@@ -95,11 +119,7 @@ __global__ void __launch_bounds__(512, 2) zb_kv8_write_kernel(const Kv8WritePara
   const int a1 = LAYOUT == 0 && turns ? j + half / 8 : a0 + 1;
   const bool any_kv = __any_sync(0xffffffffu, !is_q);
   const uint4* src = reinterpret_cast<const uint4*>(p.qkv + static_cast<size_t>(h) * HD);
-  const __nv_bfloat16* nw = !turned ? nullptr : (is_q ? p.q_norm_w : p.k_norm_w);
-  const bool normed = p.q_norm_w != nullptr || p.k_norm_w != nullptr;
-  uint4 w0 = make_uint4(0u, 0u, 0u, 0u), w1 = w0;
-  if (nw != nullptr) w0 = reinterpret_cast<const uint4*>(nw)[a0], w1 = reinterpret_cast<const uint4*>(nw)[a1];
-  const float one = p.norm_unit_offset ? 1.f : 0.f;
+  const bool normed = turned && (is_q ? p.q_norm_w : p.k_norm_w) != nullptr, any_normed = __any_sync(0xffffffffu, normed);
   const int kvh = turned ? h - p.hq : h - p.hq - p.hkv;
   uint8_t* const codes = turned ? p.k_codes : p.v_codes;
   uint8_t* const exps = turned ? p.k_exps : p.v_exps;
@@ -117,6 +137,10 @@ __global__ void __launch_bounds__(512, 2) zb_kv8_write_kernel(const Kv8WritePara
   size_t row = static_cast<size_t>(tok) * p.qkv_stride / 8;
   uint4 x0 = src[row + a0], x1 = src[row + a1];
   long long slot = kv8_slot(p, tok);
+  for (int i = threadIdx.x; i < 2 * HD; i += blockDim.x) {
+    const __nv_bfloat16* w = i < HD ? p.q_norm_w : p.k_norm_w;
+    if (w != nullptr) weights[i / HD][i % HD] = __bfloat162float(w[i % HD]) + (p.norm_unit_offset ? 1.f : 0.f);
+  }
   angles(tok, 0);
   __syncthreads();
   while (true) {
@@ -130,60 +154,76 @@ __global__ void __launch_bounds__(512, 2) zb_kv8_write_kernel(const Kv8WritePara
       slot1 = kv8_slot(p, static_cast<int>(tok1));
       if (k == 0 && tok + static_cast<long long>(kAhead) * gridDim.x < p.tokens) angles(tok + kAhead * static_cast<int>(gridDim.x), buf ^ 1);
     }
-    float f0[8], f1[8];
-    kv8_unpack8(x0, f0);
-    kv8_unpack8(x1, f1);
-    if (normed) {
-      float ss = 0.f;
+    ZbF2 f0[4] = {kv8_pair(x0.x), kv8_pair(x0.y), kv8_pair(x0.z), kv8_pair(x0.w)}, f1[4] = {kv8_pair(x1.x), kv8_pair(x1.y), kv8_pair(x1.z), kv8_pair(x1.w)};
+    if (any_normed) {
+      ZbF2 sum = zb_mul2(f0[0], f0[0]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += f0[i] * f0[i] + f1[i] * f1[i];
+      for (int i = 1; i < 4; ++i) sum = zb_fma2(f0[i], f0[i], sum);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum = zb_fma2(f1[i], f1[i], sum);
+      float ss = zb_sum2(sum);
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (nw != nullptr) {
+      if (normed) {
         const float inv = rsqrtf(ss / static_cast<float>(HD) + p.norm_eps);
-        float g0[8], g1[8];
-        kv8_unpack8(w0, g0);
-        kv8_unpack8(w1, g1);
+        const ZbF2 by = zb_pack2(inv, inv);
+        const ulonglong2* w = reinterpret_cast<const ulonglong2*>(weights[is_q ? 0 : 1]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          f0[i] = f0[i] * inv * (g0[i] + one);
-          f1[i] = f1[i] * inv * (g1[i] + one);
+        for (int i = 0; i < 2; ++i) {
+          const ulonglong2 g0 = w[2 * a0 + i], g1 = w[2 * a1 + i];
+          f0[2 * i] = zb_mul2(zb_mul2(f0[2 * i], by), g0.x), f0[2 * i + 1] = zb_mul2(zb_mul2(f0[2 * i + 1], by), g0.y);
+          f1[2 * i] = zb_mul2(zb_mul2(f1[2 * i], by), g1.x), f1[2 * i + 1] = zb_mul2(zb_mul2(f1[2 * i + 1], by), g1.y);
         }
       }
     }
     if (turns) {
-      const float4 c0 = *reinterpret_cast<const float4*>(&cs[buf][k][4 * j]), c1 = *reinterpret_cast<const float4*>(&cs[buf][k][kHalf / 2 + 4 * j]);
-      const float4 s0 = *reinterpret_cast<const float4*>(&sn[buf][k][4 * j]), s1 = *reinterpret_cast<const float4*>(&sn[buf][k][kHalf / 2 + 4 * j]);
-      const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float& x = LAYOUT == 0 ? f0[i] : (i < 4 ? f0[2 * i] : f1[2 * i - 8]);
-        float& y = LAYOUT == 0 ? f1[i] : (i < 4 ? f0[2 * i + 1] : f1[2 * i - 7]);
-        if (LAYOUT == 0 || 8 * j + i < half) {
-          const float a = x, b = y;
-          x = a * c[i] - b * s[i];
-          y = b * c[i] + a * s[i];
+      for (int q = 0; q < 2; ++q) {
+        const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(&cs[buf][k][q * (kHalf / 2) + 4 * j]), s = *reinterpret_cast<const ulonglong2*>(&sn[buf][k][q * (kHalf / 2) + 4 * j]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const ZbF2 ci = i ? c.y : c.x, si = i ? s.y : s.x;
+          if (LAYOUT == 0) {
+            ZbF2& x = f0[2 * q + i];
+            ZbF2& y = f1[2 * q + i];
+            const ZbF2 a = x, b = y;
+            x = zb_fma2(a, ci, zb_mul2(b, si ^ 0x8000000080000000ull));
+            y = zb_fma2(b, ci, zb_mul2(a, si));
+          } else {
+            float c0, c1, s0, s1, a, b;
+            zb_unpack2(ci, c0, c1);
+            zb_unpack2(si, s0, s1);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              ZbF2& v = q == 0 ? f0[2 * i + e] : f1[2 * i + e];
+              zb_unpack2(v, a, b);
+              const float cc = e ? c1 : c0, ss = e ? s1 : s0;
+              if (8 * j + 4 * q + 2 * i + e < half) v = zb_pack2(a * cc - b * ss, b * cc + a * ss);
+            }
+          }
         }
       }
     }
     if (is_q && in) {
       uint4* dst = reinterpret_cast<uint4*>(p.q_out + (static_cast<size_t>(tok) * p.hq + h) * HD);
-      dst[a0] = make_uint4(zb_pack_bf16x2(f0[0], f0[1]), zb_pack_bf16x2(f0[2], f0[3]), zb_pack_bf16x2(f0[4], f0[5]), zb_pack_bf16x2(f0[6], f0[7]));
-      dst[a1] = make_uint4(zb_pack_bf16x2(f1[0], f1[1]), zb_pack_bf16x2(f1[2], f1[3]), zb_pack_bf16x2(f1[4], f1[5]), zb_pack_bf16x2(f1[6], f1[7]));
+      dst[a0] = make_uint4(kv8_bf16x2(f0[0]), kv8_bf16x2(f0[1]), kv8_bf16x2(f0[2]), kv8_bf16x2(f0[3]));
+      dst[a1] = make_uint4(kv8_bf16x2(f1[0]), kv8_bf16x2(f1[1]), kv8_bf16x2(f1[2]), kv8_bf16x2(f1[3]));
     }
     if (any_kv) {
       uint32_t amax = 0u;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) amax = max(amax, max(kv8_abs_bits(f0[i]), kv8_abs_bits(f1[i])));
+      for (int i = 0; i < 4; ++i) amax = kv8_abs_max(kv8_abs_max(amax, f0[i]), f1[i]);
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
       if (!is_q && in && slot >= 0) {
         const uint32_t byte = kv8_exponent<INT8>(amax);
-        const float inv = kv8_inverse(byte);
+        const bool finite = byte != 255u;
+        const float by = kv8_inverse(byte);
+        const ZbF2 inv = zb_pack2(by, by);
         const size_t at = kv8_row_at(p, slot, kvh);
         uint2* dst = reinterpret_cast<uint2*>(codes + at * HD);
-        dst[a0] = make_uint2(kv8_pack4<INT8>(inv, f0[0], f0[1], f0[2], f0[3]), kv8_pack4<INT8>(inv, f0[4], f0[5], f0[6], f0[7]));
-        dst[a1] = make_uint2(kv8_pack4<INT8>(inv, f1[0], f1[1], f1[2], f1[3]), kv8_pack4<INT8>(inv, f1[4], f1[5], f1[6], f1[7]));
+        dst[a0] = make_uint2(kv8_codes4<INT8>(inv, f0[0], f0[1], finite), kv8_codes4<INT8>(inv, f0[2], f0[3], finite));
+        dst[a1] = make_uint2(kv8_codes4<INT8>(inv, f1[0], f1[1], finite), kv8_codes4<INT8>(inv, f1[2], f1[3], finite));
         if (j == 0) exps[at] = static_cast<uint8_t>(byte);
       }
     }
@@ -277,12 +317,34 @@ ZB_DEVICE void kv8_store32(void* to, const uint32_t (&x)[8]) {      // on 32 byt
                : "memory");
 }
 
+// Two codes' values times a power of two, in bf16: exact.  `from`: which bytes of a word.
+template <bool INT8>
+ZB_DEVICE void kv8_to_bf16(uint32_t w, float scale, uint32_t& lo, uint32_t& hi) {
+  const ZbF2 by = zb_pack2(scale, scale);
+  if constexpr (INT8) {
+    // byte u = code + 128 in the last place of 2^23, from which the 2^23 + 128 is taken again as the scale is multiplied
+    const uint32_t u = w ^ 0x80808080u;
+    const float off = -8388736.f * scale;
+    const ZbF2 less = zb_pack2(off, off);
+    lo = kv8_bf16x2(zb_fma2(zb_pack2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441))), by, less));
+    hi = kv8_bf16x2(zb_fma2(zb_pack2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443))), by, less));
+  } else {
+    uint32_t a, b;
+    kv8_to_half<false>(w, a, b);
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a)), y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+    lo = kv8_bf16x2(zb_mul2(zb_pack2(x.x, x.y), by));
+    hi = kv8_bf16x2(zb_mul2(zb_pack2(y.x, y.y), by));
+  }
+}
+
 // The work is a list: keys and values of every head of the first page that the sequences hold, of the second one, and so on; a CTA takes an equal,
 // contiguous part of it.  The sum over the sequences' pages tells which one a page belongs to, looked up where the page changes.  A thread has 16
-// codes of a row, 16 bytes in and 32 bytes out, of 64 rows or fewer at once, and asks for the next ones before it writes these.
+// codes of a row, 16 bytes in and 32 bytes out, of 64 rows or fewer at once (heads of up to 128: of the keys and the values), and asks for the
+// next ones before it writes these.
 template <int HD, bool INT8>
-__global__ void __launch_bounds__(256, 4) zb_kv8_read_kernel(const Kv8ReadParams p) {
+__global__ void __launch_bounds__(256, HD == 64 ? 5 : 4) zb_kv8_read_kernel(const Kv8ReadParams p) {
   constexpr int kPieces = HD / 16, kRows = 256 / kPieces, kOnce = 64 / kRows;      // rows of a pass, passes of 64 rows
+  constexpr int kBoth = HD <= 128 ? 2 : 1;
   zb_pdl_launch();
   zb_pdl_wait();
   const int most = p.max_pages * p.page_size;
@@ -296,12 +358,13 @@ __global__ void __launch_bounds__(256, 4) zb_kv8_read_kernel(const Kv8ReadParams
       p.out_table[static_cast<size_t>(s) * p.max_pages + i] = i < n && first + i < p.out_pages ? first + i : 0;
   }
   // 64 rows (or a page's rest) of a head at a time
-  const int blocks = (p.page_size + 63) / 64, per_page = 2 * p.hkv * blocks;
+  const int blocks = (p.page_size + 63) / 64, per_page = (2 / kBoth) * p.hkv * blocks;
   const long long items = static_cast<long long>(min(total, p.out_pages)) * per_page;
   const long long first = items * blockIdx.x / gridDim.x, last = items * (blockIdx.x + 1) / gridDim.x;
   if (first >= last) return;
   int left = static_cast<int>(last - first);
   int to = static_cast<int>(first / per_page), rest = static_cast<int>(first - static_cast<long long>(to) * per_page);
+  int kv = rest / (p.hkv * blocks), head = (rest - kv * p.hkv * blocks) / blocks, block = rest - (kv * p.hkv + head) * blocks;
   const int row0 = threadIdx.x / kPieces, piece = threadIdx.x % kPieces;
   int page = 0, valid = 0;
   const auto look = [&]() {
@@ -317,23 +380,27 @@ __global__ void __launch_bounds__(256, 4) zb_kv8_read_kernel(const Kv8ReadParams
   };
   look();
   struct Rows {
-    uint4 codes[kOnce];
-    uint32_t exps[kOnce];
-    __nv_bfloat16* to;
-    int rows;                                          // of the page behind this thread's first one
+    uint4 codes[kBoth][kOnce];
+    uint32_t exps[kBoth][kOnce];
+    size_t to;                                         // element of the outputs
+    int kv, rows;                                      // rows of the page behind this thread's first one
   };
   const auto load = [&](Rows& r) {
-    const int kv = rest / (p.hkv * blocks), in = rest - kv * p.hkv * blocks, head = in / blocks, at = (in - head * blocks) * 64 + row0;
+    const int at = block * 64 + row0;
     const size_t from = (static_cast<size_t>(page) * p.hkv + head) * p.page_size + at;
-    const uint4* src = reinterpret_cast<const uint4*>((kv ? p.v_codes : p.k_codes) + from * HD) + piece;
-    const uint8_t* ex = (kv ? p.v_exps : p.k_exps) + from;
-    r.to = (kv ? p.v_out : p.k_out) + ((static_cast<size_t>(to) * p.page_size + at) * p.hkv + head) * HD + piece * 16;
+    r.to = ((static_cast<size_t>(to) * p.page_size + at) * p.hkv + head) * HD + piece * 16;
+    r.kv = kv;
     r.rows = min(p.page_size - at, 64 - row0);
 #pragma unroll
-    for (int i = 0; i < kOnce; ++i) {
-      const bool some = at + i * kRows < valid;
-      r.codes[i] = some ? __ldcs(src + i * kRows * kPieces) : make_uint4(0u, 0u, 0u, 0u);
-      r.exps[i] = some ? ex[i * kRows] : 0u;
+    for (int b = 0; b < kBoth; ++b) {
+      const uint4* src = reinterpret_cast<const uint4*>((kv + b ? p.v_codes : p.k_codes) + from * HD) + piece;
+      const uint8_t* ex = (kv + b ? p.v_exps : p.k_exps) + from;
+#pragma unroll
+      for (int i = 0; i < kOnce; ++i) {
+        const bool some = at + i * kRows < valid;
+        r.codes[b][i] = some ? __ldcs(src + i * kRows * kPieces) : make_uint4(0u, 0u, 0u, 0u);
+        r.exps[b][i] = some ? ex[i * kRows] : 0u;
+      }
     }
   };
   Rows r;
@@ -341,29 +408,32 @@ __global__ void __launch_bounds__(256, 4) zb_kv8_read_kernel(const Kv8ReadParams
   while (true) {
     Rows next = r;
     if (--left > 0) {
-      if (++rest == per_page) {
-        rest = 0;
-        ++to;
-        look();
+      if (++block == blocks) {
+        block = 0;
+        if (++head == p.hkv) {
+          head = 0;
+          if (++kv == 2 / kBoth) {
+            kv = 0;
+            ++to;
+            look();
+          }
+        }
       }
       load(next);
     }
 #pragma unroll
-    for (int i = 0; i < kOnce; ++i) {
-      if (i * kRows >= r.rows) continue;
-      const float s = kv8_scale(r.exps[i]);
-      const uint32_t w[4] = {r.codes[i].x, r.codes[i].y, r.codes[i].z, r.codes[i].w};
-      uint32_t o[8];
+    for (int b = 0; b < kBoth; ++b)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t lo, hi;
-        kv8_to_half<INT8>(w[e], lo, hi);
-        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-        o[2 * e] = zb_pack_bf16x2(a.x * s, a.y * s);
-        o[2 * e + 1] = zb_pack_bf16x2(b.x * s, b.y * s);
+      for (int i = 0; i < kOnce; ++i) {
+        if (i * kRows >= r.rows) continue;
+        const float s = kv8_scale(r.exps[b][i]);
+        uint32_t o[8];
+        kv8_to_bf16<INT8>(r.codes[b][i].x, s, o[0], o[1]);
+        kv8_to_bf16<INT8>(r.codes[b][i].y, s, o[2], o[3]);
+        kv8_to_bf16<INT8>(r.codes[b][i].z, s, o[4], o[5]);
+        kv8_to_bf16<INT8>(r.codes[b][i].w, s, o[6], o[7]);
+        kv8_store32((r.kv + b ? p.v_out : p.k_out) + r.to + static_cast<size_t>(i) * kRows * p.hkv * HD, o);
       }
-      kv8_store32(r.to + static_cast<size_t>(i) * kRows * p.hkv * HD, o);
-    }
     if (left <= 0) return;
     r = next;
   }
@@ -483,7 +553,7 @@ int zb_kv8_read(const ZbKv8Read* c) {
   p.status = st->status;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(c->stream);
   const long long items = static_cast<long long>(c->out_pages) * 2 * c->hkv * ((c->page_size + 63) / 64);
-  const dim3 grid(static_cast<unsigned>(std::max(1ll, std::min(items, 4ll * st->num_sms))));
+  const dim3 grid(static_cast<unsigned>(std::max(1ll, std::min(c->hd == 256 ? items : items / 2, (c->hd == 64 ? 5ll : 4ll) * st->num_sms))));
   const bool int8 = c->int8 != 0;
   if (c->hd == 64) zb_launch(int8 ? zb_kv8_read_kernel<64, true> : zb_kv8_read_kernel<64, false>, grid, dim3(256), 0, s, p);
   else if (c->hd == 128) zb_launch(int8 ? zb_kv8_read_kernel<128, true> : zb_kv8_read_kernel<128, false>, grid, dim3(256), 0, s, p);
