@@ -3,11 +3,11 @@
 
     python examples/llm/main.py --model=<repo dir | .safetensors | index.json | hf://org/repo | s3://... | gs://... | https://...> [--prompt=...]
         [--system=...] [--seqlen=2048] [--topk=1] [--temperature=1.0] [--seed=0] [--no-chat-template] [--profile]
-        [--backend=b200|vanilla|attnd] [--attnd-ip=IP:PORT]
+        [--backend=b200|vanilla|attnd] [--attnd-ip=IP:PORT] [--kv-cache=fp8|int8]
 
 --backend picks the attention implementation (default: this library's paged kernels; `vanilla` is PyTorch SDPA on K/V
 gathered from the pages); --attnd-ip registers a remote attention daemon at IP:PORT and prefers it (dense decoder
-models, one conversation).  --system puts a system message in front of the first turn (chat template only).
+models, one conversation).  --kv-cache holds keys and values in 8 bits, half the memory of bf16.  --system puts a system message in front of the first turn (chat template only).
 
 Without --prompt an interactive chat loop starts (history in ~/.llm_chat_history).  For
 tensor / expert parallelism launch one process per GPU:
@@ -52,6 +52,7 @@ class Args:
     cpu: bool = False
     backend: Optional[str] = None
     attnd_ip: Optional[str] = None
+    kv_cache: Optional[str] = None
     help = __doc__
 
 
@@ -157,9 +158,11 @@ def main(argv=None) -> int:
         model.set_attention_backend(backend, addr)
         log.info("attention backend: %s%s", backend, f" at {addr[0]}:{addr[1]}" if addr else "")
     page = 64
+    if args.kv_cache and backend != "b200":
+        raise SystemExit(f"--kv-cache={args.kv_cache} goes with the b200 backend")
     engine = Engine(model, num_pages=(args.seqlen + page - 1) // page + 2, page_size=page, max_batch=1,
                     max_seq_len=args.seqlen, max_prefill_tokens=min(8192, args.seqlen),
-                    use_graphs=False if backend == "attnd" else None)     # the daemon is reached from the host: no graph
+                    use_graphs=False if backend == "attnd" else None, kv_dtype=args.kv_cache)     # the daemon is reached from the host: no graph
     strategy = SamplingStrategy(topk=args.topk, temperature=args.temperature)
     session = Session(engine, args.seqlen, strategy, cfg.eos_ids(), args.seed)
     template = None if args.no_chat_template or tok is None else hub.chat_template(getattr(cfg, "model_type", "llama"))

@@ -42,6 +42,7 @@ class Args:
     topk: int = 1
     temperature: float = 1.0
     window_ms: float = 20.0
+    kv_cache: Optional[str] = None      # fp8 or int8: the key / value cache in 8 bits
     cpu: bool = False
     help = __doc__
 
@@ -57,7 +58,7 @@ def main(argv=None) -> int:
     cfg = model.config
     page = 64 if device.type == "cuda" else 16
     pages = args.pages or args.max_batch * ((args.seqlen + page - 1) // page) + 1
-    engine = Engine(model, num_pages=pages, page_size=page, max_batch=args.max_batch, max_seq_len=args.seqlen)
+    engine = Engine(model, num_pages=pages, page_size=page, max_batch=args.max_batch, max_seq_len=args.seqlen, kv_dtype=args.kv_cache)
     eos = cfg.eos_ids() if hasattr(cfg, "eos_ids") else []
     server = Server(engine, tok, comm, model_name=os.path.basename(args.model.rstrip("/")),
                     template=hub.chat_template(getattr(cfg, "model_type", "llama")), bos=getattr(cfg, "bos_token_id", None),

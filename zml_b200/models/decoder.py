@@ -35,6 +35,15 @@ class AttnMeta:
     max_q_len: Optional[int] = None               # new tokens of the longest sequence (prefill)
     plans: dict = field(default_factory=dict)     # what the layers derive from this step's metadata once (by their own keys)
 
+    def kv_pages(self, page_size: int) -> Optional[int]:
+        """Pages that the sequences of a varlen batch hold together, where their lengths are known on the host."""
+        if self.seq_lens_host is None:
+            return None
+        n = self.plans.get(("kv_pages", page_size))
+        if n is None:
+            n = self.plans[("kv_pages", page_size)] = sum(-(-x // page_size) for x in self.seq_lens_host)
+        return n
+
 
 class DecoderModel:
     """Base of the decoder models: one tensor-parallel rank.  A model provides `hidden_states(ids, meta, kv_cache)` and
@@ -44,6 +53,8 @@ class DecoderModel:
     KERNEL_SOURCES: Optional[tuple] = None
     # True when the model's kernels also run in fp32 on the GPU
     FP32_ON_GPU = False
+    # True when the model's attention also takes a key / value cache in 8 bits (`ops.kv8`)
+    QUANT_KV = False
     # True: varlen batches (prompts and portions of them) run without programmatic dependent launch
     SERIAL_PREFILL = False
 
@@ -66,6 +77,15 @@ class DecoderModel:
     def alloc_kv_cache(self, num_pages: int, page_size: int):
         """The paged cache, as `hidden_states` takes it."""
         return torch.zeros(self.kv_cache_shape(num_pages, page_size), dtype=self.dtype, device=self.device)
+
+    def alloc_quant_kv_cache(self, num_pages: int, page_size: int, dtype):
+        """The paged cache in 8 bits: `dtype` is "fp8" or "int8" (`ops.kv8`)."""
+        if not self.QUANT_KV:
+            raise ValueError(f"{type(self).__name__} has no key / value cache in 8 bits")
+        if self.dtype != torch.bfloat16:
+            raise ValueError(f"a key / value cache in 8 bits goes with bfloat16 models, not {self.dtype}")
+        layers, two, pages, page, heads, hd = self.kv_cache_shape(num_pages, page_size)
+        return ops.QuantKVCache(layers, pages, page, heads, hd, ops.kv8.kv_dtype(dtype), self.device)
 
     def decode_splits(self, batch: int, max_seq_len: int) -> int:
         """KV chunks per sequence of a decode step (part of the key of captured graphs)."""

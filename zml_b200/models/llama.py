@@ -128,6 +128,7 @@ class LayerWeights:
 
 class LlamaModel(DecoderModel):
     """Weights of one tensor-parallel rank plus the forward pass over a flattened token batch."""
+    QUANT_KV = True
 
     def __init__(self, config: LlamaConfig, comm: Optional[Comm] = None, device="cpu",
                  dtype=torch.bfloat16):
@@ -359,6 +360,9 @@ class LlamaModel(DecoderModel):
 
     def attention_from_qkv(self, lw: LayerWeights, qkv, meta: AttnMeta, kc, vc):
         c = self.config
+        quant = isinstance(kc, ops.QuantKV)
+        if quant and self.attn_backend != "b200":
+            raise ValueError(f"the {self.attn_backend} backend does not read a key / value cache in 8 bits")
         if self.attn_backend == "attnd":
             return self._attention_attnd(lw, qkv, meta)
         q = ops.rope_kvwrite(qkv, meta.positions, meta.slot_mapping, self.inv_freq, kc, vc, self.hq,
@@ -368,8 +372,9 @@ class LlamaModel(DecoderModel):
         if self.attn_backend == "vanilla":
             from ..ops import baseline as impl
         if meta.is_prefill:
+            more = {"kv_pages": meta.kv_pages(kc.page_size)} if quant else {}
             a = impl.paged_prefill(q, kc, vc, meta.block_table, meta.seq_lens, meta.q_start,
-                                   window=c.sliding_window, total_q_blocks=meta.total_q_blocks, max_seq_len=meta.max_seq_len)
+                                   window=c.sliding_window, total_q_blocks=meta.total_q_blocks, max_seq_len=meta.max_seq_len, **more)
         else:
             a = impl.paged_decode(q, kc, vc, meta.block_table, meta.seq_lens, window=c.sliding_window,
                                   num_splits=meta.num_splits, max_seq_len=meta.max_seq_len)

@@ -385,8 +385,9 @@ class Qwen35Model(LlamaModel):
                              self.hkv, c.hd, self.rope_layout, self.rot_dim, 1.0, lw.q_norm, lw.k_norm,
                              c.rms_norm_eps, True)
         if meta.is_prefill:
+            more = {"kv_pages": meta.kv_pages(kc.page_size)} if isinstance(kc, ops.QuantKV) else {}
             a = ops.paged_prefill(q, kc, vc, meta.block_table, meta.seq_lens, meta.q_start,
-                                  total_q_blocks=meta.total_q_blocks, max_seq_len=meta.max_seq_len)
+                                  total_q_blocks=meta.total_q_blocks, max_seq_len=meta.max_seq_len, **more)
         else:
             a = ops.paged_decode(q, kc, vc, meta.block_table, meta.seq_lens, num_splits=meta.num_splits,
                                  max_seq_len=meta.max_seq_len)

@@ -43,6 +43,8 @@ def rmsnorm(x, weight, eps=1e-5, residual=None, unit_offset=False, out=None):
 
 def rope_kvwrite(qkv, positions, slot_mapping, inv_freq, k_cache, v_cache, hq, hkv, hd, layout=0, rot_dim=None,
                  attn_factor=1.0, q_norm_w=None, k_norm_w=None, norm_eps=1e-6, norm_unit_offset=False, q_out=None):
+    if not isinstance(k_cache, torch.Tensor):
+        raise TypeError("this path has no key / value cache in 8 bits")
     t = qkv.shape[0]
     q, k, v = qkv.split([hq * hd, hkv * hd, hkv * hd], dim=-1)
     q, k, v = q.reshape(t, hq, hd), k.reshape(t, hkv, hd), v.reshape(t, hkv, hd)

@@ -328,13 +328,24 @@ def _plan(index, b, hq, hkv, hd, max_len) -> tuple[int, int]:
 
 
 _TICKETS: dict = {}
+_CAPTURED: dict = {}
+CAPTURED_TICKETS = 1 << 20
 
 
 def _tickets(q, index: int, stream: int, n: int):
     """At least n zeros (int32) that no other call in flight uses; the kernel leaves zeros behind.  The calls of one stream follow one another and
-    share theirs; a captured call has its own, cleared by every replay, since graphs may be replayed on any streams."""
+    share theirs.  Graphs may be replayed on any streams, so a captured call has its own for good: a piece of a stock that an earlier eager call
+    has cleared, or, where there is none or it has come to an end, an allocation that every replay clears."""
     if _capturing():
-        return q.new_zeros((n,), dtype=torch.int32)
+        stock = _CAPTURED.get(index)
+        if stock is None or stock[1] + n > CAPTURED_TICKETS:
+            return q.new_zeros((n,), dtype=torch.int32)
+        stock[1] += n
+        return stock[0][stock[1] - n:stock[1]]
+    if index not in _CAPTURED:
+        stock = q.new_zeros((CAPTURED_TICKETS,), dtype=torch.int32)
+        torch.cuda.current_stream(index).synchronize()                       # whatever stream replays
+        _CAPTURED[index] = [stock, 0]
     got = _TICKETS.get((index, stream))
     if got is None or got.numel() < n:
         if len(_TICKETS) >= 256:
@@ -372,7 +383,7 @@ def paged_decode(q, k: QuantKV, v: QuantKV, block_table, seq_lens, scale: Option
     work = tickets = 0
     if numbers:                                                              # the parts of a list leave sums, and draw tickets
         partial = q.new_empty((numbers,), dtype=torch.float32)
-        ticket = _tickets(q, index, stream, b * hq)
+        ticket = _tickets(q, index, stream, b * hkv * -(-hq // (8 * hkv)))
         work, tickets = partial.data_ptr(), ticket.data_ptr()
     kc = k._codes
     rc = _lib.lib().zb_kv8_decode(_DECODE(

@@ -106,7 +106,8 @@ def _bucket(n: int) -> int:
 class Engine:
     def __init__(self, model, num_pages: int, page_size: int = 64, max_batch: int = 64,
                  max_seq_len: int = 4096, max_prefill_tokens: int = 8192, use_graphs: Optional[bool] = None,
-                 history_steps: int = 1024, num_state_slots: Optional[int] = None):
+                 history_steps: int = 1024, num_state_slots: Optional[int] = None, kv_dtype: Optional[str] = None):
+        """`kv_dtype`: "fp8" or "int8" for a key / value cache in 8 bits (`ops.kv8`), about half the memory of the model's dtype."""
         self.model = model
         self.device = model.device
         self.page_size = page_size
@@ -115,7 +116,7 @@ class Engine:
         self.max_pages = (max_seq_len + page_size - 1) // page_size
         self.max_prefill_tokens = max_prefill_tokens
         self.pool = PagePool(num_pages)
-        self.kv_cache = model.alloc_kv_cache(num_pages, page_size)
+        self.kv_cache = model.alloc_kv_cache(num_pages, page_size) if kv_dtype is None else model.alloc_quant_kv_cache(num_pages, page_size, kv_dtype)
         self.on_gpu = self.device.type == "cuda"
         self.use_graphs = self.on_gpu if use_graphs is None else (use_graphs and self.on_gpu)
         self.history_steps = history_steps
