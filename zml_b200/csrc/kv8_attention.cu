@@ -21,7 +21,7 @@
 // * The reference that scores are taken from, and that of the values' scales, move only when a score exceeds its reference by 2^8 or a scale its own:
 //   the weights stay below 2^15, and a warp looks for that with one vote, where keeping the very maximum takes three shuffles a column
 //   and a multiplication of all accumulators nearly every time.
-// * Every warp has a ring of tiles of 32 keys of its own and waits for nobody while it streams; the sums of a CTA's four warps (two, for heads of 256)
+// * Every warp has a ring of tiles of 32 keys (heads of 256: 16) of its own and waits for nobody while it streams; the sums of a CTA's four warps
 //   meet in shared memory in the end.  (One ring for eight warps, fed by tensor-map copies: 130 clocks an SM for each of a tile's four copies, and
 //   2 us at each end of a pair in which the SM's memory stood still.  CTAs that walk over equal parts of a list of all tiles: even, but nearly every
 //   pair is cut, and a CTA that joins one or begins another stands still for 3 us.  128 x 1024 keys of 4 heads: 39 and 36 us, now 28.)
@@ -40,7 +40,6 @@
 namespace {
 
 constexpr uint32_t kKernelKv8Decode = 41;
-constexpr int kTile = 32;                       // keys
 constexpr int kMaxBatch = 8192;                 // sequences whose lengths a CTA looks at: beyond, pairs are not cut
 constexpr int kMinChunk = 8;                    // tiles: two for each warp
 constexpr float kNoScore = -3.402823466e38f;    // the reference in front of the first key
@@ -100,19 +99,29 @@ ZB_DEVICE uint2 lds64(uint32_t at) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
   return v;
 }
+ZB_DEVICE uint32_t lds16(uint32_t at) {
+  uint32_t v;
+  asm volatile("{.reg .b16 h; ld.shared.u16 h, [%1]; cvt.u32.u16 %0, h;}" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
 ZB_DEVICE uint32_t lds32(uint32_t at) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
   return v;
 }
 
-// Key (of a warp's 32) in row `g` of the idx-th group of eight rows.  Four keys of a thread are neighbours, one word of exponents; in the low bits,
-// rows g = 2 i and 2 i + 1 differ so that their pieces of S^T's operand lie in different halves of the banks, and rows g = 2 t (or 2 t + 1) over
-// t so that eight lanes of O^T's operand meet eight banks.
+// Keys of a tile: two groups of eight rows of an operand's 16, twice that for heads of up to 128.
+template <int HD>
+constexpr int kv8_groups() { return HD == 256 ? 2 : 4; }
+
+// Key of a tile in row `g` of the idx-th group of eight rows.  A thread's keys are neighbours, one word of exponents; in the low bits, rows
+// g = 2 i and 2 i + 1 differ so that their pieces of S^T's operand lie in different halves of the banks, and rows g = 2 t (or 2 t + 1) over t
+// so that eight lanes of O^T's operand meet eight banks.
 template <int HD>
 ZB_DEVICE int kv8_key(int g, int idx) {
   if constexpr (HD == 64) return 4 * ((g & 4) | ((((g >> 2) ^ g) & 1) << 1) | ((g >> 1) & 1)) + idx;
-  else return 4 * (g ^ ((g >> 1) & 1)) + (idx ^ (2 * (g >> 2)));
+  else if constexpr (HD == 128) return 4 * (g ^ ((g >> 1) & 1)) + (idx ^ (2 * (g >> 2)));
+  else return 2 * (((g & 1) << 2) | (((g ^ (g >> 1)) & 1) << 1) | (g >> 2)) + idx;
 }
 // What the idx-th key's offset in a swizzled tile differs from the first one's by.
 template <int HD>
@@ -164,6 +173,7 @@ ZB_DEVICE void copies_wait() {
 struct Kv8Span {
   int len, first, tile0, tiles;      // keys first .. len - 1, in tiles tile0 .. tile0 + tiles - 1
 };
+template <int kTile>
 ZB_DEVICE Kv8Span kv8_span(const Kv8DecodeParams& p, int seq) {
   Kv8Span s;
   s.len = kv8_len(p.seq_lens, seq, p.max_pages * p.page_size);
@@ -185,9 +195,10 @@ ZB_DEVICE void kv8_cut(Kv8Work& w) {
   w.end = w.begin + each + (w.nth < longer ? 1 : 0);
 }
 // false: there are fewer chunks.  `tiles`: shared memory for a number of each sequence.
+template <int kTile>
 ZB_DEVICE bool kv8_work(const Kv8DecodeParams& p, Kv8Work& w, int* tiles) {
   const int pairs = p.hkv * p.blocks;
-  for (int s = threadIdx.x; s < p.batch; s += blockDim.x) tiles[s] = kv8_span(p, s).tiles;
+  for (int s = threadIdx.x; s < p.batch; s += blockDim.x) tiles[s] = kv8_span<kTile>(p, s).tiles;
   __syncthreads();
   const int total = kv8_total(p.batch, [&](int s) { return tiles[s]; });
   int length = 0, chunks = 0;
@@ -219,7 +230,7 @@ ZB_DEVICE bool kv8_work(const Kv8DecodeParams& p, Kv8Work& w, int* tiles) {
   if (at >= chunks) return false;
   int before;
   kv8_locate(p.batch, at, [&](int s) { return chunks_of(s) * pairs; }, w.seq, before);
-  w.span = kv8_span(p, w.seq);
+  w.span = kv8_span<kTile>(p, w.seq);
   w.chunks = chunks_of(w.seq);
   w.pair = (at - before) / w.chunks;
   w.nth = (at - before) - w.pair * w.chunks;
@@ -236,21 +247,23 @@ ZB_DEVICE bool kv8_work(const Kv8DecodeParams& p, Kv8Work& w, int* tiles) {
 
 template <int HD, int NB>
 struct Kv8Sizes {
+  static constexpr int kGroups = kv8_groups<HD>(), kTile = 8 * kGroups;      // keys of a tile
   static constexpr int kTileBytes = kTile * HD;
   static constexpr int kStageBytes = 2 * kTileBytes;
   static constexpr int kStages = HD == 64 ? 6 : 3;
-  static constexpr int kWarps = HD == 256 ? 2 : 4, kCtas = HD == 128 && NB == 2 ? 1 : 2;       // of a CTA, and CTAs on an SM
+  static constexpr int kWarps = 4, kCtas = 2;                       // of a CTA, and CTAs on an SM
   static constexpr int kWarpBytes = kStages * kStageBytes;
   static constexpr int kPitch = HD + 4;                             // floats of a row of sums
   static constexpr int kSums = (kWarps / 2) * 8 * NB * kPitch;      // half of the warps leave theirs, the others add to them
-  static constexpr int kSmem = kWarps * (kWarpBytes + kStages * 2 * kTile) + kSums * 4 + (kWarps + 1) * 8 * NB * 8 + 1024;
+  static constexpr int kSmem = kWarps * (kWarpBytes + kStages * 2 * kTile) + (kWarps + 1) * 8 * NB * 8 + 1024;
+  static_assert(kSums * 4 <= kWarps * kWarpBytes, "the sums lie over the rings");
   static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
 template <int HD, int NB, bool INT8, bool CLUSTER>
 __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB>::kWarps, Kv8Sizes<HD, NB>::kCtas) zb_kv8_decode_kernel(const Kv8DecodeParams p) {
   using Z = Kv8Sizes<HD, NB>;
-  constexpr int kStages = Z::kStages, kWarps = Z::kWarps, kRows = 8 * NB, kSteps = HD / 16, kSubs = HD > 128 ? 2 : 1, kPieces = HD / 64;
+  constexpr int kStages = Z::kStages, kWarps = Z::kWarps, kTile = Z::kTile, kGroups = Z::kGroups, kMt = kGroups / 2, kRows = 8 * NB, kSteps = HD / 16, kSubs = HD > 128 ? 2 : 1, kPieces = HD / 64;
   extern __shared__ uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   zb_pdl_launch();
@@ -261,18 +274,18 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB>::kWarps, Kv8Sizes<HD, NB
     const int index = blockIdx.x / p.parts, pairs = p.hkv * p.blocks;
     w.seq = index / pairs;
     w.pair = index - w.seq * pairs;
-    w.span = kv8_span(p, w.seq);
+    w.span = kv8_span<Z::kTile>(p, w.seq);
     w.nth = blockIdx.x - index * p.parts;
     w.chunks = p.parts;
     w.slot = 0;
     kv8_cut(w);
   } else {
-    if (!kv8_work(p, w, reinterpret_cast<int*>(smem))) return;
+    if (!kv8_work<Z::kTile>(p, w, reinterpret_cast<int*>(smem))) return;
   }
   const uint32_t smem_at = zb_smem_u32(smem), stages_at = smem_at + warp * Z::kWarpBytes;
   const uint32_t exps_at = smem_at + kWarps * Z::kWarpBytes + warp * kStages * 2 * kTile;
-  float* const sums = reinterpret_cast<float*>(smem + kWarps * (Z::kWarpBytes + kStages * 2 * kTile));      // [half of the warps][row][kPitch]
-  float* const stats = sums + Z::kSums;                                                                     // [warp, all][row][reference, sum]
+  float* const sums = reinterpret_cast<float*>(smem);  // [half of the warps][row][kPitch], over the rings
+  float* const stats = reinterpret_cast<float*>(smem + kWarps * (Z::kWarpBytes + kStages * 2 * kTile));      // [warp, all][row][reference, sum]
 
   // copies run kStages - 1 tiles ahead
   const int kvh = w.pair / p.blocks, row0 = (w.pair - kvh * p.blocks) * kRows, rows = min(kRows, p.group - row0);
@@ -282,9 +295,9 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB>::kWarps, Kv8Sizes<HD, NB
   const uint32_t copy_to = HD == 256 ? (line & 1) * kTile * 128 + (line >> 1) * 128 + ((in_line ^ (line >> 1)) << 4) : line * 128 + ((in_line ^ line) << 4);
   const auto fetch = [&]() {
     if (f_tile < w.end) {
-      const int nth = f_nth & 15;
-      if (nth == 0) {                                  // pages of the next 16 tiles, 16 keys a lane
-        const int tile = f_tile + (lane >> 1) * kWarps, key = (w.span.tile0 + tile) * kTile + (lane & 1) * 16;
+      const int nth = f_nth & (32 / kMt - 1);
+      if (nth == 0) {                                  // pages of the next 32 groups of 16 keys, one a lane
+        const int tile = f_tile + (lane / kMt) * kWarps, key = (w.span.tile0 + tile) * kTile + (lane % kMt) * 16;
         const bool some = tile < w.end && key < w.span.len && key + 16 > w.span.first;
         f_pages = some ? bt[key / p.page_size] : 0;
         if (static_cast<uint32_t>(f_pages) >= static_cast<uint32_t>(p.num_pages)) {
@@ -295,24 +308,21 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB>::kWarps, Kv8Sizes<HD, NB
         f_pages = ((f_pages * p.hkv + kvh) * p.page_size + key % p.page_size) >> 4;
         if (!some) f_pages = -1;
       }
-      const int unit0 = __shfl_sync(0xffffffffu, f_pages, 2 * nth), unit1 = __shfl_sync(0xffffffffu, f_pages, 2 * nth + 1);
       const uint32_t to = stages_at + f_stage * Z::kStageBytes;
-      constexpr int kCopies = kTile * HD / 512;
+      constexpr int kCopies = 16 * HD / 512;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int unit = half ? unit1 : unit0;
+      for (int part = 0; part < kMt; ++part) {
+        const int unit = __shfl_sync(0xffffffffu, f_pages, kMt * nth + part);
         const size_t from = static_cast<size_t>(max(unit, 0)) * (16 * HD) + lane * 16;
 #pragma unroll
-        for (int i = 0; i < kCopies / 2; ++i) {
-          const int n = half * (kCopies / 2) + i;
+        for (int i = 0; i < kCopies; ++i) {
+          const int n = part * kCopies + i;
           const uint32_t at = HD == 256 ? n * 256 + (copy_to ^ (((2 * n) & 7) << 4)) : n * 512 + (copy_to ^ ((n & 1) << 6));
           copy16(to + at, p.k_codes + from + i * 512, unit >= 0);
           copy16(to + Z::kTileBytes + at, p.v_codes + from + i * 512, unit >= 0);
         }
-      }
-      if (lane < 4) {                                  // exponents: keys, values of the first 16, of the others
-        const int unit = (lane >> 1) ? unit1 : unit0;
-        copy16(exps_at + f_stage * 2 * kTile + (lane & 1) * kTile + (lane >> 1) * 16, ((lane & 1) ? p.v_exps : p.k_exps) + static_cast<size_t>(max(unit, 0)) * 16, unit >= 0);
+        if (lane < 2)                                  // exponents of the keys, of the values
+          copy16(exps_at + f_stage * 2 * kTile + lane * kTile + part * 16, (lane ? p.v_exps : p.k_exps) + static_cast<size_t>(max(unit, 0)) * 16, unit >= 0);
       }
       if (++f_stage == kStages) f_stage = 0;
       ++f_nth;
@@ -325,11 +335,11 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB>::kWarps, Kv8Sizes<HD, NB
 
   const int g = lane >> 2, t4 = lane & 3;
   // what this thread reads of a stage: keys of row g in S^T = K Q^T, of rows 2 t4 and 2 t4 + 1 in O^T = V^T P^T, and the exponents of the former
-  const uint32_t ex_off = kv8_key<HD>(g, 0) & ~3;
+  const uint32_t ex_off = kv8_key<HD>(g, 0) & ~(kGroups - 1);
   const uint32_t k_off = kv8_at<HD>(kv8_key<HD>(g, 0), t4);
   const uint32_t v_off0 = Z::kTileBytes + kv8_at<HD>(kv8_key<HD>(2 * t4, 0), HD == 64 ? g >> 1 : g) + (HD == 64 ? (g & 1) * 8 : 0);
   const uint32_t v_off1 = Z::kTileBytes + kv8_at<HD>(kv8_key<HD>(2 * t4 + 1, 0), HD == 64 ? g >> 1 : g) + (HD == 64 ? (g & 1) * 8 : 0);
-  const uint32_t turn = HD != 64 && g >= 4 ? 0x1032 : 0x3210;      // kv8_key's order of the four
+  const uint32_t turn = HD == 128 && g >= 4 ? 0x1032 : 0x3210;     // kv8_key's order of the four
   int stage = 0;
   {
       // queries (e4m3: f16, two registers for 16 columns; int8: both parts of 32 columns), and what a score has to be multiplied by (columns 2 t4,
@@ -388,28 +398,28 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB>::kWarps, Kv8Sizes<HD, NB
       float unit = __uint_as_float(((254u + kLift) << 23) - power);
 
       // A tile's work is S^T = K Q^T (products), the weights (weigh), and O^T += V^T P^T (multiply).  The last one runs beside the next tile's first:
-      // neither waits for the other, and a tile's conversions fill the time of the other's products.  The tile's values wait in registers (HD 256:
-      // there are none left; their stage is kept).
+      // neither waits for the other, and a tile's conversions fill the time of the other's products.  The tile's values wait in registers.
       constexpr int kWords = HD == 64 ? 2 : 4;
-      constexpr bool KEEP = HD <= 128;
-      uint32_t v[KEEP ? kSubs : 1][2][4][kWords], pb[NB][4];
-      float s[NB][2][4];
+      uint32_t v[kSubs][kMt][4][kWords], pb[NB][kGroups];
+      float s[NB][kMt][4];
 #pragma unroll
-      for (int i = 0; i < 8 * kWords * (KEEP ? kSubs : 1); ++i) v[i / (8 * kWords)][(i / (4 * kWords)) & 1][(i / kWords) & 3][i % kWords] = 0u;
+      for (int i = 0; i < kSubs * kMt * 4 * kWords; ++i) v[i / (kMt * 4 * kWords)][(i / (4 * kWords)) % kMt][(i / kWords) & 3][i % kWords] = 0u;
 #pragma unroll
-      for (int b = 0; b < NB; ++b) pb[b][0] = pb[b][1] = pb[b][2] = pb[b][3] = 0u;
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) pb[b][i] = 0u;
 
       const auto products = [&](uint32_t at) {
         const uint32_t k_at = at + k_off;
-        int n[INT8 ? NB : 1][2][2][4];                 // int8: the products of the two parts of a query
-        float f[INT8 ? 1 : NB][2][2][4];               // e4m3: two sums, so that no product waits for the one before it
+        int n[INT8 ? NB : 1][kMt][2][4];               // int8: the products of the two parts of a query
+        float f[INT8 ? 1 : NB][kMt][2][4];             // e4m3: two sums, so that no product waits for the one before it
 #pragma unroll
         for (int c = 0; c < kPieces; ++c) {
-          uint4 x[4];                                  // piece c of four keys
+          uint4 x[kGroups];                            // piece c of the keys
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = lds128(((k_at ^ kv8_step<HD>(i)) ^ ((c & 1) << 6)) + (c >> 1) * kTile * 128);
+          for (int i = 0; i < kGroups; ++i) x[i] = lds128(((k_at ^ kv8_step<HD>(i)) ^ ((c & 1) << 6)) + (c >> 1) * kTile * 128);
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt) {
+          for (int mt = 0; mt < kMt; ++mt) {
             const uint32_t y[4] = {x[2 * mt].x, x[2 * mt].y, x[2 * mt].z, x[2 * mt].w}, z[4] = {x[2 * mt + 1].x, x[2 * mt + 1].y, x[2 * mt + 1].z, x[2 * mt + 1].w};
             if constexpr (INT8) {
 #pragma unroll
@@ -440,7 +450,7 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB>::kWarps, Kv8Sizes<HD, NB
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < 4 * kMt; ++i) {
             if constexpr (INT8) s[b][i >> 2][i & 3] = fmaf(256.f, static_cast<float>(n[b][i >> 2][0][i & 3]), static_cast<float>(n[b][i >> 2][1][i & 3]));
             else s[b][i >> 2][i & 3] = f[b][i >> 2][0][i & 3] + f[b][i >> 2][1][i & 3];
           }
@@ -484,47 +494,49 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB>::kWarps, Kv8Sizes<HD, NB
         }
       };
       const auto multiply_all = [&]() {
-        if constexpr (KEEP) {
 #pragma unroll
-          for (int sub = 0; sub < kSubs; ++sub)
+        for (int sub = 0; sub < kSubs; ++sub)
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt) multiply(sub, mt, v[sub][mt]);
-        }
+          for (int mt = 0; mt < kMt; ++mt) multiply(sub, mt, v[sub][mt]);
       };
 
-      // !WHOLE: some of the 32 keys lie behind the end or in front of the window
+      // !WHOLE: some of the keys lie behind the end or in front of the window
       const auto weigh = [&](auto whole, uint32_t at, uint32_t ex, int key0) {
         constexpr bool WHOLE = decltype(whole)::value;
-        const uint32_t k_exps = __byte_perm(lds32(ex), 0u, turn), v_exps = __byte_perm(lds32(ex + kTile), 0u, turn);
-        if constexpr (KEEP) {
+        uint32_t k_exps, v_exps;
+        if constexpr (kGroups == 4) k_exps = __byte_perm(lds32(ex), 0u, turn), v_exps = __byte_perm(lds32(ex + kTile), 0u, turn);
+        else k_exps = lds16(ex), v_exps = lds16(ex + kTile);
 #pragma unroll
-          for (int sub = 0; sub < kSubs; ++sub)
+        for (int sub = 0; sub < kSubs; ++sub)
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt) read(at, WHOLE ? -1 : key0, sub, mt, v[sub][mt]);
-        }
-        bool see[4];
-        uint32_t ve[4];                                // scales of the values, as bits: larger ones are larger numbers
+          for (int mt = 0; mt < kMt; ++mt) read(at, WHOLE ? -1 : key0, sub, mt, v[sub][mt]);
+        bool see[kGroups];
+        uint32_t ve[kGroups], ve_most = 0u;            // scales of the values, as bits: larger ones are larger numbers
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kGroups; ++i) {
           const int key = key0 + kv8_key<HD>(g, i);
           see[i] = WHOLE || (key >= w.span.first && key < w.span.len);
           ve[i] = see[i] ? kv8_scale_of(v_exps, i) : 0u;
+          ve_most = max(ve_most, ve[i]);
         }
-        const uint32_t ve_most = max(max(ve[0], ve[1]), max(ve[2], ve[3]));
         bool moves = ve_most > power;
+        float most[NB][2];
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NB; ++b) {
+          most[b][0] = most[b][1] = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < kGroups; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               float& x = s[b][i >> 1][(i & 1) * 2 + j];
               x = see[i] ? x * (__uint_as_float(kv8_scale_of(k_exps, i)) * factor[b][j]) : -INFINITY;
+              most[b][j] = fmaxf(most[b][j], x);
             }
+        }
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) moves = moves || fmaxf(fmaxf(s[b][0][j], s[b][0][j + 2]), fmaxf(s[b][1][j], s[b][1][j + 2])) > m[b][j] + kSlack;
+          for (int j = 0; j < 2; ++j) moves = moves || most[b][j] > m[b][j] + kSlack;
         if (__any_sync(0xffffffffu, moves)) {
           // a row that is NaN has the byte 255: its scale stays an infinity, and its codes of zero make a NaN of it
           const uint32_t now = max(power, __reduce_max_sync(0xffffffffu, min(ve_most, 253u << 23))), grown = (now - power) >> 23;
@@ -535,7 +547,7 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB>::kWarps, Kv8Sizes<HD, NB
           for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              float mx = fmaxf(fmaxf(s[b][0][j], s[b][0][j + 2]), fmaxf(s[b][1][j], s[b][1][j + 2]));
+              float mx = most[b][j];
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16)), m[b][j]);
@@ -549,28 +561,18 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB>::kWarps, Kv8Sizes<HD, NB
               }
             }
         }
-        float vs[4];
+        float vs[kGroups];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) vs[i] = __uint_as_float(ve[i]) * unit;
+        for (int i = 0; i < kGroups; ++i) vs[i] = __uint_as_float(ve[i]) * unit;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < kGroups; ++i) {
             const float p0 = zb_ex2(s[b][i >> 1][(i & 1) * 2] - m[b][0]), p1 = zb_ex2(s[b][i >> 1][(i & 1) * 2 + 1] - m[b][1]);
             l[b][0] += p0;
             l[b][1] += p1;
             pb[b][i] = transpose8(pack_half2(p0 * vs[i], p1 * vs[i]));
           }
-        if constexpr (!KEEP) {
-#pragma unroll
-          for (int sub = 0; sub < kSubs; ++sub)
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
-              uint32_t x[4][kWords];
-              read(at, WHOLE ? -1 : key0, sub, mt, x);
-              multiply(sub, mt, x);
-            }
-        }
       };
 
       for (int t = w.begin + warp; t < w.end; t += kWarps) {
@@ -811,16 +813,16 @@ int zb_kv8_decode_plan(int batch, int hq, int hkv, int hd, int max_len, long lon
   if (hkv <= 0 || hq <= 0 || hq % hkv != 0 || (hd != 64 && hd != 128 && hd != 256)) return INT_MIN;
   ZbDeviceState* st = zb_device_state();
   if (!st) return INT_MIN;
-  const int block = rows_of(hd, hq / hkv), blocks = (hq / hkv + block - 1) / block, rows = std::min(hq / hkv, block), warps = hd == 256 ? 2 : 4;
-  const long long pairs = static_cast<long long>(batch) * hkv * blocks, longest = std::max(1, (max_len + kTile - 1) / kTile), tiles = pairs * longest;
+  const int block = rows_of(hd, hq / hkv), blocks = (hq / hkv + block - 1) / block, rows = std::min(hq / hkv, block), warps = 4, tile = hd == 256 ? 16 : 32;
+  const long long pairs = static_cast<long long>(batch) * hkv * blocks, longest = std::max(1, (max_len + tile - 1) / tile), tiles = pairs * longest;
   if (tiles > 0x3fffffffll) return INT_MIN;
-  const int most = st->num_sms * (hd == 128 && block == 16 ? 1 : 2);
+  const int most = st->num_sms * 2;
   int size = 1;
   while (size < 16 && size * warps < longest) size *= 2;
   if (pairs * size <= most && size * warps * 2 >= longest) return -size;
   // No sequence is long, and there is no room to cut one: a CTA for each pair, which need not look at the other lengths (128 x 1024 keys of 4
   // heads: 28.5 us, 31.5 with that look)
-  if (batch > kMaxBatch || (2 * pairs > most && longest <= 64)) return -1;
+  if (batch > kMaxBatch || (2 * pairs > most && longest * tile <= 2048)) return -1;
   const int parts = static_cast<int>(std::min<long long>(tiles, most));
   *floats = slots_of(parts) * rows * (hd + 2);
   return parts;
@@ -882,7 +884,7 @@ int zb_kv8_decode(const ZbKv8Decode* c) {
   p.window = c->window;
   p.scale_log2 = c->scale * 1.4426950408889634f;
   p.status = st->status;
-  if (pairs * std::max<long long>(1, (static_cast<long long>(c->max_pages) * page_size + kTile - 1) / kTile) > 0x3fffffffll) return -34;
+  if (pairs * std::max<long long>(1, (static_cast<long long>(c->max_pages) * page_size + 15) / 16) > 0x3fffffffll) return -34;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(c->stream);
   const int n = static_cast<int>(pairs);
   if (hd == 64) return block == 8 ? launch_decode<64, 1>(p, c->int8 != 0, cluster, n, s) : launch_decode<64, 2>(p, c->int8 != 0, cluster, n, s);
