@@ -27,7 +27,7 @@ for _name in ("zb_kv8_write", "zb_kv8_read", "zb_kv8_decode"):
     _lib.register_signature(_name, C.c_int, [C.c_void_p])
 _lib.register_signature("zb_kv8_decode_plan", C.c_int, [C.c_int] * 5 + [C.c_void_p])
 _WRITE = struct.Struct("12P 2q 9i 2f").pack
-_READ = struct.Struct("10P 8i").pack
+_READ = struct.Struct("10P 10i").pack
 _DECODE = struct.Struct("11P q 10i f").pack
 
 # names that the engine and the command line take -> type of the codes
@@ -274,14 +274,21 @@ def paged_read(k: QuantKV, v: QuantKV, block_table, seq_lens, num_pages: Optiona
         return _paged_read_cpu(k, v, block_table, seq_lens, n)
     if _current() != index:
         with torch.cuda.device(index):
-            return paged_read(k, v, block_table, seq_lens, num_pages)
-    kd = block_table.new_empty((n, page_size, heads, hd), dtype=torch.bfloat16)
-    vd = torch.empty_like(kd)
-    table = torch.empty_like(block_table)
+            return _read(k, v, block_table, seq_lens, page_size, width, n)
+    return _read(k, v, block_table, seq_lens, page_size, width, n)
+
+
+def _read(k, v, block_table, seq_lens, size, width, n):
+    """`paged_read` into n pages of `size` tokens, `width` of a sequence at most, on the current device."""
+    pages, heads, page_size, hd = k._shape
     kc = k._codes
+    kd = block_table.new_empty((n, size, heads, hd), dtype=torch.bfloat16)
+    vd = torch.empty_like(kd)
+    table = block_table.new_empty((block_table.shape[0], width))
     rc = _lib.lib().zb_kv8_read(_READ(
         kc.data_ptr(), k._exponents.data_ptr(), v._codes.data_ptr(), v._exponents.data_ptr(), kd.data_ptr(), vd.data_ptr(), block_table.data_ptr(),
-        seq_lens.data_ptr(), table.data_ptr(), _stream(index), b, heads, hd, page_size, width, pages, n, kc.dtype is torch.int8))
+        seq_lens.data_ptr(), table.data_ptr(), _stream(k._index), block_table.shape[0], heads, hd, page_size, block_table.shape[1], pages, size, width, n,
+        kc.dtype is torch.int8))
     if rc:
         _lib.check(rc, "zb_kv8_read")
     return kd, vd, table
@@ -397,9 +404,10 @@ def paged_decode(q, k: QuantKV, v: QuantKV, block_table, seq_lens, scale: Option
 
 def paged_prefill(q, k: QuantKV, v: QuantKV, block_table, seq_lens, q_start, scale: Optional[float] = None, window: int = 0, out=None,
                   total_q_blocks: Optional[int] = None, impl: str = "auto", max_seq_len: Optional[int] = None, kv_pages: Optional[int] = None):
-    """`ops.paged_prefill` on a quantised cache: the sequences are read back to bf16 (`paged_read`; `kv_pages` is its `num_pages`), and the bf16
-    kernels attend to that.  Prompts are bound by their products: reading back moves 6 bytes a key, head and column once, where every query of
-    the group makes 4 operations of them; the workspace lives as long as the call."""
+    """`ops.paged_prefill` on a quantised cache: the sequences are read back to bf16 pages of 64 tokens, which is what the tcgen05 kernels take
+    (`kv_pages`: pages of the cache that they hold together, where the caller knows it), and the bf16 kernels attend to that.  Prompts are bound
+    by their products: reading back moves 6 bytes a key, head and column once, where every query of the group makes 4 operations of
+    them; the workspace lives as long as the call."""
     page_size = _pair(k, v)[2]
     b, width = _table(k, block_table, seq_lens)
     _queries(q, k, out)
@@ -407,11 +415,16 @@ def paged_prefill(q, k: QuantKV, v: QuantKV, block_table, seq_lens, q_start, sca
     if q_start.shape != (b + 1,):
         raise ValueError(f"q_start has one number more than the {b} sequences, got {tuple(q_start.shape)}")
     from . import paged_prefill as bf16_prefill
-    if k._index >= 0 and _current() != k._index:
-        with torch.cuda.device(k._index):
-            return paged_prefill(q, k, v, block_table, seq_lens, q_start, scale, window, out, total_q_blocks, impl, max_seq_len, kv_pages)
-    if kv_pages is None and max_seq_len is not None:
-        kv_pages = b * min(width, -(-max_seq_len // page_size))
-    kd, vd, table = paged_read(k, v, block_table, seq_lens, kv_pages)
+    if k._index < 0:
+        kd, vd, table = paged_read(k, v, block_table, seq_lens, kv_pages)
+    else:
+        if _current() != k._index:
+            with torch.cuda.device(k._index):
+                return paged_prefill(q, k, v, block_table, seq_lens, q_start, scale, window, out, total_q_blocks, impl, max_seq_len, kv_pages)
+        most = width * page_size if max_seq_len is None else min(max_seq_len, width * page_size)
+        n = b * -(-most // 64)
+        if kv_pages is not None:                                             # at most 63 tokens behind each sequence
+            n = min(n, kv_pages * page_size // 64 + b)
+        kd, vd, table = _read(k, v, block_table, seq_lens, 64, -(-width * page_size // 64), n)
     a = bf16_prefill(q, kd, vd, table, seq_lens, q_start, scale, window, out=out, total_q_blocks=total_q_blocks, impl=impl, max_seq_len=max_seq_len)
     return a if out is None or a is out else out.copy_(a)
