@@ -646,3 +646,155 @@ def test_prefill(case, dtype):
     prefill_case(*case, dtype, device="cuda")
     prefill_case(*case, dtype, device="cuda", max_seq_len=max(lens), kv_pages=sum(-(-n // case[4]) for n in lens))
     ops.raise_on_status()
+
+
+# ------------------------------------------------------------------ how a decode call is shared out
+def shared_out(lens, hq, hkv, hd, bound=None):
+    """"cluster", "warp" or "chunks" (zb_kv8_decode_plan): a cluster or a CTA for each pair of a sequence and a key head, a warp, or chunks."""
+    parts, _ = kv8._plan(0, len(lens), hq, hkv, hd, max(lens) if bound is None else bound)
+    return "chunks" if parts > 0 else "warp" if parts == 0 else "cluster"
+
+
+MANY = [(i * 37) % 90 for i in range(310)]                       # 0 .. 89 keys
+UNEVEN = [3000 if i % 9 == 0 else 5 * i for i in range(100)]
+SHARED = [
+    # kind, lens, hq, hkv, hd, page, more
+    ("warp", MANY, 2, 2, 64, 16, {}),
+    ("warp", MANY, 6, 2, 128, 64, {}),
+    ("warp", MANY, 6, 2, 256, 32, {}),
+    ("warp", MANY, 26, 2, 64, 64, dict(window=20)),
+    ("warp", MANY, 36, 2, 128, 48, dict(window=64)),
+    ("warp", MANY, 24, 2, 256, 16, dict(window=1)),
+    ("chunks", UNEVEN, 4, 2, 64, 64, {}),
+    ("chunks", UNEVEN, 12, 2, 128, 16, dict(window=1500)),
+    ("chunks", UNEVEN, 32, 2, 128, 64, {}),
+    ("chunks", UNEVEN, 16, 2, 256, 48, dict(window=2047)),
+    ("chunks", [9000, 0, 2500, 1, 20000, 64], 5, 5, 64, 64, {}),
+    ("chunks", [9000, 0, 2500, 1, 20000, 64], 16, 4, 256, 64, {}),
+    ("cluster", [700, 64, 0, 1], 4, 2, 128, 64, {}),
+    ("cluster", [1000] + [900 - i for i in range(199)], 2, 1, 128, 64, {}),
+]
+
+
+@gpu
+@DTYPES
+@pytest.mark.parametrize("case", SHARED, ids=lambda c: f"{c[0]}-{len(c[1])}x{c[2]}-{c[3]}x{c[4]}")
+def test_decode_however_it_is_shared_out(case, dtype):
+    kind, lens, hq, hkv, hd, page, more = case
+    assert shared_out(lens, hq, hkv, hd) == kind
+    decode_case(lens, hq, hkv, hd, page, dtype, device="cuda", max_seq_len=max(lens), **more)
+    ops.raise_on_status()
+
+
+@gpu
+@DTYPES
+@pytest.mark.parametrize("kind,lens,hkv", [("warp", [33] * 310, 1), ("chunks", [40, 6000, 33, 2500], 2), ("cluster", [300, 40], 2)])
+def test_decode_rows_that_are_nan_however_it_is_shared_out(kind, lens, hkv, dtype):
+    """One key, and one value, of one sequence each: NaN there, in no other sequence or head, and nowhere when the window hides them."""
+    k, v, table, sl = paged(lens, hkv, 64, 128, dtype, 5, "cuda")
+    q = torch.randn(len(lens), 4 * hkv, 128, device="cuda").bfloat16()
+    assert shared_out(lens, 4 * hkv, hkv, 128) == kind
+    for cache, seq in ((k, 0), (v, 1)):
+        page = int(table[seq, 0])
+        cache.exponents[page, 0, 3] = 255
+        cache.codes.view(torch.uint8)[page, 0, 3] = 0
+    got = ops.paged_decode(q, k, v, table, sl, max_seq_len=max(lens)).isnan().view(len(lens), hkv, -1)
+    want = torch.zeros(len(lens), hkv, 1, dtype=torch.bool, device="cuda")
+    want[:2, 0] = True
+    assert torch.equal(got, want.expand_as(got))
+    assert not bool(ops.paged_decode(q, k, v, table, sl, window=29, max_seq_len=max(lens)).isnan().any())
+
+
+@gpu
+def test_decode_of_more_sequences_than_are_cut():
+    """8200 sequences: none is cut, however long."""
+    lens = [4000 if i == 8000 else i % 6 for i in range(8200)]
+    assert shared_out(lens, 2, 1, 64) == "warp"
+    k, v, table, sl = paged(lens, 1, 16, 64, INT8, 5, "cuda")
+    q = torch.randn(len(lens), 2, 64, device="cuda").bfloat16()
+    out = ops.paged_decode(q, k, v, table, sl)
+    at = torch.tensor([0, 1, 5, 4095, 4096, 7999, 8000, 8001, 8199], device="cuda")
+    check_attention(out[at], q[at], k, v, table[at], sl[at], None, 0.125, 0)
+    for n in range(0, len(lens), 1000):
+        part = slice(n, n + 1000)
+        few = ops.paged_decode(q[part], k, v, table[part], sl[part]).float()
+        assert float((few - out[part].float()).abs().max()) <= 2.0 ** -7 * float(few.abs().max())      # a rounding to bf16 on each side
+
+
+@gpu
+@pytest.mark.parametrize("stock", ["stock", "none", "at its end"])
+def test_decode_of_cut_pairs_in_graphs_and_streams(stock, monkeypatch):
+    """Captured calls that draw tickets: of a stock, or of an allocation of their own.  Lengths change on the device between replays, two graphs run on
+    two streams at once, and eager calls run beside them."""
+    lens = [[9000, 40, 2000, 64], [1, 33, 500, 0], [0, 8999, 64, 4000]]
+    assert shared_out(lens[0], 16, 4, 128) == "chunks"
+    k, v, table, _ = paged([9000, 9000, 9000, 9000], 4, 64, 128, E4M3, 5, "cuda")
+    q = torch.randn(4, 16, 128, device="cuda").bfloat16()
+    sls = [torch.tensor(n, dtype=torch.int32, device="cuda") for n in lens]
+    want = [ops.paged_decode(q, k, v, table, n) for n in sls]
+    for i, n in enumerate(lens):
+        check_attention(want[i], q, k, v, table, sls[i], None, 1 / math.sqrt(128), 0)
+    if stock == "none":
+        monkeypatch.setattr(kv8, "_CAPTURED", {})
+    elif stock == "at its end":
+        monkeypatch.setattr(kv8, "CAPTURED_TICKETS", 1)
+    graphs, outs, now = [], [], []
+    for _ in range(2):
+        n = sls[0].clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append([ops.paged_decode(q, k, v, table, n) for _ in range(2)])
+        graphs.append(g)
+        now.append(n)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for i in range(9):
+        pick = [i % 3, (i + 1) % 3]
+        for n, p in zip(now, pick):
+            n.copy_(sls[p])
+        torch.cuda.synchronize()
+        for st, g in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+        with torch.cuda.stream(streams[2]):
+            eager = [ops.paged_decode(q, k, v, table, sls[j]) for j in range(3)]
+        torch.cuda.synchronize()
+        for o, p in zip(outs, pick):
+            assert torch.equal(o[0], want[p]) and torch.equal(o[1], want[p])
+        for j in range(3):
+            assert torch.equal(eager[j], want[j])
+
+
+# ------------------------------------------------------------------ prompts over pages of any size
+@gpu
+@pytest.mark.parametrize("page", [16, 48, 64, 112, 128, 320])
+def test_prompts_over_pages_of_any_size(page):
+    """The reader's pages for prompts hold 64 tokens: the same rows whatever the cache's pages hold, zeros behind a sequence's end."""
+    lens = [0, 1, 63, 64, 65, 700, 129]
+    k, v, table, sl = paged(lens, 2, page, 128, INT8, 5, "cuda")
+    width = -(-table.shape[1] * page // 64)
+    held = [-(-n // 64) for n in lens]
+    kd, vd, t = kv8._read(k, v, table, sl, 64, width, sum(held))
+    at = 0
+    for i, (n, m) in enumerate(zip(lens, held)):
+        assert t[i].tolist() == list(range(at, at + m)) + [0] * (width - m)
+        for got, cache in ((kd, k), (vd, v)):
+            rows = got[at:at + m].reshape(m * 64, 2, 128)
+            assert torch.equal(rows[:n].double(), sequence64(cache, table[i], n)) and not bool(rows[n:].any())
+        at += m
+    ops.raise_on_status()
+    parts = [(1, 0), (63, 1), (64, 200), (65, 0), (130, 570)]
+    for more in ({}, dict(max_seq_len=700, kv_pages=sum(-(-(a + b) // page) for a, b in parts)), dict(max_seq_len=700)):
+        prefill_case(parts, 8, 2, 128, page, 0, E4M3, "cuda", **more)
+    prefill_case(parts, 8, 2, 64, page, 100, INT8, "cuda")
+    ops.raise_on_status()
+
+
+@gpu
+def test_prompts_report_a_page_that_is_none():
+    k, v, table, sl = paged([100], 2, 16, 64, E4M3, 5, "cuda")
+    q = torch.randn(3, 4, 64, device="cuda").bfloat16()
+    for bad in (-1, k.codes.shape[0]):
+        table[0, 5] = bad
+        ops.paged_prefill(q, k, v, table, sl, torch.tensor([0, 3], dtype=torch.int32, device="cuda"))
+        with pytest.raises(ops.KernelError):
+            ops.raise_on_status()

@@ -28,8 +28,8 @@
 // * A CTA takes a chunk of a (sequence, key head) pair.  The lengths on the device decide how long chunks are, so that a captured launch serves any
 //   of them: the smallest length that leaves no more chunks than the GPU holds CTAs, an even share where there are more pairs than that.  Chunks of a
 //   cut pair leave their sums in the workspace, and the last one to finish, which a ticket of the pair tells, joins them.
-//   CLUSTER, for work that would leave a warp only a tile or two: a cluster of up to 16 CTAs takes a pair, and the sums of the CTAs meet through
-//   distributed shared memory: no ticket, no workspace.
+//   For work that would leave a warp only a tile or two, a cluster of up to 16 CTAs takes a pair, and the sums of the CTAs meet through
+//   distributed shared memory: no ticket, no workspace.  Many short pairs get a warp each (zb_kv8_decode_plan).
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -245,13 +245,19 @@ ZB_DEVICE bool kv8_work(const Kv8DecodeParams& p, Kv8Work& w, int* tiles) {
   return true;
 }
 
-template <int HD, int NB>
+// How pairs are shared out: chunks of them to CTAs (kChunks), each to a cluster of CTAs, or a CTA (kCluster), or each to a warp (kWarp).
+enum Kv8Mode { kChunks, kCluster, kWarp };
+
+template <int HD, int NB, Kv8Mode MODE>
 struct Kv8Sizes {
   static constexpr int kGroups = kv8_groups<HD>(), kTile = 8 * kGroups;      // keys of a tile
   static constexpr int kTileBytes = kTile * HD;
   static constexpr int kStageBytes = 2 * kTileBytes;
-  static constexpr int kStages = HD == 64 ? 6 : 3;
-  static constexpr int kWarps = 4, kCtas = 2;                       // of a CTA, and CTAs on an SM
+  // A warp for each pair of heads of 64 has registers and shared memory for 15 on an SM, of three stages: 8000 pairs of 30 keys take 16.0 us, where 12 of
+  // four stages take 18.0 and 8 of six 23.3
+  static constexpr bool kMany = HD == 64 && NB == 1 && MODE == kWarp;
+  static constexpr int kStages = HD == 64 && !kMany ? 6 : 3;
+  static constexpr int kWarps = MODE == kWarp ? 1 : 4, kCtas = (kMany ? 15 : 8) / kWarps;      // of a CTA, and CTAs on an SM
   static constexpr int kWarpBytes = kStages * kStageBytes;
   static constexpr int kPitch = HD + 4;                             // floats of a row of sums
   static constexpr int kSums = (kWarps / 2) * 8 * NB * kPitch;      // half of the warps leave theirs, the others add to them
@@ -260,27 +266,28 @@ struct Kv8Sizes {
   static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
-template <int HD, int NB, bool INT8, bool CLUSTER>
-__global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB>::kWarps, Kv8Sizes<HD, NB>::kCtas) zb_kv8_decode_kernel(const Kv8DecodeParams p) {
-  using Z = Kv8Sizes<HD, NB>;
-  constexpr int kStages = Z::kStages, kWarps = Z::kWarps, kTile = Z::kTile, kGroups = Z::kGroups, kMt = kGroups / 2, kRows = 8 * NB, kSteps = HD / 16, kSubs = HD > 128 ? 2 : 1, kPieces = HD / 64;
+template <int HD, int NB, bool INT8, Kv8Mode MODE>
+__global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB, MODE>::kWarps, Kv8Sizes<HD, NB, MODE>::kCtas) zb_kv8_decode_kernel(const Kv8DecodeParams p) {
+  using Z = Kv8Sizes<HD, NB, MODE>;
+  constexpr int kStages = Z::kStages, kWarps = Z::kWarps, kTile = Z::kTile, kGroups = Z::kGroups, kMt = kGroups / 2, kRows = 8 * NB, kSteps = HD / 16;
+  constexpr int kSubs = HD > 128 ? 2 : 1, kPieces = HD / 64;
   extern __shared__ uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   zb_pdl_launch();
   zb_pdl_wait();
   uint8_t* const smem = smem_raw + ((1024u - (zb_smem_u32(smem_raw) & 1023u)) & 1023u);
   Kv8Work w;
-  if constexpr (CLUSTER) {
+  if constexpr (MODE != kChunks) {
     const int index = blockIdx.x / p.parts, pairs = p.hkv * p.blocks;
     w.seq = index / pairs;
     w.pair = index - w.seq * pairs;
-    w.span = kv8_span<Z::kTile>(p, w.seq);
+    w.span = kv8_span<kTile>(p, w.seq);
     w.nth = blockIdx.x - index * p.parts;
     w.chunks = p.parts;
     w.slot = 0;
     kv8_cut(w);
   } else {
-    if (!kv8_work<Z::kTile>(p, w, reinterpret_cast<int*>(smem))) return;
+    if (!kv8_work<kTile>(p, w, reinterpret_cast<int*>(smem))) return;
   }
   const uint32_t smem_at = zb_smem_u32(smem), stages_at = smem_at + warp * Z::kWarpBytes;
   const uint32_t exps_at = smem_at + kWarps * Z::kWarpBytes + warp * kStages * 2 * kTile;
@@ -341,459 +348,478 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB>::kWarps, Kv8Sizes<HD, NB
   const uint32_t v_off1 = Z::kTileBytes + kv8_at<HD>(kv8_key<HD>(2 * t4 + 1, 0), HD == 64 ? g >> 1 : g) + (HD == 64 ? (g & 1) * 8 : 0);
   const uint32_t turn = HD == 128 && g >= 4 ? 0x1032 : 0x3210;     // kv8_key's order of the four
   int stage = 0;
-  {
-      // queries (e4m3: f16, two registers for 16 columns; int8: both parts of 32 columns), and what a score has to be multiplied by (columns 2 t4,
-      // 2 t4 + 1 of each block of eight)
-      uint32_t qf[NB][kSteps][2];
-      float factor[NB][2];
+  // queries (e4m3: f16, two registers for 16 columns; int8: both parts of 32 columns), and what a score has to be multiplied by (columns 2 t4,
+  // 2 t4 + 1 of each block of eight)
+  uint32_t qf[NB][kSteps][2];
+  float factor[NB][2];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int r = b * 8 + g;
+    const __nv_bfloat16* src = p.q + static_cast<size_t>(w.seq) * p.q_stride + static_cast<size_t>(kvh * p.group + row0 + min(r, rows - 1)) * HD;
+    uint2 raw[kSteps];
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      raw[i] = *reinterpret_cast<const uint2*>(src + (t4 + 4 * (i >> 2)) * 16 + (i & 3) * 4);
+      if (r >= rows) raw[i] = make_uint2(0u, 0u);
+      const uint32_t x = raw[i].x & 0x7fff7fffu, y = raw[i].y & 0x7fff7fffu;
+      top = max(max(top, max(x >> 16, x & 0xffffu)), max(y >> 16, y & 0xffffu));
+    }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int e = min(max((INT8 ? 268 : 267) - static_cast<int>(top >> 7), 1), 253);      // exponent of 2^14 or 2^13 over 2^floor(log2 top)
+    const float up = __uint_as_float(static_cast<uint32_t>(e) << 23);
+    const float down = __uint_as_float(top >= 0x7f80u ? 0x7fffffffu : static_cast<uint32_t>(254 - e) << 23);      // no numbers, no scores
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const float2 x = zb_unpack_bf16x2(raw[i].x), y = zb_unpack_bf16x2(raw[i].y);
+      if constexpr (INT8) {
+        const float f[4] = {x.x * up, x.y * up, y.x * up, y.y * up};
+        uint32_t hi = 0u, lo = 0u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int n = min(max(__float2int_rn(f[j]), -32639), 32639), h = (n + 128) >> 8;
+          hi |= (static_cast<uint32_t>(h) & 255u) << (8 * j);
+          lo |= (static_cast<uint32_t>(n) & 255u) << (8 * j);
+        }
+        qf[b][i & ~1][i & 1] = hi;
+        qf[b][i | 1][i & 1] = lo;
+      } else {
+        qf[b][i][0] = pack_half2(x.x * up, x.y * up);
+        qf[b][i][1] = pack_half2(y.x * up, y.y * up);
+      }
+    }
+    factor[b][0] = __shfl_sync(0xffffffffu, down, 8 * t4) * p.scale_log2;
+    factor[b][1] = __shfl_sync(0xffffffffu, down, 8 * t4 + 4) * p.scale_log2;
+  }
+  float o[NB][kSteps][4];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) o[b][i][0] = o[b][i][1] = o[b][i][2] = o[b][i][3] = 0.f;
+  float m[NB][2], l[NB][2];                       // references, and the sums of this thread's keys
+#pragma unroll
+  for (int b = 0; b < NB; ++b) m[b][0] = m[b][1] = kNoScore, l[b][0] = l[b][1] = 0.f;
+  uint32_t power = (kLift + 1) << 23;              // what the values' scales are relative to, as bits
+  float unit = __uint_as_float(((254u + kLift) << 23) - power);
+
+  // A tile's work is S^T = K Q^T (products), the weights (weigh), and O^T += V^T P^T (multiply).  The last one runs beside the next tile's first:
+  // neither waits for the other, and a tile's conversions fill the time of the other's products.  The tile's values wait in registers.
+  constexpr int kWords = HD == 64 ? 2 : 4;
+  uint32_t v[kSubs][kMt][4][kWords], pb[NB][kGroups];
+  float s[NB][kMt][4];
+#pragma unroll
+  for (int i = 0; i < kSubs * kMt * 4 * kWords; ++i) v[i / (kMt * 4 * kWords)][(i / (4 * kWords)) % kMt][(i / kWords) & 3][i % kWords] = 0u;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) pb[b][i] = 0u;
+
+  const auto products = [&](uint32_t at) {
+    const uint32_t k_at = at + k_off;
+    int n[INT8 ? NB : 1][kMt][2][4];               // int8: the products of the two parts of a query
+    float f[INT8 ? 1 : NB][kMt][2][4];             // e4m3: two sums, so that no product waits for the one before it
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c) {
+      uint4 x[kGroups];                            // piece c of the keys
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) x[i] = lds128(((k_at ^ kv8_step<HD>(i)) ^ ((c & 1) << 6)) + (c >> 1) * kTile * 128);
+#pragma unroll
+      for (int mt = 0; mt < kMt; ++mt) {
+        const uint32_t y[4] = {x[2 * mt].x, x[2 * mt].y, x[2 * mt].z, x[2 * mt].w}, z[4] = {x[2 * mt + 1].x, x[2 * mt + 1].y, x[2 * mt + 1].z, x[2 * mt + 1].w};
+        if constexpr (INT8) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+              for (int part = 0; part < 2; ++part) {
+                const uint32_t b0 = qf[b][4 * c + 2 * h + part][0], b1 = qf[b][4 * c + 2 * h + part][1];
+                if (c + h == 0) mma_int8_first(n[b][mt][part], y[2 * h], z[2 * h], y[2 * h + 1], z[2 * h + 1], b0, b1);
+                else mma_int8(n[b][mt][part], y[2 * h], z[2 * h], y[2 * h + 1], z[2 * h + 1], b0, b1);
+              }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t a0, a1, a2, a3;
+            kv8_to_half<false>(y[i], a0, a2);
+            kv8_to_half<false>(z[i], a1, a3);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              if (c == 0 && i < 2) mma_f16_first(f[b][mt][i], a0, a1, a2, a3, qf[b][i][0], qf[b][i][1]);
+              else mma_f16(f[b][mt][i & 1], a0, a1, a2, a3, qf[b][4 * c + i][0], qf[b][4 * c + i][1]);
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 4 * kMt; ++i) {
+        if constexpr (INT8) s[b][i >> 2][i & 3] = fmaf(256.f, static_cast<float>(n[b][i >> 2][0][i & 3]), static_cast<float>(n[b][i >> 2][1][i & 3]));
+        else s[b][i >> 2][i & 3] = f[b][i >> 2][0][i & 3] + f[b][i >> 2][1][i & 3];
+      }
+  };
+
+  // values of half `mt` of the tile's keys, columns of half `sub` of a head of 256: keys of rows 2 t4, 2 t4 + 1, and the same eight rows further
+  const auto read = [&](uint32_t at, int key0, int sub, int mt, uint32_t (&x)[4][kWords]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int idx = 2 * mt + (k >> 1);
+      const uint32_t from = ((at + ((k & 1) ? v_off1 : v_off0)) ^ kv8_step<HD>(idx)) + sub * kTile * 128;
+      if constexpr (HD == 64) {
+        const uint2 y = lds64(from);
+        x[k][0] = y.x, x[k][1] = y.y;
+      } else {
+        const uint4 y = lds128(from);
+        x[k][0] = y.x, x[k][1] = y.y, x[k][2] = y.z, x[k][3] = y.w;
+      }
+      // codes of rows that nobody sees may be anything, e4m3's NaN, too
+      const int key = key0 + kv8_key<HD>(2 * t4 + (k & 1), idx);
+      if (key0 >= 0 && (key < w.span.first || key >= w.span.len)) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) x[k][i] = 0u;
+      }
+    }
+  };
+  const auto multiply = [&](int sub, int mt, const uint32_t (&x)[4][kWords]) {
+    // columns of a word: pairs of keys of each
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      uint32_t a[4], c[4];
+      kv8_to_half<INT8>(__byte_perm(x[0][i], x[1][i], 0x5140), a[0], a[1]);
+      kv8_to_half<INT8>(__byte_perm(x[2][i], x[3][i], 0x5140), a[2], a[3]);
+      kv8_to_half<INT8>(__byte_perm(x[0][i], x[1][i], 0x7362), c[0], c[1]);
+      kv8_to_half<INT8>(__byte_perm(x[2][i], x[3][i], 0x7362), c[2], c[3]);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const int r = b * 8 + g;
-        const __nv_bfloat16* src = p.q + static_cast<size_t>(w.seq) * p.q_stride + static_cast<size_t>(kvh * p.group + row0 + min(r, rows - 1)) * HD;
-        uint2 raw[kSteps];
-        uint32_t top = 0u;
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          raw[i] = *reinterpret_cast<const uint2*>(src + (t4 + 4 * (i >> 2)) * 16 + (i & 3) * 4);
-          if (r >= rows) raw[i] = make_uint2(0u, 0u);
-          const uint32_t x = raw[i].x & 0x7fff7fffu, y = raw[i].y & 0x7fff7fffu;
-          top = max(max(top, max(x >> 16, x & 0xffffu)), max(y >> 16, y & 0xffffu));
-        }
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = min(max((INT8 ? 268 : 267) - static_cast<int>(top >> 7), 1), 253);      // exponent of 2^14 or 2^13 over 2^floor(log2 top)
-        const float up = __uint_as_float(static_cast<uint32_t>(e) << 23);
-        const float down = __uint_as_float(top >= 0x7f80u ? 0x7fffffffu : static_cast<uint32_t>(254 - e) << 23);      // no numbers, no scores
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          const float2 x = zb_unpack_bf16x2(raw[i].x), y = zb_unpack_bf16x2(raw[i].y);
-          if constexpr (INT8) {
-            const float f[4] = {x.x * up, x.y * up, y.x * up, y.y * up};
-            uint32_t hi = 0u, lo = 0u;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int n = min(max(__float2int_rn(f[j]), -32639), 32639), h = (n + 128) >> 8;
-              hi |= (static_cast<uint32_t>(h) & 255u) << (8 * j);
-              lo |= (static_cast<uint32_t>(n) & 255u) << (8 * j);
-            }
-            qf[b][i & ~1][i & 1] = hi;
-            qf[b][i | 1][i & 1] = lo;
-          } else {
-            qf[b][i][0] = pack_half2(x.x * up, x.y * up);
-            qf[b][i][1] = pack_half2(y.x * up, y.y * up);
-          }
-        }
-        factor[b][0] = __shfl_sync(0xffffffffu, down, 8 * t4) * p.scale_log2;
-        factor[b][1] = __shfl_sync(0xffffffffu, down, 8 * t4 + 4) * p.scale_log2;
+        mma_f16(o[b][sub * 8 + 2 * i], a[0], a[1], a[2], a[3], pb[b][2 * mt], pb[b][2 * mt + 1]);
+        mma_f16(o[b][sub * 8 + 2 * i + 1], c[0], c[1], c[2], c[3], pb[b][2 * mt], pb[b][2 * mt + 1]);
       }
-      float o[NB][kSteps][4];
+    }
+  };
+  const auto multiply_all = [&]() {
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+    for (int sub = 0; sub < kSubs; ++sub)
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) o[b][i][0] = o[b][i][1] = o[b][i][2] = o[b][i][3] = 0.f;
-      float m[NB][2], l[NB][2];                       // references, and the sums of this thread's keys
-#pragma unroll
-      for (int b = 0; b < NB; ++b) m[b][0] = m[b][1] = kNoScore, l[b][0] = l[b][1] = 0.f;
-      uint32_t power = (kLift + 1) << 23;              // what the values' scales are relative to, as bits
-      float unit = __uint_as_float(((254u + kLift) << 23) - power);
+      for (int mt = 0; mt < kMt; ++mt) multiply(sub, mt, v[sub][mt]);
+  };
 
-      // A tile's work is S^T = K Q^T (products), the weights (weigh), and O^T += V^T P^T (multiply).  The last one runs beside the next tile's first:
-      // neither waits for the other, and a tile's conversions fill the time of the other's products.  The tile's values wait in registers.
-      constexpr int kWords = HD == 64 ? 2 : 4;
-      uint32_t v[kSubs][kMt][4][kWords], pb[NB][kGroups];
-      float s[NB][kMt][4];
+  // !WHOLE: some of the keys lie behind the end or in front of the window
+  const auto weigh = [&](auto whole, uint32_t at, uint32_t ex, int key0) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    uint32_t k_exps, v_exps;
+    if constexpr (kGroups == 4) k_exps = __byte_perm(lds32(ex), 0u, turn), v_exps = __byte_perm(lds32(ex + kTile), 0u, turn);
+    else k_exps = lds16(ex), v_exps = lds16(ex + kTile);
 #pragma unroll
-      for (int i = 0; i < kSubs * kMt * 4 * kWords; ++i) v[i / (kMt * 4 * kWords)][(i / (4 * kWords)) % kMt][(i / kWords) & 3][i % kWords] = 0u;
+    for (int sub = 0; sub < kSubs; ++sub)
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+      for (int mt = 0; mt < kMt; ++mt) read(at, WHOLE ? -1 : key0, sub, mt, v[sub][mt]);
+    bool see[kGroups];
+    uint32_t ve[kGroups], ve_most = 0u;            // scales of the values, as bits: larger ones are larger numbers
 #pragma unroll
-        for (int i = 0; i < kGroups; ++i) pb[b][i] = 0u;
-
-      const auto products = [&](uint32_t at) {
-        const uint32_t k_at = at + k_off;
-        int n[INT8 ? NB : 1][kMt][2][4];               // int8: the products of the two parts of a query
-        float f[INT8 ? 1 : NB][kMt][2][4];             // e4m3: two sums, so that no product waits for the one before it
+    for (int i = 0; i < kGroups; ++i) {
+      const int key = key0 + kv8_key<HD>(g, i);
+      see[i] = WHOLE || (key >= w.span.first && key < w.span.len);
+      ve[i] = see[i] ? kv8_scale_of(v_exps, i) : 0u;
+      ve_most = max(ve_most, ve[i]);
+    }
+    bool moves = ve_most > power;
+    float most[NB][2];
 #pragma unroll
-        for (int c = 0; c < kPieces; ++c) {
-          uint4 x[kGroups];                            // piece c of the keys
+    for (int b = 0; b < NB; ++b) {
+      most[b][0] = most[b][1] = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < kGroups; ++i) x[i] = lds128(((k_at ^ kv8_step<HD>(i)) ^ ((c & 1) << 6)) + (c >> 1) * kTile * 128);
+      for (int i = 0; i < kGroups; ++i)
 #pragma unroll
-          for (int mt = 0; mt < kMt; ++mt) {
-            const uint32_t y[4] = {x[2 * mt].x, x[2 * mt].y, x[2 * mt].z, x[2 * mt].w}, z[4] = {x[2 * mt + 1].x, x[2 * mt + 1].y, x[2 * mt + 1].z, x[2 * mt + 1].w};
-            if constexpr (INT8) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                  for (int part = 0; part < 2; ++part) {
-                    const uint32_t b0 = qf[b][4 * c + 2 * h + part][0], b1 = qf[b][4 * c + 2 * h + part][1];
-                    if (c + h == 0) mma_int8_first(n[b][mt][part], y[2 * h], z[2 * h], y[2 * h + 1], z[2 * h + 1], b0, b1);
-                    else mma_int8(n[b][mt][part], y[2 * h], z[2 * h], y[2 * h + 1], z[2 * h + 1], b0, b1);
-                  }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                uint32_t a0, a1, a2, a3;
-                kv8_to_half<false>(y[i], a0, a2);
-                kv8_to_half<false>(z[i], a1, a3);
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                  if (c == 0 && i < 2) mma_f16_first(f[b][mt][i], a0, a1, a2, a3, qf[b][i][0], qf[b][i][1]);
-                  else mma_f16(f[b][mt][i & 1], a0, a1, a2, a3, qf[b][4 * c + i][0], qf[b][4 * c + i][1]);
-                }
-              }
-            }
-          }
+        for (int j = 0; j < 2; ++j) {
+          float& x = s[b][i >> 1][(i & 1) * 2 + j];
+          x = see[i] ? x * (__uint_as_float(kv8_scale_of(k_exps, i)) * factor[b][j]) : -INFINITY;
+          most[b][j] = fmaxf(most[b][j], x);
         }
+    }
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int i = 0; i < 4 * kMt; ++i) {
-            if constexpr (INT8) s[b][i >> 2][i & 3] = fmaf(256.f, static_cast<float>(n[b][i >> 2][0][i & 3]), static_cast<float>(n[b][i >> 2][1][i & 3]));
-            else s[b][i >> 2][i & 3] = f[b][i >> 2][0][i & 3] + f[b][i >> 2][1][i & 3];
-          }
-      };
-
-      // values of half `mt` of the tile's keys, columns of half `sub` of a head of 256: keys of rows 2 t4, 2 t4 + 1, and the same eight rows further
-      const auto read = [&](uint32_t at, int key0, int sub, int mt, uint32_t (&x)[4][kWords]) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int idx = 2 * mt + (k >> 1);
-          const uint32_t from = ((at + ((k & 1) ? v_off1 : v_off0)) ^ kv8_step<HD>(idx)) + sub * kTile * 128;
-          if constexpr (HD == 64) {
-            const uint2 y = lds64(from);
-            x[k][0] = y.x, x[k][1] = y.y;
-          } else {
-            const uint4 y = lds128(from);
-            x[k][0] = y.x, x[k][1] = y.y, x[k][2] = y.z, x[k][3] = y.w;
-          }
-          // codes of rows that nobody sees may be anything, e4m3's NaN, too
-          const int key = key0 + kv8_key<HD>(2 * t4 + (k & 1), idx);
-          if (key0 >= 0 && (key < w.span.first || key >= w.span.len)) {
-#pragma unroll
-            for (int i = 0; i < kWords; ++i) x[k][i] = 0u;
-          }
-        }
-      };
-      const auto multiply = [&](int sub, int mt, const uint32_t (&x)[4][kWords]) {
-        // columns of a word: pairs of keys of each
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-          uint32_t a[4], c[4];
-          kv8_to_half<INT8>(__byte_perm(x[0][i], x[1][i], 0x5140), a[0], a[1]);
-          kv8_to_half<INT8>(__byte_perm(x[2][i], x[3][i], 0x5140), a[2], a[3]);
-          kv8_to_half<INT8>(__byte_perm(x[0][i], x[1][i], 0x7362), c[0], c[1]);
-          kv8_to_half<INT8>(__byte_perm(x[2][i], x[3][i], 0x7362), c[2], c[3]);
-#pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            mma_f16(o[b][sub * 8 + 2 * i], a[0], a[1], a[2], a[3], pb[b][2 * mt], pb[b][2 * mt + 1]);
-            mma_f16(o[b][sub * 8 + 2 * i + 1], c[0], c[1], c[2], c[3], pb[b][2 * mt], pb[b][2 * mt + 1]);
-          }
-        }
-      };
-      const auto multiply_all = [&]() {
-#pragma unroll
-        for (int sub = 0; sub < kSubs; ++sub)
-#pragma unroll
-          for (int mt = 0; mt < kMt; ++mt) multiply(sub, mt, v[sub][mt]);
-      };
-
-      // !WHOLE: some of the keys lie behind the end or in front of the window
-      const auto weigh = [&](auto whole, uint32_t at, uint32_t ex, int key0) {
-        constexpr bool WHOLE = decltype(whole)::value;
-        uint32_t k_exps, v_exps;
-        if constexpr (kGroups == 4) k_exps = __byte_perm(lds32(ex), 0u, turn), v_exps = __byte_perm(lds32(ex + kTile), 0u, turn);
-        else k_exps = lds16(ex), v_exps = lds16(ex + kTile);
-#pragma unroll
-        for (int sub = 0; sub < kSubs; ++sub)
-#pragma unroll
-          for (int mt = 0; mt < kMt; ++mt) read(at, WHOLE ? -1 : key0, sub, mt, v[sub][mt]);
-        bool see[kGroups];
-        uint32_t ve[kGroups], ve_most = 0u;            // scales of the values, as bits: larger ones are larger numbers
-#pragma unroll
-        for (int i = 0; i < kGroups; ++i) {
-          const int key = key0 + kv8_key<HD>(g, i);
-          see[i] = WHOLE || (key >= w.span.first && key < w.span.len);
-          ve[i] = see[i] ? kv8_scale_of(v_exps, i) : 0u;
-          ve_most = max(ve_most, ve[i]);
-        }
-        bool moves = ve_most > power;
-        float most[NB][2];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          most[b][0] = most[b][1] = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < kGroups; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float& x = s[b][i >> 1][(i & 1) * 2 + j];
-              x = see[i] ? x * (__uint_as_float(kv8_scale_of(k_exps, i)) * factor[b][j]) : -INFINITY;
-              most[b][j] = fmaxf(most[b][j], x);
-            }
-        }
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) moves = moves || most[b][j] > m[b][j] + kSlack;
-        if (__any_sync(0xffffffffu, moves)) {
-          // a row that is NaN has the byte 255: its scale stays an infinity, and its codes of zero make a NaN of it
-          const uint32_t now = max(power, __reduce_max_sync(0xffffffffu, min(ve_most, 253u << 23))), grown = (now - power) >> 23;
-          const float shrink = grown > 126u ? 0.f : __uint_as_float((127u - grown) << 23);
-          power = now;
-          unit = __uint_as_float(((254u + kLift) << 23) - now);
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float mx = most[b][j];
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-              mx = fmaxf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16)), m[b][j]);
-              const float c = zb_ex2(m[b][j] - mx);
-              m[b][j] = mx;
-              l[b][j] *= c;
-#pragma unroll
-              for (int i = 0; i < kSteps; ++i) {
-                o[b][i][j] *= c * shrink;
-                o[b][i][j + 2] *= c * shrink;
-              }
-            }
-        }
-        float vs[kGroups];
-#pragma unroll
-        for (int i = 0; i < kGroups; ++i) vs[i] = __uint_as_float(ve[i]) * unit;
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int i = 0; i < kGroups; ++i) {
-            const float p0 = zb_ex2(s[b][i >> 1][(i & 1) * 2] - m[b][0]), p1 = zb_ex2(s[b][i >> 1][(i & 1) * 2 + 1] - m[b][1]);
-            l[b][0] += p0;
-            l[b][1] += p1;
-            pb[b][i] = transpose8(pack_half2(p0 * vs[i], p1 * vs[i]));
-          }
-      };
-
-      for (int t = w.begin + warp; t < w.end; t += kWarps) {
-        copies_wait<kStages - 2>();
-        __syncwarp();                                  // everybody's copies of this tile have landed, and the last tile has been read
-        fetch();
-        const int key0 = (w.span.tile0 + t) * kTile;
-        const uint32_t at = stages_at + stage * Z::kStageBytes, ex = exps_at + stage * 2 * kTile + ex_off;
-        if (w.span.len > 0) {
-          products(at);
-          multiply_all();
-          if (key0 >= w.span.first && key0 + kTile <= w.span.len) weigh(std::true_type(), at, ex, key0);
-          else weigh(std::false_type(), at, ex, key0);
-        }
-        if (++stage == kStages) stage = 0;
-      }
-      multiply_all();
-
-      // The CTA's sums: the warps' references, then half of the warps leave their sums, the others add theirs.  A thread's columns of a row are
-      // neighbours, eight of them (HD 64), or 16 of each 128.
-      const int out_row = w.seq * p.hkv * p.group + kvh * p.group + row0;
-      constexpr int kPitch = Z::kPitch, kHalf = kWarps / 2, kFours = HD / 4;
-      const float power_of = __uint_as_float(power - (kLift << 23));
+      for (int j = 0; j < 2; ++j) moves = moves || most[b][j] > m[b][j] + kSlack;
+    if (__any_sync(0xffffffffu, moves)) {
+      // a row that is NaN has the byte 255: its scale stays an infinity, and its codes of zero make a NaN of it
+      const uint32_t now = max(power, __reduce_max_sync(0xffffffffu, min(ve_most, 253u << 23))), grown = (now - power) >> 23;
+      const float shrink = grown > 126u ? 0.f : __uint_as_float((127u - grown) << 23);
+      power = now;
+      unit = __uint_as_float(((254u + kLift) << 23) - now);
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float sum = l[b][j];
-          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-          if (g == 0) *reinterpret_cast<float2*>(stats + (warp * kRows + b * 8 + 2 * t4 + j) * 2) = make_float2(m[b][j], sum);
+          float mx = most[b][j];
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16)), m[b][j]);
+          const float c = zb_ex2(m[b][j] - mx);
+          m[b][j] = mx;
+          l[b][j] *= c;
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i) {
+            o[b][i][j] *= c * shrink;
+            o[b][i][j + 2] *= c * shrink;
+          }
         }
-      __syncthreads();
+    }
+    float vs[kGroups];
 #pragma unroll
-      for (int turns = 0; turns < 2; ++turns) {
-        if ((warp >= kHalf) == (turns == 0)) {
+    for (int i = 0; i < kGroups; ++i) vs[i] = __uint_as_float(ve[i]) * unit;
 #pragma unroll
-          for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int r = b * 8 + 2 * t4 + j;
-              if (r >= rows) continue;
-              float top = kNoScore;
-#pragma unroll
-              for (int k = 0; k < kWarps; ++k) top = fmaxf(top, stats[(k * kRows + r) * 2]);
-              const float by = zb_ex2(m[b][j] - top) * power_of;
-#pragma unroll
-              for (int i = 0; i < kSteps; i += 2) {
-                const int col = HD == 64 ? g * 8 + 2 * i : (i >> 3) * 128 + g * 16 + 2 * (i & 7);
-                float4* dst = reinterpret_cast<float4*>(sums + ((turns == 0 ? warp - kHalf : warp) * kRows + r) * kPitch + col);
-                float4 x = make_float4(o[b][i][j] * by, o[b][i][j + 2] * by, o[b][i + 1][j] * by, o[b][i + 1][j + 2] * by);
-                if (turns == 1) {
-                  const float4 y = *dst;
-                  x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
-                }
-                *dst = x;
-              }
-            }
-        }
-        __syncthreads();
+      for (int i = 0; i < kGroups; ++i) {
+        const float p0 = zb_ex2(s[b][i >> 1][(i & 1) * 2] - m[b][0]), p1 = zb_ex2(s[b][i >> 1][(i & 1) * 2 + 1] - m[b][1]);
+        l[b][0] += p0;
+        l[b][1] += p1;
+        pb[b][i] = transpose8(pack_half2(p0 * vs[i], p1 * vs[i]));
       }
-      // the CTA's sums of a row and four columns
-      const auto sum_of = [&](int r, int col, float& top, float& sum) {
-        top = kNoScore, sum = 0.f;
+  };
+
+  for (int t = w.begin + warp; t < w.end; t += kWarps) {
+    copies_wait<kStages - 2>();
+    __syncwarp();                                  // everybody's copies of this tile have landed, and the last tile has been read
+    fetch();
+    const int key0 = (w.span.tile0 + t) * kTile;
+    const uint32_t at = stages_at + stage * Z::kStageBytes, ex = exps_at + stage * 2 * kTile + ex_off;
+    if (w.span.len > 0) {
+      products(at);
+      multiply_all();
+      if (key0 >= w.span.first && key0 + kTile <= w.span.len) weigh(std::true_type(), at, ex, key0);
+      else weigh(std::false_type(), at, ex, key0);
+    }
+    if (++stage == kStages) stage = 0;
+  }
+  multiply_all();
+
+  // A thread's columns of a row are neighbours, eight of them (HD 64), or 16 of each 128.
+  const auto column = [&](int i) { return HD == 64 ? g * 8 + 2 * i : (i >> 3) * 128 + g * 16 + 2 * (i & 7); };
+  const int out_row = w.seq * p.hkv * p.group + kvh * p.group + row0;
+  const auto put = [&](int r, int col, const float4& x, float sum) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;    // a row that sees nothing is zero
+    *reinterpret_cast<uint2*>(p.out + static_cast<size_t>(out_row + r) * HD + col) = make_uint2(zb_pack_bf16x2(x.x * inv, x.y * inv), zb_pack_bf16x2(x.z * inv, x.w * inv));
+  };
+  const float power_of = __uint_as_float(power - (kLift << 23));
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) top = fmaxf(top, stats[(k * kRows + r) * 2]);
+  for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) {
-          const float2 st = *reinterpret_cast<const float2*>(stats + (k * kRows + r) * 2);
-          sum += zb_ex2(st.x - top) * st.y;
-        }
-        float4 x = *reinterpret_cast<const float4*>(sums + r * kPitch + col);
+    for (int j = 0; j < 2; ++j) {
+      l[b][j] += __shfl_xor_sync(0xffffffffu, l[b][j], 4);
+      l[b][j] += __shfl_xor_sync(0xffffffffu, l[b][j], 8);
+      l[b][j] += __shfl_xor_sync(0xffffffffu, l[b][j], 16);
+    }
+  if constexpr (MODE == kWarp) {
 #pragma unroll
-        for (int k = 1; k < kHalf; ++k) {
-          const float4 y = *reinterpret_cast<const float4*>(sums + (k * kRows + r) * kPitch + col);
-          x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
-        }
-        return x;
-      };
-      const auto put = [&](int r, int col, const float4& x, float sum) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;              // a row that sees nothing is zero
-        *reinterpret_cast<uint2*>(p.out + static_cast<size_t>(out_row + r) * HD + col) = make_uint2(zb_pack_bf16x2(x.x * inv, x.y * inv), zb_pack_bf16x2(x.z * inv, x.w * inv));
-      };
-      if constexpr (CLUSTER) {
-        const bool alone = w.chunks == 1;
-        for (int i = threadIdx.x; i < rows * kFours; i += 32 * kWarps) {
-          const int r = i / kFours, col = 4 * (i - r * kFours);
-          float top, sum;
-          const float4 x = sum_of(r, col, top, sum);
-          if (alone) {
-            put(r, col, x, sum);
-          } else {
-            *reinterpret_cast<float4*>(sums + r * kPitch + col) = x;
-            if (col == 0) *reinterpret_cast<float2*>(stats + (kWarps * kRows + r) * 2) = make_float2(top, sum);
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = b * 8 + 2 * t4 + j;
+        if (r >= rows) continue;
+#pragma unroll
+        for (int i = 0; i < kSteps; i += 2)
+          put(r, column(i), make_float4(o[b][i][j] * power_of, o[b][i][j + 2] * power_of, o[b][i + 1][j] * power_of, o[b][i + 1][j + 2] * power_of), l[b][j]);
+      }
+    return;
+  }
+  // The CTA's sums: the warps' references, then half of the warps leave their sums, the others add theirs.
+  constexpr int kPitch = Z::kPitch, kHalf = kWarps / 2, kFours = HD / 4;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (g == 0) *reinterpret_cast<float2*>(stats + (warp * kRows + b * 8 + 2 * t4 + j) * 2) = make_float2(m[b][j], l[b][j]);
+  __syncthreads();
+#pragma unroll
+  for (int turns = 0; turns < 2; ++turns) {
+    if ((warp >= kHalf) == (turns == 0)) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int r = b * 8 + 2 * t4 + j;
+          if (r >= rows) continue;
+          float top = kNoScore;
+#pragma unroll
+          for (int k = 0; k < kWarps; ++k) top = fmaxf(top, stats[(k * kRows + r) * 2]);
+          const float by = zb_ex2(m[b][j] - top) * power_of;
+#pragma unroll
+          for (int i = 0; i < kSteps; i += 2) {
+            float4* dst = reinterpret_cast<float4*>(sums + ((turns == 0 ? warp - kHalf : warp) * kRows + r) * kPitch + column(i));
+            float4 x = make_float4(o[b][i][j] * by, o[b][i][j + 2] * by, o[b][i + 1][j] * by, o[b][i + 1][j + 2] * by);
+            if (turns == 1) {
+              const float4 y = *dst;
+              x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+            }
+            *dst = x;
           }
         }
-        if (alone) return;
-        // those of the cluster's CTAs, each of which finishes a share of the columns
-        __syncwarp();
-        zb_cluster_arrive();
-        zb_cluster_wait();
-        const uint32_t sums_at = zb_smem_u32(sums), stats_at = zb_smem_u32(stats + kWarps * kRows * 2);
-        for (int i = w.nth + p.parts * threadIdx.x; i < rows * kFours; i += p.parts * 32 * kWarps) {
-          const int r = i / kFours, col = 4 * (i - r * kFours);
-          float top = kNoScore, sum = 0.f;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int c0 = 0; c0 < p.parts; c0 += 8) {
-            float2 st[8];
-            float4 x[8];
+    }
+    __syncthreads();
+  }
+  // the CTA's sums of a row and four columns
+  const auto sum_of = [&](int r, int col, float& top, float& sum) {
+    top = kNoScore, sum = 0.f;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              if (c0 + c >= p.parts) continue;
-              st[c] = load_peer2(zb_mapa(stats_at + r * 8, c0 + c));
-              x[c] = load_peer4(zb_mapa(sums_at + (r * kPitch + col) * 4, c0 + c));
-            }
+    for (int k = 0; k < kWarps; ++k) top = fmaxf(top, stats[(k * kRows + r) * 2]);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              if (c0 + c >= p.parts) continue;
-              const float up = fmaxf(top, st[c].x), was = zb_ex2(top - up), by = zb_ex2(st[c].x - up);
-              acc.x = acc.x * was + by * x[c].x, acc.y = acc.y * was + by * x[c].y, acc.z = acc.z * was + by * x[c].z, acc.w = acc.w * was + by * x[c].w;
-              sum = sum * was + by * st[c].y;
-              top = up;
-            }
-          }
-          put(r, col, acc, sum);
-        }
-        __syncwarp();
-        zb_cluster_arrive();                           // nobody leaves while another one reads its shared memory
-        zb_cluster_wait();
-        return;
+    for (int k = 0; k < kWarps; ++k) {
+      const float2 st = *reinterpret_cast<const float2*>(stats + (k * kRows + r) * 2);
+      sum += zb_ex2(st.x - top) * st.y;
+    }
+    float4 x = *reinterpret_cast<const float4*>(sums + r * kPitch + col);
+#pragma unroll
+    for (int k = 1; k < kHalf; ++k) {
+      const float4 y = *reinterpret_cast<const float4*>(sums + (k * kRows + r) * kPitch + col);
+      x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+    }
+    return x;
+  };
+  if constexpr (MODE == kCluster) {
+    const bool alone = w.chunks == 1;
+    for (int i = threadIdx.x; i < rows * kFours; i += 32 * kWarps) {
+      const int r = i / kFours, col = 4 * (i - r * kFours);
+      float top, sum;
+      const float4 x = sum_of(r, col, top, sum);
+      if (alone) {
+        put(r, col, x, sum);
       } else {
-        const bool complete = w.chunks == 1;
-        const auto slot_at = [&](int nth, int r) { return static_cast<size_t>(w.slot + nth) * p.rows + r; };
-        for (int i = threadIdx.x; i < rows * kFours; i += 32 * kWarps) {
-          const int r = i / kFours, col = 4 * (i - r * kFours);
-          float top, sum;
-          const float4 x = sum_of(r, col, top, sum);
-          if (complete) {
-            put(r, col, x, sum);
-          } else {
-            *reinterpret_cast<float4*>(p.part_o + slot_at(w.nth, r) * HD + col) = x;
-            if (col == 0) p.part_ml[slot_at(w.nth, r)] = make_float2(top, sum);
-          }
+        *reinterpret_cast<float4*>(sums + r * kPitch + col) = x;
+        if (col == 0) *reinterpret_cast<float2*>(stats + (kWarps * kRows + r) * 2) = make_float2(top, sum);
+      }
+    }
+    if (alone) return;
+    // those of the cluster's CTAs, each of which finishes a share of the columns
+    __syncwarp();
+    zb_cluster_arrive();
+    zb_cluster_wait();
+    const uint32_t sums_at = zb_smem_u32(sums), stats_at = zb_smem_u32(stats + kWarps * kRows * 2);
+    for (int i = w.nth + p.parts * threadIdx.x; i < rows * kFours; i += p.parts * 32 * kWarps) {
+      const int r = i / kFours, col = 4 * (i - r * kFours);
+      float top = kNoScore, sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int c0 = 0; c0 < p.parts; c0 += 8) {
+        float2 st[8];
+        float4 x[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          if (c0 + c >= p.parts) continue;
+          st[c] = load_peer2(zb_mapa(stats_at + r * 8, c0 + c));
+          x[c] = load_peer4(zb_mapa(sums_at + (r * kPitch + col) * 4, c0 + c));
         }
-        if (complete) return;
-        __shared__ uint32_t drawn;
-        __syncthreads();                               // all of the CTA's sums are written
-        if (threadIdx.x == 0) {
-          __threadfence();
-          uint32_t* ticket = p.tickets + static_cast<size_t>(w.seq) * p.hkv * p.blocks + w.pair;
-          drawn = atomicAdd(ticket, 1u);
-          if (drawn == static_cast<uint32_t>(w.chunks - 1)) *ticket = 0u;      // for the next launch
-          __threadfence();
-        }
-        __syncthreads();
-        if (drawn != static_cast<uint32_t>(w.chunks - 1)) return;
-        // a warp for each row: the weights of 32 chunks at a time, one a lane, and the sums of 16
-        for (int r = warp; r < rows; r += kWarps) {
-          float top = kNoScore, sum = 0.f;
-          float acc[HD / 32];
 #pragma unroll
-          for (int j = 0; j < HD / 32; ++j) acc[j] = 0.f;
-          for (int i0 = 0; i0 < w.chunks; i0 += 32) {
-            constexpr int kOnce = HD == 256 ? 8 : 16;
-            const int most = min(32, w.chunks - i0);
-            const float2 ml = lane < most ? __ldcg(&p.part_ml[slot_at(i0 + lane, r)]) : make_float2(kNoScore, 0.f);
-            float x[kOnce][HD / 32];
-            const auto load = [&](int i1) {
-#pragma unroll
-              for (int i = 0; i < kOnce; ++i)
-#pragma unroll
-                for (int j = 0; j < HD / 32; ++j) x[i][j] = i1 + i < most ? __ldcg(p.part_o + slot_at(i0 + i1 + i, r) * HD + lane + 32 * j) : 0.f;
-            };
-            load(0);
-            const float up = fmaxf(top, zb_warp_max(ml.x)), was = zb_ex2(top - up), f = zb_ex2(ml.x - up);
-            top = up;
-            sum = sum * was + zb_warp_sum(f * ml.y);
-#pragma unroll
-            for (int j = 0; j < HD / 32; ++j) acc[j] *= was;
-            for (int i1 = 0; i1 < most; i1 += kOnce) {
-              if (i1 > 0) load(i1);
-#pragma unroll
-              for (int i = 0; i < kOnce; ++i) {
-                const float by = __shfl_sync(0xffffffffu, f, (i1 + i) & 31);
-#pragma unroll
-                for (int j = 0; j < HD / 32; ++j) acc[j] += by * x[i][j];
-              }
-            }
-          }
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-          for (int j = 0; j < HD / 32; ++j) p.out[static_cast<size_t>(out_row + r) * HD + lane + 32 * j] = __float2bfloat16(acc[j] * inv);
+        for (int c = 0; c < 8; ++c) {
+          if (c0 + c >= p.parts) continue;
+          const float up = fmaxf(top, st[c].x), was = zb_ex2(top - up), by = zb_ex2(st[c].x - up);
+          acc.x = acc.x * was + by * x[c].x, acc.y = acc.y * was + by * x[c].y, acc.z = acc.z * was + by * x[c].z, acc.w = acc.w * was + by * x[c].w;
+          sum = sum * was + by * st[c].y;
+          top = up;
         }
       }
+      put(r, col, acc, sum);
+    }
+    __syncwarp();
+    zb_cluster_arrive();                           // nobody leaves while another one reads its shared memory
+    zb_cluster_wait();
+    return;
+  } else {
+    const bool complete = w.chunks == 1;
+    const auto slot_at = [&](int nth, int r) { return static_cast<size_t>(w.slot + nth) * p.rows + r; };
+    for (int i = threadIdx.x; i < rows * kFours; i += 32 * kWarps) {
+      const int r = i / kFours, col = 4 * (i - r * kFours);
+      float top, sum;
+      const float4 x = sum_of(r, col, top, sum);
+      if (complete) {
+        put(r, col, x, sum);
+      } else {
+        *reinterpret_cast<float4*>(p.part_o + slot_at(w.nth, r) * HD + col) = x;
+        if (col == 0) p.part_ml[slot_at(w.nth, r)] = make_float2(top, sum);
+      }
+    }
+    if (complete) return;
+    __shared__ uint32_t drawn;
+    __syncthreads();                               // all of the CTA's sums are written
+    if (threadIdx.x == 0) {
+      __threadfence();
+      uint32_t* ticket = p.tickets + static_cast<size_t>(w.seq) * p.hkv * p.blocks + w.pair;
+      drawn = atomicAdd(ticket, 1u);
+      if (drawn == static_cast<uint32_t>(w.chunks - 1)) *ticket = 0u;      // for the next launch
+      __threadfence();
+    }
+    __syncthreads();
+    if (drawn != static_cast<uint32_t>(w.chunks - 1)) return;
+    // a warp for each row: the weights of 32 chunks at a time, one a lane, and the sums of 16
+    for (int r = warp; r < rows; r += kWarps) {
+      float top = kNoScore, sum = 0.f;
+      float acc[HD / 32];
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j) acc[j] = 0.f;
+      for (int i0 = 0; i0 < w.chunks; i0 += 32) {
+        constexpr int kOnce = HD == 256 ? 8 : 16;
+        const int most = min(32, w.chunks - i0);
+        const float2 ml = lane < most ? __ldcg(&p.part_ml[slot_at(i0 + lane, r)]) : make_float2(kNoScore, 0.f);
+        float x[kOnce][HD / 32];
+        const auto load = [&](int i1) {
+#pragma unroll
+          for (int i = 0; i < kOnce; ++i)
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j) x[i][j] = i1 + i < most ? __ldcg(p.part_o + slot_at(i0 + i1 + i, r) * HD + lane + 32 * j) : 0.f;
+        };
+        load(0);
+        const float up = fmaxf(top, zb_warp_max(ml.x)), was = zb_ex2(top - up), f = zb_ex2(ml.x - up);
+        top = up;
+        sum = sum * was + zb_warp_sum(f * ml.y);
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) acc[j] *= was;
+        for (int i1 = 0; i1 < most; i1 += kOnce) {
+          if (i1 > 0) load(i1);
+#pragma unroll
+          for (int i = 0; i < kOnce; ++i) {
+            const float by = __shfl_sync(0xffffffffu, f, (i1 + i) & 31);
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j) acc[j] += by * x[i][j];
+          }
+        }
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j) p.out[static_cast<size_t>(out_row + r) * HD + lane + 32 * j] = __float2bfloat16(acc[j] * inv);
+    }
   }
 }
 
-template <int HD, int NB, bool INT8, bool CLUSTER>
+template <int HD, int NB, bool INT8, Kv8Mode MODE>
 int launch_decode(const Kv8DecodeParams& p, int pairs, cudaStream_t stream) {
-  using Z = Kv8Sizes<HD, NB>;
-  const auto kernel = zb_kv8_decode_kernel<HD, NB, INT8, CLUSTER>;
+  using Z = Kv8Sizes<HD, NB, MODE>;
+  const auto kernel = zb_kv8_decode_kernel<HD, NB, INT8, MODE>;
   static bool configured[16] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 16) return -21;
   cudaError_t e = cudaSuccess;
   if (!configured[dev]) {
     e = zb_config_smem(kernel, Z::kSmem);
-    if (CLUSTER && e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);      // 16 CTAs
+    if (MODE == kCluster && e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);      // 16 CTAs
     if (e != cudaSuccess) return static_cast<int>(e);
     configured[dev] = true;
   }
-  if (CLUSTER) e = zb_launch_cluster(kernel, dim3(static_cast<unsigned>(pairs * p.parts)), dim3(32 * Z::kWarps), Z::kSmem, stream, p.parts, p);
+  if (MODE == kCluster) e = zb_launch_cluster(kernel, dim3(static_cast<unsigned>(pairs * p.parts)), dim3(32 * Z::kWarps), Z::kSmem, stream, p.parts, p);
+  else if (MODE == kWarp) e = zb_launch(kernel, dim3(static_cast<unsigned>(pairs)), dim3(32), Z::kSmem, stream, p);
   else e = zb_launch(kernel, dim3(static_cast<unsigned>(pairs <= p.parts ? p.parts : pairs + p.parts)), dim3(32 * Z::kWarps), Z::kSmem, stream, p);
   zb_count_launch(1);
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
+template <int HD, int NB, bool INT8>
+int launch_decode(const Kv8DecodeParams& p, Kv8Mode mode, int pairs, cudaStream_t stream) {
+  if (mode == kWarp) return launch_decode<HD, NB, INT8, kWarp>(p, pairs, stream);
+  return mode == kCluster ? launch_decode<HD, NB, INT8, kCluster>(p, pairs, stream) : launch_decode<HD, NB, INT8, kChunks>(p, pairs, stream);
+}
 template <int HD, int NB>
-int launch_decode(const Kv8DecodeParams& p, bool int8, bool cluster, int pairs, cudaStream_t stream) {
-  if (cluster) return int8 ? launch_decode<HD, NB, true, true>(p, pairs, stream) : launch_decode<HD, NB, false, true>(p, pairs, stream);
-  return int8 ? launch_decode<HD, NB, true, false>(p, pairs, stream) : launch_decode<HD, NB, false, false>(p, pairs, stream);
+int launch_decode(const Kv8DecodeParams& p, bool int8, Kv8Mode mode, int pairs, cudaStream_t stream) {
+  return int8 ? launch_decode<HD, NB, true>(p, mode, pairs, stream) : launch_decode<HD, NB, false>(p, mode, pairs, stream);
 }
 
 // Chunks of cut pairs: at most as many as there are CTAs, or, where there are more pairs, two for each even share that such a pair has.
@@ -805,7 +831,7 @@ int rows_of(int hd, int group) { return group > 8 && hd <= 128 ? 16 : 8; }
 
 extern "C" {
 
-// How a call is cut: CTAs of a cluster as a negative number, or the CTAs that share the chunks, and (in *floats) the fp32 numbers of its workspace, which
+// How a call is cut: CTAs of a cluster as a negative number, 0 for a warp for each pair, or the CTAs that share the chunks, and (in *floats) the fp32 numbers of its workspace, which
 // needs no particular contents.  max_len: keys of the longest sequence, or a bound of them; any number gives right results.
 int zb_kv8_decode_plan(int batch, int hq, int hkv, int hd, int max_len, long long* floats) {
   *floats = 0;
@@ -820,9 +846,12 @@ int zb_kv8_decode_plan(int batch, int hq, int hkv, int hd, int max_len, long lon
   int size = 1;
   while (size < 16 && size * warps < longest) size *= 2;
   if (pairs * size <= most && size * warps * 2 >= longest) return -size;
-  // No sequence is long, and there is no room to cut one: a CTA for each pair, which need not look at the other lengths (128 x 1024 keys of 4
-  // heads: 28.5 us, 31.5 with that look)
-  if (batch > kMaxBatch || (2 * pairs > most && longest * tile <= 2048)) return -1;
+  // More pairs than CTAs, none of them long: a warp for each, where a CTA for each takes a turn per 296 of them, most of it spent on getting
+  // under way (us, heads of 128, a warp / a CTA: 512 pairs of 40, 300, 1000 keys 5.2 / 8.1, 13.4 / 16.1, 32.3 / 27.6, 1024 pairs of 1000 44.9 / 51.3,
+  // 8000 of 30 28.8 / 93.2)
+  if (batch > kMaxBatch || (pairs > most && longest * tile <= 2048 && longest * tile * most <= pairs * 300)) return 0;
+  // Too many to cut: a CTA for each, which need not look at the other lengths (512 pairs of 1024 keys: 28.5 us, 31.5 with that look)
+  if (2 * pairs > most && longest * tile <= 2048) return -1;
   const int parts = static_cast<int>(std::min<long long>(tiles, most));
   *floats = slots_of(parts) * rows * (hd + 2);
   return parts;
@@ -850,7 +879,7 @@ int zb_kv8_decode(const ZbKv8Decode* c) {
   if (page_size <= 0 || page_size % 16 != 0 || c->num_pages <= 0 || static_cast<long long>(c->num_pages) * hkv * page_size > 0x7fffffffll ||
       static_cast<long long>(c->max_pages) * page_size > 0x7fffff00ll)
     return -31;
-  if (c->parts == 0 || c->parts < -16 || c->parts > 65536) return -33;
+  if (c->parts < -16 || c->parts > 65536) return -33;
   ZbDeviceState* st = zb_device_state();
   if (!st) return -20;
   const int block = rows_of(hd, hq / hkv);
@@ -870,13 +899,14 @@ int zb_kv8_decode(const ZbKv8Decode* c) {
   p.rows = std::min(p.group, block);
   const long long pairs = static_cast<long long>(c->batch) * hkv * p.blocks;
   if (pairs > 0x3ffffff) return -34;
-  const bool cluster = c->parts < 0;
-  p.parts = cluster ? -c->parts : c->parts;
+  const Kv8Mode mode = c->parts > 0 ? kChunks : c->parts < 0 ? kCluster : kWarp;
+  p.parts = std::max({1, c->parts, -c->parts});
   p.part_o = c->work;
-  p.part_ml = reinterpret_cast<float2*>(c->work + slots_of(c->parts) * p.rows * hd);
   p.tickets = c->tickets;
-  if (!cluster && c->batch > kMaxBatch) return -33;
-  if (!cluster && (c->work == nullptr || c->tickets == nullptr)) return -33;
+  if (mode == kChunks) {
+    if (c->batch > kMaxBatch || c->work == nullptr || c->tickets == nullptr) return -33;
+    p.part_ml = reinterpret_cast<float2*>(c->work + slots_of(c->parts) * p.rows * hd);
+  }
   p.q_stride = c->q_stride;
   p.page_size = page_size;
   p.max_pages = c->max_pages;
@@ -887,9 +917,9 @@ int zb_kv8_decode(const ZbKv8Decode* c) {
   if (pairs * std::max<long long>(1, (static_cast<long long>(c->max_pages) * page_size + 15) / 16) > 0x3fffffffll) return -34;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(c->stream);
   const int n = static_cast<int>(pairs);
-  if (hd == 64) return block == 8 ? launch_decode<64, 1>(p, c->int8 != 0, cluster, n, s) : launch_decode<64, 2>(p, c->int8 != 0, cluster, n, s);
-  if (hd == 128) return block == 8 ? launch_decode<128, 1>(p, c->int8 != 0, cluster, n, s) : launch_decode<128, 2>(p, c->int8 != 0, cluster, n, s);
-  return launch_decode<256, 1>(p, c->int8 != 0, cluster, n, s);
+  if (hd == 64) return block == 8 ? launch_decode<64, 1>(p, c->int8 != 0, mode, n, s) : launch_decode<64, 2>(p, c->int8 != 0, mode, n, s);
+  if (hd == 128) return block == 8 ? launch_decode<128, 1>(p, c->int8 != 0, mode, n, s) : launch_decode<128, 2>(p, c->int8 != 0, mode, n, s);
+  return launch_decode<256, 1>(p, c->int8 != 0, mode, n, s);
 }
 
 }  // extern "C"

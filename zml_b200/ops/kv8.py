@@ -321,7 +321,7 @@ _PLANS: dict = {}
 
 def _plan(index, b, hq, hkv, hd, max_len) -> tuple[int, int]:
     """(how a decode call is cut, numbers of its workspace): a function of its sizes."""
-    key = (index, b, hq, hkv, hd, -(-max_len // 32))
+    key = (index, b, hq, hkv, hd, -(-max_len // 16))
     got = _PLANS.get(key)
     if got is None:
         n = C.c_longlong()
