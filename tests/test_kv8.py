@@ -798,3 +798,61 @@ def test_prompts_report_a_page_that_is_none():
         ops.paged_prefill(q, k, v, table, sl, torch.tensor([0, 3], dtype=torch.int32, device="cuda"))
         with pytest.raises(ops.KernelError):
             ops.raise_on_status()
+
+
+def check_prompt_edges(device):
+    """Lengths that reach beyond the table count as far as it goes, and below zero as none; sequences without keys, a table without columns, and rows
+    behind the last sequence, which are left as they are."""
+    k, v, table, _ = paged([128, 128, 128], 2, 64, 64, E4M3, 5, device)
+    q = torch.randn(9, 4, 64, generator=torch.Generator().manual_seed(4)).bfloat16().to(device)
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=device)
+    starts = ints(0, 3, 3, 6)
+    want = ops.paged_prefill(q[:6], k, v, table, ints(128, 0, 128), starts)
+    assert torch.equal(ops.paged_prefill(q[:6], k, v, table, ints(10 ** 6, -5, 129), starts), want)
+    check_attention(want, q, k, v, table, ints(128, 0, 128), starts.tolist(), 0.125, 0)
+    if device != "cpu":
+        out = torch.full((9, 4, 64), 7.0, dtype=torch.bfloat16, device=device)
+        assert ops.paged_prefill(q, k, v, table, ints(128, 0, 128), starts, out=out) is out
+        assert torch.equal(out[:6], want) and bool((out[6:] == 7).all())
+        ops.raise_on_status()
+    for bt, more in ((table, dict(max_seq_len=0, kv_pages=0)), (table, {}), (table[:, :0].contiguous(), {})):
+        none = ops.paged_prefill(q[:0], k, v, bt, ints(0, 0, 0), ints(0, 0, 0, 0), **more)
+        assert none.shape == (0, 4, 64)
+        assert ops.paged_read(k, v, bt, ints(0, 0, 0), num_pages=0)[0].shape == (0, 64, 2, 64)
+        assert not bool(ops.paged_decode(q[:3], k, v, bt, ints(0, 0, 0)).any())
+    if device != "cpu":
+        ops.raise_on_status()
+
+
+def test_prompt_edges_cpu():
+    check_prompt_edges("cpu")
+
+
+@gpu
+def test_prompt_edges():
+    check_prompt_edges("cuda")
+
+
+@gpu
+@pytest.mark.parametrize("shift", [1, 2, 4])
+def test_outputs_at_any_address(shift):
+    """Outputs that start on 2, 4 or 8 bytes."""
+    lens = [70, 200]
+    k, v, table, sl = paged(lens, 2, 64, 128, E4M3, 5, "cuda")
+    q = torch.randn(2, 8, 128, generator=torch.Generator().manual_seed(6)).bfloat16().cuda()
+    at = lambda *shape: torch.full((math.prod(shape) + 8,), 7.0, dtype=torch.bfloat16, device="cuda")
+    flat = at(2, 8, 128)
+    out = flat[shift:shift + 2048].view(2, 8, 128)
+    assert ops.paged_decode(q, k, v, table, sl, out=out) is out
+    assert torch.equal(out, ops.paged_decode(q, k, v, table, sl)) and bool((flat[:shift] == 7).all()) and bool((flat[shift + 2048:] == 7).all())
+    qkv = torch.randn(3, 12 * 128, generator=torch.Generator().manual_seed(7)).bfloat16().cuda()
+    pos, freq = torch.arange(3, dtype=torch.int32, device="cuda"), torch.ones(64, device="cuda")
+    slots = torch.arange(3, dtype=torch.int32, device="cuda")
+    flat = at(3, 8, 128)
+    out = flat[shift:shift + 3072].view(3, 8, 128)
+    assert ops.rope_kvwrite(qkv, pos, slots, freq, k, v, 8, 2, 128, q_out=out) is out
+    want = ops.rope_kvwrite(qkv, pos, slots, freq, k, v, 8, 2, 128)
+    err = (out.double() - want.double()).abs()                # two kernels: each rounds once to bf16, fp32 before that
+    assert bool((err <= 2 * 2.0 ** -8 * want.double().abs() + 2.0 ** -17).all())
+    assert bool((flat[:shift] == 7).all()) and bool((flat[shift + 3072:] == 7).all())
+    ops.raise_on_status()

@@ -322,6 +322,7 @@ struct Kv8ReadParams {
   const int32_t* block_table;
   const int32_t* seq_lens;
   int32_t* out_table;          // [batch, out_width]
+  int32_t* out_lens;           // [batch]: seq_lens within what the block table has, or null
   int batch, hkv, log_pieces, page_size, max_pages, num_pages, out_size, out_width, out_pages;      // pieces: of 16 columns
   uint32_t inverse;            // 2^32 over the pieces of a token's row, rounded up
   ZbStatus* status;
@@ -370,6 +371,7 @@ __global__ void __launch_bounds__(kReadThreads, kReadCtas) zb_kv8_read_kernel(co
     zb_record_error(p.status, ZB_ERR_BOUNDS, kKernelKv8Read, 1u, static_cast<uint32_t>(total));
   for (int s = blockIdx.x; s < p.batch; s += gridDim.x) {
     const int first = kv8_total(s, pages_of), n = pages_of(s);
+    if (p.out_lens != nullptr && threadIdx.x == 0) p.out_lens[s] = kv8_len(p.seq_lens, s, most);
     for (int i = threadIdx.x; i < p.out_width; i += blockDim.x)
       p.out_table[static_cast<size_t>(s) * p.out_width + i] = i < n && first + i < p.out_pages ? first + i : 0;
   }
@@ -490,6 +492,7 @@ struct ZbKv8Read {
   const int32_t* block_table;
   const int32_t* seq_lens;
   int32_t* out_table;
+  int32_t* out_lens;                               // or null
   void* stream;
   int batch, hkv, hd, page_size, max_pages, num_pages;
   int out_size, out_width, out_pages, int8;         // tokens of a page that is written, pages of a row of out_table, pages that there are
@@ -560,6 +563,7 @@ int zb_kv8_read(const ZbKv8Read* c) {
   p.block_table = c->block_table;
   p.seq_lens = c->seq_lens;
   p.out_table = c->out_table;
+  p.out_lens = c->out_lens;
   p.batch = c->batch;
   p.hkv = c->hkv;
   p.log_pieces = c->hd == 64 ? 2 : c->hd == 128 ? 3 : 4;

@@ -861,7 +861,7 @@ int zb_kv8_decode_plan(int batch, int hq, int hkv, int hd, int max_len, long lon
 struct ZbKv8Decode {
   const void* q;                                   // [batch, hq, hd], rows on 8 bytes
   const void *k_codes, *k_exps, *v_codes, *v_exps;  // contiguous, on 16 bytes
-  void* out;                                       // [batch, hq, hd], contiguous
+  void* out;                                       // [batch, hq, hd], contiguous, on 8 bytes
   const int32_t* block_table;
   const int32_t* seq_lens;
   float* work;                                     // the numbers that the plan asked for
@@ -880,6 +880,7 @@ int zb_kv8_decode(const ZbKv8Decode* c) {
       static_cast<long long>(c->max_pages) * page_size > 0x7fffff00ll)
     return -31;
   if (c->parts < -16 || c->parts > 65536) return -33;
+  if (((reinterpret_cast<uintptr_t>(c->q) | reinterpret_cast<uintptr_t>(c->out)) & 7) != 0 || c->q_stride % 4 != 0) return -32;
   ZbDeviceState* st = zb_device_state();
   if (!st) return -20;
   const int block = rows_of(hd, hq / hkv);

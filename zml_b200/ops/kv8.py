@@ -27,7 +27,7 @@ for _name in ("zb_kv8_write", "zb_kv8_read", "zb_kv8_decode"):
     _lib.register_signature(_name, C.c_int, [C.c_void_p])
 _lib.register_signature("zb_kv8_decode_plan", C.c_int, [C.c_int] * 5 + [C.c_void_p])
 _WRITE = struct.Struct("12P 2q 9i 2f").pack
-_READ = struct.Struct("10P 10i").pack
+_READ = struct.Struct("11P 10i").pack
 _DECODE = struct.Struct("11P q 10i f").pack
 
 # names that the engine and the command line take -> type of the codes
@@ -278,8 +278,9 @@ def paged_read(k: QuantKV, v: QuantKV, block_table, seq_lens, num_pages: Optiona
     return _read(k, v, block_table, seq_lens, page_size, width, n)
 
 
-def _read(k, v, block_table, seq_lens, size, width, n):
-    """`paged_read` into n pages of `size` tokens, `width` of a sequence at most, on the current device."""
+def _read(k, v, block_table, seq_lens, size, width, n, lens=None):
+    """`paged_read` into n pages of `size` tokens, `width` of a sequence at most, on the current device.  `lens` takes the lengths that were read:
+    no more than the block table has, none below zero."""
     pages, heads, page_size, hd = k._shape
     kc = k._codes
     kd = block_table.new_empty((n, size, heads, hd), dtype=torch.bfloat16)
@@ -287,7 +288,7 @@ def _read(k, v, block_table, seq_lens, size, width, n):
     table = block_table.new_empty((block_table.shape[0], width))
     rc = _lib.lib().zb_kv8_read(_READ(
         kc.data_ptr(), k._exponents.data_ptr(), v._codes.data_ptr(), v._exponents.data_ptr(), kd.data_ptr(), vd.data_ptr(), block_table.data_ptr(),
-        seq_lens.data_ptr(), table.data_ptr(), _stream(k._index), block_table.shape[0], heads, hd, page_size, block_table.shape[1], pages, size, width, n,
+        seq_lens.data_ptr(), table.data_ptr(), 0 if lens is None else lens.data_ptr(), _stream(k._index), block_table.shape[0], heads, hd, page_size, block_table.shape[1], pages, size, width, n,
         kc.dtype is torch.int8))
     if rc:
         _lib.check(rc, "zb_kv8_read")
@@ -384,6 +385,8 @@ def paged_decode(q, k: QuantKV, v: QuantKV, block_table, seq_lens, scale: Option
         s0 = hq * hd
     if out is None:
         out = q.new_empty((b, hq, hd))
+    elif out.data_ptr() % 8:                                                 # and writes as many
+        return out.copy_(paged_decode(q, k, v, block_table, seq_lens, scale, window, max_seq_len))
     most = width * page_size
     parts, numbers = _plan(index, b, hq, hkv, hd, most if max_seq_len is None else min(max_seq_len, most))
     stream = _stream(index)
@@ -414,9 +417,12 @@ def paged_prefill(q, k: QuantKV, v: QuantKV, block_table, seq_lens, q_start, sca
     _ints(k._index, "q_start", q_start)
     if q_start.shape != (b + 1,):
         raise ValueError(f"q_start has one number more than the {b} sequences, got {tuple(q_start.shape)}")
+    if q.shape[0] == 0:
+        return q.new_empty(q.shape) if out is None else out
     from . import paged_prefill as bf16_prefill
     if k._index < 0:
         kd, vd, table = paged_read(k, v, block_table, seq_lens, kv_pages)
+        lens = seq_lens.clamp(0, width * page_size)
     else:
         if _current() != k._index:
             with torch.cuda.device(k._index):
@@ -425,6 +431,7 @@ def paged_prefill(q, k: QuantKV, v: QuantKV, block_table, seq_lens, q_start, sca
         n = b * -(-most // 64)
         if kv_pages is not None:                                             # at most 63 tokens behind each sequence
             n = min(n, kv_pages * page_size // 64 + b)
-        kd, vd, table = _read(k, v, block_table, seq_lens, 64, -(-width * page_size // 64), n)
-    a = bf16_prefill(q, kd, vd, table, seq_lens, q_start, scale, window, out=out, total_q_blocks=total_q_blocks, impl=impl, max_seq_len=max_seq_len)
+        lens = torch.empty_like(seq_lens)
+        kd, vd, table = _read(k, v, block_table, seq_lens, 64, -(-width * page_size // 64), max(1, n), lens)
+    a = bf16_prefill(q, kd, vd, table, lens, q_start, scale, window, out=out, total_q_blocks=total_q_blocks, impl=impl, max_seq_len=max_seq_len)
     return a if out is None or a is out else out.copy_(a)
