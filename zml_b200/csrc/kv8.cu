@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(512, 2) zb_kv8_write_kernel(const Kv8WritePara
   constexpr int kLanes = HD / 16, kHalf = HD / 2;
   // cosines and sines; angle i lies where a thread's eight are two pieces of 16 bytes, neighbouring threads' beside each other
   __shared__ __align__(16) float cs[2][kAhead][kHalf], sn[2][kAhead][kHalf];
-  __shared__ __align__(16) float weights[2][HD];       // of queries' and keys' norms
+  __shared__ __align__(16) float weights[2][HD];       // of queries' and keys' norms, laid out alike
   __shared__ long long rows[2][kAhead];
   zb_pdl_launch();
   zb_pdl_wait();
@@ -151,7 +151,8 @@ __global__ void __launch_bounds__(512, 2) zb_kv8_write_kernel(const Kv8WritePara
   uint4 x0 = src[static_cast<size_t>(tok) * p.qkv_stride / 8 + a0], x1 = src[static_cast<size_t>(tok) * p.qkv_stride / 8 + a1];
   for (int i = threadIdx.x; i < 2 * HD; i += blockDim.x) {
     const __nv_bfloat16* w = i < HD ? p.q_norm_w : p.k_norm_w;
-    if (w != nullptr) weights[i / HD][i % HD] = __bfloat162float(w[i % HD]) + (p.norm_unit_offset ? 1.f : 0.f);
+    const int n = i % HD;
+    if (w != nullptr) weights[i / HD][((n >> 2) & 1) * kHalf + (n >> 3) * 4 + (n & 3)] = __bfloat162float(w[n]) + (p.norm_unit_offset ? 1.f : 0.f);
   }
   ahead(tok, 0);
   __syncthreads();
@@ -179,7 +180,7 @@ __global__ void __launch_bounds__(512, 2) zb_kv8_write_kernel(const Kv8WritePara
         const ulonglong2* w = reinterpret_cast<const ulonglong2*>(weights[is_q ? 0 : 1]);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const ulonglong2 g0 = w[2 * a0 + i], g1 = w[2 * a1 + i];
+          const ulonglong2 g0 = w[i * (HD / 8) + a0], g1 = w[i * (HD / 8) + a1];
           f0[2 * i] = zb_mul2(zb_mul2(f0[2 * i], by), g0.x), f0[2 * i + 1] = zb_mul2(zb_mul2(f0[2 * i + 1], by), g0.y);
           f1[2 * i] = zb_mul2(zb_mul2(f1[2 * i], by), g1.x), f1[2 * i + 1] = zb_mul2(zb_mul2(f1[2 * i + 1], by), g1.y);
         }

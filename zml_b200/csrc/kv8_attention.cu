@@ -24,12 +24,16 @@
 // * Every warp has a ring of tiles of 32 keys (heads of 256: 16) of its own and waits for nobody while it streams; the sums of a CTA's four warps
 //   meet in shared memory in the end.  (One ring for eight warps, fed by tensor-map copies: 130 clocks an SM for each of a tile's four copies, and
 //   2 us at each end of a pair in which the SM's memory stood still.  CTAs that walk over equal parts of a list of all tiles: even, but nearly every
-//   pair is cut, and a CTA that joins one or begins another stands still for 3 us.  128 x 1024 keys of 4 heads: 39 and 36 us, now 28.)
+//   pair is cut, and a CTA that joins one or begins another stands still for 3 us.  128 x 1024 keys of 4 heads: 39 and 36 us, now 29.)
 // * A CTA takes a chunk of a (sequence, key head) pair.  The lengths on the device decide how long chunks are, so that a captured launch serves any
 //   of them: the smallest length that leaves no more chunks than the GPU holds CTAs, an even share where there are more pairs than that.  Chunks of a
 //   cut pair leave their sums in the workspace, and the last one to finish, which a ticket of the pair tells, joins them.
 //   For work that would leave a warp only a tile or two, a cluster of up to 16 CTAs takes a pair, and the sums of the CTAs meet through
 //   distributed shared memory: no ticket, no workspace.  Many short pairs get a warp each (zb_kv8_decode_plan).
+// Bound by memory where sequences are long: one of 131072 keys, 8 key heads of 128, 50.5 us, 5.4 TB/s (82 % of a copy's rate; 38 us where the keys lie
+// in L2); 128 of 1024 keys, 32 / 4 heads of 128, 29.1 us, 4.7 TB/s.  A launch has some 4.5 us that are not streaming: lengths, table and the first
+// keys one after the other, and the sums at the end; sequences of unequal lengths that are not cut add the wait for the longest
+// (32 of 128 - 2048 keys, 8 key heads of 128: 22.3 us, 3.3 TB/s).
 #include <algorithm>
 #include <climits>
 #include <type_traits>
