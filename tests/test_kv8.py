@@ -673,6 +673,9 @@ SHARED = [
     ("chunks", [9000, 0, 2500, 1, 20000, 64], 16, 4, 256, 64, {}),
     ("cluster", [700, 64, 0, 1], 4, 2, 128, 64, {}),
     ("cluster", [1000] + [900 - i for i in range(199)], 2, 1, 128, 64, {}),
+    ("cluster", [5000, 300, 4999, 0], 4, 2, 64, 64, {}),
+    ("cluster", [5000, 300, 4999, 0], 10, 2, 128, 48, dict(window=3000)),
+    ("cluster", [5000, 300, 4999, 0], 10, 2, 256, 16, {}),
 ]
 
 
@@ -688,7 +691,7 @@ def test_decode_however_it_is_shared_out(case, dtype):
 
 @gpu
 @DTYPES
-@pytest.mark.parametrize("kind,lens,hkv", [("warp", [33] * 310, 1), ("chunks", [40, 6000, 33, 2500], 2), ("cluster", [300, 40], 2)])
+@pytest.mark.parametrize("kind,lens,hkv", [("warp", [33] * 310, 1), ("chunks", [40, 20000, 33, 2500], 2), ("cluster", [300, 40], 2)])
 def test_decode_rows_that_are_nan_however_it_is_shared_out(kind, lens, hkv, dtype):
     """One key, and one value, of one sequence each: NaN there, in no other sequence or head, and nowhere when the window hides them."""
     k, v, table, sl = paged(lens, hkv, 64, 128, dtype, 5, "cuda")

@@ -28,8 +28,8 @@
 // * A CTA takes a chunk of a (sequence, key head) pair.  The lengths on the device decide how long chunks are, so that a captured launch serves any
 //   of them: the smallest length that leaves no more chunks than the GPU holds CTAs, an even share where there are more pairs than that.  Chunks of a
 //   cut pair leave their sums in the workspace, and the last one to finish, which a ticket of the pair tells, joins them.
-//   For work that would leave a warp only a tile or two, a cluster of up to 16 CTAs takes a pair, and the sums of the CTAs meet through
-//   distributed shared memory: no ticket, no workspace.  Many short pairs get a warp each (zb_kv8_decode_plan).
+//   Few pairs of up to 256 keys a warp get a cluster of up to 16 CTAs each, and the sums of the CTAs meet through distributed shared memory: no
+//   ticket, no workspace.  Many short pairs get a warp each (zb_kv8_decode_plan).
 // Bound by memory where sequences are long: one of 131072 keys, 8 key heads of 128, 50.5 us, 5.4 TB/s (82 % of a copy's rate; 38 us where the keys lie
 // in L2); 128 of 1024 keys, 32 / 4 heads of 128, 29.1 us, 4.7 TB/s.  A launch has some 4.5 us that are not streaming: lengths, table and the first
 // keys one after the other, and the sums at the end; sequences of unequal lengths that are not cut add the wait for the longest
@@ -847,9 +847,14 @@ int zb_kv8_decode_plan(int batch, int hq, int hkv, int hd, int max_len, long lon
   const long long pairs = static_cast<long long>(batch) * hkv * blocks, longest = std::max(1, (max_len + tile - 1) / tile), tiles = pairs * longest;
   if (tiles > 0x3fffffffll) return INT_MIN;
   const int most = st->num_sms * 2;
+  // CTAs for a pair: as many as give each warp a tile and fit on the GPU at once.  Of clusters of 16 only half as many fit, as each lies within a part of the
+  // GPU (16 pairs of 8000 keys: 17.5 us in clusters of 16, 13.7 of eight)
   int size = 1;
-  while (size < 16 && size * warps < longest) size *= 2;
-  if (pairs * size <= most && size * warps * 2 >= longest) return -size;
+  while (size < 16 && size * warps < longest && pairs * size * 2 <= (size == 8 ? most / 2 : most)) size *= 2;
+  // Up to 256 keys a warp a cluster is better than chunks, which look at all lengths and join through memory (us, heads of 128, a cluster / chunks: 8 pairs of
+  // 5000 and 10000 keys 8.5 / 10.2, 10.4 / 12.4, 64 of 4000 15.6 / 18.7, 128 of 1800 15.1 / 17.6), also where lengths differ (64 of
+  // 500 - 4000 14.2 / 14.4; 16 of 300 - 8000 11.7 / 11.0); beyond, the longest sequence keeps the others waiting (64 of 100 - 8000 21.8 / 18.6)
+  if (pairs * size <= most && longest * tile <= size * warps * 256) return -size;
   // More pairs than CTAs, none of them long: a warp for each, where a CTA for each takes a turn per 296 of them, most of it spent on getting
   // under way (us, heads of 128, a warp / a CTA: 512 pairs of 40, 300, 1000 keys 5.2 / 8.1, 13.4 / 16.1, 32.3 / 27.6, 1024 pairs of 1000 44.9 / 51.3,
   // 8000 of 30 28.8 / 93.2)
