@@ -158,8 +158,11 @@ def _ints(index: int, name: str, t) -> None:
 
 
 def _table(k: QuantKV, block_table, seq_lens) -> tuple[int, int]:
-    _ints(k._index, "block_table", block_table)
-    _ints(k._index, "seq_lens", seq_lens)
+    index = k._index
+    if (block_table.dtype is not torch.int32 or seq_lens.dtype is not torch.int32 or block_table.get_device() != index or seq_lens.get_device() != index
+            or not block_table.is_contiguous() or not seq_lens.is_contiguous()):
+        _ints(index, "block_table", block_table)
+        _ints(index, "seq_lens", seq_lens)
     shape = block_table.shape
     if len(shape) != 2 or seq_lens.shape != shape[:1]:
         raise ValueError(f"block_table [batch, pages] with seq_lens [batch], got {tuple(shape)} and {tuple(seq_lens.shape)}")
@@ -384,7 +387,7 @@ def paged_decode(q, k: QuantKV, v: QuantKV, block_table, seq_lens, scale: Option
         q = q.clone(memory_format=torch.contiguous_format)                   # the kernel reads 8 bytes of a row at a time
         s0 = hq * hd
     if out is None:
-        out = q.new_empty((b, hq, hd))
+        out = torch.empty_like(q) if s0 == hq * hd else q.new_empty((b, hq, hd))      # 1.4 us where new_empty takes 2.0
     elif out.data_ptr() % 8:                                                 # and writes as many
         return out.copy_(paged_decode(q, k, v, block_table, seq_lens, scale, window, max_seq_len))
     most = width * page_size
