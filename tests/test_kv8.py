@@ -848,14 +848,13 @@ def test_outputs_at_any_address(shift):
     out = flat[shift:shift + 2048].view(2, 8, 128)
     assert ops.paged_decode(q, k, v, table, sl, out=out) is out
     assert torch.equal(out, ops.paged_decode(q, k, v, table, sl)) and bool((flat[:shift] == 7).all()) and bool((flat[shift + 2048:] == 7).all())
-    qkv = torch.randn(3, 12 * 128, generator=torch.Generator().manual_seed(7)).bfloat16().cuda()
-    pos, freq = torch.arange(3, dtype=torch.int32, device="cuda"), torch.ones(64, device="cuda")
-    slots = torch.arange(3, dtype=torch.int32, device="cuda")
-    flat = at(3, 8, 128)
-    out = flat[shift:shift + 3072].view(3, 8, 128)
-    assert ops.rope_kvwrite(qkv, pos, slots, freq, k, v, 8, 2, 128, q_out=out) is out
-    want = ops.rope_kvwrite(qkv, pos, slots, freq, k, v, 8, 2, 128)
+    qkv = torch.randn(5, 12 * 128, generator=torch.Generator().manual_seed(7)).bfloat16().cuda()
+    pos, freq = torch.arange(5, dtype=torch.int32, device="cuda"), torch.ones(64, device="cuda")
+    flat = at(5, 8, 128)
+    out = flat[shift:shift + 5 * 8 * 128].view(5, 8, 128)
+    assert ops.rope_kvwrite(qkv, pos, pos, freq, k, v, 8, 2, 128, q_out=out) is out
+    want = ops.rope_kvwrite(qkv, pos, pos, freq, k, v, 8, 2, 128)
     err = (out.double() - want.double()).abs()                # two kernels: each rounds once to bf16, fp32 before that
     assert bool((err <= 2 * 2.0 ** -8 * want.double().abs() + 2.0 ** -17).all())
-    assert bool((flat[:shift] == 7).all()) and bool((flat[shift + 3072:] == 7).all())
+    assert bool((flat[:shift] == 7).all()) and bool((flat[shift + 5 * 8 * 128:] == 7).all())
     ops.raise_on_status()
