@@ -140,3 +140,19 @@ def test_serving_many_requests(kind):
     same = sum(a == b for x, y in zip(alone, served) for a, b in zip(x, y))
     assert all(len(x) == 12 for x in served) and same >= 0.75 * 12 * len(prompts)
     ops.raise_on_status()
+
+
+@gpu
+def test_graphs_of_short_and_long_sequences_are_apart():
+    """A step that was captured for short sequences is not replayed for long ones: their launches are planned by the longest sequence."""
+    m = model(device="cuda")
+    prompts = [tokens(10), tokens(3000, 4)]
+
+    def run(**kw):
+        e = Engine(m, num_pages=80, page_size=64, max_batch=4, max_seq_len=4096, kv_dtype="fp8", **kw)
+        return e, [e.generate([p], max_new_tokens=6)[0][0] for p in prompts]
+    e, captured = run()
+    plans = [e._plan_splits(1, n) for n in (16, 3006)]
+    assert plans[0] != plans[1] and {key[3] for key in e._graphs} == set(plans)
+    assert captured == run(use_graphs=False)[1]
+    ops.raise_on_status()

@@ -102,6 +102,12 @@ class QuantKVCache:
     def nbytes(self) -> int:
         return self.codes.numel() + self.exponents.numel()
 
+    def decode_plan(self, batch: int, hq: int, max_seq_len: int) -> int:
+        """A number for how `paged_decode` of these sizes is launched on the GPU: a captured launch serves any lengths, but is the one that the
+        `max_seq_len` of its capture asked for."""
+        k = self[0, 0]
+        return _plan(k._index, batch, hq, k._shape[1], k._shape[3], max_seq_len)[0]
+
 
 def kv_dtype(name) -> torch.dtype:
     """The code type that "fp8", "int8" or a torch dtype names."""

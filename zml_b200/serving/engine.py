@@ -30,7 +30,7 @@ import torch
 from .. import ops
 from ..models.common import SamplingStrategy
 from ..models.decoder import AttnMeta
-from ..ops import _lib
+from ..ops import QuantKVCache, _lib
 
 
 class OutOfPages(RuntimeError):
@@ -353,7 +353,11 @@ class Engine:
         return self._decode_step(bb, SamplingStrategy(), self._plan_splits(bb, max_total), max_total, None)[:b]
 
     def _plan_splits(self, batch: int, max_seq_len: int) -> int:
-        return self.model.decode_splits(batch, max_seq_len) if self.on_gpu else 1
+        if not self.on_gpu:
+            return 1
+        if isinstance(self.kv_cache, QuantKVCache):      # its kernel plans by itself: graphs are kept apart by that plan
+            return self.kv_cache.decode_plan(batch, self.model.hq, max_seq_len)
+        return self.model.decode_splits(batch, max_seq_len)
 
     def _upload_decode(self, bb: int, st: torch.Tensor, bt: torch.Tensor, stats: Optional[GenerationStats]) -> None:
         """Device state of the first bb batch rows: st [5, bb] = token, position, length, cache slot (negative: none) and
