@@ -15,7 +15,7 @@
 // * f16 does not hold every product p_j s_vj: s_vj is taken relative to the largest one so far, which rescales the accumulators like the reference
 //   of the scores does, and the weight times 2^7: what f16 drops lies 2^-32 below.
 // * The contraction may take the columns of a head in any order, the output columns may lie anywhere, and so may the keys in the rows, so every
-//   thread reads its operands as whole 16-byte pieces of a row and the exponents of its four keys as one word.  Rows are 128 bytes in shared memory
+//   thread reads its operands as whole 16-byte pieces of a row and the exponents of its keys (four; two of a head of 256) as one word.  Rows are 128 bytes in shared memory
 //   (half a row of a head of 256, two rows of a head of 64) in the 128-byte swizzle of the tensor-map copy; kv8_key says which key lies in
 //   which row, so that the pieces that eight neighbouring lanes read lie in different banks, in both products.
 // * The reference that scores are taken from, and that of the values' scales, move only when a score exceeds its reference by 2^8 or a scale its own:
@@ -835,8 +835,8 @@ int rows_of(int hd, int group) { return group > 8 && hd <= 128 ? 16 : 8; }
 
 extern "C" {
 
-// How a call is cut: CTAs of a cluster as a negative number, 0 for a warp for each pair, or the CTAs that share the chunks, and (in *floats) the fp32 numbers of its workspace, which
-// needs no particular contents.  max_len: keys of the longest sequence, or a bound of them; any number gives right results.
+// How a call is cut: CTAs of a cluster as a negative number, 0 for a warp for each pair, or the CTAs that share the chunks, and (in *floats) the
+// fp32 numbers of its workspace, which needs no particular contents.  max_len: keys of the longest sequence, or a bound of them; any number gives right results.
 int zb_kv8_decode_plan(int batch, int hq, int hkv, int hd, int max_len, long long* floats) {
   *floats = 0;
   if (batch <= 0) return 0;
@@ -874,7 +874,7 @@ struct ZbKv8Decode {
   const int32_t* block_table;
   const int32_t* seq_lens;
   float* work;                                     // the numbers that the plan asked for
-  uint32_t* tickets;                               // [batch * hkv * blocks of queries] where the plan is a list: zero before the call, and after it
+  uint32_t* tickets;                               // [batch * hkv * blocks of queries] where the plan is chunks: zero before the call, and after it
   void* stream;
   long long q_stride;
   int batch, hq, hkv, hd, page_size, max_pages, num_pages, window, int8, parts;

@@ -297,8 +297,8 @@ def _read(k, v, block_table, seq_lens, size, width, n, lens=None):
     table = block_table.new_empty((block_table.shape[0], width))
     rc = _lib.lib().zb_kv8_read(_READ(
         kc.data_ptr(), k._exponents.data_ptr(), v._codes.data_ptr(), v._exponents.data_ptr(), kd.data_ptr(), vd.data_ptr(), block_table.data_ptr(),
-        seq_lens.data_ptr(), table.data_ptr(), 0 if lens is None else lens.data_ptr(), _stream(k._index), block_table.shape[0], heads, hd, page_size, block_table.shape[1], pages, size, width, n,
-        kc.dtype is torch.int8))
+        seq_lens.data_ptr(), table.data_ptr(), 0 if lens is None else lens.data_ptr(), _stream(k._index), block_table.shape[0], heads, hd, page_size,
+        block_table.shape[1], pages, size, width, n, kc.dtype is torch.int8))
     if rc:
         _lib.check(rc, "zb_kv8_read")
     return kd, vd, table
@@ -400,7 +400,7 @@ def paged_decode(q, k: QuantKV, v: QuantKV, block_table, seq_lens, scale: Option
     parts, numbers = _plan(index, b, hq, hkv, hd, most if max_seq_len is None else min(max_seq_len, most))
     stream = _stream(index)
     work = tickets = 0
-    if numbers:                                                              # the parts of a list leave sums, and draw tickets
+    if numbers:                                                               # chunks leave sums, and draw tickets
         partial = q.new_empty((numbers,), dtype=torch.float32)
         ticket = _tickets(q, index, stream, b * hkv * -(-hq // (8 * hkv)))
         work, tickets = partial.data_ptr(), ticket.data_ptr()
