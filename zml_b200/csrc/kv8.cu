@@ -339,12 +339,12 @@ template <bool INT8>
 ZB_DEVICE void kv8_to_bf16(uint32_t w, float scale, uint32_t& lo, uint32_t& hi) {
   const ZbF2 by = zb_pack2(scale, scale);
   if constexpr (INT8) {
-    // byte u = code + 128 in the last place of 2^23, from which the 2^23 + 128 is taken again as the scale is multiplied
+    // byte u = code + 128 in the last place of 2^23, from which the 2^23 + 128 is taken again, exactly, before the scale is multiplied: their product
+    // is an infinity under scales of 2^105 and more, which rows of numbers above 2.6e33 have
     const uint32_t u = w ^ 0x80808080u;
-    const float off = -8388736.f * scale;
-    const ZbF2 less = zb_pack2(off, off);
-    lo = kv8_bf16x2(zb_fma2(zb_pack2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441))), by, less));
-    hi = kv8_bf16x2(zb_fma2(zb_pack2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443))), by, less));
+    const ZbF2 less = zb_pack2(-8388736.f, -8388736.f);
+    lo = kv8_bf16x2(zb_mul2(zb_add2(zb_pack2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441))), less), by));
+    hi = kv8_bf16x2(zb_mul2(zb_add2(zb_pack2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443))), less), by));
   } else {
     uint32_t a, b;
     kv8_to_half<false>(w, a, b);
