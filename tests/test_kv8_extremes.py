@@ -8,6 +8,7 @@ import torch
 
 from test_kv8 import DTYPES, gpu, values64
 from zml_b200 import ops
+from zml_b200.ops import kv8
 
 
 # ------------------------------------------------------------------ reader
@@ -40,4 +41,73 @@ def test_every_code_under_large_scales_cpu(dtype):
 @DTYPES
 def test_every_code_under_large_scales(dtype):
     check_every_code(dtype, "cuda")
+    ops.raise_on_status()
+
+
+# ------------------------------------------------------------------ attention of single tokens
+def shared_out(lens, hq, hkv, hd, bound):
+    parts, _ = kv8._plan(0, len(lens), hq, hkv, hd, bound)
+    return "chunks" if parts > 0 else "warp" if parts == 0 else "cluster"
+
+
+# lengths, the bound of them that the launch is planned by: a warp, one CTA, or chunks take the first sequence, tiles in turn among the warps of a CTA
+WAYS = pytest.mark.parametrize("kind,lens,bound", [("warp", [200] * 310, 200), ("cluster", [200], 1), ("chunks", [200, 20000, 33, 2500], 20000)],
+                               ids=["warp", "cluster", "chunks"])
+
+
+def sequences(lens, hkv, hd, dtype, device, page=64):
+    """A cache in which sequence i holds the pages after those of sequence i - 1, all of it zeros: keys, values, table, lengths, first page of each."""
+    held = [-(-n // page) for n in lens]
+    first = [sum(held[:i]) for i in range(len(lens))]
+    table = torch.zeros(len(lens), max(held), dtype=torch.int32)
+    for i, (a, m) in enumerate(zip(first, held)):
+        table[i, :m] = torch.arange(a, a + m, dtype=torch.int32)
+    k, v = (ops.QuantKV.alloc(sum(held), hkv, page, hd, dtype, device) for _ in range(2))
+    k.exponents.fill_(127)
+    v.exponents.fill_(127)
+    return k, v, table.to(device), torch.tensor(lens, dtype=torch.int32, device=device), first
+
+
+def put(cache, first, keys, rows):
+    """Rows `keys` of the one head of the sequence whose pages begin at `first`."""
+    codes, exponents = kv8.quantize(rows.float(), cache.codes.dtype)
+    page, at = (first + keys // 64).to(cache.device), (keys % 64).to(cache.device)
+    cache.codes.view(torch.uint8)[page, 0, at] = codes.view(torch.uint8).to(cache.device)
+    cache.exponents[page, 0, at] = exponents.to(cache.device)
+
+
+def scale_of_log2(x):
+    """A float32 scale whose product with log2(e), in float32, is x."""
+    f = torch.tensor(x / 1.4426950408889634, dtype=torch.float32)
+    for _ in range(8):
+        if float(f * torch.tensor(1.4426950408889634)) == x:
+            return float(f)
+        f = torch.nextafter(f, torch.tensor(float("inf")) if float(f * torch.tensor(1.4426950408889634)) < x else torch.tensor(0.0))
+    raise AssertionError("no such scale")
+
+
+@gpu
+@DTYPES
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@WAYS
+def test_scores_where_fp32_counts_in_sixteens(kind, lens, bound, hd, dtype):
+    """Scores of 2^27 + 16 and, later in the same warp, 2^27 + 32, in units of log2: the second key outweighs the first by 2^16, more than f16 holds over the
+    slack that weights have.  Both scores are exact: 8 x 64 x 2^14 and one or two, times 16.  What is left of the first key is 2^-16, and the second value is
+    rounded as a weight (2^-11) and to bf16 (2^-8)."""
+    assert shared_out(lens, 1, 1, hd, bound) == kind
+    k, v, table, sl, first = sequences(lens, 1, hd, dtype, "cuda")
+    near = torch.zeros(hd)
+    near[:8], near[8] = 64.0, 1.0
+    far = near.clone()
+    far[8] = 2.0
+    g = torch.Generator().manual_seed(3)
+    va, vb = (kv8._values(*kv8.quantize(torch.randn(hd, generator=g), dtype)) for _ in range(2))
+    later = 4 * (16 if hd == 256 else 32) + 7
+    put(k, first[0], torch.tensor([5, later]), torch.stack([near, far]))
+    put(v, first[0], torch.tensor([5, later]), torch.stack([va, vb]))
+    q = torch.zeros(len(lens), 1, hd, dtype=torch.bfloat16, device="cuda")
+    q[:, 0, :8], q[:, 0, 8] = 2.0 ** 14, 1.0
+    out = ops.paged_decode(q, k, v, table, sl, scale=scale_of_log2(16.0), max_seq_len=bound)[0, 0].double().cpu()
+    va, vb = va.double(), vb.double()
+    assert bool(((out - vb).abs() <= (2.0 ** -8 + 2.0 ** -11) * vb.abs() + 2.0 ** -15 * (va.abs() + vb.abs())).all()), out
     ops.raise_on_status()

@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB, MODE>::kWarps, Kv8Sizes<
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) moves = moves || most[b][j] > m[b][j] + kSlack;
+      for (int j = 0; j < 2; ++j) moves = moves || most[b][j] - m[b][j] > kSlack;      // m + kSlack is m or m + 16 from 2^27 on
     if (__any_sync(0xffffffffu, moves)) {
       // a row that is NaN has the byte 255: its scale stays an infinity, and its codes of zero make a NaN of it
       const uint32_t now = max(power, __reduce_max_sync(0xffffffffu, min(ve_most, 253u << 23))), grown = (now - power) >> 23;
