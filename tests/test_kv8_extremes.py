@@ -6,7 +6,7 @@ bf16, 2^-11 in f16.
 import pytest
 import torch
 
-from test_kv8 import DTYPES, gpu, values64
+from test_kv8 import DTYPES, INT8, gpu, sequence64, values64
 from zml_b200 import ops
 from zml_b200.ops import kv8
 
@@ -110,4 +110,88 @@ def test_scores_where_fp32_counts_in_sixteens(kind, lens, bound, hd, dtype):
     out = ops.paged_decode(q, k, v, table, sl, scale=scale_of_log2(16.0), max_seq_len=bound)[0, 0].double().cpu()
     va, vb = va.double(), vb.double()
     assert bool(((out - vb).abs() <= (2.0 ** -8 + 2.0 ** -11) * vb.abs() + 2.0 ** -15 * (va.abs() + vb.abs())).all()), out
+    ops.raise_on_status()
+
+
+def check_closely(out, q, k, v, table, lens, scale, which, int8):
+    """Rows `which` of a decode call against 64 bits, each key with its own share of the tolerance.
+
+    bf16 rounds the result (2^-8); a weight is rounded to f16 (2^-11), or lies among f16's subnormals (half a step of 2^-24, where the largest p s_v
+    of the row is 2^7 or more): 2^-32 of the largest p s_v, times a code.  A score is a sum of hd products in fp32 and three roundings, (hd + 8) 2^-24 of the sum of
+    their magnitudes; queries beside int8 keys are rounded to half a unit where the row's largest is 2^14 or more (2^-15), so a score is off by that
+    times the sum of the key's magnitudes.  exp2 gives 2^-21; a key's error acts on the sum of values and on the sum of weights.  Weights below 2^-126 of the
+    reference, which is up to 2^8 below the largest, may vanish."""
+    hd, hkv = q.shape[2], k.codes.shape[1]
+    group = q.shape[1] // hkv
+    most_code = 128.0 if int8 else 448.0
+    for i in which:
+        n = int(lens[i])
+        ks, vs = sequence64(k, table[i], n), sequence64(v, table[i], n)
+        scales = torch.exp2(v.exponents[table[i, :-(-n // 64)].long()].double() - 127.0).transpose(1, 2).reshape(-1, hkv)[:n]
+        for h in range(q.shape[1]):
+            kh, vh, qh = ks[:, h // group], vs[:, h // group], q[i, h].double()
+            delta = (hd + 8) * 2.0 ** -24 * abs(scale) * (kh.abs() @ qh.abs()) + 2.0 ** -21
+            if int8:
+                delta = delta + 2.0 ** -15 * float(qh.abs().max()) * abs(scale) * kh.abs().sum(-1)
+            p = torch.softmax((kh @ qh) * scale, 0)
+            want, mag = p @ vh, p @ vh.abs()
+            gone = torch.where(p < 2.0 ** -116 * p.max(), p, 0.0) @ vh.abs()
+            tol = (2.0 ** -8 * want.abs() + 2.0 ** -11 * mag + (p * delta) @ vh.abs() + (p @ delta) * mag + gone
+                   + n * 2.0 ** -32 * most_code * float((p * scales[:, h // group]).max()) + 2.0 ** -130)
+            err = (out[i, h].double() - want).abs()
+            assert bool((err <= tol).all()), (i, h, float((err / tol).max()), float((err - tol).max()))
+
+
+@gpu
+@DTYPES
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("up", [26, 40, 100])
+@WAYS
+def test_large_values_that_nobody_looks_at(kind, lens, bound, up, hd, dtype):
+    """One value row is 2^up times as large as the others, and its key's score 60 below theirs or far lower: it must not cost the others their digits (2^100 and
+    60 below, it is what the result is made of).  A second query head of the same key head looks at that key and at no other."""
+    assert shared_out(lens, 2, 1, hd, bound) == kind
+    g = torch.Generator().manual_seed(up + hd)
+    n = lens[0]
+    for place in (0, 70, n - 1):
+        for low in (60.0, 600.0):
+            k, v, table, sl, first = sequences(lens, 1, hd, dtype, "cuda")
+            ks, vs = torch.randn(n, hd, generator=g) * 0.1, torch.randn(n, hd, generator=g)
+            ks[:, 0] = 0.0
+            ks[place] = 0.0
+            ks[place, 0] = -low                           # a code times a power of two
+            vs[place] *= 2.0 ** up
+            put(k, first[0], torch.arange(n), ks)
+            put(v, first[0], torch.arange(n), vs)
+            q = torch.randn(len(lens), 2, hd, generator=g).bfloat16()
+            q[:, 0, 0], q[:, 1, 0] = 1.0, -1.0
+            q = q.cuda()
+            out = ops.paged_decode(q, k, v, table, sl, scale=1.0, max_seq_len=bound)
+            check_closely(out, q, k, v, table, sl, 1.0, [0], dtype is INT8)
+    ops.raise_on_status()
+
+
+@gpu
+@DTYPES
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("step,down", [(12.0, 5.0), (12.0, 17.0), (12.0, 30.0), (-12.0, -5.0), (-12.0, -30.0), (0.3, 1.0), (0.3, -1.0), (7.0, 0.0)])
+@WAYS
+def test_scores_and_values_that_climb_and_fall(kind, lens, bound, step, down, hd, dtype):
+    """Along a sequence scores rise by `step` (in units of log2) every 13 keys while values shrink by 2^down: what the weights are taken from moves with
+    nearly every tile, in both directions, and the first or the last keys make the result."""
+    assert shared_out(lens, 3, 1, hd, bound) == kind
+    g = torch.Generator().manual_seed(hd)
+    n = lens[0]
+    k, v, table, sl, first = sequences(lens, 1, hd, dtype, "cuda")
+    ks, vs = torch.randn(n, hd, generator=g) * 0.05, torch.randn(n, hd, generator=g)
+    at = torch.arange(n) // 13
+    ks[:, 0] = (step * at.float()).bfloat16().float()
+    vs *= torch.exp2(-down * (at.float() - 7.0))[:, None].clamp(2.0 ** -110, 2.0 ** 110)
+    put(k, first[0], torch.arange(n), ks)
+    put(v, first[0], torch.arange(n), vs)
+    q = torch.randn(len(lens), 3, hd, generator=g).bfloat16()
+    q[:, :, 0] = torch.tensor([1.0, 0.25, -1.0])
+    q = q.cuda()
+    out = ops.paged_decode(q, k, v, table, sl, scale=0.6931471805599453, max_seq_len=bound)
+    check_closely(out, q, k, v, table, sl, 0.6931471805599453, [0], dtype is INT8)
     ops.raise_on_status()

@@ -12,15 +12,17 @@
 //   the same conversions and products on this GPU, and more of them.)  A query row is scaled by a power of two to a largest magnitude in [2^13,
 //   2^14), exactly, and that power is taken out of its scores.  int8 has a product of its own for S^T, m16n8k32 with int32 sums, without
 //   conversions: the query is 256 times one int8 number and another (the largest of a row in [2^14, 2^15), half a unit is lost).
-// * f16 does not hold every product p_j s_vj: s_vj is taken relative to the largest one so far, which rescales the accumulators like the reference
-//   of the scores does, and the weight times 2^7: what f16 drops lies 2^-32 below.
+// * f16 does not hold every product p_j s_vj: every query head has a second reference, a power of two u with which its largest p_j s_vj so far is
+//   between 2^7 and 2^15, and which rescales its accumulators like the reference of the scores does.  What f16 drops lies 2^-32 below that head's largest
+//   product, whatever the scales of values are whose keys it does not look at.  (One power for all heads, taken from the scales alone, is two instructions a weight
+//   less and loses everything 2^32 below the largest scale, whether or not it has any weight.)
 // * The contraction may take the columns of a head in any order, the output columns may lie anywhere, and so may the keys in the rows, so every
 //   thread reads its operands as whole 16-byte pieces of a row and the exponents of its keys (four; two of a head of 256) as one word.  Rows are 128 bytes in shared memory
 //   (half a row of a head of 256, two rows of a head of 64) in the 128-byte swizzle of the tensor-map copy; kv8_key says which key lies in
 //   which row, so that the pieces that eight neighbouring lanes read lie in different banks, in both products.
-// * The reference that scores are taken from, and that of the values' scales, move only when a score exceeds its reference by 2^8 or a scale its own:
-//   the weights stay below 2^15, and a warp looks for that with one vote, where keeping the very maximum takes three shuffles a column
-//   and a multiplication of all accumulators nearly every time.
+// * Both references move only when a p_j exceeds 2^8 or a p_j s_vj u 2^15: a warp looks for that with one vote, where keeping the very maximum takes three
+//   shuffles a column and a multiplication of all accumulators nearly every time.  The reference of scores is a whole number, so that both rescale by
+//   powers of two, exactly.
 // * Every warp has a ring of tiles of 32 keys (heads of 256: 16) of its own and waits for nobody while it streams; the sums of a CTA's four warps
 //   meet in shared memory in the end.  (One ring for eight warps, fed by tensor-map copies: 130 clocks an SM for each of a tile's four copies, and
 //   2 us at each end of a pair in which the SM's memory stood still.  CTAs that walk over equal parts of a list of all tiles: even, but nearly every
@@ -47,8 +49,10 @@ constexpr uint32_t kKernelKv8Decode = 41;
 constexpr int kMaxBatch = 8192;                 // sequences whose lengths a CTA looks at: beyond, pairs are not cut
 constexpr int kMinChunk = 8;                    // tiles: two for each warp
 constexpr float kNoScore = -3.402823466e38f;    // the reference in front of the first key
-constexpr float kSlack = 8.f;                   // in units of log2: how far a score may exceed its reference
-constexpr uint32_t kLift = 7;                   // log2 of what weights are multiplied by
+constexpr float kMostP = 256.f;                 // what p_j may grow to before the references move
+constexpr float kMostWeight = 32768.f;          // and p_j s_vj u, which is an f16 number
+constexpr int kLift = 7;                        // log2 of what the largest p_j s_vj u is, at least, when they have moved
+constexpr int kMostUnit = 237, kLeastUnit = 7;  // u is 2^-120 to 2^110, as exponent bytes: 1 / u, and p_j u, are numbers, too
 
 struct Kv8DecodeParams {
   const __nv_bfloat16* q;
@@ -404,8 +408,9 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB, MODE>::kWarps, Kv8Sizes<
   float m[NB][2], l[NB][2];                       // references, and the sums of this thread's keys
 #pragma unroll
   for (int b = 0; b < NB; ++b) m[b][0] = m[b][1] = kNoScore, l[b][0] = l[b][1] = 0.f;
-  uint32_t power = (kLift + 1) << 23;              // what the values' scales are relative to, as bits
-  float unit = __uint_as_float(((254u + kLift) << 23) - power);
+  int unit[NB][2];                                // exponent bytes of u
+#pragma unroll
+  for (int b = 0; b < NB; ++b) unit[b][0] = unit[b][1] = kMostUnit;
 
   // A tile's work is S^T = K Q^T (products), the weights (weigh), and O^T += V^T P^T (multiply).  The last one runs beside the next tile's first:
   // neither waits for the other, and a tile's conversions fill the time of the other's products.  The tile's values wait in registers.
@@ -520,69 +525,79 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB, MODE>::kWarps, Kv8Sizes<
     for (int sub = 0; sub < kSubs; ++sub)
 #pragma unroll
       for (int mt = 0; mt < kMt; ++mt) read(at, WHOLE ? -1 : key0, sub, mt, v[sub][mt]);
-    bool see[kGroups];
-    uint32_t ve[kGroups], ve_most = 0u;            // scales of the values, as bits: larger ones are larger numbers
+    float vs[kGroups];                             // scales of the values; a row that is NaN has the byte 255, an infinity, and its codes of zero make a NaN of it
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
       const int key = key0 + kv8_key<HD>(g, i);
-      see[i] = WHOLE || (key >= w.span.first && key < w.span.len);
-      ve[i] = see[i] ? kv8_scale_of(v_exps, i) : 0u;
-      ve_most = max(ve_most, ve[i]);
-    }
-    bool moves = ve_most > power;
-    float most[NB][2];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      most[b][0] = most[b][1] = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < kGroups; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float& x = s[b][i >> 1][(i & 1) * 2 + j];
-          x = see[i] ? x * (__uint_as_float(kv8_scale_of(k_exps, i)) * factor[b][j]) : -INFINITY;
-          most[b][j] = fmaxf(most[b][j], x);
-        }
-    }
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) moves = moves || most[b][j] - m[b][j] > kSlack;      // m + kSlack is m or m + 16 from 2^27 on
-    if (__any_sync(0xffffffffu, moves)) {
-      // a row that is NaN has the byte 255: its scale stays an infinity, and its codes of zero make a NaN of it
-      const uint32_t now = max(power, __reduce_max_sync(0xffffffffu, min(ve_most, 253u << 23))), grown = (now - power) >> 23;
-      const float shrink = grown > 126u ? 0.f : __uint_as_float((127u - grown) << 23);
-      power = now;
-      unit = __uint_as_float(((254u + kLift) << 23) - now);
+      const bool see = WHOLE || (key >= w.span.first && key < w.span.len);
+      vs[i] = see ? __uint_as_float(kv8_scale_of(v_exps, i)) : 0.f;
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float mx = most[b][j];
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16)), m[b][j]);
-          const float c = zb_ex2(m[b][j] - mx);
-          m[b][j] = mx;
-          l[b][j] *= c;
-#pragma unroll
-          for (int i = 0; i < kSteps; ++i) {
-            o[b][i][j] *= c * shrink;
-            o[b][i][j + 2] *= c * shrink;
-          }
+          float& x = s[b][i >> 1][(i & 1) * 2 + j];
+          x = see ? x * (__uint_as_float(kv8_scale_of(k_exps, i)) * factor[b][j]) : -INFINITY;
         }
     }
-    float vs[kGroups];
+    float weight[NB][kGroups][2], sum[NB][2];
+    const auto weights = [&]() {                   // true: the references have to move
+      float most_p = 0.f, most = 0.f;
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i) vs[i] = __uint_as_float(ve[i]) * unit;
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+        for (int j = 0; j < 2; ++j) {
+          const float u = __uint_as_float(static_cast<uint32_t>(unit[b][j]) << 23);
+          sum[b][j] = 0.f;
 #pragma unroll
-      for (int i = 0; i < kGroups; ++i) {
-        const float p0 = zb_ex2(s[b][i >> 1][(i & 1) * 2] - m[b][0]), p1 = zb_ex2(s[b][i >> 1][(i & 1) * 2 + 1] - m[b][1]);
-        l[b][0] += p0;
-        l[b][1] += p1;
-        pb[b][i] = transpose8(pack_half2(p0 * vs[i], p1 * vs[i]));
-      }
+          for (int i = 0; i < kGroups; ++i) {
+            const float x = zb_ex2(s[b][i >> 1][(i & 1) * 2 + j] - m[b][j]);
+            sum[b][j] += x;
+            weight[b][i][j] = x * u * vs[i];
+            most_p = fmaxf(most_p, x);
+            most = fmaxf(most, weight[b][i][j]);
+          }
+        }
+      return most_p > kMostP || most > kMostWeight;
+    };
+    if (__any_sync(0xffffffffu, weights())) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const auto over_keys = [](float x) {
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          };
+          float mx = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < kGroups; ++i) mx = fmaxf(mx, s[b][i >> 1][(i & 1) * 2 + j]);
+          mx = fmaxf(ceilf(over_keys(mx)), m[b][j]);
+          const int rise = static_cast<int>(fminf(mx - m[b][j], 512.f));       // whole; no number (no references yet, infinities): 0 or 512
+          m[b][j] = mx;
+          float most = 0.f;
+#pragma unroll
+          for (int i = 0; i < kGroups; ++i) most = fmaxf(most, zb_ex2(s[b][i >> 1][(i & 1) * 2 + j] - mx) * fminf(vs[i], __uint_as_float(253u << 23)));
+          const int lower = 254 + kLift - static_cast<int>(__float_as_uint(over_keys(most)) >> 23);      // with which this tile's largest is 2^7 to 2^8
+          const int now = max(min(min(unit[b][j] + rise, lower), kMostUnit), kLeastUnit), fall = unit[b][j] + rise - now;
+          unit[b][j] = now;
+          l[b][j] *= __uint_as_float(static_cast<uint32_t>(max(127 - rise, 0)) << 23);
+          const float shrink = __uint_as_float(static_cast<uint32_t>(max(127 - fall, 0)) << 23);
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i) {
+            o[b][i][j] *= shrink;
+            o[b][i][j + 2] *= shrink;
+          }
+        }
+      weights();
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) l[b][j] += sum[b][j];
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) pb[b][i] = transpose8(pack_half2(weight[b][i][0], weight[b][i][1]));
+    }
   };
 
   for (int t = w.begin + warp; t < w.end; t += kWarps) {
@@ -608,7 +623,7 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB, MODE>::kWarps, Kv8Sizes<
     const float inv = sum == 0.f ? 0.f : 1.f / sum;    // a row that sees nothing is zero
     *reinterpret_cast<uint2*>(p.out + static_cast<size_t>(out_row + r) * HD + col) = make_uint2(zb_pack_bf16x2(x.x * inv, x.y * inv), zb_pack_bf16x2(x.z * inv, x.w * inv));
   };
-  const float power_of = __uint_as_float(power - (kLift << 23));
+  const auto one_over = [&](int b, int j) { return __uint_as_float(static_cast<uint32_t>(254 - unit[b][j]) << 23); };
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -624,9 +639,10 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB, MODE>::kWarps, Kv8Sizes<
       for (int j = 0; j < 2; ++j) {
         const int r = b * 8 + 2 * t4 + j;
         if (r >= rows) continue;
+        const float by = one_over(b, j);
 #pragma unroll
         for (int i = 0; i < kSteps; i += 2)
-          put(r, column(i), make_float4(o[b][i][j] * power_of, o[b][i][j + 2] * power_of, o[b][i + 1][j] * power_of, o[b][i + 1][j + 2] * power_of), l[b][j]);
+          put(r, column(i), make_float4(o[b][i][j] * by, o[b][i][j + 2] * by, o[b][i + 1][j] * by, o[b][i + 1][j + 2] * by), l[b][j]);
       }
     return;
   }
@@ -650,7 +666,7 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB, MODE>::kWarps, Kv8Sizes<
           float top = kNoScore;
 #pragma unroll
           for (int k = 0; k < kWarps; ++k) top = fmaxf(top, stats[(k * kRows + r) * 2]);
-          const float by = zb_ex2(m[b][j] - top) * power_of;
+          const float by = zb_ex2(m[b][j] - top) * one_over(b, j);
 #pragma unroll
           for (int i = 0; i < kSteps; i += 2) {
             float4* dst = reinterpret_cast<float4*>(sums + ((turns == 0 ? warp - kHalf : warp) * kRows + r) * kPitch + column(i));
