@@ -6,7 +6,7 @@ bf16, 2^-11 in f16.
 import pytest
 import torch
 
-from test_kv8 import DTYPES, INT8, gpu, sequence64, values64
+from test_kv8 import DTYPES, E4M3, INT8, gpu, sequence64, values64
 from zml_b200 import ops
 from zml_b200.ops import kv8
 
@@ -194,4 +194,59 @@ def test_scores_and_values_that_climb_and_fall(kind, lens, bound, step, down, hd
     q = q.cuda()
     out = ops.paged_decode(q, k, v, table, sl, scale=0.6931471805599453, max_seq_len=bound)
     check_closely(out, q, k, v, table, sl, 0.6931471805599453, [0], dtype is INT8)
+    ops.raise_on_status()
+
+
+# ------------------------------------------------------------------ writer
+TOP = [3.3895313892515355e38, 3.3762e38, 3.36e38, 3.3e38, 3.29e38, 3.2e38, 2.99e38, 2.98e38, 2.9e38, 1.7e38, 1e38]
+
+
+def check_top(cache, x):
+    """Rows x [tokens, heads, hd] of finite numbers up to bf16's largest: they stand for finite numbers, within half a step, or within a whole one where the
+    next step would be 2^128."""
+    got = values64(cache)[0, :, :x.shape[0]].transpose(0, 1).cpu()
+    back = read_back(cache, x.shape[0]).double().cpu()
+    assert torch.equal(got, back) and bool((back.abs() < 2.0 ** 128).all())
+    s = torch.exp2(cache.exponents[0, :, :x.shape[0]].t().double().cpu() - 127.0)[..., None]
+    x = x.double().cpu()
+    step = s * torch.ones_like(x)
+    if cache.codes.dtype is E4M3:
+        step = s * torch.exp2(torch.floor(torch.log2((x.abs() / s).clamp_min(2.0 ** -6)))) / 8
+    full = (back.abs() + step) >= 2.0 ** 128
+    assert bool(((x - back).abs() <= torch.where(full, step, step / 2)).all())
+
+
+def top_rows():
+    x = torch.randn(2 * len(TOP), 1, 64, generator=torch.Generator().manual_seed(1)) * 1e37
+    for i, t in enumerate(TOP):
+        x[2 * i, 0, 7 * i % 64], x[2 * i + 1, 0, (11 * i + 3) % 64] = t, -t
+    return x.bfloat16()
+
+
+@DTYPES
+def test_rows_up_to_the_largest_number_stay_finite_cpu(dtype):
+    x = top_rows()
+    cache = ops.QuantKV.alloc(1, 1, 32, 64, dtype)
+    codes, exps = kv8.quantize(x[:, 0], dtype)
+    cache.codes.view(torch.uint8)[0, 0, :len(x)], cache.exponents[0, 0, :len(x)] = codes.view(torch.uint8), exps
+    check_top(cache, x)
+
+
+@gpu
+@DTYPES
+@pytest.mark.parametrize("shift", [0, 1])
+def test_rows_up_to_the_largest_number_stay_finite(dtype, shift):
+    x = top_rows()
+    n = len(x)
+    buf = torch.zeros(n, 3 * 64 + 8, dtype=torch.bfloat16, device="cuda")
+    qkv = buf[:, shift:shift + 3 * 64]
+    qkv[:, 64:128], qkv[:, 128:] = x[:, 0].cuda(), x[:, 0].cuda()
+    k, v = (ops.QuantKV.alloc(1, 1, 32, 64, dtype, "cuda") for _ in range(2))
+    ids = torch.arange(n, dtype=torch.int32, device="cuda")
+    ops.rope_kvwrite(qkv, torch.zeros_like(ids), ids, torch.ones(32, device="cuda"), k, v, 1, 1, 64)
+    check_top(k, x)                                       # position 0 turns nothing
+    check_top(v, x)
+    codes, exps = kv8.quantize(x[:, 0], dtype)
+    for c in (k, v):
+        assert torch.equal(c.codes.view(torch.uint8)[0, 0, :n].cpu(), codes.view(torch.uint8)) and torch.equal(c.exponents[0, 0, :n].cpu(), exps)
     ops.raise_on_status()

@@ -233,8 +233,14 @@ __global__ void __launch_bounds__(512, 2) zb_kv8_write_kernel(const Kv8WritePara
         const ZbF2 inv = zb_pack2(by, by);
         const size_t at = static_cast<size_t>(row) + static_cast<size_t>(kvh) * p.page_size;
         uint2* dst = reinterpret_cast<uint2*>(codes + at * HD);
-        dst[a0] = make_uint2(kv8_codes4<INT8>(inv, f0[0], f0[1], finite), kv8_codes4<INT8>(inv, f0[2], f0[3], finite));
-        dst[a1] = make_uint2(kv8_codes4<INT8>(inv, f1[0], f1[1], finite), kv8_codes4<INT8>(inv, f1[2], f1[3], finite));
+        uint2 c0 = make_uint2(kv8_codes4<INT8>(inv, f0[0], f0[1], finite), kv8_codes4<INT8>(inv, f0[2], f0[3], finite));
+        uint2 c1 = make_uint2(kv8_codes4<INT8>(inv, f1[0], f1[1], finite), kv8_codes4<INT8>(inv, f1[2], f1[3], finite));
+        if (byte == kv8_top<INT8>()) {
+          c0 = make_uint2(kv8_below_top<INT8>(c0.x), kv8_below_top<INT8>(c0.y));
+          c1 = make_uint2(kv8_below_top<INT8>(c1.x), kv8_below_top<INT8>(c1.y));
+        }
+        dst[a0] = c0;
+        dst[a1] = c1;
         if (j == 0) exps[at] = static_cast<uint8_t>(byte);
       }
     }
@@ -305,7 +311,10 @@ __global__ void __launch_bounds__(256) zb_kv8_write_any_kernel(const Kv8WritePar
     const float inv = kv8_inverse(byte);
     const size_t at = kv8_row_at(p, slot, turned ? h - p.hq : h - p.hq - p.hkv);
     uint8_t* dst = (turned ? p.k_codes : p.v_codes) + at * hd;
-    for (int a = 0; a < hd / 32; ++a) dst[lane + 32 * a] = static_cast<uint8_t>(kv8_pack4<INT8>(inv, f[a], 0.f, 0.f, 0.f));
+    for (int a = 0; a < hd / 32; ++a) {
+      const uint32_t code = kv8_pack4<INT8>(inv, f[a], 0.f, 0.f, 0.f);
+      dst[lane + 32 * a] = static_cast<uint8_t>(byte == kv8_top<INT8>() ? kv8_below_top<INT8>(code) : code);
+    }
     if (lane == 0) (turned ? p.k_exps : p.v_exps)[at] = static_cast<uint8_t>(byte);
   }
 }

@@ -4,7 +4,8 @@
 // (e4m3) and 127 (int8), and its codes are x / 2^k, which is exact, rounded to the cache's type.  A power of two costs e4m3 nothing (a floating
 // format is as fine anywhere in its range) and int8 half a bit on average; in return codes times scale are bf16 numbers, so that attention over
 // prompts on a bf16 copy of the cache sees the very keys and values that attention of single tokens sees, and a scale is one byte, k + 127.
-// A row that holds an infinity or a NaN has the exponent byte 255 and codes of zero: it reads as NaN.
+// A row that holds an infinity or a NaN has the exponent byte 255 and codes of zero: it reads as NaN.  A number that would round to 2^128 takes the code below:
+// what is finite reads as finite.
 // Codes are [pages, kv_heads, page_size, HD], exponents [pages, kv_heads, page_size]: a page of one head is contiguous.
 #pragma once
 #include <cuda_bf16.h>
@@ -55,6 +56,15 @@ ZB_DEVICE uint32_t kv8_pack4(float inv, float x0, float x1, float x2, float x3) 
     const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(x2 * inv, x3 * inv), __NV_SATFINITE, __NV_E4M3);
     return a | (b << 16);
   }
+}
+// The largest exponent byte of finite rows, under which codes of 64 (int8) or 256 (e4m3) stand for 2^128, and four of its codes with those replaced by
+// the ones below, 63 and 240.  There are none above them.
+template <bool INT8>
+constexpr uint32_t kv8_top() { return INT8 ? 249u : 247u; }
+template <bool INT8>
+ZB_DEVICE uint32_t kv8_below_top(uint32_t w) {
+  if constexpr (INT8) return w - (__vcmpeq4(w, 0x40404040u) & 0x01010101u) + (__vcmpeq4(w, 0xc0c0c0c0u) & 0x01010101u);
+  else return w - (__vcmpeq4(w & 0x7f7f7f7fu, 0x78787878u) & 0x01010101u);
 }
 ZB_DEVICE uint32_t kv8_abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 

@@ -2,8 +2,9 @@
 
 A row is one token's key (or value) of one head, x of `hd` numbers.  Its scale is the smallest power of two 2^k with max |x| <= R 2^k, R = 448 for
 float8_e4m3fn and 127 for int8; its codes are x / 2^k rounded to the cache's type, and it stands for codes * 2^k, which are bf16 numbers: reading
-back is exact.  The scale is held as the byte k + 127.  A row that holds an infinity or a NaN has the byte 255 and codes of zero, and reads as
-NaN.  A row takes hd + 1 bytes where the bf16 cache has 2 hd.
+back is exact.  (A number that would round to 2^128 takes the code below, so that what is finite reads as finite.)  The scale is held as the byte
+k + 127.  A row that holds an infinity or a NaN has the byte 255 and codes of zero, and reads as NaN.  A row takes hd + 1 bytes where the bf16
+cache has 2 hd.
 
 The ops of the bf16 cache take a `QuantKV` in the place of a cache tensor: `ops.rope_kvwrite`, `ops.paged_decode`, `ops.paged_prefill`;
 `ops.paged_read` reads sequences back to bf16.  `QuantKVCache` is the whole cache of a model, indexed as the engine's bf16 tensor is.
@@ -137,6 +138,8 @@ def quantize(x: torch.Tensor, dtype=torch.float8_e4m3fn):
     byte = (exp - 1 - e + (2 * frac > m) + 127).clamp_min(MIN_EXPONENT)
     y = torch.where(ok[..., None], xf * _power(254 - byte)[..., None], 0.0)
     y = y.round() if dtype is torch.int8 else y
+    top, most = (249, 63.0) if dtype is torch.int8 else (247, 240.0)         # the largest byte, and its largest code below 2^128
+    y = torch.where((byte == top)[..., None], y.clamp(-most, most), y)
     return y.to(dtype), torch.where(ok, byte, NAN_EXPONENT).to(torch.uint8)
 
 
