@@ -6,7 +6,7 @@ bf16, 2^-11 in f16.
 import pytest
 import torch
 
-from test_kv8 import DTYPES, E4M3, INT8, gpu, sequence64, values64
+from test_kv8 import DTYPES, E4M3, INT8, gpu, paged, sequence64, values64
 from zml_b200 import ops
 from zml_b200.ops import kv8
 
@@ -250,3 +250,43 @@ def test_rows_up_to_the_largest_number_stay_finite(dtype, shift):
     for c in (k, v):
         assert torch.equal(c.codes.view(torch.uint8)[0, 0, :n].cpu(), codes.view(torch.uint8)) and torch.equal(c.exponents[0, 0, :n].cpu(), exps)
     ops.raise_on_status()
+
+
+# ------------------------------------------------------------------ prompts
+@DTYPES
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_a_bound_of_the_lengths_that_is_too_small_changes_nothing(device, dtype):
+    """`max_seq_len` chooses the kernel of `ops.paged_prefill`, whatever the cache."""
+    k, v, table, sl = paged([300, 70, 500], 2, 64, 128, dtype, 5, device)
+    q = torch.randn(30, 4, 128, generator=torch.Generator().manual_seed(4)).bfloat16().to(device)
+    starts = torch.tensor([0, 10, 20, 30], dtype=torch.int32, device=device)
+    want = ops.paged_prefill(q, k, v, table, sl, starts, impl="mma")
+    for bound in (1, 64, 100, 10 ** 6):
+        assert torch.equal(ops.paged_prefill(q, k, v, table, sl, starts, max_seq_len=bound, impl="mma"), want)
+    if device != "cpu":
+        ops.raise_on_status()
+
+
+@gpu
+@pytest.mark.parametrize("page", [16, 64, 128])
+def test_sequences_that_the_workspace_has_no_room_for(page):
+    """`kv_pages` below what the sequences hold: reported, and those that do not fit have outputs of zero and see nobody else's keys.  The first ones are
+    as they were."""
+    lens = [130, 70, 500]
+    k, v, table, sl = paged(lens, 2, page, 128, E4M3, 5, "cuda")
+    q = torch.randn(30, 4, 128, generator=torch.Generator().manual_seed(4)).bfloat16().cuda()
+    starts = torch.tensor([0, 10, 20, 30], dtype=torch.int32, device="cuda")
+    want = ops.paged_prefill(q, k, v, table, sl, starts)
+    ops.raise_on_status()
+    for total, whole in ((256, 2), (128, 2), (0, 1)):                            # tokens of the pages; room for 64 more behind each sequence
+        got = ops.paged_prefill(q, k, v, table, sl, starts, kv_pages=total // page)
+        with pytest.raises(ops.KernelError):
+            ops.raise_on_status()
+        assert torch.equal(got[:10 * whole], want[:10 * whole]) and not bool(got[10 * whole:].any())
+
+
+def test_sequences_that_the_workspace_has_no_room_for_cpu():
+    k, v, table, sl = paged([130, 70], 2, 64, 64, E4M3, 5)
+    q = torch.randn(4, 4, 64).bfloat16()
+    with pytest.raises(ValueError):
+        ops.paged_prefill(q, k, v, table, sl, torch.tensor([0, 2, 4], dtype=torch.int32), kv_pages=4)

@@ -332,7 +332,7 @@ struct Kv8ReadParams {
   const int32_t* block_table;
   const int32_t* seq_lens;
   int32_t* out_table;          // [batch, out_width]
-  int32_t* out_lens;           // [batch]: seq_lens within what the block table has, or null
+  int32_t* out_lens;           // [batch]: seq_lens within what the block table has, zero where the sequence is not read whole; or null
   int batch, hkv, log_pieces, page_size, max_pages, num_pages, out_size, out_width, out_pages;      // pieces: of 16 columns
   uint32_t inverse;            // 2^32 over the pieces of a token's row, rounded up
   ZbStatus* status;
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kReadThreads, kReadCtas) zb_kv8_read_kernel(co
     zb_record_error(p.status, ZB_ERR_BOUNDS, kKernelKv8Read, 1u, static_cast<uint32_t>(total));
   for (int s = blockIdx.x; s < p.batch; s += gridDim.x) {
     const int first = kv8_total(s, pages_of), n = pages_of(s);
-    if (p.out_lens != nullptr && threadIdx.x == 0) p.out_lens[s] = kv8_len(p.seq_lens, s, most);
+    if (p.out_lens != nullptr && threadIdx.x == 0) p.out_lens[s] = first + n <= p.out_pages ? kv8_len(p.seq_lens, s, most) : 0;
     for (int i = threadIdx.x; i < p.out_width; i += blockDim.x)
       p.out_table[static_cast<size_t>(s) * p.out_width + i] = i < n && first + i < p.out_pages ? first + i : 0;
   }

@@ -436,7 +436,8 @@ def paged_prefill(q, k_cache, v_cache, block_table, seq_lens, q_start, scale: fl
     `max_seq_len`: keys of the longest sequence, where the caller knows it (else the block table's width); it chooses the kernel only.
     `impl`: "auto" (the tcgen05 kernel where it applies and is the faster one), "tc" (require it) or "mma" (the mma.sync kernel).  `ext` (CUDA
     only, with `out`): a `gqa.AttnExt`, see `ops.gqa`.  `QuantKV` caches are read back to bf16 first (`ops.kv8`; no `ext`); `kv_pages`: pages
-    that the sequences hold together, where the caller knows it, which sizes that workspace.
+    that the sequences hold together, where the caller knows it, which sizes that workspace (sequences that do not fit are reported, and their
+    outputs are zero).
     """
     if isinstance(k_cache, QuantKV) or isinstance(v_cache, QuantKV):
         if ext is not None:

@@ -292,7 +292,7 @@ def paged_read(k: QuantKV, v: QuantKV, block_table, seq_lens, num_pages: Optiona
 
 def _read(k, v, block_table, seq_lens, size, width, n, lens=None):
     """`paged_read` into n pages of `size` tokens, `width` of a sequence at most, on the current device.  `lens` takes the lengths that were read:
-    no more than the block table has, none below zero."""
+    no more than the block table has, none below zero, and zero for a sequence that the n pages do not hold whole."""
     pages, heads, page_size, hd = k._shape
     kc = k._codes
     kd = block_table.new_empty((n, size, heads, hd), dtype=torch.bfloat16)
@@ -419,10 +419,11 @@ def paged_decode(q, k: QuantKV, v: QuantKV, block_table, seq_lens, scale: Option
 
 def paged_prefill(q, k: QuantKV, v: QuantKV, block_table, seq_lens, q_start, scale: Optional[float] = None, window: int = 0, out=None,
                   total_q_blocks: Optional[int] = None, impl: str = "auto", max_seq_len: Optional[int] = None, kv_pages: Optional[int] = None):
-    """`ops.paged_prefill` on a quantised cache: the sequences are read back to bf16 pages of 64 tokens, which is what the tcgen05 kernels take
-    (`kv_pages`: pages of the cache that they hold together, where the caller knows it), and the bf16 kernels attend to that.  Prompts are bound
-    by their products: reading back moves 6 bytes a key, head and column once, where every query of the group makes 4 operations of
-    them; the workspace lives as long as the call."""
+    """`ops.paged_prefill` on a quantised cache: the sequences are read back to bf16 pages of 64 tokens, which is what the tcgen05 kernels take, and the
+    bf16 kernels attend to that.  Prompts are bound by their products: reading back moves 6 bytes a key, head and column once, where every query
+    of the group makes 4 operations of them.  The workspace lives as long as the call; it holds what the block table could name, or, less,
+    `kv_pages` pages of the cache: what the sequences hold together, where the caller knows it.  Sequences that do not fit into that are
+    reported (`raise_on_status`), and their outputs are zero.  `max_seq_len` chooses the kernel only."""
     page_size = _pair(k, v)[2]
     b, width = _table(k, block_table, seq_lens)
     _queries(q, k, out)
@@ -439,8 +440,7 @@ def paged_prefill(q, k: QuantKV, v: QuantKV, block_table, seq_lens, q_start, sca
         if _current() != k._index:
             with torch.cuda.device(k._index):
                 return paged_prefill(q, k, v, block_table, seq_lens, q_start, scale, window, out, total_q_blocks, impl, max_seq_len, kv_pages)
-        most = width * page_size if max_seq_len is None else min(max_seq_len, width * page_size)
-        n = b * -(-most // 64)
+        n = b * -(-width * page_size // 64)
         if kv_pages is not None:                                             # at most 63 tokens behind each sequence
             n = min(n, kv_pages * page_size // 64 + b)
         lens = torch.empty_like(seq_lens)
