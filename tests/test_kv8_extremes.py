@@ -290,3 +290,18 @@ def test_sequences_that_the_workspace_has_no_room_for_cpu():
     q = torch.randn(4, 4, 64).bfloat16()
     with pytest.raises(ValueError):
         ops.paged_prefill(q, k, v, table, sl, torch.tensor([0, 2, 4], dtype=torch.int32), kv_pages=4)
+
+
+@DTYPES
+@pytest.mark.parametrize("group", [1, 2])
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_prompts_over_a_table_without_columns(device, group, dtype):
+    """New tokens of sequences that have no pages at all see nothing: the bf16 kernels are given a table with a column, which they read whatever the lengths are."""
+    k, v, _, _ = paged([5, 9], 2, 64, 64, dtype, 5, device)
+    i32 = dict(dtype=torch.int32, device=device)
+    q = torch.ones(70, 2 * group, 64, dtype=torch.bfloat16, device=device)
+    out = ops.paged_prefill(q, k, v, torch.zeros(2, 0, **i32), torch.tensor([0, 3], **i32), torch.tensor([0, 1, 70], **i32))
+    assert out.shape == q.shape and not bool(out.any())
+    if device != "cpu":
+        assert kv8._read(k, v, torch.zeros(2, 0, **i32), torch.tensor([0, 3], **i32), 64, 1, 1)[2].tolist() == [[0], [0]]
+        ops.raise_on_status()

@@ -444,6 +444,7 @@ def paged_prefill(q, k: QuantKV, v: QuantKV, block_table, seq_lens, q_start, sca
         if kv_pages is not None:                                             # at most 63 tokens behind each sequence
             n = min(n, kv_pages * page_size // 64 + b)
         lens = torch.empty_like(seq_lens)
-        kd, vd, table = _read(k, v, block_table, seq_lens, 64, -(-width * page_size // 64), max(1, n), lens)
+        columns = max(1, -(-width * page_size // 64))                        # the bf16 kernels read the first one, whatever the lengths are
+        kd, vd, table = _read(k, v, block_table, seq_lens, 64, columns, max(1, n), lens)
     a = bf16_prefill(q, kd, vd, table, lens, q_start, scale, window, out=out, total_q_blocks=total_q_blocks, impl=impl, max_seq_len=max_seq_len)
     return a if out is None or a is out else out.copy_(a)
