@@ -3,6 +3,9 @@
 Oracles are restatements in 64 bits; tolerances are derived beside their tests.  A rounding to a format is off by at most half a step: 2^-8 relative in
 bf16, 2^-11 in f16.
 """
+import threading
+import time
+
 import pytest
 import torch
 
@@ -305,3 +308,31 @@ def test_prompts_over_a_table_without_columns(device, group, dtype):
     if device != "cpu":
         assert kv8._read(k, v, torch.zeros(2, 0, **i32), torch.tensor([0, 3], **i32), 64, 1, 1)[2].tolist() == [[0], [0]]
         ops.raise_on_status()
+
+
+# ------------------------------------------------------------------ tickets of captured calls
+def test_captures_in_several_threads_draw_different_tickets(monkeypatch):
+    """What a captured call takes of the stock is its own, wherever threads take turns: the stock's counter gives way whenever it is written."""
+    class Slow(list):
+        def __setitem__(self, at, value):
+            super().__setitem__(at, value)
+            time.sleep(1e-4)
+
+    stock = Slow([torch.zeros(1 << 16, dtype=torch.int32), 0])
+    monkeypatch.setattr(kv8, "_CAPTURED", {0: stock})
+    monkeypatch.setattr(kv8, "_capturing", lambda: True)
+    got, q = [], torch.zeros(1)
+
+    def capture():
+        for n in range(1, 40):
+            t = kv8._tickets(q, 0, 0, n)
+            got.append((t.data_ptr(), t.data_ptr() + 4 * t.numel()))
+
+    threads = [threading.Thread(target=capture) for _ in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    got.sort()
+    assert len(got) == 6 * 39 and all(a[1] <= b[0] for a, b in zip(got, got[1:]))
+    assert got[0][0] == stock[0].data_ptr() and got[-1][1] <= stock[0].data_ptr() + 4 * (1 << 16)

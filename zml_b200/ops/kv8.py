@@ -16,6 +16,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import struct
+import threading
 from typing import Optional
 
 import torch
@@ -348,7 +349,8 @@ def _plan(index, b, hq, hkv, hd, max_len) -> tuple[int, int]:
 
 
 _TICKETS: dict = {}
-_CAPTURED: dict = {}
+_CAPTURED: dict = {}                                                      # device -> [stock, how much of it captured calls have]
+_STOCK = threading.Lock()                                                 # captures of several threads take pieces of one stock
 CAPTURED_TICKETS = 1 << 20
 
 
@@ -357,15 +359,18 @@ def _tickets(q, index: int, stream: int, n: int):
     share theirs.  Graphs may be replayed on any streams, so a captured call has its own for good: a piece of a stock that an earlier eager call
     has cleared, or, where there is none or it has come to an end, an allocation that every replay clears."""
     if _capturing():
-        stock = _CAPTURED.get(index)
-        if stock is None or stock[1] + n > CAPTURED_TICKETS:
-            return q.new_zeros((n,), dtype=torch.int32)
-        stock[1] += n
-        return stock[0][stock[1] - n:stock[1]]
+        with _STOCK:
+            stock = _CAPTURED.get(index)
+            if stock is not None and stock[1] + n <= CAPTURED_TICKETS:
+                at = stock[1]
+                stock[1] = at + n
+                return stock[0][at:at + n]
+        return q.new_zeros((n,), dtype=torch.int32)
     if index not in _CAPTURED:
         stock = q.new_zeros((CAPTURED_TICKETS,), dtype=torch.int32)
         torch.cuda.current_stream(index).synchronize()                       # whatever stream replays
-        _CAPTURED[index] = [stock, 0]
+        with _STOCK:
+            _CAPTURED.setdefault(index, [stock, 0])                          # another thread's may be in use already
     got = _TICKETS.get((index, stream))
     if got is None or got.numel() < n:
         if len(_TICKETS) >= 256:
