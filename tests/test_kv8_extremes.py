@@ -3,6 +3,9 @@
 Oracles are restatements in 64 bits; tolerances are derived beside their tests.  A rounding to a format is off by at most half a step: 2^-8 relative in
 bf16, 2^-11 in f16.
 """
+import os
+import subprocess
+import sys
 import threading
 import time
 
@@ -336,3 +339,37 @@ def test_captures_in_several_threads_draw_different_tickets(monkeypatch):
     got.sort()
     assert len(got) == 6 * 39 and all(a[1] <= b[0] for a, b in zip(got, got[1:]))
     assert got[0][0] == stock[0].data_ptr() and got[-1][1] <= stock[0].data_ptr() + 4 * (1 << 16)
+
+
+# ------------------------------------------------------------------ the bounds-checking build
+_BOUNDS_WORKER = """
+import torch
+from zml_b200 import ops
+from zml_b200.models.llama import PRESETS, LlamaConfig, LlamaModel
+from zml_b200.ops import _lib
+from zml_b200.serving import Engine
+assert _lib.bounds_check_build()
+m = LlamaModel(LlamaConfig.from_hf(dict(PRESETS["tiny-llama-test"])), device="cuda").init_random(seed=3, std=0.05)
+for page, pages in ((128, 7), (16, 40), (320, 3), (64, 11)):
+    prompts = [[(7 * i + j) % 1000 for i in range(n)] for j, n in enumerate((300, 50, 129) if page != 320 else (500,))]
+    e = Engine(m, num_pages=pages, page_size=page, max_batch=4, max_seq_len=640, kv_dtype="fp8", use_graphs=False)
+    outs = e.generate(prompts, max_new_tokens=3)[0]
+    assert all(len(o) == 3 for o in outs)
+    ops.raise_on_status()
+print("CLEAN", flush=True)
+"""
+
+
+@gpu
+def test_the_bounds_checking_build_knows_the_pages_of_the_copy(tmp_path):
+    """Attention over prompts reads a copy in pages of 64 tokens, of which there are more than pages of 128 in the cache: page numbers of the copy are no
+    offence."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    so = os.path.join(root, "zml_b200", "_C", "libzb_cuda_bc.so")
+    if not os.path.exists(so):
+        from zml_b200 import _build
+        _build.build_cuda(extra_flags=["-DZB_BOUNDS_CHECK", "-rdc=true"], variant="bc")
+    script = tmp_path / "w.py"
+    script.write_text(_BOUNDS_WORKER)
+    r = subprocess.run([sys.executable, str(script)], capture_output=True, text=True, timeout=600, env={**os.environ, "ZB_CUDA_LIB": so, "PYTHONPATH": root})
+    assert r.returncode == 0 and "CLEAN" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]

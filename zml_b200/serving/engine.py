@@ -149,7 +149,9 @@ class Engine:
             model.alloc_state(self.num_slots + 1)
         if self.on_gpu:
             # read by the bounds-checking build of the library only: the extents kernel arguments do not carry
-            _lib.set_bounds_extents(num_pages, self.num_slots + 1 if self.stateful else 0)
+            # (of an 8-bit cache, whose own kernels always check: the copy for prompts, in pages of 64 tokens)
+            pages = num_pages if kv_dtype is None else num_pages * -(-page_size // 64)
+            _lib.set_bounds_extents(pages, self.num_slots + 1 if self.stateful else 0)
 
     # ------------------------------------------------------------------ helpers
     def set_seed(self, seed: int) -> None:
