@@ -119,7 +119,7 @@ def test_scores_where_fp32_counts_in_sixteens(kind, lens, bound, hd, dtype):
     ops.raise_on_status()
 
 
-def check_closely(out, q, k, v, table, lens, scale, which, int8):
+def check_closely(out, q, k, v, table, lens, scale, which, int8, window=0):
     """Rows `which` of a decode call against 64 bits, each key with its own share of the tolerance.
 
     bf16 rounds the result (2^-8); a weight is rounded to f16 (2^-11), or lies among f16's subnormals (half a step of 2^-24, where the largest p s_v
@@ -133,7 +133,9 @@ def check_closely(out, q, k, v, table, lens, scale, which, int8):
     for i in which:
         n = int(lens[i])
         ks, vs = sequence64(k, table[i], n), sequence64(v, table[i], n)
-        scales = torch.exp2(v.exponents[table[i, :-(-n // 64)].long()].double() - 127.0).transpose(1, 2).reshape(-1, hkv)[:n]
+        scales = torch.exp2(v.exponents[table[i, :-(-n // v.page_size)].long()].double() - 127.0).transpose(1, 2).reshape(-1, hkv)[:n]
+        first = max(0, n - window) if window else 0
+        n, ks, vs, scales = n - first, ks[first:], vs[first:], scales[first:]
         for h in range(q.shape[1]):
             kh, vh, qh = ks[:, h // group], vs[:, h // group], q[i, h].double()
             delta = (hd + 8) * 2.0 ** -24 * abs(scale) * (kh.abs() @ qh.abs()) + 2.0 ** -21
