@@ -873,9 +873,13 @@ int zb_kv8_decode_plan(int batch, int hq, int hkv, int hd, int max_len, long lon
   if (pairs * size <= most && longest * tile <= size * warps * 256) return -size;
   // More pairs than CTAs, none of them long: a warp for each, where a CTA for each takes a turn per 296 of them, most of it spent on getting
   // under way (us, heads of 128, a warp / a CTA: 512 pairs of 40, 300, 1000 keys 5.2 / 8.1, 13.4 / 16.1, 32.3 / 27.6, 1024 pairs of 1000 44.9 / 51.3,
-  // 8000 of 30 28.8 / 93.2)
+  // 8000 of 30 28.8 / 93.2).  Up to 2048 keys, as a warp is alone with its pair: 4096 pairs of 1000, 2000, 4000 keys 162 / 166, 309 / 307, 604 / 591, but
+  // eight of 1000, 2048, 4000 among 4088 of 100: 41 / 64, 61 / 66, 95 / 70
   if (batch > kMaxBatch || (pairs > most && longest * tile <= 2048 && longest * tile * most <= pairs * 300)) return 0;
-  // Too many to cut: a CTA for each, which need not look at the other lengths (512 pairs of 1024 keys: 28.5 us, 31.5 with that look)
+  // Too many to cut: a CTA for each, which need not look at the other lengths.  Up to 2048 keys, as a CTA is alone with its pair: that is what one long
+  // sequence costs among short ones, where of sequences of equal or evenly spread lengths chunks are 1 - 3 us slower at any length (us, heads of 128, 8 of
+  // a sequence, a CTA / chunks: 32 sequences of 1000, 2000, 3000 keys 15.2 / 16.4, 25.0 / 26.4, 34.4 / 35.7, 128 - 2048 21.6 / 22.9, 200 - 3000 29.0 / 30.2;
+  // one of 1000, 2048, 3000, 8000 among 31 of 100 9.6 / 9.4, 14.9 / 11.1, 20.5 / 11.5, 47.0 / 19.4, among 63 11.2 / 12.6, 16.4 / 14.0, 22.0 / 15.1, 49.4 / 17.7)
   if (2 * pairs > most && longest * tile <= 2048) return -1;
   const int parts = static_cast<int>(std::min<long long>(tiles, most));
   *floats = slots_of(parts) * rows * (hd + 2);
