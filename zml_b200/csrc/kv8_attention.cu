@@ -10,12 +10,14 @@
 //   128 are 32 registers.  P^T reaches its operand layout by transposes of 8 x 8.
 // * e4m3 and int8 are subsets of f16: codes are converted two at a time and multiplied by m16n8k16 with fp32 sums.  (m16n8k32 of e4m3 is made of
 //   the same conversions and products on this GPU, and more of them.)  A query row is scaled by a power of two to a largest magnitude in [2^13,
-//   2^14), exactly, and that power is taken out of its scores.  int8 has a product of its own for S^T, m16n8k32 with int32 sums, without
-//   conversions: the query is 256 times one int8 number and another (the largest of a row in [2^14, 2^15), half a unit is lost).
+//   2^14), exactly where its numbers are 2^-30 of that or more, and that power is taken out of its scores.  int8 has a product of its own for S^T,
+//   m16n8k32 with int32 sums, without conversions: the query is 256 times one int8 number and another, the largest of a row in [2^14, 2^15).  Half a unit is
+//   lost, so numbers below 2^-7 of the largest keep fewer bits than bf16 gave them, and a score moves by up to 2^-15 of the query's largest times the sum of the
+//   key's magnitudes; rounding the key to int8 moved it by up to 2^-8 of the key's largest times the sum of the query's.
 // * f16 does not hold every product p_j s_vj: every query head has a second reference, a power of two u with which its largest p_j s_vj so far is
 //   between 2^7 and 2^15, and which rescales its accumulators like the reference of the scores does.  What f16 drops lies 2^-32 below that head's largest
 //   product, whatever the scales of values are whose keys it does not look at.  (One power for all heads, taken from the scales alone, is two instructions a weight
-//   less and loses everything 2^32 below the largest scale, whether or not it has any weight.)
+//   less, 2 us of 31 for 8000 pairs of 30 keys and nothing for long ones, and loses everything 2^32 below the largest scale, whether or not that has any weight.)
 // * The contraction may take the columns of a head in any order, the output columns may lie anywhere, and so may the keys in the rows, so every
 //   thread reads its operands as whole 16-byte pieces of a row and the exponents of its keys (four; two of a head of 256) as one word.  Rows are 128 bytes in shared memory
 //   (half a row of a head of 256, two rows of a head of 64) in the 128-byte swizzle of the tensor-map copy; kv8_key says which key lies in
@@ -261,8 +263,8 @@ struct Kv8Sizes {
   static constexpr int kGroups = kv8_groups<HD>(), kTile = 8 * kGroups;      // keys of a tile
   static constexpr int kTileBytes = kTile * HD;
   static constexpr int kStageBytes = 2 * kTileBytes;
-  // A warp for each pair of heads of 64 has registers and shared memory for 15 on an SM, of three stages: 8000 pairs of 30 keys take 16.0 us, where 12 of
-  // four stages take 18.0 and 8 of six 23.3
+  // A warp for each pair of heads of 64 has registers and shared memory for 15 on an SM, of three stages: 8000 pairs of 30 keys take 17.0 us, where 12 of
+  // four stages take 19.1 and 8 of six 24.5
   static constexpr bool kMany = HD == 64 && NB == 1 && MODE == kWarp;
   static constexpr int kStages = HD == 64 && !kMany ? 6 : 3;
   static constexpr int kWarps = MODE == kWarp ? 1 : 4, kCtas = (kMany ? 15 : 8) / kWarps;      // of a CTA, and CTAs on an SM
@@ -516,7 +518,7 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB, MODE>::kWarps, Kv8Sizes<
   };
 
   // !WHOLE: some of the keys lie behind the end or in front of the window
-  const auto weigh = [&](auto whole, uint32_t at, uint32_t ex, int key0) {
+  const auto weigh = [&](auto whole, bool first, uint32_t at, uint32_t ex, int key0) {
     constexpr bool WHOLE = decltype(whole)::value;
     uint32_t k_exps, v_exps;
     if constexpr (kGroups == 4) k_exps = __byte_perm(lds32(ex), 0u, turn), v_exps = __byte_perm(lds32(ex + kTile), 0u, turn);
@@ -539,64 +541,84 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB, MODE>::kWarps, Kv8Sizes<
           x = see ? x * (__uint_as_float(kv8_scale_of(k_exps, i)) * factor[b][j]) : -INFINITY;
         }
     }
-    float weight[NB][kGroups][2], sum[NB][2];
-    const auto weights = [&]() {                   // true: the references have to move
-      float most_p = 0.f, most = 0.f;
+    float chance[NB][2][kGroups], weight[NB][2][kGroups], sum[NB][2], most_p = 0.f, most = 0.f;
+    const auto chances = [&](int b, int j) {       // p_j of a head
+      sum[b][j] = 0.f;
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float u = __uint_as_float(static_cast<uint32_t>(unit[b][j]) << 23);
-          sum[b][j] = 0.f;
-#pragma unroll
-          for (int i = 0; i < kGroups; ++i) {
-            const float x = zb_ex2(s[b][i >> 1][(i & 1) * 2 + j] - m[b][j]);
-            sum[b][j] += x;
-            weight[b][i][j] = x * u * vs[i];
-            most_p = fmaxf(most_p, x);
-            most = fmaxf(most, weight[b][i][j]);
-          }
-        }
-      return most_p > kMostP || most > kMostWeight;
+      for (int i = 0; i < kGroups; ++i) {
+        chance[b][j][i] = zb_ex2(s[b][i >> 1][(i & 1) * 2 + j] - m[b][j]);
+        sum[b][j] += chance[b][j][i];
+        most_p = fmaxf(most_p, chance[b][j][i]);
+      }
     };
-    if (__any_sync(0xffffffffu, weights())) {
+    const auto weights = [&](int b, int j) {       // p_j s_vj u
+      const float u = __uint_as_float(static_cast<uint32_t>(unit[b][j]) << 23);
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+        weight[b][j][i] = chance[b][j][i] * u * vs[i];
+        most = fmaxf(most, weight[b][j][i]);
+      }
+    };
+    if (!first) {                                  // a warp's first tile has no references yet
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
+        for (int j = 0; j < 2; ++j) chances(b, j), weights(b, j);
+    }
+    if (__any_sync(0xffffffffu, first || most_p > kMostP || most > kMostWeight)) {
+      int rise[NB][2], fall[NB][2];                // what both references rise by together, and 1 / u by
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        uint32_t tops = 0u;                        // exponent bytes of this tile's largest p_j s_vj of both columns
+#pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const auto over_keys = [](float x) {
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-            return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          };
           float mx = -INFINITY;
 #pragma unroll
           for (int i = 0; i < kGroups; ++i) mx = fmaxf(mx, s[b][i >> 1][(i & 1) * 2 + j]);
-          mx = fmaxf(ceilf(over_keys(mx)), m[b][j]);
-          const int rise = static_cast<int>(fminf(mx - m[b][j], 512.f));       // whole; no number (no references yet, infinities): 0 or 512
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(ceilf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16))), m[b][j]);
+          rise[b][j] = static_cast<int>(fminf(mx - m[b][j], 512.f));         // whole; no number (no references yet, infinities): 0 or 512
           m[b][j] = mx;
-          float most = 0.f;
+          chances(b, j);
+          float top = 0.f;
 #pragma unroll
-          for (int i = 0; i < kGroups; ++i) most = fmaxf(most, zb_ex2(s[b][i >> 1][(i & 1) * 2 + j] - mx) * fminf(vs[i], __uint_as_float(253u << 23)));
-          const int lower = 254 + kLift - static_cast<int>(__float_as_uint(over_keys(most)) >> 23);      // with which this tile's largest is 2^7 to 2^8
-          const int now = max(min(min(unit[b][j] + rise, lower), kMostUnit), kLeastUnit), fall = unit[b][j] + rise - now;
-          unit[b][j] = now;
-          l[b][j] *= __uint_as_float(static_cast<uint32_t>(max(127 - rise, 0)) << 23);
-          const float shrink = __uint_as_float(static_cast<uint32_t>(max(127 - fall, 0)) << 23);
-#pragma unroll
-          for (int i = 0; i < kSteps; ++i) {
-            o[b][i][j] *= shrink;
-            o[b][i][j + 2] *= shrink;
-          }
+          for (int i = 0; i < kGroups; ++i) top = fmaxf(top, chance[b][j][i] * fminf(vs[i], __uint_as_float(253u << 23)));
+          tops |= __float_as_uint(top) >> 23 << (16 * j);
         }
-      weights();
+        tops = __vmaxu2(tops, __shfl_xor_sync(0xffffffffu, tops, 4));
+        tops = __vmaxu2(tops, __shfl_xor_sync(0xffffffffu, tops, 8));
+        tops = __vmaxu2(tops, __shfl_xor_sync(0xffffffffu, tops, 16));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int lower = 254 + kLift - static_cast<int>(tops >> (16 * j) & 255u);      // with which this tile's largest is 2^7 to 2^8
+          const int now = max(min(min(unit[b][j] + rise[b][j], lower), kMostUnit), kLeastUnit);
+          fall[b][j] = unit[b][j] + rise[b][j] - now;
+          unit[b][j] = now;
+          weights(b, j);
+        }
+      }
+      if (!first) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            l[b][j] *= __uint_as_float(static_cast<uint32_t>(max(127 - rise[b][j], 0)) << 23);
+            const float shrink = __uint_as_float(static_cast<uint32_t>(max(127 - fall[b][j], 0)) << 23);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+              o[b][i][j] *= shrink;
+              o[b][i][j + 2] *= shrink;
+            }
+          }
+      }
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) l[b][j] += sum[b][j];
 #pragma unroll
-      for (int i = 0; i < kGroups; ++i) pb[b][i] = transpose8(pack_half2(weight[b][i][0], weight[b][i][1]));
+      for (int i = 0; i < kGroups; ++i) pb[b][i] = transpose8(pack_half2(weight[b][0][i], weight[b][1][i]));
     }
   };
 
@@ -609,8 +631,8 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB, MODE>::kWarps, Kv8Sizes<
     if (w.span.len > 0) {
       products(at);
       multiply_all();
-      if (key0 >= w.span.first && key0 + kTile <= w.span.len) weigh(std::true_type(), at, ex, key0);
-      else weigh(std::false_type(), at, ex, key0);
+      if (key0 >= w.span.first && key0 + kTile <= w.span.len) weigh(std::true_type(), t == w.begin + warp, at, ex, key0);
+      else weigh(std::false_type(), t == w.begin + warp, at, ex, key0);
     }
     if (++stage == kStages) stage = 0;
   }
@@ -864,16 +886,16 @@ int zb_kv8_decode_plan(int batch, int hq, int hkv, int hd, int max_len, long lon
   if (tiles > 0x3fffffffll) return INT_MIN;
   const int most = st->num_sms * 2;
   // CTAs for a pair: as many as give each warp a tile and fit on the GPU at once.  Of clusters of 16 only half as many fit, as each lies within a part of the
-  // GPU (16 pairs of 8000 keys: 17.5 us in clusters of 16, 13.7 of eight)
+  // GPU (16 pairs of 8000 keys: 18.0 us in clusters of 16, 13.8 of eight)
   int size = 1;
   while (size < 16 && size * warps < longest && pairs * size * 2 <= (size == 8 ? most / 2 : most)) size *= 2;
   // Up to 256 keys a warp a cluster is better than chunks, which look at all lengths and join through memory (us, heads of 128, a cluster / chunks: 8 pairs of
-  // 5000 and 10000 keys 8.5 / 10.2, 10.4 / 12.4, 64 of 4000 15.6 / 18.7, 128 of 1800 15.1 / 17.6), also where lengths differ (64 of
-  // 500 - 4000 14.2 / 14.4; 16 of 300 - 8000 11.7 / 11.0); beyond, the longest sequence keeps the others waiting (64 of 100 - 8000 21.8 / 18.6)
+  // 5000 and 10000 keys 8.7 / 10.4, 10.6 / 12.6, 64 of 4000 15.9 / 18.8, 128 of 1800 15.2 / 18.0), also where lengths differ (64 of
+  // 500 - 4000 14.3 / 14.5; 16 of 300 - 8000 11.6 / 11.1); beyond, the longest sequence keeps the others waiting (64 of 100 - 8000 21.8 / 19.0)
   if (pairs * size <= most && longest * tile <= size * warps * 256) return -size;
   // More pairs than CTAs, none of them long: a warp for each, where a CTA for each takes a turn per 296 of them, most of it spent on getting
-  // under way (us, heads of 128, a warp / a CTA: 512 pairs of 40, 300, 1000 keys 5.2 / 8.1, 13.4 / 16.1, 32.3 / 27.6, 1024 pairs of 1000 44.9 / 51.3,
-  // 8000 of 30 28.8 / 93.2).  Up to 2048 keys, as a warp is alone with its pair: 4096 pairs of 1000, 2000, 4000 keys 162 / 166, 309 / 307, 604 / 591, but
+  // under way (us, heads of 128, a warp / a CTA: 512 pairs of 40, 300, 1000 keys 5.6 / 8.2, 13.7 / 16.4, 32.8 / 28.2, 1024 pairs of 1000 45.0 / 51.7,
+  // 8000 of 30 31.1 / 97.7).  Up to 2048 keys, as a warp is alone with its pair: 4096 pairs of 1000, 2000, 4000 keys 162 / 166, 309 / 307, 604 / 591, but
   // eight of 1000, 2048, 4000 among 4088 of 100: 41 / 64, 61 / 66, 95 / 70
   if (batch > kMaxBatch || (pairs > most && longest * tile <= 2048 && longest * tile * most <= pairs * 300)) return 0;
   // Too many to cut: a CTA for each, which need not look at the other lengths.  Up to 2048 keys, as a CTA is alone with its pair: that is what one long
