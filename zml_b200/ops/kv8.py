@@ -382,7 +382,8 @@ def _tickets(q, index: int, stream: int, n: int):
 def paged_decode(q, k: QuantKV, v: QuantKV, block_table, seq_lens, scale: Optional[float] = None, window: int = 0,
                  max_seq_len: Optional[int] = None, out=None):
     """`ops.paged_decode` on a quantised cache.  The keys are split over the GPU on the device, from the lengths there (`max_seq_len` bounds
-    the launch only); any number of query heads for a key head."""
+    the launch only); any number of query heads for a key head.  Sums are fp32; weights times values' scales are f16, 2^-11 each and 2^-32 of a head's largest;
+    beside int8 keys a query's numbers are rounded to 2^-15 of its largest."""
     pages, hkv, page_size, _ = _pair(k, v)
     sequences, width = _table(k, block_table, seq_lens)
     b, hq, hd = _queries(q, k, out)
@@ -425,10 +426,10 @@ def paged_decode(q, k: QuantKV, v: QuantKV, block_table, seq_lens, scale: Option
 def paged_prefill(q, k: QuantKV, v: QuantKV, block_table, seq_lens, q_start, scale: Optional[float] = None, window: int = 0, out=None,
                   total_q_blocks: Optional[int] = None, impl: str = "auto", max_seq_len: Optional[int] = None, kv_pages: Optional[int] = None):
     """`ops.paged_prefill` on a quantised cache: the sequences are read back to bf16 pages of 64 tokens, which is what the tcgen05 kernels take, and the
-    bf16 kernels attend to that.  Prompts are bound by their products: reading back moves 6 bytes a key, head and column once, where every query
-    of the group makes 4 operations of them.  The workspace lives as long as the call; it holds what the block table could name, or, less,
-    `kv_pages` pages of the cache: what the sequences hold together, where the caller knows it.  Sequences that do not fit into that are
-    reported (`raise_on_status`), and their outputs are zero.  `max_seq_len` chooses the kernel only."""
+    bf16 kernels attend to that.  Prompts with many new tokens are bound by their products: reading back moves 6 bytes a key, head and column once,
+    where every query of the group makes 4 operations of them.  Few new tokens on a long past read the whole past back, too.  The workspace
+    lives as long as the call; it holds what the block table could name, or, less, `kv_pages` pages of the cache: what the sequences hold
+    together, where the caller knows it.  Sequences that do not fit into that are reported (`raise_on_status`), and their outputs are zero.  `max_seq_len` chooses the kernel only."""
     page_size = _pair(k, v)[2]
     b, width = _table(k, block_table, seq_lens)
     _queries(q, k, out)
