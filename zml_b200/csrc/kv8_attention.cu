@@ -16,13 +16,14 @@
 //   key's magnitudes; rounding the key to int8 moved it by up to 2^-8 of the key's largest times the sum of the query's.
 // * f16 does not hold every product p_j s_vj: every query head has a second reference, a power of two u with which its largest p_j s_vj so far is
 //   between 2^7 and 2^15, and which rescales its accumulators like the reference of the scores does.  What f16 drops lies 2^-32 below that head's largest
-//   product, whatever the scales of values are whose keys it does not look at.  (One power for all heads, taken from the scales alone, is two instructions a weight
-//   less, 2 us of 31 for 8000 pairs of 30 keys and nothing for long ones, and loses everything 2^32 below the largest scale, whether or not that has any weight.)
+//   product, whatever the scales of values are whose keys it does not look at.  (One power for all heads, taken from the scales alone, saves 3 % of
+//   groups of 16 heads, 7 % of 8000 pairs of 30 keys and nothing of long sequences with up to eight heads, and loses everything 2^32 below the largest
+//   scale, whether or not that has any weight.)
 // * The contraction may take the columns of a head in any order, the output columns may lie anywhere, and so may the keys in the rows, so every
 //   thread reads its operands as whole 16-byte pieces of a row and the exponents of its keys (four; two of a head of 256) as one word.  Rows are 128 bytes in shared memory
 //   (half a row of a head of 256, two rows of a head of 64) in the 128-byte swizzle of the tensor-map copy; kv8_key says which key lies in
 //   which row, so that the pieces that eight neighbouring lanes read lie in different banks, in both products.
-// * Both references move only when a p_j exceeds 2^8 or a p_j s_vj u 2^15: a warp looks for that with one vote, where keeping the very maximum takes three
+// * Both references move only when a thread's p_j add up to more than 2^8 or a p_j s_vj u exceeds 2^15: a warp looks for that with one vote, where keeping the very maximum takes three
 //   shuffles a column and a multiplication of all accumulators nearly every time.  The reference of scores is a whole number, so that both rescale by
 //   powers of two, exactly.
 // * Every warp has a ring of tiles of 32 keys (heads of 256: 16) of its own and waits for nobody while it streams; the sums of a CTA's four warps
@@ -51,8 +52,8 @@ constexpr uint32_t kKernelKv8Decode = 41;
 constexpr int kMaxBatch = 8192;                 // sequences whose lengths a CTA looks at: beyond, pairs are not cut
 constexpr int kMinChunk = 8;                    // tiles: two for each warp
 constexpr float kNoScore = -3.402823466e38f;    // the reference in front of the first key
-constexpr float kMostP = 256.f;                 // what p_j may grow to before the references move
-constexpr float kMostWeight = 32768.f;          // and p_j s_vj u, which is an f16 number
+constexpr float kMostP = 256.f;                 // what the p_j of a thread's keys may add up to before the references move
+constexpr unsigned short kMostWeight = 0x7800;  // and p_j s_vj u grow to: 2^15 in f16
 constexpr int kLift = 7;                        // log2 of what the largest p_j s_vj u is, at least, when they have moved
 constexpr int kMostUnit = 237, kLeastUnit = 7;  // u is 2^-120 to 2^110, as exponent bytes: 1 / u, and p_j u, are numbers, too
 
@@ -263,7 +264,7 @@ struct Kv8Sizes {
   static constexpr int kGroups = kv8_groups<HD>(), kTile = 8 * kGroups;      // keys of a tile
   static constexpr int kTileBytes = kTile * HD;
   static constexpr int kStageBytes = 2 * kTileBytes;
-  // A warp for each pair of heads of 64 has registers and shared memory for 15 on an SM, of three stages: 8000 pairs of 30 keys take 17.0 us, where 12 of
+  // A warp for each pair of heads of 64 has registers and shared memory for 15 on an SM, of three stages: 8000 pairs of 30 keys take 16.9 us, where 12 of
   // four stages take 19.1 and 8 of six 24.5
   static constexpr bool kMany = HD == 64 && NB == 1 && MODE == kWarp;
   static constexpr int kStages = HD == 64 && !kMany ? 6 : 3;
@@ -533,43 +534,52 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB, MODE>::kWarps, Kv8Sizes<
       const int key = key0 + kv8_key<HD>(g, i);
       const bool see = WHOLE || (key >= w.span.first && key < w.span.len);
       vs[i] = see ? __uint_as_float(kv8_scale_of(v_exps, i)) : 0.f;
+      const float ks = __uint_as_float(kv8_scale_of(k_exps, i));
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float& x = s[b][i >> 1][(i & 1) * 2 + j];
-          x = see ? x * (__uint_as_float(kv8_scale_of(k_exps, i)) * factor[b][j]) : -INFINITY;
-        }
+      for (int b = 0; b < NB; ++b) {
+        float& x = s[b][i >> 1][(i & 1) * 2];
+        float& y = s[b][i >> 1][(i & 1) * 2 + 1];
+        zb_unpack2(zb_mul2(zb_pack2(x, y), zb_mul2(zb_pack2(ks, ks), zb_pack2(factor[b][0], factor[b][1]))), x, y);
+        if (!see) x = y = -INFINITY;
+      }
     }
-    float chance[NB][2][kGroups], weight[NB][2][kGroups], sum[NB][2], most_p = 0.f, most = 0.f;
-    const auto chances = [&](int b, int j) {       // p_j of a head
-      sum[b][j] = 0.f;
+    // both columns' numbers go in packed pairs
+    ZbF2 chance[NB][kGroups], sum[NB];
+    uint32_t weight[NB][kGroups];
+    bool moves = false;
+    const auto chances = [&](int b) {              // p_j
+      const ZbF2 less = zb_pack2(-m[b][0], -m[b][1]);
 #pragma unroll
       for (int i = 0; i < kGroups; ++i) {
-        chance[b][j][i] = zb_ex2(s[b][i >> 1][(i & 1) * 2 + j] - m[b][j]);
-        sum[b][j] += chance[b][j][i];
-        most_p = fmaxf(most_p, chance[b][j][i]);
+        float x, y;
+        zb_unpack2(zb_add2(zb_pack2(s[b][i >> 1][(i & 1) * 2], s[b][i >> 1][(i & 1) * 2 + 1]), less), x, y);
+        chance[b][i] = zb_pack2(zb_ex2(x), zb_ex2(y));
+        sum[b] = i == 0 ? chance[b][i] : zb_add2(sum[b], chance[b][i]);
       }
+      float x, y;
+      zb_unpack2(sum[b], x, y);
+      moves = moves || x > kMostP || y > kMostP;
     };
-    const auto weights = [&](int b, int j) {       // p_j s_vj u
-      const float u = __uint_as_float(static_cast<uint32_t>(unit[b][j]) << 23);
+    const auto weights = [&](int b) {              // p_j s_vj u
+      const ZbF2 u = zb_pack2(__uint_as_float(static_cast<uint32_t>(unit[b][0]) << 23), __uint_as_float(static_cast<uint32_t>(unit[b][1]) << 23));
+      __half2 most = __float2half2_rn(0.f);
 #pragma unroll
       for (int i = 0; i < kGroups; ++i) {
-        weight[b][j][i] = chance[b][j][i] * u * vs[i];
-        most = fmaxf(most, weight[b][j][i]);
+        float x, y;
+        zb_unpack2(zb_mul2(zb_mul2(chance[b][i], u), zb_pack2(vs[i], vs[i])), x, y);
+        weight[b][i] = pack_half2(x, y);
+        most = __hmax2(most, *reinterpret_cast<const __half2*>(&weight[b][i]));
       }
+      moves = moves || __hgt(__hmax(__low2half(most), __high2half(most)), __ushort_as_half(kMostWeight));
     };
     if (!first) {                                  // a warp's first tile has no references yet
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) chances(b, j), weights(b, j);
+      for (int b = 0; b < NB; ++b) chances(b), weights(b);
     }
-    if (__any_sync(0xffffffffu, first || most_p > kMostP || most > kMostWeight)) {
+    if (__any_sync(0xffffffffu, first || moves)) {
       int rise[NB][2], fall[NB][2];                // what both references rise by together, and 1 / u by
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        uint32_t tops = 0u;                        // exponent bytes of this tile's largest p_j s_vj of both columns
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           float mx = -INFINITY;
@@ -580,12 +590,17 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB, MODE>::kWarps, Kv8Sizes<
           mx = fmaxf(ceilf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16))), m[b][j]);
           rise[b][j] = static_cast<int>(fminf(mx - m[b][j], 512.f));         // whole; no number (no references yet, infinities): 0 or 512
           m[b][j] = mx;
-          chances(b, j);
-          float top = 0.f;
-#pragma unroll
-          for (int i = 0; i < kGroups; ++i) top = fmaxf(top, chance[b][j][i] * fminf(vs[i], __uint_as_float(253u << 23)));
-          tops |= __float_as_uint(top) >> 23 << (16 * j);
         }
+        chances(b);
+        float top0 = 0.f, top1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) {
+          const float scale = fminf(vs[i], __uint_as_float(253u << 23));
+          float x, y;
+          zb_unpack2(zb_mul2(chance[b][i], zb_pack2(scale, scale)), x, y);
+          top0 = fmaxf(top0, x), top1 = fmaxf(top1, y);
+        }
+        uint32_t tops = __float_as_uint(top0) >> 23 | __float_as_uint(top1) >> 23 << 16;      // exponent bytes of this tile's largest p_j s_vj of both columns
         tops = __vmaxu2(tops, __shfl_xor_sync(0xffffffffu, tops, 4));
         tops = __vmaxu2(tops, __shfl_xor_sync(0xffffffffu, tops, 8));
         tops = __vmaxu2(tops, __shfl_xor_sync(0xffffffffu, tops, 16));
@@ -595,8 +610,8 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB, MODE>::kWarps, Kv8Sizes<
           const int now = max(min(min(unit[b][j] + rise[b][j], lower), kMostUnit), kLeastUnit);
           fall[b][j] = unit[b][j] + rise[b][j] - now;
           unit[b][j] = now;
-          weights(b, j);
         }
+        weights(b);
       }
       if (!first) {
 #pragma unroll
@@ -615,10 +630,11 @@ __global__ void __launch_bounds__(32 * Kv8Sizes<HD, NB, MODE>::kWarps, Kv8Sizes<
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
+      float x, y;
+      zb_unpack2(sum[b], x, y);
+      l[b][0] += x, l[b][1] += y;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) l[b][j] += sum[b][j];
-#pragma unroll
-      for (int i = 0; i < kGroups; ++i) pb[b][i] = transpose8(pack_half2(weight[b][0][i], weight[b][1][i]));
+      for (int i = 0; i < kGroups; ++i) pb[b][i] = transpose8(weight[b][i]);
     }
   };
 
@@ -895,7 +911,7 @@ int zb_kv8_decode_plan(int batch, int hq, int hkv, int hd, int max_len, long lon
   if (pairs * size <= most && longest * tile <= size * warps * 256) return -size;
   // More pairs than CTAs, none of them long: a warp for each, where a CTA for each takes a turn per 296 of them, most of it spent on getting
   // under way (us, heads of 128, a warp / a CTA: 512 pairs of 40, 300, 1000 keys 5.6 / 8.2, 13.7 / 16.4, 32.8 / 28.2, 1024 pairs of 1000 45.0 / 51.7,
-  // 8000 of 30 31.1 / 97.7).  Up to 2048 keys, as a warp is alone with its pair: 4096 pairs of 1000, 2000, 4000 keys 162 / 166, 309 / 307, 604 / 591, but
+  // 8000 of 30 30.9 / 97.7).  Up to 2048 keys, as a warp is alone with its pair: 4096 pairs of 1000, 2000, 4000 keys 162 / 166, 309 / 307, 604 / 591, but
   // eight of 1000, 2048, 4000 among 4088 of 100: 41 / 64, 61 / 66, 95 / 70
   if (batch > kMaxBatch || (pairs > most && longest * tile <= 2048 && longest * tile * most <= pairs * 300)) return 0;
   // Too many to cut: a CTA for each, which need not look at the other lengths.  Up to 2048 keys, as a CTA is alone with its pair: that is what one long
