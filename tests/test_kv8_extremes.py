@@ -183,11 +183,12 @@ def test_large_values_that_nobody_looks_at(kind, lens, bound, up, hd, dtype):
 @DTYPES
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("step,down", [(12.0, 5.0), (12.0, 17.0), (12.0, 30.0), (-12.0, -5.0), (-12.0, -30.0), (0.3, 1.0), (0.3, -1.0), (7.0, 0.0)])
+@pytest.mark.parametrize("hq", [3, 12])
 @WAYS
-def test_scores_and_values_that_climb_and_fall(kind, lens, bound, step, down, hd, dtype):
+def test_scores_and_values_that_climb_and_fall(kind, lens, bound, hq, step, down, hd, dtype):
     """Along a sequence scores rise by `step` (in units of log2) every 13 keys while values shrink by 2^down: what the weights are taken from moves with
     nearly every tile, in both directions, and the first or the last keys make the result."""
-    assert shared_out(lens, 3, 1, hd, bound) == kind
+    assert shared_out(lens, hq, 1, hd, bound) == kind
     g = torch.Generator().manual_seed(hd)
     n = lens[0]
     k, v, table, sl, first = sequences(lens, 1, hd, dtype, "cuda")
@@ -197,8 +198,8 @@ def test_scores_and_values_that_climb_and_fall(kind, lens, bound, step, down, hd
     vs *= torch.exp2(-down * (at.float() - 7.0))[:, None].clamp(2.0 ** -110, 2.0 ** 110)
     put(k, first[0], torch.arange(n), ks)
     put(v, first[0], torch.arange(n), vs)
-    q = torch.randn(len(lens), 3, hd, generator=g).bfloat16()
-    q[:, :, 0] = torch.tensor([1.0, 0.25, -1.0])
+    q = torch.randn(len(lens), hq, hd, generator=g).bfloat16()
+    q[:, :, 0] = torch.tensor([1.0, 0.25, -1.0]).repeat(hq // 3)
     q = q.cuda()
     out = ops.paged_decode(q, k, v, table, sl, scale=0.6931471805599453, max_seq_len=bound)
     check_closely(out, q, k, v, table, sl, 0.6931471805599453, [0], dtype is INT8)
@@ -301,14 +302,14 @@ def test_sequences_that_the_workspace_has_no_room_for_cpu():
 
 
 @DTYPES
-@pytest.mark.parametrize("group", [1, 2])
+@pytest.mark.parametrize("group,hd", [(1, 64), (2, 64), (2, 128), (1, 256)])
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
-def test_prompts_over_a_table_without_columns(device, group, dtype):
+def test_prompts_over_a_table_without_columns(device, group, hd, dtype):
     """New tokens of sequences that have no pages at all see nothing: the bf16 kernels are given a table with a column, which they read whatever the lengths are."""
-    k, v, _, _ = paged([5, 9], 2, 64, 64, dtype, 5, device)
+    k, v, _, _ = paged([5, 9], 2, 64, hd, dtype, 5, device)
     i32 = dict(dtype=torch.int32, device=device)
-    q = torch.ones(70, 2 * group, 64, dtype=torch.bfloat16, device=device)
-    out = ops.paged_prefill(q, k, v, torch.zeros(2, 0, **i32), torch.tensor([0, 3], **i32), torch.tensor([0, 1, 70], **i32))
+    q = torch.ones(320, 2 * group, hd, dtype=torch.bfloat16, device=device)
+    out = ops.paged_prefill(q, k, v, torch.zeros(2, 0, **i32), torch.tensor([0, 3], **i32), torch.tensor([0, 1, 320], **i32))
     assert out.shape == q.shape and not bool(out.any())
     if device != "cpu":
         assert kv8._read(k, v, torch.zeros(2, 0, **i32), torch.tensor([0, 3], **i32), 64, 1, 1)[2].tolist() == [[0], [0]]
