@@ -1509,8 +1509,8 @@ int zb_make_tmap_u8_2d(CUtensorMap* out, const void* base, long long rows, long 
 // column groups, kv heads) with box (64, box_rows, head_dim / 64, 1) and the 128-byte swizzle: one copy
 // brings `box_rows` consecutive slots of one head into shared memory as head_dim / 64 tiles of
 // [box_rows][64], each with 128-byte rows.  Returns 0 on success.
-int zb_make_tmap_kv_cache(CUtensorMap* out, const void* base, long long slots, int kv_heads, int head_dim,
-                          int box_rows) {
+int zb_make_tmap_kv_box(CUtensorMap* out, const void* base, long long slots, int kv_heads, int head_dim,
+                        int box_rows, int box_subs) {
   EncodeTiledFn fn = get_encode_fn();
   if (fn == nullptr) return -1;
   if ((reinterpret_cast<uintptr_t>(base) & 15) != 0 || head_dim % 64 != 0 || box_rows < 1 || box_rows > 256) return -2;
@@ -1518,12 +1518,15 @@ int zb_make_tmap_kv_cache(CUtensorMap* out, const void* base, long long slots, i
   cuuint64_t dims[4] = {64, static_cast<cuuint64_t>(slots), static_cast<cuuint64_t>(head_dim / 64),
                         static_cast<cuuint64_t>(kv_heads)};
   cuuint64_t strides[3] = {row_bytes, 128, static_cast<cuuint64_t>(head_dim) * 2};
-  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(head_dim / 64), 1};
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(box_subs), 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -3;
+}
+int zb_make_tmap_kv_cache(CUtensorMap* out, const void* base, long long slots, int kv_heads, int head_dim, int box_rows) {
+  return zb_make_tmap_kv_box(out, base, slots, kv_heads, head_dim, box_rows, head_dim / 64);      // all columns of a head
 }
 
 namespace {

@@ -12,12 +12,14 @@ import math
 import torch
 
 from . import _lib, kv8, reference
+from . import shared as _shared
 from ._lib import CollectiveTimeout, KernelError, launch_count, raise_on_status  # noqa: F401
 from .kv8 import QuantKV, QuantKVCache, paged_read  # noqa: F401
+from .shared import SharedPrefix  # noqa: F401
 
 __all__ = [
     "gemm", "linear", "row_sumsq", "RowStats", "interleave_gate_up", "rmsnorm", "rope_kvwrite", "swiglu", "embedding", "argmax", "topk_sample",
-    "paged_prefill", "paged_decode", "paged_read", "QuantKV", "QuantKVCache", "decode_plan_splits", "KernelError", "launch_count",
+    "paged_prefill", "paged_decode", "paged_read", "QuantKV", "QuantKVCache", "SharedPrefix", "decode_plan_splits", "KernelError", "launch_count",
     "raise_on_status",
 ]
 
@@ -363,9 +365,15 @@ def decode_plan_splits(batch: int, num_kv_heads: int, max_seq_len: int) -> int:
 
 def paged_decode(q, k_cache, v_cache, block_table, seq_lens, scale: float | None = None,
                  window: int = 0, num_splits: int | None = None, max_seq_len: int | None = None,
-                 out=None, ext=None):
+                 out=None, ext=None, shared=None):
     """One query token per sequence against its paged KV.  q [B, hq, hd] -> [B, hq, hd].  `ext` (CUDA only, with `out`): a
-    `gqa.AttnExt`, see `ops.gqa`.  `QuantKV` caches are read in 8 bits (`ops.kv8`; they take no `ext`, and split the keys by themselves)."""
+    `gqa.AttnExt`, see `ops.gqa`.  `QuantKV` caches are read in 8 bits (`ops.kv8`; they take no `ext`, and split the keys by themselves).
+    `shared`: a `SharedPrefix`, the sequences whose first keys are the same pages, which are then read once for all of them (`ops.shared`; bf16 caches
+    without window or `ext`, keys split by the kernel)."""
+    if shared is not None:
+        if ext is not None or window or isinstance(k_cache, QuantKV) or isinstance(v_cache, QuantKV):
+            raise ValueError("attention behind a shared prefix takes bfloat16 caches, and no window or extensions")
+        return _shared.paged_decode(q, k_cache, v_cache, block_table, seq_lens, shared, scale, out)
     if isinstance(k_cache, QuantKV) or isinstance(v_cache, QuantKV):
         if ext is not None:
             raise ValueError("attention over a quantised cache has no extensions")

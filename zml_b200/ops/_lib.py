@@ -160,7 +160,7 @@ KERNEL_NAMES = {1: "gemm_bf16", 2: "paged_decode", 3: "paged_prefill", 4: "gemm_
                 20: "rope_kvwrite", 21: "embedding", 22: "decode_advance", 24: "causal_conv1d", 25: "gated_delta_scan",
                 26: "embedding_f32", 27: "stream_conv", 28: "latent_prep", 29: "latent_attend", 30: "latent_gather", 31: "wkv_scan",
                 32: "latent_prefill_tc", 33: "latent_decode", 34: "gqa_prep", 35: "gqa_attend", 36: "channel_delta",
-                37: "gqa_pool", 38: "gated_scan", 39: "kv8_write", 40: "kv8_read", 41: "kv8_decode"}
+                37: "gqa_pool", 38: "gated_scan", 39: "kv8_write", 40: "kv8_read", 41: "kv8_decode", 42: "shared_decode"}
 
 
 class BoundsError(KernelError):
