@@ -15,12 +15,13 @@ from . import _lib, kv8, reference
 from . import shared as _shared
 from ._lib import CollectiveTimeout, KernelError, launch_count, raise_on_status  # noqa: F401
 from .kv8 import QuantKV, QuantKVCache, paged_read  # noqa: F401
+from .sampling import sample  # noqa: F401
 from .shared import SharedPrefix  # noqa: F401
 
 __all__ = [
     "gemm", "linear", "row_sumsq", "RowStats", "interleave_gate_up", "rmsnorm", "rope_kvwrite", "swiglu", "embedding", "argmax", "topk_sample",
-    "paged_prefill", "paged_decode", "paged_read", "QuantKV", "QuantKVCache", "SharedPrefix", "decode_plan_splits", "KernelError", "launch_count",
-    "raise_on_status",
+    "sample", "paged_prefill", "paged_decode", "paged_read", "QuantKV", "QuantKVCache", "SharedPrefix", "decode_plan_splits", "KernelError",
+    "launch_count", "raise_on_status",
 ]
 
 
