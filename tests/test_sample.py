@@ -125,6 +125,9 @@ def suite(device, most=60000):
     x, u = spread(64, 700, 0.3, 7)
     check(x, u, mixed(64, 8), device)
     check(x, u, {**mixed(64, 9), "top_p": 0.8}, device, dtype=torch.bfloat16)
+    # top_p is a part of the sum of the top_k, whatever min_p leaves of them
+    check(x, u, {"top_k": 300, "top_p": 0.5, "min_p": 0.05, "temperature": 0.3}, device)
+    check(x, u, {"top_k": 30, "top_p": 0.5, "min_p": 0.6}, device)
     # nearly the whole, and a tail of tiny weights
     x, u = spread(8, 4000, 6.0, 11)
     check(x, u, {"top_p": 1.0 - 2.0 ** -20}, device, most_near=4)      # the nucleus ends among weights of 1e-9, one in ten of them near

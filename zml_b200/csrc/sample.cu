@@ -8,8 +8,8 @@
 // typically 2^-36 of the largest weight.  (A sum of fp32 weights is off by 1e-7 of the whole, and among 128 thousand flat weights each is 8e-6 of it:
 // one draw in a hundred would be another token.)
 //
-// A cluster of CTAs holds a row in shared memory, a slice a CTA, and reads it from there as often as it needs; the row is not sorted.  All cuts keep
-// what is in front in the order of size, so a row ends in one of two ways:
+// A cluster of CTAs has a row, a slice a CTA, and reads it two to four times, all but the first time from L2 (shared memory for the slices would leave two
+// CTAs on an SM: 64 rows of 151936 40 us, 256 380).  The row is not sorted.  All cuts keep what is in front in the order of size, so a row ends in one of two ways:
 //   * a list: what is at least as large as a bound that is known beforehand (the k-th largest of some logits; the weight below which all of the vocabulary
 //     together is less than 1 - top_p; min_p) is usually a few hundred logits, which one CTA ranks, sums and draws from;
 //   * a cut: where these are too many, a histogram finds the smallest logit that stays and how many of its equals do, every warp sums the weights
@@ -21,12 +21,12 @@
 
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCtas = 8;
-constexpr int kMaxSlice = 49152;                     // logits of a CTA
-constexpr int kList = 1024;
-constexpr int kSmallK = 256;
+constexpr int kMaxCtas = 8;
+constexpr int kMaxVocab = 8 * 49152;                 // (an index and a weight are one number of 19 + 45 bits)
+constexpr int kList = 2048;
+constexpr int kSmallK = 600;                        // a top_k up to this ends in a list, if all goes well
 constexpr int kBins = 2048;
-constexpr int kTable = 512;                          // 2^((j + 1/2) / 512)
+constexpr int kTable = 16;                           // 2^((j + 1/2) / 16): any 32 lanes' entries are on different banks (512 entries: 7 conflicts)
 constexpr double kOne = 17592186044416.0;            // 2^44
 constexpr unsigned long long kBias = 0x4070000000000000ull;      // 256.0: a weight added to it has its 2^-44 in the last place
 
@@ -40,7 +40,7 @@ struct SampleParams {
   const int32_t* top_k;
   long long stride;
   double temperature_all, top_p_all, min_p_all;
-  int top_k_all, vocab, slice, uniforms64, vec;  // vec: every row starts on four logits
+  int top_k_all, vocab, slice, uniforms64, vec;  // slice: of a CTA, whole rows of 128 for each warp; vec: every row starts on four logits
 };
 
 using u64 = unsigned long long;
@@ -91,104 +91,114 @@ ZB_DEVICE u64 warp_upto(u64 v, int lane) {           // inclusive
   return v;
 }
 
+template <int kThreads>
 struct Shared {
+  static constexpr int kWarps = kThreads / 32;
   double table[kTable];
   union {
     struct {
       u64 cand[kList];                               // of this CTA: key << 32 | ~index, the larger, the further in front
       u64 sorted[kList];                             // CTA 0: of the cluster
-      u64 weight[kList];
+      u64 weight[kList];                             // CTA 0: of these; then those that stay, index << 45 | weight
     } list;
-    uint32_t hist[3][kBins];                         // counts, or 15 bits each of the weights
+    struct {
+      uint32_t hist[kBins];
+      u64 heavy[kBins];
+    };
   };
-  u64 part[2][kWarps];
+  u64 part[kWarps], seg[kWarps], sub[kWarps], above[kWarps];
   u64 total[kMaxCtas];                               // of every CTA
   uint32_t ties[kMaxCtas], count[kMaxCtas], best[kMaxCtas], bound[kMaxCtas], least[kMaxCtas];
-  uint32_t warp_ties[kWarps], warp_best[kWarps], warp_least[kWarps], top[kWarps * (kSmallK / kWarps + 1)], n, range[2];
+  uint32_t seg_ties[kWarps], sub_ties[kWarps], warp_best[kWarps], warp_least[kWarps], top[kThreads], n, range[2];
   u64 left;                                          // what CTA 0 has found, in every CTA
-  uint32_t found;
+  uint32_t found[2];
 };
 
 // All threads of a cluster, which is one row.
-template <typename T>
+template <typename T, int kThreads>
 struct Sampler {
+  static constexpr int kWarps = kThreads / 32, kMine = kList / kThreads;      // neighbours of a list that a thread has
   const SampleParams& p;
-  Shared& sh;
-  float* x_s;                    // the CTA's slice
-  int ctas, rank, warp, lane, from, rows, first;      // a warp has `rows` rows of 128 logits of the slice, from `first` on, four neighbours a lane
+  Shared<kThreads>& sh;
+  const T* x;                    // the row
+  int ctas, rank, warp, lane, from, end;              // the warp's part of the row, whole rows of 128 but for the row's end
+  int kind;                      // 1: only infinities count, as 1; 2: logits are scaled by 2^-100
   float top, floor_x;            // the largest logit; below floor_x weights are zero
   double top64, scale;           // log2 of a weight is (x - top) * scale
   uint32_t best;
+  bool listed;                   // the logits around the cut are in the CTAs' lists, and what is above them in sh.above
 
-  ZB_DEVICE Sampler(const SampleParams& params, Shared& shared, float* x, int log2_ctas)
-      : p(params), sh(shared), x_s(x), ctas(1 << log2_ctas), rank(blockIdx.x & (ctas - 1)), warp(threadIdx.x >> 5), lane(threadIdx.x & 31) {
-    from = rank * p.slice;
-    rows = p.slice / (128 * kWarps);
-    first = warp * rows * 128;
+  ZB_DEVICE Sampler(const SampleParams& params, Shared<kThreads>& shared, int log2_ctas)
+      : p(params), sh(shared), ctas(1 << log2_ctas), rank(blockIdx.x & (ctas - 1)), warp(threadIdx.x >> 5), lane(threadIdx.x & 31), kind(0), listed(false) {
+    x = reinterpret_cast<const T*>(p.logits) + static_cast<size_t>(blockIdx.x >> log2_ctas) * p.stride;
+    from = min(rank * p.slice + warp * (p.slice / kWarps), p.vocab);
+    end = min(from + p.slice / kWarps, p.vocab);
   }
 
-  // The weight of a logit that is not above `top`, in 2^-44, plus kBias.  z is held with 41 bits behind the point: 9 of them choose the table's entry, with the
-  // other 32 as r, around their middle, 2^r is a cubic (off by 9e-15).
+  // The weight of a logit that is not above `top`, in 2^-44, plus kBias; a NaN's is zero.  z is held with 41 bits behind the point: 4 of them choose the table's
+  // entry, and with the other 37 as r, around their middle, 2^r is a polynomial (off by 5e-16).
   ZB_DEVICE u64 biased(float x) const {
-    const double t = __fma_rn(static_cast<double>(fmaxf(x, floor_x)) - top64, scale, 3072.0);
+    const double t = __fma_rn(static_cast<double>(fmaxf(x, floor_x)) - top64, scale, 3072.0);      // 1.5 * 2^11
     const int hi = __double2hiint(t);
-    const double r = __hiloint2double(0x43300000, __double2loint(t)) - 4503601774854144.0;      // 2^52 + 2^31
-    constexpr double c1 = 0.6931471805599453 * 0x1p-41, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6;
-    const double base = sh.table[hi & (kTable - 1)];
-    const double b = __hiloint2double(__double2hiint(base) + ((hi & ~(kTable - 1)) << 11) - (1024 << 20), __double2loint(base));
-    const double q = __fma_rn(__fma_rn(r, c3, c2), r, c1) * r;
+    const double r = __hiloint2double(0x43300000 | (hi & 31), __double2loint(t)) - 4503668346847232.0;      // 2^52 + 2^36
+    constexpr double c1 = 0.6931471805599453 * 0x1p-41, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4, c5 = c4 * c1 / 5, c6 = c5 * c1 / 6;
+    const double base = sh.table[hi >> 5 & (kTable - 1)];
+    const double b = __hiloint2double(__double2hiint(base) + ((hi & ~0x1ff) << 11) - (1024 << 20), __double2loint(base));
+    const double q = __fma_rn(__fma_rn(__fma_rn(__fma_rn(__fma_rn(r, c6, c5), r, c4), r, c3), r, c2), r, c1) * r;
     return static_cast<u64>(__double_as_longlong(__fma_rn(b, q, b) + 256.0));
   }
   ZB_DEVICE u64 weight(float x) const { return biased(x) - kBias; }
 
-  template <typename F>
-  ZB_DEVICE void each(F&& f) const {                 // f(index in the slice of the first, four logits): the warp's, in order
-#pragma unroll 1
-    for (int i = 0; i < rows; ++i) {
-      const int at = first + i * 128 + lane * 4;
-      f(at, *reinterpret_cast<const float4*>(x_s + at));
-    }
+  ZB_DEVICE float fix(float v) const {               // what counts as a logit (a NaN fails every comparison and has no weight)
+    return kind == 0 ? v : kind == 1 ? (v == INFINITY ? 1.f : -INFINITY) : v * 0x1p-100f;
   }
-
-  ZB_DEVICE void load(const T* x, float& most, float& least) {
-    const auto take = [&](float v) {
-      v = v != v ? -INFINITY : v;
-      most = fmaxf(most, v);
-      least = v > -INFINITY ? fminf(least, v) : least;
-      return v;
-    };
-    most = -INFINITY, least = INFINITY;
-    const int whole = min(rows, max(0, (p.vocab - from - first) / 128));      // rows without an end
-    int i = 0;
+  // f(four logits, index of the first, distance of their indices) over the warp's part, 128 logits at a time, -inf behind the row's end.
+  template <typename F>
+  ZB_DEVICE void each(F&& f) const {
+    constexpr int kOnce = 4;
+    int i = from;
     if (p.vec) {
-#pragma unroll 4
-      for (; i < whole; ++i) {
-        const int at = first + i * 128 + lane * 4;
-        float4 v;
-        if constexpr (sizeof(T) == 4) {
-          v = *reinterpret_cast<const float4*>(x + from + at);
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(x + from + at);
-          v = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+#pragma unroll 1
+      for (; i + 128 <= end; i += 128 * kOnce) {
+        float4 v[kOnce];
+#pragma unroll
+        for (int k = 0; k < kOnce; ++k) {
+          const int at = i + k * 128 + lane * 4;
+          if (i + (k + 1) * 128 <= end) {
+            if constexpr (sizeof(T) == 4) {
+              v[k] = *reinterpret_cast<const float4*>(x + at);
+            } else {
+              const uint2 u = *reinterpret_cast<const uint2*>(x + at);
+              v[k] = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+            }
+          }
         }
-        *reinterpret_cast<float4*>(x_s + at) = make_float4(take(v.x), take(v.y), take(v.z), take(v.w));
+#pragma unroll
+        for (int k = 0; k < kOnce; ++k) {
+          if (i + (k + 1) * 128 > end) break;
+          float e[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+          if (kind != 0) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) e[j] = fix(e[j]);
+          }
+          f(e, i + k * 128 + lane * 4, 1);
+        }
       }
+      i = from + (end - from) / 128 * 128;
     }
-#pragma unroll 2
-    for (; i < rows; ++i) {
-      float v[4];
+#pragma unroll 1
+    for (; i < end; i += 128) {
+      float e[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int at = from + first + i * 128 + j * 32 + lane;
-        v[j] = at < p.vocab ? static_cast<float>(x[at]) : -INFINITY;
+        const int at = i + j * 32 + lane;
+        e[j] = at < end ? fix(static_cast<float>(x[at])) : -INFINITY;
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x_s[first + i * 128 + j * 32 + lane] = take(v[j]);
+      f(e, i + lane, 32);
     }
-    __syncwarp();
   }
 
-  // The k-th largest of at least k of the CTA's logits: each warp's largest few of its lanes' largest.
+  // The k-th largest of at least k of the CTA's logits (at most 32 a warp): each warp's largest few of its lanes' largest.
   ZB_DEVICE void find_bound(uint32_t mine, int k) {
     const int per_warp = min((k + kWarps - 1) / kWarps + 1, 32);
     for (int i = 0; i < per_warp; ++i) {
@@ -201,19 +211,20 @@ struct Sampler {
     if (threadIdx.x < kWarps * per_warp) {
       const uint32_t m = sh.top[threadIdx.x];
       int ahead = 0;
+#pragma unroll 4
       for (int j = 0; j < kWarps * per_warp; ++j) ahead += sh.top[j] > m || (sh.top[j] == m && j < static_cast<int>(threadIdx.x)) ? 1 : 0;
       if (ahead == k - 1) sh.range[0] = m;
     }
     __syncthreads();
   }
 
-  // Over the cluster, in every thread; *before: of the CTAs in front, *front: and of the warps in front.
+  // Over the cluster, in every thread.  (Another barrier has to come before the next sum.)
   ZB_DEVICE u64 sum_all(u64 v) {
     v = warp_sum(v);
-    if (lane == 0) sh.part[0][warp] = v;
+    if (lane == 0) sh.part[warp] = v;
     __syncthreads();
     if (warp == 0) {
-      u64 s = lane < kWarps ? sh.part[0][lane] : 0;
+      u64 s = lane < kWarps ? sh.part[lane] : 0;
       s = warp_sum(s);
       if (lane < ctas) st_cluster_u64(zb_mapa(zb_smem_u32(&sh.total[rank]), lane), s);
     }
@@ -223,27 +234,37 @@ struct Sampler {
     return s;
   }
 
-  // A row's logits from key `lo` on into the CTAs' lists; how many in the cluster.  (Another barrier has to come before the lists are written again.)
-  ZB_DEVICE int gather(uint32_t lo) {
-    const float bound = value_of(lo);
-    if (threadIdx.x == 0) sh.n = 0;
-    __syncthreads();
-    each([&](int at, const float4& v) {
-      if (!__any_sync(0xffffffffu, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= bound)) return;
-      const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (e[j] >= bound && from + at + j < p.vocab) {
-          const uint32_t slot = atomicAdd(&sh.n, 1u);
-          if (slot < kList) sh.list.cand[slot] = static_cast<u64>(key_of(e[j])) << 32 | static_cast<uint32_t>(~(from + at + j));
-        }
-    });
+  // Into the CTA's list, by whole warps.
+  ZB_DEVICE void append(bool some, float v, int index) {
+    const uint32_t who = __ballot_sync(0xffffffffu, some);
+    if (who == 0) return;
+    uint32_t slot = 0;
+    if (lane == 0) slot = atomicAdd(&sh.n, static_cast<uint32_t>(__popc(who)));
+    slot = __shfl_sync(0xffffffffu, slot, 0) + __popc(who & ((1u << lane) - 1u));
+    if (some && slot < kList) sh.list.cand[slot] = static_cast<u64>(key_of(v)) << 32 | static_cast<uint32_t>(~index);
+  }
+  // Every CTA's sh.n to all; how many in the cluster, more than kList: too many.
+  ZB_DEVICE int exchange_counts() {
     __syncthreads();
     if (threadIdx.x < ctas) st_cluster_u32(zb_mapa(zb_smem_u32(&sh.count[rank]), threadIdx.x), sh.n);
     cluster_sync();
     int n = 0;
     for (int c = 0; c < ctas; ++c) n += static_cast<int>(min(sh.count[c], static_cast<uint32_t>(kList + 1)));
     return n;
+  }
+  // A row's logits from key `lo` on into the CTAs' lists; how many.  (Another barrier has to come before the lists are written again.)
+  ZB_DEVICE int gather(uint32_t lo) {
+    const float bound = value_of(lo);
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+    const volatile uint32_t* n = &sh.n;
+    each([&](const float (&e)[4], int at, int step) {
+      if (!__any_sync(0xffffffffu, fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) >= bound)) return;
+      if (__shfl_sync(0xffffffffu, *n, 0) > kList) return;      // too many already
+#pragma unroll
+      for (int j = 0; j < 4; ++j) append(e[j] >= bound && at + j * step < end, e[j], at + j * step);
+    });
+    return exchange_counts();
   }
 
   // The CTAs' lists, n in all, to CTA 0, in the order of size.
@@ -257,32 +278,86 @@ struct Sampler {
     }
     cluster_sync();                                  // nobody leaves or writes its list before it has been read
     if (rank != 0) return;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const u64 mine = sh.list.weight[i];
-      int ahead = 0;
+    sort_down(sh.list.weight, sh.list.sorted, n);
+  }
+  // a[0, n) from the largest on to b: a number a thread by counting what is in front of it (256: 1.6 us), more bitonically.
+  ZB_DEVICE void sort_down(const u64* a, u64* b, int n) {
+    __syncthreads();
+    if (n <= min(kThreads, 256)) {
+      if (static_cast<int>(threadIdx.x) < n) {
+        const u64 mine = a[threadIdx.x];
+        int ahead = 0;
 #pragma unroll 8
-      for (int j = 0; j < n; ++j) ahead += sh.list.weight[j] > mine ? 1 : 0;
-      sh.list.sorted[ahead] = mine;
+        for (int j = 0; j < n; ++j) ahead += a[j] > mine || (a[j] == mine && j < static_cast<int>(threadIdx.x)) ? 1 : 0;
+        b[ahead] = mine;
+      }
+      __syncthreads();
+      return;
     }
+    // Neighbours in registers: of the distances, the smallest lie within a thread, the next ones within a warp.
+    const int size = 2 << (31 - __clz(n - 1)), i0 = kMine * threadIdx.x;
+    u64 v[kMine];
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) v[j] = i0 + j < n ? a[i0 + j] : 0;
+    const auto keep = [&](u64 mine, u64 other, int i, int k, int d) { return ((i & d) == 0) == ((i & k) == 0) ? max(mine, other) : min(mine, other); };
+#pragma unroll 1
+    for (int k = 2; k <= size; k <<= 1) {
+#pragma unroll 1
+      for (int d = k >> 1; d >= kMine; d >>= 1) {
+        u64 other[kMine];
+        if (d >= 32 * kMine) {
+          __syncthreads();
+#pragma unroll
+          for (int j = 0; j < kMine; ++j)
+            if (i0 < size) b[i0 + j] = v[j];
+          __syncthreads();
+#pragma unroll
+          for (int j = 0; j < kMine; ++j) other[j] = i0 < size ? b[(i0 ^ d) + j] : 0;
+        } else {
+#pragma unroll
+          for (int j = 0; j < kMine; ++j) other[j] = __shfl_xor_sync(0xffffffffu, v[j], d / kMine);
+        }
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) v[j] = keep(v[j], other[j], i0 + j, k, d);
+      }
+#pragma unroll
+      for (int d = kMine / 2; d > 0; d >>= 1) {
+        if (d >= k) continue;
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+          if ((j & d) != 0) continue;
+          const u64 lo = min(v[j], v[j | d]), hi = max(v[j], v[j | d]);
+          const bool down = ((i0 + j) & k) == 0;
+          v[j] = down ? hi : lo, v[j | d] = down ? lo : hi;
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kMine; ++j)
+      if (i0 < size) b[i0 + j] = v[j];
     __syncthreads();
   }
   static ZB_DEVICE uint32_t key_at(u64 c) { return static_cast<uint32_t>(c >> 32); }
   static ZB_DEVICE int index_at(u64 c) { return ~static_cast<int>(static_cast<uint32_t>(c)); }
 
-  // Sums up to each of the first n of the sorted list (CTA 0): of two neighbours a thread, those in front of the first.
-  ZB_DEVICE u64 list_before(int n, u64& w0, u64& w1, u64& all) {
-    const int i = 2 * threadIdx.x;
-    w0 = i < n ? weight(value_of(key_at(sh.list.sorted[i]))) : 0;
-    w1 = i + 1 < n ? weight(value_of(key_at(sh.list.sorted[i + 1]))) : 0;
-    const u64 upto = warp_upto(w0 + w1, lane);
-    if (lane == 31) sh.part[0][warp] = upto;
+  // Given their weights: what is in front of the first; *all: the sum of the list.
+  ZB_DEVICE u64 list_before(const u64 (&w)[kMine], u64* all) {
+    u64 mine = 0;
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) mine += w[j];
+    const u64 upto = warp_upto(mine, lane);
+    if (lane == 31) sh.part[warp] = upto;
     __syncthreads();
-    u64 before = upto - w0 - w1;
-    all = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += sh.part[0][w];
-      all += sh.part[0][w];
+    u64 before = upto - mine;
+    *all = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      const u64 y = sh.part[i];
+      if (i < warp) before += y;
+      *all += y;
     }
+    __syncthreads();
     return before;
   }
 
@@ -302,182 +377,249 @@ struct Sampler {
 
   // CTA 0: from the sorted list of n, of which those with keys from `least` on may stay; `all`: the sum that top_p is a part of, 0: the list's.
   ZB_DEVICE void draw_from_list(int row, int n, double top_p, u64 all, uint32_t least) {
-    u64 w0, w1, sum;
-    u64 before = list_before(n, w0, w1, sum);
-    const int i = 2 * threadIdx.x;
+    const int i = kMine * threadIdx.x;
+    u64 c[kMine], w[kMine], sum;
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      c[j] = i + j < n ? sh.list.sorted[i + j] : 0;
+      w[j] = i + j < n ? weight(value_of(key_at(c[j]))) : 0;
+    }
+    u64 before = list_before(w, &sum);
     const u64 need = top_p < 1.0 ? need_of(top_p, all != 0 ? all : sum) : ~0ull;
-    const bool s0 = i < n && (i == 0 || (before < need && key_at(sh.list.sorted[i]) >= least));
-    const bool s1 = i + 1 < n && before + w0 < need && key_at(sh.list.sorted[i + 1]) >= least;
-    if (i < n) sh.list.weight[i] = w0;
-    if (i + 1 < n) sh.list.weight[i + 1] = w1;
-    const int m = __syncthreads_count(s0) + __syncthreads_count(s1);      // those in front stay
-    // their sum
-    if ((s0 && i == m - 1) || (s1 && i + 1 == m - 1)) sh.left = before + w0 + (s1 ? w1 : 0);
+    int stays = 0;                                   // the first few of the list
+    u64 kept = 0;
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      if (i + j < n && (i + j == 0 || (before < need && key_at(c[j]) >= least))) {
+        ++stays;
+        kept += w[j];
+        sh.list.weight[i + j] = static_cast<u64>(static_cast<uint32_t>(0x7ffffu - index_at(c[j]))) << 45 | w[j];      // (sorted down: the lowest index first)
+      }
+      before += w[j];
+    }
+    int m = __reduce_add_sync(0xffffffffu, stays);
+    kept = warp_sum(kept);
+    if (lane == 0) sh.sub[warp] = kept, sh.sub_ties[warp] = m;
     __syncthreads();
-    const u64 kept = sh.left, target = target_of(uniform(row), kept);
-    for (int a = threadIdx.x; a < m; a += kThreads) {
-      const u64 mine = sh.list.sorted[a];
-      const uint32_t idx = static_cast<uint32_t>(mine);      // complements: larger is further in front
-      u64 s = 0;
-#pragma unroll 4
-      for (int j = 0; j < m; ++j) s += static_cast<uint32_t>(sh.list.sorted[j]) > idx ? sh.list.weight[j] : 0;
-      if (s <= target && target - s < sh.list.weight[a]) write(row, index_at(mine), value_of(key_at(mine)), kept);
+    m = 0, kept = 0;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) m += sh.sub_ties[k], kept += sh.sub[k];
+    const u64 target = target_of(uniform(row), kept);
+    constexpr u64 kWeight = (1ull << 45) - 1;
+    const auto found = [&](u64 number) {
+      const int token = 0x7ffff - static_cast<int>(number >> 45);
+      write(row, token, fix(static_cast<float>(x[token])), kept);
+    };
+    if (m <= min(kThreads, 256)) {
+      if (static_cast<int>(threadIdx.x) >= m) return;
+      const u64 mine = sh.list.weight[threadIdx.x];
+      before = 0;
+#pragma unroll 8
+      for (int j = 0; j < m; ++j) {
+        const u64 y = sh.list.weight[j];
+        before += y > mine ? y & kWeight : 0;        // (of lower index; no two have the same)
+      }
+      if (before <= target && target - before < (mine & kWeight)) found(mine);
+      return;
+    }
+    sort_down(sh.list.weight, sh.list.cand, m);
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      c[j] = i + j < m ? sh.list.cand[i + j] : 0;
+      w[j] = c[j] & kWeight;
+    }
+    before = list_before(w, &sum);
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      if (before <= target && target - before < w[j]) found(c[j]);
+      before += w[j];
     }
   }
 
-  // The largest key up to which, from above, the counts (or weights) of the logits above `floor_key` sum to at least `need`; *rest: what is needed there.
-  // A histogram over 2048 equal intervals of [value_of(lo), top], and a list of the interval that has it - or, where that is too long, what its keys have in
-  // common is looked for bit by bit.
+  // The largest key up to which, from above, the counts (or weights) of the logits above `floor_key`, from `lo` on, sum to at least `need`; *rest: what is needed
+  // there.  0: there are not as many.  A histogram of counts over 2048 equal intervals of [value_of(lo), top] tells the interval, and one more pass lists its logits.  Of weights
+  // it tells it nearly: weights above all / 4096 are summed as they are, and for the others stands an interval's middle, half a hundredth off, to either side.
+  // (Their sum is off by some all / 2^13.)  So all is listed where the sum may lie within all / 2^11 of it, and what is above that is summed (for each
+  // warp to sh.above).  What cannot be listed is looked for bit by bit.
   template <bool WEIGHTS>
-  ZB_DEVICE uint32_t search(uint32_t lo, uint32_t floor_key, u64 need, u64* rest) {
+  ZB_DEVICE uint32_t search(uint32_t lo, uint32_t floor_key, u64 need, u64 all, u64* rest) {
     const float x_lo = fmaxf(value_of(lo), -3.0e38f), span = top - x_lo, by = span > 0.f ? static_cast<float>(kBins - 1) / span : 0.f;
-    const auto bin_of = [&](float x) { return max(0, min(kBins - 1, static_cast<int>((x - x_lo) * by))); };      // grows with x
-    for (int i = threadIdx.x; i < 3 * kBins; i += kThreads) (&sh.hist[0][0])[i] = 0;
+    const float floor_value = floor_key > 0 ? value_of(floor_key) : -INFINITY;
+    const auto counts = [&](float v) { return v >= x_lo && v > floor_value; };
+    const auto bin_of = [&](float v) { return max(0, min(kBins - 1, static_cast<int>((v - x_lo) * by))); };      // grows with v
+    const float heavy_x = WEIGHTS ? __double2float_rd(fmax(top64 + log2(static_cast<double>(all) / (kOne * 4096.0)) / scale, -3.4e38)) : INFINITY;
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.hist[i] = 0, sh.heavy[i] = 0;
     __syncthreads();
-    each([&](int, const float4& v) {
-      const float e[4] = {v.x, v.y, v.z, v.w};
+    each([&](const float (&e)[4], int, int) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (!(e[j] >= x_lo) || key_of(e[j]) <= floor_key) continue;
-        const int b = bin_of(e[j]);
-        if (WEIGHTS) {
-          const u64 w = weight(e[j]);
-          atomicAdd(&sh.hist[0][b], static_cast<uint32_t>(w) & 0x7fffu);
-          atomicAdd(&sh.hist[1][b], static_cast<uint32_t>(w >> 15) & 0x7fffu);
-          atomicAdd(&sh.hist[2][b], static_cast<uint32_t>(w >> 30));
-        } else {
-          atomicAdd(&sh.hist[0][b], 1u);
+      for (int j = 0; j < 4; ++j)
+        if (counts(e[j])) {
+          if (WEIGHTS && e[j] > heavy_x) atomicAdd(&sh.heavy[bin_of(e[j])], weight(e[j]));
+          else atomicAdd(&sh.hist[bin_of(e[j])], 1u);
         }
-      }
     });
     cluster_sync();
-    if (rank == 0) {
-      // sums of four bins a thread, from the highest on
-      const int bin0 = kBins - 4 - 4 * threadIdx.x;
-      u64 b[4] = {0, 0, 0, 0};
-      for (int c = 0; c < ctas; ++c)
-#pragma unroll
-        for (int k = 0; k < (WEIGHTS ? 3 : 1); ++k)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) b[j] += static_cast<u64>(ld_cluster_u32(zb_mapa(zb_smem_u32(&sh.hist[k][bin0 + j]), c))) << (15 * k);
-      const u64 sum = b[0] + b[1] + b[2] + b[3], upto = warp_upto(sum, lane);
-      if (lane == 31) sh.part[0][warp] = upto;
-      __syncthreads();
-      u64 before = upto - sum;
-      for (int w = 0; w < warp; ++w) before += sh.part[0][w];
-      if (before < need && before + sum >= need) {
-        int j = 3;
-        while (j > 0 && before + b[j] < need) before += b[j--];
-        for (int c = 0; c < ctas; ++c) {
-          st_cluster_u64(zb_mapa(zb_smem_u32(&sh.left), c), need - before);
-          st_cluster_u32(zb_mapa(zb_smem_u32(&sh.found), c), static_cast<uint32_t>(bin0 + j));
-        }
+    // Every CTA adds up a share of the bins, from the highest on, a thread some of them.
+    constexpr int kEach = (kBins + kThreads - 1) / kThreads;      // where a row has one CTA
+    const int share = kBins >> (31 - __clz(ctas)), each_bins = (share + kThreads - 1) / kThreads, top_bin = kBins - 1 - rank * share - threadIdx.x * each_bins;
+    const auto mass_of = [&](int bin) {
+      u64 heavy = 0;
+      uint32_t n = 0;
+#pragma unroll 1
+      for (int c = 0; c < ctas; ++c) {
+        n += ld_cluster_u32(zb_mapa(zb_smem_u32(&sh.hist[bin]), c));
+        if (WEIGHTS) heavy += ld_cluster_u64(zb_mapa(zb_smem_u32(&sh.heavy[bin]), c));
       }
-      if (threadIdx.x == kThreads - 1 && before + sum < need)      // there are not as many
-        for (int c = 0; c < ctas; ++c) st_cluster_u32(zb_mapa(zb_smem_u32(&sh.found), c), ~0u);
+      return WEIGHTS ? heavy + n * weight(x_lo + (static_cast<float>(bin) + 0.5f) * (span / static_cast<float>(kBins - 1))) : n;
+    };
+    u64 mass[kEach], sum = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      mass[j] = j < each_bins && static_cast<int>(threadIdx.x) * each_bins + j < share ? mass_of(top_bin - j) : 0;
+      sum += mass[j];
     }
+    u64 upto = warp_upto(sum, lane);
+    if (lane == 31) sh.part[warp] = upto;
+    __syncthreads();
+    u64 before = upto - sum, mine = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const u64 y = sh.part[w];
+      if (w < warp) before += y;
+      mine += y;
+    }
+    if (threadIdx.x < ctas) st_cluster_u64(zb_mapa(zb_smem_u32(&sh.total[rank]), threadIdx.x), mine);
     cluster_sync();
-    const int bin = static_cast<int>(sh.found);
-    need = sh.left;
-    if (bin < 0) {
+    u64 total = 0;
+    for (int c = 0; c < ctas; ++c) {
+      if (c < rank) before += sh.total[c];
+      total += sh.total[c];
+    }
+    // the bins in which two sums are reached (counts: one)
+    const u64 off = WEIGHTS ? all >> 11 : 0;
+#pragma unroll
+    for (int i = 0; i < (WEIGHTS ? 2 : 1); ++i) {
+      const u64 goal = i == 0 ? (need > off ? need - off : 1) : need + off;
+      int bin = -1;
+      u64 at = before;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        if (bin < 0 && at < goal && at + mass[j] >= goal) bin = top_bin - j;
+        if (bin < 0) at += mass[j];
+      }
+      if (total < goal && rank == 0 && threadIdx.x == 0) bin = WEIGHTS ? 0 : kBins;      // there are not as many
+      if (bin >= 0)
+        for (int c = 0; c < ctas; ++c) {
+          if (i == 0) st_cluster_u64(zb_mapa(zb_smem_u32(&sh.left), c), goal - at);
+          st_cluster_u32(zb_mapa(zb_smem_u32(&sh.found[i]), c), static_cast<uint32_t>(bin));
+        }
+    }
+    if (threadIdx.x == 0) sh.n = 0, sh.range[0] = ~0u, sh.range[1] = 0;
+    cluster_sync();
+    const int bin_hi = static_cast<int>(sh.found[0]), bin_lo = WEIGHTS ? static_cast<int>(sh.found[1]) : bin_hi;
+    if (!WEIGHTS && bin_hi == kBins) {
       *rest = ~0ull;
       cluster_sync();
       return 0;
     }
-    const auto inside = [&](float x) { return x >= x_lo && key_of(x) > floor_key && bin_of(x) == bin; };
-    // ---- the interval's logits
-    if (threadIdx.x == 0) sh.n = 0, sh.range[0] = ~0u, sh.range[1] = 0;
-    __syncthreads();
+    // ---- the logits of these intervals
     uint32_t smallest = ~0u, largest = 0;
-    each([&](int at, const float4& v) {
-      const float e[4] = {v.x, v.y, v.z, v.w};
+    u64 above = 0;
+    uint32_t counted = 0;
+    each([&](const float (&e)[4], int index, int step) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (!inside(e[j])) continue;
-        const uint32_t key = key_of(e[j]), slot = atomicAdd(&sh.n, 1u);
-        smallest = min(smallest, key), largest = max(largest, key);
-        if (slot < kList) sh.list.cand[slot] = static_cast<u64>(key) << 32 | static_cast<uint32_t>(~(from + at + j));
+        const int b = counts(e[j]) ? bin_of(e[j]) : -1;
+        if (WEIGHTS && b > bin_hi) above += biased(e[j]), ++counted;
+        const bool in = b >= bin_lo && b <= bin_hi;
+        if (in) smallest = min(smallest, key_of(e[j])), largest = max(largest, key_of(e[j]));
+        append(in, e[j], index + j * step);
       }
     });
     smallest = __reduce_min_sync(0xffffffffu, smallest);
     largest = __reduce_max_sync(0xffffffffu, largest);
-    if (lane == 0) atomicMin(&sh.range[0], smallest), atomicMax(&sh.range[1], largest);
+    above = warp_sum(above - counted * kBias);
+    if (lane == 0) atomicMin(&sh.range[0], smallest), atomicMax(&sh.range[1], largest), sh.above[warp] = above;
     __syncthreads();
     if (threadIdx.x < ctas) {
-      st_cluster_u32(zb_mapa(zb_smem_u32(&sh.count[rank]), threadIdx.x), sh.n);
+      u64 a = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) a += sh.above[w];
+      st_cluster_u64(zb_mapa(zb_smem_u32(&sh.total[rank]), threadIdx.x), a);
       st_cluster_u32(zb_mapa(zb_smem_u32(&sh.least[rank]), threadIdx.x), sh.range[0]);
       st_cluster_u32(zb_mapa(zb_smem_u32(&sh.bound[rank]), threadIdx.x), sh.range[1]);
     }
-    cluster_sync();
-    int n = 0;
-    for (int c = 0; c < ctas; ++c) {
-      n += static_cast<int>(min(sh.count[c], static_cast<uint32_t>(kList + 1)));
-      smallest = min(smallest, sh.least[c]), largest = max(largest, sh.bound[c]);
-    }
-    if (smallest == largest) {
-      *rest = need;
+    const int n = exchange_counts();
+    u64 n_all = 0;
+    above = 0;
+    for (int c = 0; c < ctas; ++c) smallest = min(smallest, sh.least[c]), largest = max(largest, sh.bound[c]), above += sh.total[c], n_all += sh.count[c];
+    const u64 here = WEIGHTS ? (above < need ? need - above : 0) : sh.left;      // what is needed of these logits
+    if (here > 0 && smallest == largest && n_all * (WEIGHTS ? weight(value_of(smallest)) : 1) >= here) {
+      *rest = here;
+      listed = WEIGHTS && n <= kList;
       cluster_sync();
       return smallest;
     }
-    if (n <= kList) {
+    if (here > 0 && n <= kList) {
       sort_lists(n);
       if (rank == 0) {
-        u64 w0, w1, all;
-        u64 before;
-        const int i = 2 * threadIdx.x;
-        if (WEIGHTS) {
-          before = list_before(n, w0, w1, all);
-        } else {
-          before = i;
-          w0 = i < n, w1 = i + 1 < n;
-        }
+        const int i = kMine * threadIdx.x;
+        u64 w[kMine], all;
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) w[j] = i + j < n ? (WEIGHTS ? weight(value_of(key_at(sh.list.sorted[i + j]))) : 1) : 0;
+        u64 before = list_before(w, &all);
         // the first whose sum reaches it; what its equals in front of it have is part of `rest`
-        const bool here0 = i < n && before < need && before + w0 >= need, here1 = i + 1 < n && before + w0 < need && before + w0 + w1 >= need;
-        if (here0 || here1) {
-          const int at = here0 ? i : i + 1;
-          const uint32_t key = key_at(sh.list.sorted[at]);
-          u64 left = need - (here0 ? before : before + w0);
-          const u64 w = WEIGHTS ? weight(value_of(key)) : 1;
-          for (int j = at - 1; j >= 0 && key_at(sh.list.sorted[j]) == key; --j) left += w;
+        int at = -1;
+        u64 left = 0;
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+          if (i + j < n && before < here && before + w[j] >= here) at = i + j, left = here - before;
+          before += w[j];
+        }
+        uint32_t key = 0;
+        if (at >= 0) {
+          key = key_at(sh.list.sorted[at]);
+          const u64 one = WEIGHTS ? weight(value_of(key)) : 1;
+          for (int j = at - 1; j >= 0 && key_at(sh.list.sorted[j]) == key; --j) left += one;
+        }
+        if (at >= 0 || (all < here && threadIdx.x == 0))      // (0: the sum is reached below these logits)
           for (int c = 0; c < ctas; ++c) {
             st_cluster_u64(zb_mapa(zb_smem_u32(&sh.left), c), left);
-            st_cluster_u32(zb_mapa(zb_smem_u32(&sh.found), c), key);
+            st_cluster_u32(zb_mapa(zb_smem_u32(&sh.found[0]), c), key);
           }
-        }
       }
       cluster_sync();
+      const uint32_t key = sh.found[0];
       *rest = sh.left;
-      const uint32_t key = sh.found;
-      cluster_sync();
-      return key;
+      listed = WEIGHTS && key != 0;
+      if (key != 0) {
+        cluster_sync();
+        return key;
+      }
     }
-    // ---- bit by bit, from the highest one in which they differ: whether what has it set is enough
-    uint32_t prefix = smallest;
-    for (int bit = 31 - __clz(smallest ^ largest); bit >= 0; --bit) {
-      const uint32_t mask = ~((1u << bit) - 1u), want = (prefix & (mask << 1)) | 1u << bit;
+    // ---- bit by bit, from the highest one: whether what has it set is enough.  (A logit of 16 bits has no others.)
+    uint32_t prefix = 0;
+    for (int bit = 31; bit >= (sizeof(T) == 2 && kind != 2 ? 16 : 0); --bit) {
+      const uint32_t mask = ~((1u << bit) - 1u), want = prefix | 1u << bit;
       u64 sum = 0;
-      each([&](int, const float4& v) {
-        const float e[4] = {v.x, v.y, v.z, v.w};
+      each([&](const float (&e)[4], int, int) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (inside(e[j]) && (key_of(e[j]) & mask) == want) sum += WEIGHTS ? weight(e[j]) : 1;
+          if (counts(e[j]) && (key_of(e[j]) & mask) == want) sum += WEIGHTS ? weight(e[j]) : 1;
       });
       cluster_sync();
       sum = sum_all(sum);
-      if (sum >= need) {
-        prefix = want;
-      } else {
-        need -= sum;
-        prefix = want & ~(1u << bit);
-      }
+      if (sum >= need) prefix = want;
+      else need -= sum;
     }
     cluster_sync();
+    // (of negative numbers in 16 bits, the complement's low bits are ones)
+    if (sizeof(T) == 2 && kind != 2 && (prefix & 0x80000000u) == 0) prefix |= 0xffffu;
     *rest = need;
     return prefix;
   }
 
   ZB_DEVICE void run(int row) {
-    const T* x = reinterpret_cast<const T*>(p.logits) + static_cast<size_t>(row) * p.stride;
     const double t = p.temperature != nullptr ? p.temperature[row] : p.temperature_all;
     const double top_p = p.top_p != nullptr ? p.top_p[row] : p.top_p_all;
     const double min_p = p.min_p != nullptr ? p.min_p[row] : p.min_p_all;
@@ -485,17 +627,26 @@ struct Sampler {
     if (!(t > 0.0) || top_p <= 0.0) top_k = 1;
     if (top_k <= 0 || top_k > p.vocab) top_k = p.vocab;
     bool small_k = top_k > 1 && top_k <= kSmallK && top_k < p.vocab;
+    // If every CTA has j logits from some bound on, the row has ctas * j of them: the smallest of the CTAs' j-th largest is at most the row's.
+    const int j_th = (top_k + ctas - 1) / ctas;
+    small_k = small_k && j_th <= kThreads;
 
     // ---- the row, its largest logit and its smallest one
-    float most, lowest;
-    load(x, most, lowest);
+    float most = -INFINITY, lowest = INFINITY;
+    each([&](const float (&e)[4], int, int) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        most = fmaxf(most, e[j]);
+        lowest = e[j] > -INFINITY ? fminf(lowest, e[j]) : lowest;
+      }
+    });
     for (int j = threadIdx.x; j < kTable; j += kThreads) sh.table[j] = exp2((j + 0.5) / kTable);
     const uint32_t my_best = key_of(most);
     {
       const uint32_t b = __reduce_max_sync(0xffffffffu, my_best), l = __reduce_min_sync(0xffffffffu, key_of(lowest));
       if (lane == 0) sh.warp_best[warp] = b, sh.warp_least[warp] = l;
     }
-    if (small_k) find_bound(my_best, top_k);
+    if (small_k) find_bound(my_best, j_th);
     else __syncthreads();
     zb_cluster_wait();                               // every CTA runs
     if (threadIdx.x < ctas) {
@@ -503,12 +654,12 @@ struct Sampler {
       for (int w = 0; w < kWarps; ++w) b = max(b, sh.warp_best[w]), l = min(l, sh.warp_least[w]);
       st_cluster_u32(zb_mapa(zb_smem_u32(&sh.best[rank]), threadIdx.x), b);
       st_cluster_u32(zb_mapa(zb_smem_u32(&sh.least[rank]), threadIdx.x), l);
-      st_cluster_u32(zb_mapa(zb_smem_u32(&sh.bound[rank]), threadIdx.x), small_k ? sh.range[0] : 0u);
+      st_cluster_u32(zb_mapa(zb_smem_u32(&sh.bound[rank]), threadIdx.x), small_k ? sh.range[0] : ~0u);
     }
     cluster_sync();
-    uint32_t row_least = ~0u, bound = 0;
+    uint32_t row_least = ~0u, bound = ~0u;
     best = 0;
-    for (int c = 0; c < ctas; ++c) best = max(best, sh.best[c]), row_least = min(row_least, sh.least[c]), bound = max(bound, sh.bound[c]);
+    for (int c = 0; c < ctas; ++c) best = max(best, sh.best[c]), row_least = min(row_least, sh.least[c]), bound = min(bound, sh.bound[c]);
     top = value_of(best);
     if (top == -INFINITY) {                          // nothing is allowed
       if (rank == 0 && threadIdx.x == 0) {
@@ -518,19 +669,13 @@ struct Sampler {
       return;                                        // (alike in all CTAs, and none writes to another one any more)
     }
     if (top == INFINITY) {                           // infinities are alike, and all else is nothing beside them
-      each([&](int at, const float4& v) {
-        *reinterpret_cast<float4*>(x_s + at) = make_float4(v.x == INFINITY ? 1.f : -INFINITY, v.y == INFINITY ? 1.f : -INFINITY, v.z == INFINITY ? 1.f : -INFINITY, v.w == INFINITY ? 1.f : -INFINITY);
-      });
-      __syncwarp();
+      kind = 1;
       top = 1.f;
       best = row_least = key_of(1.f);
       bound = min(bound, best);
     }
-    if (t > 1e37 && (top > 1e30f || value_of(row_least) < -1e30f)) {      // so that the scale below leaves them alike
-      each([&](int at, const float4& v) {
-        *reinterpret_cast<float4*>(x_s + at) = make_float4(v.x * 0x1p-100f, v.y * 0x1p-100f, v.z * 0x1p-100f, v.w * 0x1p-100f);
-      });
-      __syncwarp();
+    if (kind == 0 && t > 1e37 && (top > 1e30f || value_of(row_least) < -1e30f)) {      // so that the scale below leaves them alike
+      kind = 2;
       top *= 0x1p-100f;
       best = key_of(top), row_least = key_of(value_of(row_least) * 0x1p-100f), bound = key_of(value_of(bound) * 0x1p-100f);
     }
@@ -558,7 +703,7 @@ struct Sampler {
       stay = 1;
     } else {
       if (small_k) {
-        const int n = gather(max(bound, least));
+        const int n = gather(top_p < 1.0 ? bound : max(bound, least));      // (top_p is of the sum of all top_k)
         if (n <= kList) {
           sort_lists(n);
           if (rank == 0) draw_from_list(row, min(n, top_k), top_p, 0, least);
@@ -566,28 +711,29 @@ struct Sampler {
         }
         cluster_sync();
       }
-      if (top_k < p.vocab) cut = search<false>(row_least, 0u, top_k, &stay);
-      u64 all = 0;
+      if (top_k < p.vocab) cut = search<false>(row_least, 0u, top_k, 0, &stay);
       if (top_p < 1.0) {
-        u64 above = 0;
-        uint32_t n = 0;
-        each([&](int, const float4& v) {
-          const float e[4] = {v.x, v.y, v.z, v.w};
+        const float cut_x = value_of(cut);
+        u64 sum = 0;
+        uint32_t counted = 0;
+        each([&](const float (&e)[4], int, int) {
+          if (cut == 0) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const u64 w = biased(e[j]);
-            if (cut == 0 || key_of(e[j]) > cut) above += w, ++n;
+            for (int j = 0; j < 4; ++j) sum += biased(e[j]);
+            counted += 4;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (e[j] > cut_x) sum += biased(e[j]), ++counted;
           }
         });
-        above = sum_all(above - n * kBias);
+        const u64 above = sum_all(sum - counted * kBias), at_cut = cut > 0 ? weight(cut_x) : 0, all = above + (cut > 0 ? stay * at_cut : 0), need = need_of(top_p, all);
         cluster_sync();
-        const u64 at_cut = cut > 0 ? weight(value_of(cut)) : 0;
-        all = above + (cut > 0 ? stay * at_cut : 0);
-        // All logits below this weight together are less than 1 - top_p of the sum (half of that, for what sums are rounded by)
+        // All logits below this weight together are less than 1 - top_p of the sum (half of that, for what sums are rounded by).
         const double z = log2(static_cast<double>(all) / kOne * (1.0 - top_p) / (2.0 * p.vocab)) - 1e-6;
-        const uint32_t enough = max(key_of(__double2float_rd(fmax(top64 + z / scale, -3.4e38))), 1u);
-        const u64 need = need_of(top_p, all);
-        if (enough > cut) {
+        const uint32_t enough = max(key_of(__double2float_rd(fmax(top64 + z / scale, -3.4e38))), row_least);
+        // (a nucleus has at least need / 2^44 logits)
+        if (enough > cut && (need >> 44) < kList) {
           const int n = gather(max(enough, least));
           if (n <= kList) {
             sort_lists(n);
@@ -599,117 +745,106 @@ struct Sampler {
         if (above >= need) {
           u64 rest;
           const uint32_t old = cut;
-          cut = search<true>(max(enough, row_least), old, need, &rest);
+          cut = search<true>(enough, old, need, all, &rest);
           const u64 w = weight(value_of(cut));
           stay = (rest + w - 1) / w;
         } else {
           stay = (need - above + at_cut - 1) / at_cut;
         }
-      } else if (least > cut) {
-        const int n = gather(least);
-        if (n <= kList) {
-          sort_lists(n);
-          if (rank == 0) draw_from_list(row, n, 2.0, 0, least);
-          return;
-        }
-        cluster_sync();
       }
       if (least > cut) {
         cut = least;
         stay = ~0ull;
+        listed = false;
       }
     }
 
-    // ---- what stays, warp after warp and CTA after CTA
-    u64 mass = 0;
-    uint32_t ties = 0, counted = 0;
+    // ---- what stays, CTA after CTA, warp after warp, and of the drawn one's warp eighth after eighth
     const float cut_x = value_of(cut);
-    each([&](int, const float4& v) {
-      const float e[4] = {v.x, v.y, v.z, v.w};
-      if (cut == 0) {
+    u64 mass;
+    uint32_t ties;
+    const auto sum_part = [&]() {                    // of the warp's part
+      mass = 0, ties = 0;
+      uint32_t counted = 0;
+      each([&](const float (&e)[4], int, int) {
+        if (cut == 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mass += biased(e[j]);
-        counted += 4;
-      } else if (__any_sync(0xffffffffu, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= cut_x)) {
+          for (int j = 0; j < 4; ++j) mass += biased(e[j]);
+          counted += 4;
+        } else if (fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) >= cut_x) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (e[j] > cut_x) mass += biased(e[j]), ++counted;
-          ties += e[j] == cut_x ? 1 : 0;
+          for (int j = 0; j < 4; ++j) {
+            if (e[j] > cut_x) mass += biased(e[j]), ++counted;
+            ties += e[j] == cut_x ? 1 : 0;
+          }
         }
+      });
+      mass = warp_sum(mass - counted * kBias);
+      ties = __reduce_add_sync(0xffffffffu, ties);
+    };
+    if (listed) {
+      mass = 0, ties = 0;
+      for (int i = lane; i < static_cast<int>(sh.n); i += 32) {
+        const u64 c = sh.list.cand[i];
+        if (index_at(c) < from || index_at(c) >= end) continue;
+        if (key_at(c) > cut) mass += weight(value_of(key_at(c)));
+        ties += key_at(c) == cut ? 1 : 0;
       }
-    });
-    mass = warp_sum(mass - counted * kBias);
-    ties = __reduce_add_sync(0xffffffffu, ties);
-    if (lane == 0) sh.part[1][warp] = mass, sh.warp_ties[warp] = ties;
+      mass = warp_sum(mass) + sh.above[warp];
+      ties = __reduce_add_sync(0xffffffffu, ties);
+    } else {
+      sum_part();
+    }
+    if (lane == 0) sh.seg[warp] = mass, sh.seg_ties[warp] = ties;
     __syncthreads();
     if (threadIdx.x < ctas) {
       u64 s = 0;
       uint32_t n = 0;
-      for (int w = 0; w < kWarps; ++w) s += sh.part[1][w], n += sh.warp_ties[w];
+      for (int w = 0; w < kWarps; ++w) s += sh.seg[w], n += sh.seg_ties[w];
       st_cluster_u64(zb_mapa(zb_smem_u32(&sh.total[rank]), threadIdx.x), s);
       st_cluster_u32(zb_mapa(zb_smem_u32(&sh.ties[rank]), threadIdx.x), n);
     }
     cluster_sync();
     const u64 tie_weight = cut > 0 ? weight(cut_x) : 0;
-    const auto kept = [&](u64 m, uint32_t n, u64& room) {      // of a part, whose equals of the cut stay as far as there is room
+    u64 room = stay;
+    const auto kept = [&](u64 m, uint32_t n) {       // of a part, whose equals of the cut stay as far as there is room
       const u64 k = min(static_cast<u64>(n), room);
       room -= k;
       return m + k * tie_weight;
     };
-    u64 all = 0, room = stay;
-    for (int c = 0; c < ctas; ++c) all += kept(sh.total[c], sh.ties[c], room);
+    u64 all = 0;
+    for (int c = 0; c < ctas; ++c) all += kept(sh.total[c], sh.ties[c]);
     u64 target = target_of(uniform(row), all);
     room = stay;
-    for (int c = 0; c < ctas; ++c) {
-      const u64 before = room, here = kept(sh.total[c], sh.ties[c], room);
-      if (target >= here) {
-        target -= here;
-        continue;
-      }
-      if (c != rank) return;                         // (nobody's shared memory is read from another CTA any more)
-      room = before;
-      break;
-    }
-    for (int w = 0; w < kWarps; ++w) {
-      const u64 before = room, here = kept(sh.part[1][w], sh.warp_ties[w], room);
-      if (target >= here) {
-        target -= here;
-        continue;
-      }
-      if (w != warp) return;
-      room = before;
-      break;
-    }
-#pragma unroll 1
-    for (int i = 0; i < rows; ++i) {
-      const int at = first + i * 128 + lane * 4;
-      const float4 v = *reinterpret_cast<const float4*>(x_s + at);
-      const float e[4] = {v.x, v.y, v.z, v.w};
-      uint32_t mine = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) mine += cut > 0 && e[j] == cut_x ? 1 : 0;
-      uint32_t upto = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t n = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += n;
-      }
-      u64 tie = upto - mine, w[4], sum = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        w[j] = cut == 0 || e[j] > cut_x ? weight(e[j]) : 0;
-        if (cut > 0 && e[j] == cut_x && tie++ < room) w[j] = tie_weight;
-        sum += w[j];
-      }
-      room -= min(room, static_cast<u64>(__shfl_sync(0xffffffffu, upto, 31)));
-      const u64 sums = warp_upto(sum, lane), row_sum = __shfl_sync(0xffffffffu, sums, 31);
-      if (row_sum > target) {
-        u64 s = sums - sum;
-        if (s <= target && sums > target) {
-          int j = 0;
-          while (s + w[j] <= target) s += w[j++];
-          write(row, from + at + j, e[j], all);
+    const auto pick = [&](const u64* m, const uint32_t* n, int parts) {      // the part that has the target
+      for (int i = 0; i < parts; ++i) {
+        const u64 before = room, here = kept(m[i], n[i]);
+        if (target < here) {
+          room = before;
+          return i;
         }
+        target -= here;
+      }
+      return parts - 1;                              // (there is one)
+    };
+    if (pick(sh.total, sh.ties, ctas) != rank) return;      // (nobody's shared memory is read from another CTA any more)
+    const int owner = pick(sh.seg, sh.seg_ties, kWarps), share = p.slice / kWarps, base = rank * p.slice + owner * share, eighth = (share / kWarps + 31) / 32 * 32;
+    from = min(base + warp * eighth, min(base + share, p.vocab));
+    end = min(from + eighth, min(base + share, p.vocab));
+    sum_part();
+    if (lane == 0) sh.sub[warp] = mass, sh.sub_ties[warp] = ties;
+    __syncthreads();
+    if (pick(sh.sub, sh.sub_ties, kWarps) != warp) return;
+    for (int i = from; i < end; i += 32) {
+      const int at = i + lane;
+      const float v = at < end ? fix(static_cast<float>(x[at])) : -INFINITY;
+      const bool tie = cut > 0 && at < end && v == cut_x;
+      const uint32_t tied = __ballot_sync(0xffffffffu, tie);
+      const u64 w = tie ? (static_cast<u64>(__popc(tied & ((1u << lane) - 1u))) < room ? tie_weight : 0) : cut == 0 || v > cut_x ? weight(v) : 0;
+      room -= min(room, static_cast<u64>(__popc(tied)));
+      const u64 upto = warp_upto(w, lane), row_sum = __shfl_sync(0xffffffffu, upto, 31);
+      if (row_sum > target) {
+        if (upto > target && upto - w <= target) write(row, at, v, all);
         return;
       }
       target -= row_sum;
@@ -717,35 +852,36 @@ struct Sampler {
   }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) zb_sample_kernel(const SampleParams p, int log2_ctas) {
-  extern __shared__ __align__(16) float x_s[];       // [slice]
-  __shared__ Shared sh;
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) zb_sample_kernel(const SampleParams p, int log2_ctas) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  Shared<kThreads>& sh = *reinterpret_cast<Shared<kThreads>*>(raw);
   zb_cluster_arrive();                               // every CTA runs before another one writes to its shared memory
   zb_pdl_launch();
   zb_pdl_wait();
-  Sampler<T> s(p, sh, x_s, log2_ctas);
+  Sampler<T, kThreads> s(p, sh, log2_ctas);
   s.run(blockIdx.x >> log2_ctas);
 }
 
-// CTAs of a row: as many as keep its slices small enough for two on an SM, and more while that fills the GPU.
-int ctas_of(int rows, int vocab, int sms) {
-  int log2 = 0;
-  while (log2 < 3 && ((vocab + (1 << log2) - 1) >> log2) > 20480) ++log2;
-  while (log2 < 3 && (static_cast<long long>(rows) << log2) < 2 * sms && (vocab >> log2) > 4 * kThreads) ++log2;
-  return log2;
-}
-
-template <typename T>
-int launch(SampleParams& p, int rows, cudaStream_t s) {
-  const int log2 = ctas_of(rows, p.vocab, zb_num_sms()), unit = 128 * kWarps;
+template <typename T, int kThreads>
+int launch(SampleParams& p, int rows, int log2, cudaStream_t s) {
+  const int unit = 128 * kThreads / 32;
   p.slice = ((p.vocab + (1 << log2) - 1) / (1 << log2) + unit - 1) / unit * unit;
-  p.vec = reinterpret_cast<uintptr_t>(p.logits) % (4 * sizeof(T)) == 0 && (rows == 1 || p.stride % 4 == 0);
   static bool configured[16] = {};
-  if (const int rc = zb_config_smem_once(zb_sample_kernel<T>, kMaxSlice * 4, configured)) return rc;
-  const cudaError_t e = zb_launch_cluster(zb_sample_kernel<T>, dim3(static_cast<unsigned>(rows) << log2), dim3(kThreads), p.slice * 4, s, 1 << log2, p, log2);
+  if (const int rc = zb_config_smem_once(zb_sample_kernel<T, kThreads>, sizeof(Shared<kThreads>), configured)) return rc;
+  const cudaError_t e = zb_launch_cluster(zb_sample_kernel<T, kThreads>, dim3(static_cast<unsigned>(rows) << log2), dim3(kThreads), sizeof(Shared<kThreads>), s, 1 << log2, p, log2);
   zb_count_launch(1);
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
+}
+
+// Eight CTAs of a row, of fewer for short ones; as many threads as the rows leave room for.
+template <typename T>
+int launch(SampleParams& p, int rows, cudaStream_t s) {
+  int log2 = 3;
+  while (log2 > 0 && (p.vocab >> log2) < 2048) --log2;
+  p.vec = reinterpret_cast<uintptr_t>(p.logits) % (4 * sizeof(T)) == 0 && (rows == 1 || p.stride % 4 == 0);
+  const long long ctas = static_cast<long long>(rows) << log2;
+  return ctas <= 2 * zb_num_sms() ? launch<T, 512>(p, rows, log2, s) : launch<T, 256>(p, rows, log2, s);
 }
 
 }  // namespace
@@ -769,7 +905,7 @@ struct ZbSample {
 
 int zb_sample(const ZbSample* c) {
   if (c->rows <= 0) return 0;
-  if (c->vocab <= 0 || c->vocab > kMaxSlice * kMaxCtas || c->rows > (1 << 24)) return -30;
+  if (c->vocab <= 0 || c->vocab > kMaxVocab || c->rows > (1 << 24)) return -30;
   if (c->uniforms == nullptr && c->rng == nullptr) return -31;
   if (!zb_device_state()) return -20;
   SampleParams p = {};
