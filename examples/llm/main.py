@@ -2,12 +2,13 @@
 """LLM CLI (the reference's `examples/llm`): load a HF-format checkpoint and chat with it.
 
     python examples/llm/main.py --model=<repo dir | .safetensors | index.json | hf://org/repo | s3://... | gs://... | https://...> [--prompt=...]
-        [--system=...] [--seqlen=2048] [--topk=1] [--temperature=1.0] [--seed=0] [--no-chat-template] [--profile]
-        [--backend=b200|vanilla|attnd] [--attnd-ip=IP:PORT] [--kv-cache=fp8|int8]
+        [--system=...] [--seqlen=2048] [--topk=1] [--temperature=1.0] [--top-p=1.0] [--min-p=0.0] [--seed=0]
+        [--no-chat-template] [--profile] [--backend=b200|vanilla|attnd] [--attnd-ip=IP:PORT] [--kv-cache=fp8|int8]
 
 --backend picks the attention implementation (default: this library's paged kernels; `vanilla` is PyTorch SDPA on K/V
 gathered from the pages); --attnd-ip registers a remote attention daemon at IP:PORT and prefers it (dense decoder
-models, one conversation).  --kv-cache holds keys and values in 8 bits, half the memory of bf16.  --system puts a system message in front of the first turn (chat template only).
+models, one conversation).  --kv-cache holds keys and values in 8 bits, half the memory of bf16.  --top-p and --min-p cut the tokens that are drawn from,
+with --topk=0 among all.  --system puts a system message in front of the first turn (chat template only).
 
 Without --prompt an interactive chat loop starts (history in ~/.llm_chat_history).  For
 tensor / expert parallelism launch one process per GPU:
@@ -45,6 +46,8 @@ class Args:
     seqlen: int = 2048
     topk: int = 1
     temperature: float = 1.0
+    top_p: float = 1.0
+    min_p: float = 0.0
     seed: int = 0
     max_new_tokens: int = 0
     no_chat_template: bool = False
@@ -163,7 +166,7 @@ def main(argv=None) -> int:
     engine = Engine(model, num_pages=(args.seqlen + page - 1) // page + 2, page_size=page, max_batch=1,
                     max_seq_len=args.seqlen, max_prefill_tokens=min(8192, args.seqlen),
                     use_graphs=False if backend == "attnd" else None, kv_dtype=args.kv_cache)     # the daemon is reached from the host: no graph
-    strategy = SamplingStrategy(topk=args.topk, temperature=args.temperature)
+    strategy = SamplingStrategy(topk=args.topk, temperature=args.temperature, top_p=args.top_p, min_p=args.min_p)
     session = Session(engine, args.seqlen, strategy, cfg.eos_ids(), args.seed)
     template = None if args.no_chat_template or tok is None else hub.chat_template(getattr(cfg, "model_type", "llama"))
     chat = Chat(session, tok, template, getattr(cfg, "bos_token_id", None), comm.rank, comm, args.system)

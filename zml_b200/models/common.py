@@ -30,9 +30,22 @@ class Phase(Enum):
 
 @dataclass
 class SamplingStrategy:
-    """topk == 1 is greedy; otherwise top-k then Gumbel-max at `temperature` (zml/nn.zig:1999-2005)."""
+    """topk == 1 is greedy; otherwise top-k then Gumbel-max at `temperature` (zml/nn.zig:1999-2005).  With `top_p` below 1 or `min_p` above 0, with more
+    than 128 candidates, or with a negative `topk` (no such cut), the token is drawn by `ops.sample`; beside `top_p` or `min_p` topk 0 is no cut, too."""
     topk: int = 1
     temperature: float = 1.0
+    top_p: float = 1.0
+    min_p: float = 0.0
+
+    @property
+    def cuts(self) -> bool:
+        """Whether `ops.sample` draws."""
+        return self.topk != 1 and (self.top_p < 1.0 or self.min_p > 0.0 or self.topk < 0 or self.topk > 128)
+
+    @property
+    def draws(self) -> bool:
+        """Whether random numbers are used up."""
+        return self.topk > 1 or self.cuts
 
 
 @dataclass

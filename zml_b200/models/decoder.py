@@ -33,6 +33,7 @@ class AttnMeta:
     q_start_host: Optional[list] = None           # host copy of q_start (prefill), for splitting a chunk by sequences
     seq_lens_host: Optional[list] = None          # host copy of seq_lens (prefill)
     max_q_len: Optional[int] = None               # new tokens of the longest sequence (prefill)
+    shared: Optional[ops.SharedPrefix] = None     # decode: sequences whose first keys are the same pages
     plans: dict = field(default_factory=dict)     # what the layers derive from this step's metadata once (by their own keys)
 
     def kv_pages(self, page_size: int) -> Optional[int]:
@@ -55,6 +56,8 @@ class DecoderModel:
     FP32_ON_GPU = False
     # True when the model's attention also takes a key / value cache in 8 bits (`ops.kv8`)
     QUANT_KV = False
+    # True when the model's decode attention takes `AttnMeta.shared`
+    SHARED_PREFIX = False
     # True: varlen batches (prompts and portions of them) run without programmatic dependent launch
     SERIAL_PREFILL = False
 
@@ -121,6 +124,12 @@ class DecoderModel:
         """Token ids int32 [B] from vocab-parallel logits.  `rng`: device-side {seed, draw counter} of
         `ops.topk_sample` (the serving engine's, so that graph replays draw fresh noise)."""
         comm = self.comm
+        if strategy.cuts:
+            # Under a split vocabulary every rank draws from the gathered logits (column j of rank r is token r * v_per + j), from the same number.
+            lg = logits if comm.world == 1 else comm.all_gather(logits.contiguous(), dim=1)
+            if rng is None:
+                rng = torch.tensor([seed, step], dtype=torch.int64, device=lg.device)
+            return ops.sample(lg, None, strategy.temperature, max(strategy.topk, 0), strategy.top_p, strategy.min_p, rng=rng)
         rng = rng if (rng is not None and logits.is_cuda) else None
         if comm.world == 1:
             if strategy.topk <= 1:

@@ -129,6 +129,7 @@ class LayerWeights:
 class LlamaModel(DecoderModel):
     """Weights of one tensor-parallel rank plus the forward pass over a flattened token batch."""
     QUANT_KV = True
+    SHARED_PREFIX = True
 
     def __init__(self, config: LlamaConfig, comm: Optional[Comm] = None, device="cpu",
                  dtype=torch.bfloat16):
@@ -376,8 +377,9 @@ class LlamaModel(DecoderModel):
             a = impl.paged_prefill(q, kc, vc, meta.block_table, meta.seq_lens, meta.q_start,
                                    window=c.sliding_window, total_q_blocks=meta.total_q_blocks, max_seq_len=meta.max_seq_len, **more)
         else:
+            more = {"shared": meta.shared} if meta.shared is not None else {}
             a = impl.paged_decode(q, kc, vc, meta.block_table, meta.seq_lens, window=c.sliding_window,
-                                  num_splits=meta.num_splits, max_seq_len=meta.max_seq_len)
+                                  num_splits=meta.num_splits, max_seq_len=meta.max_seq_len, **more)
         return a.reshape(a.shape[0], self.hq * c.hd)
 
     def attention(self, lw: LayerWeights, n1, meta: AttnMeta, kc, vc):

@@ -11,7 +11,9 @@ per token with a 4-byte device->host read each step, this engine
 * captures one whole decode step (all layers, sampling, feeding the token back,
   advancing positions / slots on the device) in a CUDA graph per batch bucket, so
   that a decode step costs one graph launch and no host synchronisation,
-* reads generated tokens back in blocks from an on-device history.
+* reads generated tokens back in blocks from an on-device history,
+* with `share_prefixes`, keeps the whole pages that several running prompts begin with once: they are computed and stored
+  once, and the decode attention reads them once for all of them (`ops.shared`).
 
 One Engine instance lives in each tensor-parallel rank; all ranks execute the same
 schedule (SPMD), so no control traffic is needed.
@@ -43,6 +45,8 @@ class PagePool:
     def __init__(self, num_pages: int):
         self.num_pages = num_pages
         self.free = list(range(num_pages - 1, 0, -1))
+        self.more: dict[int, int] = {}           # page -> holders beside the first
+        self.on_free = None                      # called with a page that nobody holds any more
 
     def alloc(self, n: int) -> list[int]:
         if n > len(self.free):
@@ -51,7 +55,25 @@ class PagePool:
         del self.free[len(self.free) - n:]
         return out
 
+    def share(self, pages: list[int]) -> None:
+        """One more holder of pages that are held."""
+        for p in pages:
+            self.more[p] = self.more.get(p, 0) + 1
+
     def release(self, pages: list[int]) -> None:
+        if self.more or self.on_free is not None:
+            kept = []
+            for p in pages:
+                n = self.more.get(p, 0)
+                if n > 1:
+                    self.more[p] = n - 1
+                elif n == 1:
+                    del self.more[p]
+                else:
+                    kept.append(p)
+                    if self.on_free is not None:
+                        self.on_free(p)
+            pages = kept
         self.free.extend(reversed(pages))
 
     @property
@@ -70,6 +92,7 @@ class Request:
     finished: bool = False
     ttft_ms: Optional[float] = None
     slot: int = -1               # row in the model's recurrent-state pool (hybrid models)
+    common: int = 0              # leading pages that were there when the request came (`share_prefixes`)
 
     @property
     def total_len(self) -> int:
@@ -106,8 +129,10 @@ def _bucket(n: int) -> int:
 class Engine:
     def __init__(self, model, num_pages: int, page_size: int = 64, max_batch: int = 64,
                  max_seq_len: int = 4096, max_prefill_tokens: int = 8192, use_graphs: Optional[bool] = None,
-                 history_steps: int = 1024, num_state_slots: Optional[int] = None, kv_dtype: Optional[str] = None):
-        """`kv_dtype`: "fp8" or "int8" for a key / value cache in 8 bits (`ops.kv8`), about half the memory of the model's dtype."""
+                 history_steps: int = 1024, num_state_slots: Optional[int] = None, kv_dtype: Optional[str] = None, share_prefixes: bool = False):
+        """`kv_dtype`: "fp8" or "int8" for a key / value cache in 8 bits (`ops.kv8`), about half the memory of the model's dtype.
+        `share_prefixes`: prompts that begin with the same whole pages as one that is running hold these pages together with it - the answers to
+        one prompt, requests behind one system prompt."""
         self.model = model
         self.device = model.device
         self.page_size = page_size
@@ -118,6 +143,9 @@ class Engine:
         self.pool = PagePool(num_pages)
         self.kv_cache = model.alloc_kv_cache(num_pages, page_size) if kv_dtype is None else model.alloc_quant_kv_cache(num_pages, page_size, kv_dtype)
         self.on_gpu = self.device.type == "cuda"
+        self.share_prefixes = bool(share_prefixes)
+        self._prefixes: dict = {}                # (page in front, tokens of a page) -> page that holds their keys
+        self._prefix_of: dict = {}               # page -> its entry there
         self.use_graphs = self.on_gpu if use_graphs is None else (use_graphs and self.on_gpu)
         self.history_steps = history_steps
         self._graphs: dict = {}
@@ -147,6 +175,12 @@ class Engine:
         self.stateful = hasattr(model, "alloc_state")
         if self.stateful:
             model.alloc_state(self.num_slots + 1)
+        if self.share_prefixes:
+            self._check_sharing(kv_dtype)
+            self.pool.on_free = self._forget
+            # members, offsets and lengths of the groups of a decode step: rows of one tensor
+            self.d_groups = torch.zeros((3, mb + 1), **i32)
+            self._groups_used = False
         if self.on_gpu:
             # read by the bounds-checking build of the library only: the extents kernel arguments do not carry
             # (of an 8-bit cache, whose own kernels always check: the copy for prompts, in pages of 64 tokens)
@@ -181,21 +215,145 @@ class Engine:
             stats.h2d_bytes += host.numel() * host.element_size()
         return host.to(self.device, non_blocking=True) if self.on_gpu else host
 
-    def new_request(self, prompt: Seq[int], max_new_tokens: int) -> Request:
+    def new_request(self, prompt: Seq[int], max_new_tokens: int, share: bool = False) -> Request:
+        """`share` (with `share_prefixes`): for a caller that computes its requests' prompts in the order in which it makes them, and all of them."""
         r = Request(list(prompt), max_new_tokens, self._next_rid)
+        shared: list[int] = []
         if not r.prompt:
             raise ValueError("empty prompt: a request needs at least one token (e.g. the begin-of-text token)")
         self._next_rid += 1
         need = (len(r.prompt) + max_new_tokens + self.page_size - 1) // self.page_size
         if need > self.max_pages:
             raise ValueError(f"request needs {need} pages, engine allows {self.max_pages} per sequence")
-        r.pages = self.pool.alloc(need)
+        share = share and self.share_prefixes
+        if share:
+            shared = self._find_prefix(r.prompt)
+        r.pages = shared + self.pool.alloc(need - len(shared))
+        self.pool.share(shared)
         try:
             self._take_slot(r)
         except OutOfPages:
             self.pool.release(r.pages)
             raise
+        if share:
+            r.common = len(shared)
+            r.computed = len(shared) * self.page_size
+            self._enter_prefix(r)
         return r
+
+    # ------------------------------------------------------------------ pages that several requests begin with
+    def _check_sharing(self, kv_dtype) -> None:
+        c, m = self.model.config, self.model
+        if not m.SHARED_PREFIX or self.stateful:
+            raise ValueError(f"{type(m).__name__} does not share the pages of prompts")
+        if kv_dtype is not None:
+            raise ValueError("a key / value cache in 8 bits does not go with shared pages")
+        if getattr(c, "sliding_window", 0):
+            raise ValueError("attention within a window does not go with shared pages")
+        if getattr(m, "attn_backend", "b200") != "b200":
+            raise ValueError(f"the {m.attn_backend} backend does not share pages")
+        if self.on_gpu and (m.dtype != torch.bfloat16 or c.hd not in ops.shared.HEAD_DIMS or (self.page_size not in (16, 32) and self.page_size % 64)
+                            or self.max_batch > ops.shared.MAX_BATCH):
+            raise ValueError(f"shared pages are for bfloat16 models with heads of {ops.shared.HEAD_DIMS}, pages of 16, 32 or a multiple of 64 tokens and up to "
+                             f"{ops.shared.MAX_BATCH} sequences")
+
+    def _page_keys(self, prompt, pages):
+        """((page in front, its tokens), page) of the whole pages of a prompt, without the one that has its last token: that one is always computed,
+        its logits are needed."""
+        ps, before = self.page_size, 0
+        for i in range((len(prompt) - 1) // ps):
+            page = yield (before, tuple(prompt[i * ps:(i + 1) * ps])), i
+            before = pages[i] if page is None else page
+
+    def _find_prefix(self, prompt) -> list[int]:
+        found: list[int] = []
+        keys = self._page_keys(prompt, found)
+        try:
+            key, _ = next(keys)
+            while True:
+                page = self._prefixes.get(key)
+                if page is None:
+                    break
+                found.append(page)
+                key, _ = keys.send(page)
+        except StopIteration:
+            pass
+        return found
+
+    def _enter_prefix(self, r: Request) -> None:
+        for key, i in self._page_keys(r.prompt, r.pages):
+            if key not in self._prefixes:
+                self._prefixes[key] = r.pages[i]
+                self._prefix_of[r.pages[i]] = key
+
+    def _forget(self, page: int) -> None:
+        key = self._prefix_of.pop(page, None)
+        if key is not None:
+            self._prefixes.pop(key, None)
+
+    @contextlib.contextmanager
+    def _sharing(self):
+        """What an exception leaves behind - pages that nobody has computed - is not found by later requests."""
+        try:
+            yield
+        except BaseException:
+            self._prefixes.clear()
+            self._prefix_of.clear()
+            raise
+
+    def _share_groups(self, rows) -> Optional[torch.Tensor]:
+        """rows: (batch row, request) -> the groups of a decode step, int32 [3, max_batch + 1] on the host, or None where too few keys are shared.  Requests whose
+        first page is the same are one group over the pages that all of them have in front, or, where that saves more, a group
+        for each of their longer common beginnings."""
+        ps, families = self.page_size, {}
+        for row, r in rows:
+            families.setdefault(r.pages[0], []).append((row, r))
+        groups = []
+        for members in families.values():
+            if len(members) < 2:
+                continue
+            # in the order of their pages, whoever shares most with a request is its neighbour
+            whole = sorted((r.pages[:(len(r.prompt) - 1) // ps], row) for row, r in members)
+            lcp = [next((i for i, (x, y) in enumerate(zip(a, b)) if x != y), min(len(a), len(b))) for (a, _), (b, _) in zip(whole, whole[1:])]
+            split = {}
+            for (w, row), n in zip(whole, map(max, lcp + [0], [0] + lcp)):
+                split.setdefault(tuple(w[:n]), []).append(row)
+            one = [([row for _, row in whole], min(lcp))]
+            many = [(rows_, len(k)) for k, rows_ in split.items() if len(rows_) > 1 and k]
+            groups += max(one, many, key=lambda g: sum((len(m) - 1) * n for m, n in g))
+        saved = sum((len(m) - 1) * n for m, n in groups) * ps
+        if saved * self._key_bytes() < self.SHARE_BYTES:
+            return None
+        host = self._host(3, self.max_batch + 1).zero_()
+        at = 0
+        for g, (m, n) in enumerate(groups):
+            host[0, at:at + len(m)] = torch.tensor(m, dtype=torch.int32)
+            at += len(m)
+            host[1, g + 1:] = at
+            host[2, g] = n * ps
+        return host
+
+    # Bytes of keys and values of a layer that sharing has to spare in a step before it is used: below, the kernel's further parts take longer than the keys.
+    SHARE_BYTES = 64 << 20
+
+    def _key_bytes(self) -> int:
+        return 4 * self.model.hkv * self.model.config.hd
+
+    def _set_groups(self, rows, stats) -> None:
+        """Uploads the groups of the next decode steps."""
+        if not self.share_prefixes:
+            return
+        host = self._share_groups(rows)
+        self._groups_used = host is not None
+        if host is not None:
+            if stats is not None:
+                stats.h2d_bytes += host.numel() * 4
+            self.d_groups.copy_(host, non_blocking=True)
+
+    def _shared(self, b: int):
+        if not self.share_prefixes or not self._groups_used:
+            return None
+        return ops.SharedPrefix(self.d_groups[0, :b], self.d_groups[1, :b + 1], self.d_groups[2, :b])
 
     def _take_slot(self, r: Request) -> None:
         if self.stateful:
@@ -221,7 +379,7 @@ class Engine:
 
     def release(self, r: Request) -> None:
         self.pool.release(r.pages)
-        r.pages = []
+        r.pages, r.common = [], 0
         if r.slot >= 0:
             self.slot_free.append(r.slot)
             r.slot = -1
@@ -290,7 +448,7 @@ class Engine:
         with self._varlen_launches():
             if rows:
                 toks = self.model.forward(ids, meta, self.kv_cache, strategy, self.seed, 0, rng=self.d_rng)
-                if strategy is not None and strategy.topk > 1:
+                if strategy is not None and strategy.draws:
                     ops.advance_rng(self.d_rng)
             else:
                 self.model.hidden_states(ids, meta, self.kv_cache)
@@ -350,6 +508,7 @@ class Engine:
         rows[:3, b:], rows[3, b:], rows[4, b:] = 0, -1, self.scratch_slot
         self._tables(bt.numpy(), [r for r, _, _ in chunk])
         self._upload_decode(bb, st, bt, None)
+        self._set_groups([], None)
         self.d_step.zero_()
         max_total = self.max_pages * ps
         return self._decode_step(bb, SamplingStrategy(), self._plan_splits(bb, max_total), max_total, None)[:b]
@@ -376,7 +535,7 @@ class Engine:
     # ------------------------------------------------------------------ decode
     def _decode_body(self, b: int, strategy, num_splits, max_seq_len):
         meta = AttnMeta(False, self.d_pos[:b], self.d_slot[:b], self.d_bt[:b], self.d_seq[:b],
-                        num_splits=num_splits, max_seq_len=max_seq_len,
+                        num_splits=num_splits, max_seq_len=max_seq_len, shared=self._shared(b),
                         q_start=self.d_qs[:b + 1] if self.stateful else None,
                         state_slots=self.d_sslot[:b] if self.stateful else None)
         lg = self.model.logits(self.model.hidden_states(self.d_ids[:b], meta, self.kv_cache))
@@ -408,7 +567,7 @@ class Engine:
         next replay)."""
         if not self.use_graphs:
             return self._decode_body(b, strategy, num_splits, max_seq_len)
-        key = (b, strategy.topk, float(strategy.temperature), num_splits)
+        key = (b, strategy.topk, float(strategy.temperature), float(strategy.top_p), float(strategy.min_p), num_splits, self.share_prefixes and self._groups_used)
         g = self._graphs.get(key)
         if g is None:
             while len(self._graphs) >= self.max_graphs:          # sampling settings come from requests: bound the cache
@@ -448,6 +607,10 @@ class Engine:
         """Generates up to max_new_tokens per prompt.  Token ids go host -> device from pinned
         memory, generated ids come back device -> host in blocks of `sync_interval` steps.
         Returns (outputs, stats); stats times are device times (CUDA events)."""
+        with self._sharing():
+            return self._generate(prompts, max_new_tokens, strategy, eos_ids, sync_interval, seed)
+
+    def _generate(self, prompts, max_new_tokens, strategy, eos_ids, sync_interval, seed):
         strategy = strategy or SamplingStrategy()
         self.set_seed(seed)
         stats = GenerationStats()
@@ -459,7 +622,7 @@ class Engine:
         reqs: list[Request] = []
         try:
             for p in prompts:
-                reqs.append(self.new_request(p, max_new_tokens))
+                reqs.append(self.new_request(p, max_new_tokens, share=True))
         except Exception:
             for r in reqs:                       # a request that does not fit must not strand the pages of the others
                 self.release(r)
@@ -502,6 +665,7 @@ class Engine:
                 st[4, i] = r.slot
             bt[i, :len(r.pages)] = torch.tensor(r.pages, dtype=torch.int32)
         self._upload_decode(bb, st, bt, stats)
+        self._set_groups(list(enumerate(reqs)), stats)
         self.d_ids[:b].copy_(torch.cat([first_tok[r.rid] for r in reqs]))
         self.d_step.zero_()
         max_total = max(pos) + max_new_tokens
@@ -577,6 +741,10 @@ class Engine:
 
         On a multi-rank job every rank calls this with the same arguments; a rank that stopped or left is noticed
         on the host before the next block is launched (`Comm.check_peers`)."""
+        with self._sharing():
+            return self._serve(prompts, max_new_tokens, strategy, eos_ids, sync_interval, seed, arrivals, on_tokens)
+
+    def _serve(self, prompts, max_new_tokens, strategy, eos_ids, sync_interval, seed, arrivals, on_tokens):
         strategy = strategy or SamplingStrategy()
         self.set_seed(seed)
         stats = GenerationStats()
@@ -647,7 +815,7 @@ class Engine:
             while waiting and free_rows and (arrivals is None or arrivals[waiting[0]] <= block):
                 idx = waiting[0]
                 try:
-                    r = self.new_request(prompts[idx], budget[idx])
+                    r = self.new_request(prompts[idx], budget[idx], share=True)
                 except OutOfPages:
                     if not running and not fresh:
                         raise
@@ -694,6 +862,7 @@ class Engine:
                 live[list(running)] = True
                 slot_h = torch.where(live, slot_h, torch.full_like(slot_h, -1))
                 self._upload_decode(bb, torch.stack([ids_h, pos_h, pos_h + 1, slot_h.to(torch.int32), ss_h]), bt_h, stats)
+                self._set_groups([(row, r) for row, (_, r) in running.items()], stats)
             # ---------------- one decode block
             left = max(budget[idx] - len(outputs[idx]) for idx, _ in running.values())
             n = max(1, min(sync_interval, self.history_steps, left))
@@ -786,6 +955,7 @@ class Session:
         eng.d_bt[0, :len(self.req.pages)] = torch.tensor(self.req.pages, **i32)
         if eng.stateful:
             eng.d_sslot[:1] = torch.tensor([self.req.slot], **i32)
+        eng._set_groups([], None)
         splits = eng._plan_splits(1, self.max_tokens)
         pending = [self._next]
         done = False

@@ -5,9 +5,9 @@ The reference stops at the chat CLI (examples/llm); this is the small piece a de
 `Engine.serve`.  Requests are collected for a short window (`batch_window_s`) or until `max_queue` of them wait, then
 run as one `Engine.serve` call, which batches them continuously on the device; requests that arrive while a batch runs
 wait for the next one.  `"stream": true` answers with server-sent events, one per decode block.  A request may set
-`stop` (strings that end the answer), `temperature`, `top_k` (at most 128, the widest the sampler draws from) and
-`seed`; requests of one batch share their sampling settings, so a batch is the waiting requests whose settings equal those of the oldest one, and the others run
-in a later batch.  On a multi-rank job every rank calls `Server.run()`: rank 0 owns the socket and the queue and
+`stop` (strings that end the answer), `temperature`, `top_k` (at most 128; beside `top_p` or `min_p` any number),
+`top_p`, `min_p` and `seed`; requests of one batch share their sampling settings, so a batch is the waiting requests
+whose settings equal those of the oldest one, and the others run in a later batch.  On a multi-rank job every rank calls `Server.run()`: rank 0 owns the socket and the queue and
 broadcasts each batch (token ids, budgets, sampling settings) so that all ranks enter `Engine.serve` with the same
 arguments; an idle tick is broadcast too, so that the heartbeat of `Comm.check_peers` keeps running while no request is
 in flight.
@@ -78,7 +78,7 @@ class _Request:
     finished: float = 0.0
     stream: bool = False
     chunks: "queue.Queue" = field(default_factory=queue.Queue)       # (new tokens, finished) per decode block
-    sampling: tuple = (1, 1.0, 0)                                    # (top-k, temperature, seed)
+    sampling: tuple = (1, 1.0, 0)                                    # (top-k, temperature, seed), and top-p, min-p where one of them cuts
     stop: tuple = ()                                                 # strings that end the answer (not included in it)
 
 
@@ -120,10 +120,20 @@ class Server:
         return self.queue.qsize() + len(self._held)
 
     def _sampling(self, body: dict) -> tuple:
-        """(top-k, temperature, seed) of a request.  Without `temperature` and `top_k` the server's strategy applies;
-        `temperature: 0` is greedy; a positive temperature without `top_k` draws from the server's k when that is more
-        than 1, else from the MAX_TOP_K best tokens."""
+        """(top-k, temperature, seed) of a request, and behind them top-p and min-p where one of these cuts.  What the body
+        does not set is as in the server's strategy; `temperature: 0` is greedy; a positive temperature without `top_k`
+        draws from the server's k when that is more than 1, else from the MAX_TOP_K best tokens.  `top_p` or `min_p` that
+        cut ask for a draw, too, without `top_k` or the server's k from all tokens that they leave; beside them `top_k` may
+        be any number."""
         k, t = None, None
+        cut = {"top_p": float(self.strategy.top_p), "min_p": float(self.strategy.min_p)}
+        for name in cut:
+            v = body.get(name)
+            if v is not None:
+                if isinstance(v, bool) or not isinstance(v, (int, float)) or not 0 <= v <= 1:
+                    raise ValueError(f"'{name}' must be a number from 0 to 1")
+                cut[name] = round(float(v), 3)          # as the temperature below
+        cuts = cut["top_p"] < 1.0 or cut["min_p"] > 0.0
         if body.get("temperature") is not None:
             t = body["temperature"]
             if isinstance(t, bool) or not isinstance(t, (int, float)) or t < 0 or t != t:
@@ -133,19 +143,22 @@ class Server:
             k = body["top_k"]
             if isinstance(k, bool) or not isinstance(k, int) or k == 0 or k < -1:
                 raise ValueError("'top_k' must be a positive integer (or -1 for the widest supported)")
-            k = MAX_TOP_K if k == -1 else min(k, MAX_TOP_K)
+            k = (0 if k == -1 else k) if cuts else MAX_TOP_K if k == -1 else min(k, MAX_TOP_K)
         seed = body.get("seed", 0)
         if seed is None:
             seed = 0
         if isinstance(seed, bool) or not isinstance(seed, int):
             raise ValueError("'seed' must be an integer")
-        if t is None and k is None:
-            return int(self.strategy.topk), float(self.strategy.temperature), int(seed)
+        asked = any(body.get(name) is not None for name in cut)
         if t == 0.0:
             return 1, 1.0, int(seed)
-        if k is None:
-            k = int(self.strategy.topk) if self.strategy.topk > 1 else MAX_TOP_K
-        return int(k), float(self.strategy.temperature if t is None else t), int(seed)
+        if t is None and k is None and not asked:
+            k = int(self.strategy.topk)
+        elif k is None:
+            greedy = t is None and not cuts and not self.strategy.draws
+            k = int(self.strategy.topk) if self.strategy.topk > 1 else 1 if greedy else 0 if cuts else MAX_TOP_K
+        sampling = k, float(self.strategy.temperature if t is None else t), int(seed)
+        return (*sampling, cut["top_p"], cut["min_p"]) if cuts and k != 1 else sampling
 
     def submit(self, body: dict, chat: bool) -> _Request:
         """Validates a request body and queues it; raises ValueError with the message for a 400 answer."""
@@ -376,8 +389,8 @@ class Server:
                 if batch[i].stream:
                     batch[i].chunks.put((list(toks), fin))
         try:
-            topk, temperature, seed = sampling
-            outs, _ = self.engine.serve(prompts, budgets, SamplingStrategy(topk=topk, temperature=temperature), self.eos_ids,
+            topk, temperature, seed, *cuts = sampling
+            outs, _ = self.engine.serve(prompts, budgets, SamplingStrategy(topk, temperature, *cuts), self.eos_ids,
                                         seed=seed, on_tokens=on_tokens)
             err = None
         except Exception as e:                  # noqa: BLE001 - reported to the callers, the server keeps running
