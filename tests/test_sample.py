@@ -264,3 +264,33 @@ def test_refusals_on_the_gpu():
         ops.sample(x.cuda(), u)
     with pytest.raises(ValueError):
         ops.sample(x.cuda(), u.cuda(), temperature=torch.ones(3))
+
+
+def long_cuts(device, dtype=torch.float32):
+    """Cuts that leave more than a list holds, or nearly so: of many logits, of few distinct ones, of many that are nearly alike, of such without weight."""
+    vocab = 30000
+    g = torch.Generator().manual_seed(5)
+    alike = 1.0 + torch.randperm(vocab, generator=g).float() * 2.0 ** -22                   # all of one bin, and all different (in 32 bits)
+    few = torch.tensor([0.0, 1e-3, 2e-3, -4.0])[torch.randint(0, 4, (vocab,), generator=g)]
+    rows = torch.stack([spread(1, vocab, 2.5, 1)[0][0], spread(1, vocab, 0.4, 2)[0][0], alike, few, torch.zeros(vocab), spread(1, vocab, 2.0, 3, masked=0.7)[0][0]])
+    u = torch.rand(len(rows), generator=g, dtype=torch.float64)
+    for k in (0, 601, 2048, 2049, 9000, vocab - 1):
+        for p in (1.0, 0.9, 0.4):
+            check(rows, u, {"top_k": k, "top_p": p}, device, dtype)
+    check(rows, u, {"top_k": 5000, "top_p": 0.97, "min_p": 0.02, "temperature": 1.3}, device, dtype)
+    for p in (1.0, 0.999, 1.0 - 1e-9):
+        near = len(rows) if p == 1.0 - 1e-9 else 0    # (what is behind this nucleus is as much as 30000 weights are rounded by: 8.5e-10)
+        check(rows, u, {"top_k": 9000, "top_p": p, "temperature": 0.05}, device, dtype, near)      # the 9000th has no weight
+        check(rows, u, {"top_p": p, "temperature": 0.3}, device, dtype, near)
+    check(rows * 1e30, u, {"top_p": 0.6, "temperature": 1e30}, device, dtype)
+    check(rows, u, {"top_k": 7000, "top_p": 0.6, "temperature": math.inf}, device, dtype)
+
+
+def test_long_cuts_cpu():
+    long_cuts("cpu")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_cuts(dtype):
+    long_cuts("cuda", dtype)

@@ -10,12 +10,15 @@
 //
 // A cluster of CTAs has a row, a slice a CTA, and reads it two to four times, all but the first time from L2 (shared memory for the slices would leave two
 // CTAs on an SM: 64 rows of 151936 40 us, 256 380).  The row is not sorted.  All cuts keep what is in front in the order of size, so a row ends in one of two ways:
-//   * a list: what is at least as large as a bound that is known beforehand (the k-th largest of some logits; the weight below which all of the vocabulary
-//     together is less than 1 - top_p; min_p) is usually a few hundred logits, which one CTA ranks, sums and draws from;
-//   * a cut: where these are too many, a histogram finds the smallest logit that stays and how many of its equals do, every warp sums the weights
-//     of its part, and the warp that has the drawn one looks for it.
-// What bounds it: the logits' bytes for many rows, beside some 30 instructions of a weight where the whole row's sum is needed; for few rows the passes' and
-// the cluster's barriers' latency.
+//   * a list: what is at least as large as a bound - the k-th largest of some logits; the weight below which all of the vocabulary together is less than
+//     1 - top_p; the end of the bin of a histogram in which the cut is - is usually a few hundred logits, which one CTA ranks, sums and draws from;
+//   * a cut: where these are too many, one more pass sums the weights above the histogram's bins that may have the cut and lists what is in them, 11 bits of
+//     a logit at a time tell which of these is the smallest that stays and how many of its equals do, and the warp that has the drawn one looks for it.
+// The histogram has a bin for each 2^-9 .. 2^-4 of the weights' logarithm and counts logits, in the pass that sums all weights; a bin's edges bound the weights in it (a
+// histogram over the logits after that pass, with the weights of each bin's middle, and a list tried beforehand: 256 rows with flat logits 322 us, now 257).
+// What bounds it: the logits' bytes for many rows, beside some 30 instructions of a weight where the whole row's sum is needed, some 40 with the histogram's; for few rows
+// the passes' and the cluster's barriers' latency.  Measured, with logits in L2 as a model leaves them: 1 row of 128256 with top_p 15 us, 32 rows with settings of their
+// own 39, 64 rows of 151936 without a cut 35, 128 rows of 248320 with top_k 50 and top_p 55 (127 MB: 2.3 TB/s), 256 rows of 151936 with a nucleus of 80 thousand 257.
 #include "common.cuh"
 #include "host_api.h"
 
@@ -95,23 +98,21 @@ template <int kThreads>
 struct Shared {
   static constexpr int kWarps = kThreads / 32;
   double table[kTable];
+  u64 cand[kList];                                   // of this CTA: key << 32 | ~index, the larger, the further in front
   union {
-    struct {
-      u64 cand[kList];                               // of this CTA: key << 32 | ~index, the larger, the further in front
-      u64 sorted[kList];                             // CTA 0: of the cluster
-      u64 weight[kList];                             // CTA 0: of these; then those that stay, index << 45 | weight
-    } list;
-    struct {
-      uint32_t hist[kBins];
-      u64 heavy[kBins];
-    };
+    u64 sorted[kList];                               // CTA 0: of the cluster
+    uint32_t hist[kBins];
+  };
+  union {
+    u64 weight[kList];                               // CTA 0: of these; then those that stay, index << 45 | weight
+    u64 sums[kBins];
   };
   u64 part[kWarps], seg[kWarps], sub[kWarps], above[kWarps];
-  u64 total[kMaxCtas];                               // of every CTA
+  u64 total[kMaxCtas], lower[kMaxCtas];              // of every CTA
   uint32_t ties[kMaxCtas], count[kMaxCtas], best[kMaxCtas], bound[kMaxCtas], least[kMaxCtas];
   uint32_t seg_ties[kWarps], sub_ties[kWarps], warp_best[kWarps], warp_least[kWarps], top[kThreads], n, range[2];
-  u64 left;                                          // what CTA 0 has found, in every CTA
-  uint32_t found[2];
+  u64 left;                                          // what one thread of the cluster has found, in every CTA
+  uint32_t found[3];
 };
 
 // All threads of a cluster, which is one row.
@@ -126,6 +127,7 @@ struct Sampler {
   float top, floor_x;            // the largest logit; below floor_x weights are zero
   double top64, scale;           // log2 of a weight is (x - top) * scale
   uint32_t best;
+  int bin_from, bin_shift;       // see count_bins
   bool listed;                   // the logits around the cut are in the CTAs' lists, and what is above them in sh.above
 
   ZB_DEVICE Sampler(const SampleParams& params, Shared<kThreads>& shared, int log2_ctas)
@@ -137,8 +139,9 @@ struct Sampler {
 
   // The weight of a logit that is not above `top`, in 2^-44, plus kBias; a NaN's is zero.  z is held with 41 bits behind the point: 4 of them choose the table's
   // entry, and with the other 37 as r, around their middle, 2^r is a polynomial (off by 5e-16).
-  ZB_DEVICE u64 biased(float x) const {
-    const double t = __fma_rn(static_cast<double>(fmaxf(x, floor_x)) - top64, scale, 3072.0);      // 1.5 * 2^11
+  ZB_DEVICE double log2_of(float x) const { return __fma_rn(static_cast<double>(fmaxf(x, floor_x)) - top64, scale, 3072.0); }      // 1.5 * 2^11
+  ZB_DEVICE u64 biased(float x) const { return power(log2_of(x)); }
+  ZB_DEVICE u64 power(double t) const {
     const int hi = __double2hiint(t);
     const double r = __hiloint2double(0x43300000 | (hi & 31), __double2loint(t)) - 4503668346847232.0;      // 2^52 + 2^36
     constexpr double c1 = 0.6931471805599453 * 0x1p-41, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4, c5 = c4 * c1 / 5, c6 = c5 * c1 / 6;
@@ -234,14 +237,22 @@ struct Sampler {
     return s;
   }
 
-  // Into the CTA's list, by whole warps.
-  ZB_DEVICE void append(bool some, float v, int index) {
-    const uint32_t who = __ballot_sync(0xffffffffu, some);
-    if (who == 0) return;
+  // Four of a lane's logits into the CTA's list, by whole warps.
+  ZB_DEVICE void append(const bool (&some)[4], const float (&v)[4], int index, int step) {
+    uint32_t who[4];
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) who[j] = __ballot_sync(0xffffffffu, some[j]), n += __popc(who[j]);
+    if (n == 0) return;
     uint32_t slot = 0;
-    if (lane == 0) slot = atomicAdd(&sh.n, static_cast<uint32_t>(__popc(who)));
-    slot = __shfl_sync(0xffffffffu, slot, 0) + __popc(who & ((1u << lane) - 1u));
-    if (some && slot < kList) sh.list.cand[slot] = static_cast<u64>(key_of(v)) << 32 | static_cast<uint32_t>(~index);
+    if (lane == 0) slot = atomicAdd(&sh.n, static_cast<uint32_t>(n));
+    slot = __shfl_sync(0xffffffffu, slot, 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t mine = slot + __popc(who[j] & ((1u << lane) - 1u));
+      if (some[j] && mine < kList) sh.cand[mine] = static_cast<u64>(key_of(v[j])) << 32 | static_cast<uint32_t>(~(index + j * step));
+      slot += __popc(who[j]);
+    }
   }
   // Every CTA's sh.n to all; how many in the cluster, more than kList: too many.
   ZB_DEVICE int exchange_counts() {
@@ -261,81 +272,80 @@ struct Sampler {
     each([&](const float (&e)[4], int at, int step) {
       if (!__any_sync(0xffffffffu, fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) >= bound)) return;
       if (__shfl_sync(0xffffffffu, *n, 0) > kList) return;      // too many already
+      bool in[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) append(e[j] >= bound && at + j * step < end, e[j], at + j * step);
+      for (int j = 0; j < 4; ++j) in[j] = e[j] >= bound && at + j * step < end;
+      append(in, e, at, step);
     });
     return exchange_counts();
   }
 
-  // The CTAs' lists, n in all, to CTA 0, in the order of size.
-  ZB_DEVICE void sort_lists(int n) {
+  // The CTAs' lists, n in all, of keys from `least` on, to CTA 0, in the order of size.
+  ZB_DEVICE void sort_lists(int n, uint32_t least) {
     if (rank == 0) {
       for (int i = threadIdx.x; i < n; i += kThreads) {
         int c = 0, at = i;
         while (at >= static_cast<int>(sh.count[c])) at -= sh.count[c++];
-        sh.list.weight[i] = ld_cluster_u64(zb_mapa(zb_smem_u32(&sh.list.cand[at]), c));
+        sh.sorted[i] = ld_cluster_u64(zb_mapa(zb_smem_u32(&sh.cand[at]), c));
       }
     }
     cluster_sync();                                  // nobody leaves or writes its list before it has been read
-    if (rank != 0) return;
-    sort_down(sh.list.weight, sh.list.sorted, n);
+    if (rank == 0) sort_down(sh.sorted, sh.weight, n, static_cast<u64>(least) << 32, static_cast<u64>(best) << 32 | 0xffffffffu);
   }
-  // a[0, n) from the largest on to b: a number a thread by counting what is in front of it (256: 1.6 us), more bitonically.
-  ZB_DEVICE void sort_down(const u64* a, u64* b, int n) {
+  // a[0, n), of numbers in [lo, hi] and no two alike, from the largest on, by counting what is in front of each: of all, or (1016: 3 us, bitonically 12) of an interval of 2048.
+  // b, sh.cand: space.
+  ZB_DEVICE void sort_down(u64* a, u64* b, int n, u64 lo, u64 hi) {
     __syncthreads();
     if (n <= min(kThreads, 256)) {
+      int ahead = 0;
+      u64 mine = 0;
       if (static_cast<int>(threadIdx.x) < n) {
-        const u64 mine = a[threadIdx.x];
-        int ahead = 0;
+        mine = a[threadIdx.x];
 #pragma unroll 8
-        for (int j = 0; j < n; ++j) ahead += a[j] > mine || (a[j] == mine && j < static_cast<int>(threadIdx.x)) ? 1 : 0;
-        b[ahead] = mine;
+        for (int j = 0; j < n; ++j) ahead += a[j] > mine ? 1 : 0;
       }
+      __syncthreads();
+      if (static_cast<int>(threadIdx.x) < n) a[ahead] = mine;
       __syncthreads();
       return;
     }
-    // Neighbours in registers: of the distances, the smallest lie within a thread, the next ones within a warp.
-    const int size = 2 << (31 - __clz(n - 1)), i0 = kMine * threadIdx.x;
-    u64 v[kMine];
+    constexpr int kOwn = kBins / kThreads;
+    uint32_t* ends = reinterpret_cast<uint32_t*>(sh.cand) + 1;      // of the intervals, from the highest on: ends[-1] is 0
+    const int shift = max(0, 53 - __clzll(static_cast<long long>(hi - lo)));
+    const auto interval = [&](u64 v) { return static_cast<int>((hi - v) >> shift); };
+    for (int i = threadIdx.x; i <= kBins; i += kThreads) ends[i - 1] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) atomicAdd(&ends[interval(a[i])], 1u);
+    __syncthreads();
+    uint32_t count[kOwn], mine = 0;
 #pragma unroll
-    for (int j = 0; j < kMine; ++j) v[j] = i0 + j < n ? a[i0 + j] : 0;
-    const auto keep = [&](u64 mine, u64 other, int i, int k, int d) { return ((i & d) == 0) == ((i & k) == 0) ? max(mine, other) : min(mine, other); };
-#pragma unroll 1
-    for (int k = 2; k <= size; k <<= 1) {
-#pragma unroll 1
-      for (int d = k >> 1; d >= kMine; d >>= 1) {
-        u64 other[kMine];
-        if (d >= 32 * kMine) {
-          __syncthreads();
+    for (int j = 0; j < kOwn; ++j) mine += count[j] = ends[threadIdx.x * kOwn + j];
+    uint32_t upto = mine;
 #pragma unroll
-          for (int j = 0; j < kMine; ++j)
-            if (i0 < size) b[i0 + j] = v[j];
-          __syncthreads();
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    if (lane == 31) sh.seg_ties[warp] = upto;
+    __syncthreads();
+    upto -= mine;
 #pragma unroll
-          for (int j = 0; j < kMine; ++j) other[j] = i0 < size ? b[(i0 ^ d) + j] : 0;
-        } else {
+    for (int w = 0; w < kWarps; ++w) upto += w < warp ? sh.seg_ties[w] : 0;
 #pragma unroll
-          for (int j = 0; j < kMine; ++j) other[j] = __shfl_xor_sync(0xffffffffu, v[j], d / kMine);
-        }
-#pragma unroll
-        for (int j = 0; j < kMine; ++j) v[j] = keep(v[j], other[j], i0 + j, k, d);
-      }
-#pragma unroll
-      for (int d = kMine / 2; d > 0; d >>= 1) {
-        if (d >= k) continue;
-#pragma unroll
-        for (int j = 0; j < kMine; ++j) {
-          if ((j & d) != 0) continue;
-          const u64 lo = min(v[j], v[j | d]), hi = max(v[j], v[j | d]);
-          const bool down = ((i0 + j) & k) == 0;
-          v[j] = down ? hi : lo, v[j | d] = down ? lo : hi;
-        }
-      }
+    for (int j = 0; j < kOwn; ++j) {
+      ends[threadIdx.x * kOwn + j] = upto;           // where it begins, until its numbers are there
+      upto += count[j];
     }
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kMine; ++j)
-      if (i0 < size) b[i0 + j] = v[j];
+    for (int i = threadIdx.x; i < n; i += kThreads) b[atomicAdd(&ends[interval(a[i])], 1u)] = a[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const u64 v = b[i];
+      const int at = interval(v), first = ends[at - 1], last = ends[at];
+      int ahead = first;
+      for (int j = first; j < last; ++j) ahead += b[j] > v ? 1 : 0;
+      a[ahead] = v;
+    }
     __syncthreads();
   }
   static ZB_DEVICE uint32_t key_at(u64 c) { return static_cast<uint32_t>(c >> 32); }
@@ -381,7 +391,7 @@ struct Sampler {
     u64 c[kMine], w[kMine], sum;
 #pragma unroll
     for (int j = 0; j < kMine; ++j) {
-      c[j] = i + j < n ? sh.list.sorted[i + j] : 0;
+      c[j] = i + j < n ? sh.sorted[i + j] : 0;
       w[j] = i + j < n ? weight(value_of(key_at(c[j]))) : 0;
     }
     u64 before = list_before(w, &sum);
@@ -393,7 +403,7 @@ struct Sampler {
       if (i + j < n && (i + j == 0 || (before < need && key_at(c[j]) >= least))) {
         ++stays;
         kept += w[j];
-        sh.list.weight[i + j] = static_cast<u64>(static_cast<uint32_t>(0x7ffffu - index_at(c[j]))) << 45 | w[j];      // (sorted down: the lowest index first)
+        sh.weight[i + j] = static_cast<u64>(static_cast<uint32_t>(0x7ffffu - index_at(c[j]))) << 45 | w[j];      // (sorted down: the lowest index first)
       }
       before += w[j];
     }
@@ -412,20 +422,20 @@ struct Sampler {
     };
     if (m <= min(kThreads, 256)) {
       if (static_cast<int>(threadIdx.x) >= m) return;
-      const u64 mine = sh.list.weight[threadIdx.x];
+      const u64 mine = sh.weight[threadIdx.x];
       before = 0;
 #pragma unroll 8
       for (int j = 0; j < m; ++j) {
-        const u64 y = sh.list.weight[j];
+        const u64 y = sh.weight[j];
         before += y > mine ? y & kWeight : 0;        // (of lower index; no two have the same)
       }
       if (before <= target && target - before < (mine & kWeight)) found(mine);
       return;
     }
-    sort_down(sh.list.weight, sh.list.cand, m);
+    sort_down(sh.weight, sh.sorted, m, static_cast<u64>(0x80000 - p.vocab) << 45, (1ull << 63) + ((1ull << 63) - 1));
 #pragma unroll
     for (int j = 0; j < kMine; ++j) {
-      c[j] = i + j < m ? sh.list.cand[i + j] : 0;
+      c[j] = i + j < m ? sh.weight[i + j] : 0;
       w[j] = c[j] & kWeight;
     }
     before = list_before(w, &sum);
@@ -436,105 +446,213 @@ struct Sampler {
     }
   }
 
-  // The largest key up to which, from above, the counts (or weights) of the logits above `floor_key`, from `lo` on, sum to at least `need`; *rest: what is needed
-  // there.  0: there are not as many.  A histogram of counts over 2048 equal intervals of [value_of(lo), top] tells the interval, and one more pass lists its logits.  Of weights
-  // it tells it nearly: weights above all / 4096 are summed as they are, and for the others stands an interval's middle, half a hundredth off, to either side.
-  // (Their sum is off by some all / 2^13.)  So all is listed where the sum may lie within all / 2^11 of it, and what is above that is summed (for each
-  // warp to sh.above).  What cannot be listed is looked for bit by bit.
-  template <bool WEIGHTS>
-  ZB_DEVICE uint32_t search(uint32_t lo, uint32_t floor_key, u64 need, u64 all, u64* rest) {
-    const float x_lo = fmaxf(value_of(lo), -3.0e38f), span = top - x_lo, by = span > 0.f ? static_cast<float>(kBins - 1) / span : 0.f;
-    const float floor_value = floor_key > 0 ? value_of(floor_key) : -INFINITY;
-    const auto counts = [&](float v) { return v >= x_lo && v > floor_value; };
-    const auto bin_of = [&](float v) { return max(0, min(kBins - 1, static_cast<int>((v - x_lo) * by))); };      // grows with v
-    const float heavy_x = WEIGHTS ? __double2float_rd(fmax(top64 + log2(static_cast<double>(all) / (kOne * 4096.0)) / scale, -3.4e38)) : INFINITY;
-    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.hist[i] = 0, sh.heavy[i] = 0;
+  // ---- the cuts of rows that are too long for a list
+  // Counts of the logits with weights of 2^z_from or more, in up to 2048 bins of equal length on the weights' logarithm (the high word of log2_of: 2^-9 or
+  // more; from the row's smallest logit on).  With `list` they are listed, too, until there are too many.  Returns the thread's sum of weights.
+  ZB_DEVICE u64 count_bins(double z_from, uint32_t row_least, bool sums, bool list) {
+    bin_from = max(__double2hiint(log2_of(value_of(row_least))), __double2hiint(3072.0 + z_from));
+    bin_shift = max(0, 21 - __clz(__double2hiint(3072.0) - bin_from));
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.hist[i] = 0;
+    if (threadIdx.x == 0) sh.n = list ? 0 : kList + 1;
     __syncthreads();
-    each([&](const float (&e)[4], int, int) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (counts(e[j])) {
-          if (WEIGHTS && e[j] > heavy_x) atomicAdd(&sh.heavy[bin_of(e[j])], weight(e[j]));
-          else atomicAdd(&sh.hist[bin_of(e[j])], 1u);
-        }
-    });
-    cluster_sync();
-    // Every CTA adds up a share of the bins, from the highest on, a thread some of them.
-    constexpr int kEach = (kBins + kThreads - 1) / kThreads;      // where a row has one CTA
-    const int share = kBins >> (31 - __clz(ctas)), each_bins = (share + kThreads - 1) / kThreads, top_bin = kBins - 1 - rank * share - threadIdx.x * each_bins;
-    const auto mass_of = [&](int bin) {
-      u64 heavy = 0;
-      uint32_t n = 0;
-#pragma unroll 1
-      for (int c = 0; c < ctas; ++c) {
-        n += ld_cluster_u32(zb_mapa(zb_smem_u32(&sh.hist[bin]), c));
-        if (WEIGHTS) heavy += ld_cluster_u64(zb_mapa(zb_smem_u32(&sh.heavy[bin]), c));
-      }
-      return WEIGHTS ? heavy + n * weight(x_lo + (static_cast<float>(bin) + 0.5f) * (span / static_cast<float>(kBins - 1))) : n;
-    };
-    u64 mass[kEach], sum = 0;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      mass[j] = j < each_bins && static_cast<int>(threadIdx.x) * each_bins + j < share ? mass_of(top_bin - j) : 0;
-      sum += mass[j];
-    }
-    u64 upto = warp_upto(sum, lane);
-    if (lane == 31) sh.part[warp] = upto;
-    __syncthreads();
-    u64 before = upto - sum, mine = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const u64 y = sh.part[w];
-      if (w < warp) before += y;
-      mine += y;
-    }
-    if (threadIdx.x < ctas) st_cluster_u64(zb_mapa(zb_smem_u32(&sh.total[rank]), threadIdx.x), mine);
-    cluster_sync();
-    u64 total = 0;
-    for (int c = 0; c < ctas; ++c) {
-      if (c < rank) before += sh.total[c];
-      total += sh.total[c];
-    }
-    // the bins in which two sums are reached (counts: one)
-    const u64 off = WEIGHTS ? all >> 11 : 0;
-#pragma unroll
-    for (int i = 0; i < (WEIGHTS ? 2 : 1); ++i) {
-      const u64 goal = i == 0 ? (need > off ? need - off : 1) : need + off;
-      int bin = -1;
-      u64 at = before;
-#pragma unroll
-      for (int j = 0; j < kEach; ++j) {
-        if (bin < 0 && at < goal && at + mass[j] >= goal) bin = top_bin - j;
-        if (bin < 0) at += mass[j];
-      }
-      if (total < goal && rank == 0 && threadIdx.x == 0) bin = WEIGHTS ? 0 : kBins;      // there are not as many
-      if (bin >= 0)
-        for (int c = 0; c < ctas; ++c) {
-          if (i == 0) st_cluster_u64(zb_mapa(zb_smem_u32(&sh.left), c), goal - at);
-          st_cluster_u32(zb_mapa(zb_smem_u32(&sh.found[i]), c), static_cast<uint32_t>(bin));
-        }
-    }
-    if (threadIdx.x == 0) sh.n = 0, sh.range[0] = ~0u, sh.range[1] = 0;
-    cluster_sync();
-    const int bin_hi = static_cast<int>(sh.found[0]), bin_lo = WEIGHTS ? static_cast<int>(sh.found[1]) : bin_hi;
-    if (!WEIGHTS && bin_hi == kBins) {
-      *rest = ~0ull;
-      cluster_sync();
-      return 0;
-    }
-    // ---- the logits of these intervals
-    uint32_t smallest = ~0u, largest = 0;
-    u64 above = 0;
+    u64 sum = 0;
     uint32_t counted = 0;
-    each([&](const float (&e)[4], int index, int step) {
+    const volatile uint32_t* listed_so_far = &sh.n;
+    each([&](const float (&e)[4], int at, int step) {
+      int d[4], most = -1;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int b = counts(e[j]) ? bin_of(e[j]) : -1;
-        if (WEIGHTS && b > bin_hi) above += biased(e[j]), ++counted;
-        const bool in = b >= bin_lo && b <= bin_hi;
-        if (in) smallest = min(smallest, key_of(e[j])), largest = max(largest, key_of(e[j]));
-        append(in, e[j], index + j * step);
+        const double t = log2_of(e[j]);
+        if (sums) sum += power(t);
+        d[j] = __double2hiint(t) - bin_from;
+        most = max(most, d[j]);
       }
+      counted += 4;
+      if (!__any_sync(0xffffffffu, most >= 0)) return;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (d[j] >= 0) atomicAdd(&sh.hist[d[j] >> bin_shift], 1u);
+      if (list) {
+        if (__shfl_sync(0xffffffffu, *listed_so_far, 0) > kList) list = false;
+        const bool in[4] = {d[0] >= 0, d[1] >= 0, d[2] >= 0, d[3] >= 0};
+        append(in, e, at, step);
+      }
+    });
+    return sums ? sum - counted * kBias : 0;
+  }
+  ZB_DEVICE u64 at_edge(int bin) const {              // the weight where a bin begins
+    return power(__hiloint2double(min(bin_from + (bin << bin_shift), __double2hiint(3072.0)), 0)) - kBias;
+  }
+  // The key of the smallest logit that is in a bin or above it: 5 bits of it at a time, a lane each.
+  ZB_DEVICE uint32_t key_of_bin(int bin) const {
+    if (bin <= 0) bin = 0;
+    const int from_hi = bin_from + (bin << bin_shift);
+    uint32_t lo = 0;                                 // the last one that is below
+#pragma unroll 1
+    for (int shift = 27; shift > -5; shift -= 5) {
+      const int by = max(shift, 0);
+      const uint32_t key = lo + (static_cast<uint32_t>(lane) << by);
+      const bool below = key >= lo && (key < key_of(floor_x) || (key <= best && __double2hiint(log2_of(value_of(key))) < from_hi));
+      lo += static_cast<uint32_t>(31 - __clz(__ballot_sync(0xffffffffu, below) | 1u)) << by;
+    }
+    return lo + 1;
+  }
+  // Where the counts (or weights) of the bins, from the highest on, reach `need`: of weights, not above *first and not below *last, by the weights at the bins' edges (one more or
+  // less, for their roundings).  Returns how many logits there are from *last on; 0: the counts do not reach it.  Of counts, sh.left is what is needed of the bin.
+  ZB_DEVICE uint32_t bracket(bool weights, u64 need, int* first, int* last) {
+    cluster_sync();
+    constexpr int kEach = (kBins + kThreads - 1) / kThreads;      // where a row has one CTA
+    const int share = kBins >> (31 - __clz(ctas)), each_bins = (share + kThreads - 1) / kThreads, top_bin = kBins - 1 - rank * share - threadIdx.x * each_bins;
+    uint32_t n[kEach], counted = 0;
+    u64 up = 0, low = 0;
+    const auto most_of = [&](int j) { return weights ? n[j] * (at_edge(top_bin - j + 1) + 1) : n[j]; };
+    const auto least_of = [&](int j) { return weights ? n[j] * (max(at_edge(top_bin - j), 1ull) - 1) : n[j]; };
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      n[j] = 0;
+      if (j < each_bins && static_cast<int>(threadIdx.x) * each_bins + j < share) {
+#pragma unroll
+        for (int c = 0; c < kMaxCtas; ++c)
+          if (c < ctas) n[j] += ld_cluster_u32(zb_mapa(zb_smem_u32(&sh.hist[top_bin - j]), c));
+        up += most_of(j), low += least_of(j), counted += n[j];
+      }
+    }
+    u64 up_before = warp_upto(up, lane), low_before = warp_upto(low, lane);
+    uint32_t before = counted;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += y;
+    }
+    if (lane == 31) sh.part[warp] = up_before, sh.seg[warp] = low_before, sh.seg_ties[warp] = before;
+    __syncthreads();
+    up_before -= up, low_before -= low, before -= counted;
+    up = low = 0, counted = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) up_before += sh.part[w], low_before += sh.seg[w], before += sh.seg_ties[w];
+      up += sh.part[w], low += sh.seg[w], counted += sh.seg_ties[w];
+    }
+    if (threadIdx.x < ctas) {
+      st_cluster_u64(zb_mapa(zb_smem_u32(&sh.total[rank]), threadIdx.x), up);
+      st_cluster_u64(zb_mapa(zb_smem_u32(&sh.lower[rank]), threadIdx.x), low);
+      st_cluster_u32(zb_mapa(zb_smem_u32(&sh.ties[rank]), threadIdx.x), counted);
+    }
+    cluster_sync();
+    up = low = 0, counted = 0;
+    for (int c = 0; c < ctas; ++c) {
+      if (c < rank) up_before += sh.total[c], low_before += sh.lower[c], before += sh.ties[c];
+      up += sh.total[c], low += sh.lower[c], counted += sh.ties[c];
+    }
+    const auto tell = [&](int which, int bin, uint32_t upto, u64 left) {
+      for (int c = 0; c < ctas; ++c) {
+        st_cluster_u32(zb_mapa(zb_smem_u32(&sh.found[which]), c), static_cast<uint32_t>(bin));
+        if (which == 0) continue;
+        st_cluster_u32(zb_mapa(zb_smem_u32(&sh.found[2]), c), upto);
+        st_cluster_u64(zb_mapa(zb_smem_u32(&sh.left), c), left);
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const u64 most = most_of(j), least = least_of(j);
+      before += n[j];
+      if (up_before < need && up_before + most >= need) tell(0, top_bin - j, 0, 0);
+      if (low_before < need && low_before + least >= need) tell(1, top_bin - j, before, need - low_before);
+      up_before += most, low_before += least;
+    }
+    if (rank == 0 && threadIdx.x == 0) {
+      if (up < need) tell(0, 0, 0, 0);
+      if (low < need) tell(1, 0, weights ? counted : 0, 0);
+    }
+    cluster_sync();
+    *first = static_cast<int>(sh.found[0]), *last = static_cast<int>(sh.found[1]);
+    return sh.found[2];
+  }
+  // The largest key from which on, downwards from `hi`, the counts (or weights) sum to `need`, which those from `lo` on do; *rest: what is needed there.
+  // 11 bits of it at a time; over(f): f(logit) of the thread's.
+  template <typename Over>
+  ZB_DEVICE uint32_t narrow(bool weights, uint32_t lo, uint32_t hi, u64 need, u64* rest, Over&& over) {
+    if (lo == hi) cluster_sync();                    // (as if there were a round: nobody reads what the caller's next steps write)
+    while (lo != hi) {
+      const int shift = max(0, 21 - __clz(hi - lo));
+      for (int i = threadIdx.x; i < kBins; i += kThreads) sh.sums[i] = 0;
+      __syncthreads();
+      over([&](float v) {
+        const uint32_t key = key_of(v);
+        if (key >= lo && key <= hi) atomicAdd(&sh.sums[(key - lo) >> shift], weights ? weight(v) : 1ull);
+      });
+      cluster_sync();
+      constexpr int kEach = (kBins + kThreads - 1) / kThreads;
+      const int share = kBins >> (31 - __clz(ctas)), each_bins = (share + kThreads - 1) / kThreads, top_bin = kBins - 1 - rank * share - threadIdx.x * each_bins;
+      u64 sum[kEach], before = 0, mine = 0;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        sum[j] = 0;
+        if (j < each_bins && static_cast<int>(threadIdx.x) * each_bins + j < share) {
+#pragma unroll
+          for (int c = 0; c < kMaxCtas; ++c)
+            if (c < ctas) sum[j] += ld_cluster_u64(zb_mapa(zb_smem_u32(&sh.sums[top_bin - j]), c));
+          mine += sum[j];
+        }
+      }
+      const u64 upto = warp_upto(mine, lane);
+      if (lane == 31) sh.part[warp] = upto;
+      if (threadIdx.x == 0) sh.found[0] = 0, sh.left = need;      // (of a sum that does not reach it)
+      __syncthreads();
+      before = upto - mine, mine = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += sh.part[w];
+        mine += sh.part[w];
+      }
+      if (threadIdx.x < ctas) st_cluster_u64(zb_mapa(zb_smem_u32(&sh.total[rank]), threadIdx.x), mine);
+      cluster_sync();
+      for (int c = 0; c < rank; ++c) before += sh.total[c];
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        if (before < need && before + sum[j] >= need)
+          for (int c = 0; c < ctas; ++c) {
+            st_cluster_u32(zb_mapa(zb_smem_u32(&sh.found[0]), c), static_cast<uint32_t>(top_bin - j));
+            st_cluster_u64(zb_mapa(zb_smem_u32(&sh.left), c), need - before);
+          }
+        before += sum[j];
+      }
+      cluster_sync();
+      lo += sh.found[0] << shift;
+      hi = min(hi, lo + ((1u << shift) - 1u));
+      need = sh.left;
+    }
+    *rest = need;
+    return lo;
+  }
+  // The key above which `need` (of counts: sh.left of the logits in the bins) is not reached; *rest: what is needed there.  The logits of the bins [last, first]
+  // that are above floor_key go into the CTAs' lists, the weights of those above the bins into sh.above.
+  ZB_DEVICE uint32_t cut_in(bool weights, int first, int last, uint32_t floor_key, u64 need, u64* rest) {
+    const uint32_t from_key = max(key_of_bin(last), floor_key + 1);
+    const float x_from = value_of(from_key), x_above = first + 1 < kBins ? value_of(max(key_of_bin(first + 1), from_key)) : INFINITY;
+    const u64 left = sh.left;
+    if (threadIdx.x == 0) sh.n = 0, sh.range[0] = ~0u, sh.range[1] = 0;
+    __syncthreads();
+    uint32_t smallest = ~0u, largest = 0, counted = 0;
+    u64 above = 0;
+    each([&](const float (&e)[4], int index, int step) {
+      bool in[4], some = false, over = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        in[j] = e[j] >= x_from && e[j] < x_above;
+        some |= in[j];
+        over |= e[j] >= x_above;
+      }
+      if (__any_sync(0xffffffffu, over)) {           // (lanes that take no part would not be faster)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) above += biased(e[j] >= x_above ? e[j] : -INFINITY);
+        counted += 4;
+      }
+      if (!__any_sync(0xffffffffu, some)) return;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (in[j]) smallest = min(smallest, key_of(e[j])), largest = max(largest, key_of(e[j]));
+      append(in, e, index, step);
     });
     smallest = __reduce_min_sync(0xffffffffu, smallest);
     largest = __reduce_max_sync(0xffffffffu, largest);
@@ -549,74 +667,50 @@ struct Sampler {
       st_cluster_u32(zb_mapa(zb_smem_u32(&sh.least[rank]), threadIdx.x), sh.range[0]);
       st_cluster_u32(zb_mapa(zb_smem_u32(&sh.bound[rank]), threadIdx.x), sh.range[1]);
     }
-    const int n = exchange_counts();
-    u64 n_all = 0;
-    above = 0;
-    for (int c = 0; c < ctas; ++c) smallest = min(smallest, sh.least[c]), largest = max(largest, sh.bound[c]), above += sh.total[c], n_all += sh.count[c];
-    const u64 here = WEIGHTS ? (above < need ? need - above : 0) : sh.left;      // what is needed of these logits
-    if (here > 0 && smallest == largest && n_all * (WEIGHTS ? weight(value_of(smallest)) : 1) >= here) {
-      *rest = here;
-      listed = WEIGHTS && n <= kList;
-      cluster_sync();
-      return smallest;
+    exchange_counts();
+    above = 0, listed = true;
+    for (int c = 0; c < ctas; ++c) {
+      smallest = min(smallest, sh.least[c]), largest = max(largest, sh.bound[c]), above += sh.total[c];
+      listed = listed && sh.count[c] <= kList;
     }
-    if (here > 0 && n <= kList) {
-      sort_lists(n);
-      if (rank == 0) {
-        const int i = kMine * threadIdx.x;
-        u64 w[kMine], all;
-#pragma unroll
-        for (int j = 0; j < kMine; ++j) w[j] = i + j < n ? (WEIGHTS ? weight(value_of(key_at(sh.list.sorted[i + j]))) : 1) : 0;
-        u64 before = list_before(w, &all);
-        // the first whose sum reaches it; what its equals in front of it have is part of `rest`
-        int at = -1;
-        u64 left = 0;
-#pragma unroll
-        for (int j = 0; j < kMine; ++j) {
-          if (i + j < n && before < here && before + w[j] >= here) at = i + j, left = here - before;
-          before += w[j];
-        }
-        uint32_t key = 0;
-        if (at >= 0) {
-          key = key_at(sh.list.sorted[at]);
-          const u64 one = WEIGHTS ? weight(value_of(key)) : 1;
-          for (int j = at - 1; j >= 0 && key_at(sh.list.sorted[j]) == key; --j) left += one;
-        }
-        if (at >= 0 || (all < here && threadIdx.x == 0))      // (0: the sum is reached below these logits)
-          for (int c = 0; c < ctas; ++c) {
-            st_cluster_u64(zb_mapa(zb_smem_u32(&sh.left), c), left);
-            st_cluster_u32(zb_mapa(zb_smem_u32(&sh.found[0]), c), key);
-          }
-      }
-      cluster_sync();
-      const uint32_t key = sh.found[0];
-      *rest = sh.left;
-      listed = WEIGHTS && key != 0;
-      if (key != 0) {
-        cluster_sync();
-        return key;
-      }
-    }
-    // ---- bit by bit, from the highest one: whether what has it set is enough.  (A logit of 16 bits has no others.)
-    uint32_t prefix = 0;
-    for (int bit = 31; bit >= (sizeof(T) == 2 && kind != 2 ? 16 : 0); --bit) {
-      const uint32_t mask = ~((1u << bit) - 1u), want = prefix | 1u << bit;
-      u64 sum = 0;
+    need = weights ? need - above : left;
+    const int n = static_cast<int>(sh.n);
+    if (listed)
+      return narrow(weights, smallest, largest, need, rest, [&](auto&& f) {
+        for (int i = threadIdx.x; i < n; i += kThreads) f(value_of(key_at(sh.cand[i])));
+      });
+    return narrow(weights, smallest, largest, need, rest, [&](auto&& f) {
       each([&](const float (&e)[4], int, int) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (counts(e[j]) && (key_of(e[j]) & mask) == want) sum += WEIGHTS ? weight(e[j]) : 1;
+          if (e[j] == e[j]) f(e[j]);
       });
-      cluster_sync();
-      sum = sum_all(sum);
-      if (sum >= need) prefix = want;
-      else need -= sum;
+    });
+  }
+  // The weights of the warp's part above a cut.
+  ZB_DEVICE u64 sum_above(uint32_t cut) const {
+    const float cut_x = value_of(cut);
+    u64 sum = 0;
+    uint32_t counted = 0;
+    each([&](const float (&e)[4], int, int) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum += biased(e[j] > cut_x ? e[j] : -INFINITY);
+      counted += 4;
+    });
+    return warp_sum(sum - counted * kBias);
+  }
+  // Where the cut is among the lists: the weights of the warp's part above it, and how many equal it.
+  ZB_DEVICE void sum_lists(uint32_t cut, u64* mass, uint32_t* ties) const {
+    u64 m = 0;
+    uint32_t t = 0;
+    for (int i = lane; i < static_cast<int>(sh.n); i += 32) {
+      const u64 c = sh.cand[i];
+      if (index_at(c) < from || index_at(c) >= end) continue;
+      if (key_at(c) > cut) m += weight(value_of(key_at(c)));
+      t += key_at(c) == cut ? 1 : 0;
     }
-    cluster_sync();
-    // (of negative numbers in 16 bits, the complement's low bits are ones)
-    if (sizeof(T) == 2 && kind != 2 && (prefix & 0x80000000u) == 0) prefix |= 0xffffu;
-    *rest = need;
-    return prefix;
+    *mass = warp_sum(m) + sh.above[warp];
+    *ties = __reduce_add_sync(0xffffffffu, t);
   }
 
   ZB_DEVICE void run(int row) {
@@ -682,7 +776,7 @@ struct Sampler {
     // Within bounds that change nothing: the next number below the largest has a weight of zero at 900 already, and at 1e37 all finite ones are alike.
     top64 = top;
     const double next = best > 0x00800000u ? top64 - static_cast<double>(value_of(best - 1)) : 1.0;
-    scale = t > 0.0 ? fmin(1.4426950408889634 / fmin(t, 1e37), 900.0 / next) : 1.0;
+    scale = fmin(t > 0.0 ? 1.4426950408889634 / fmin(t, 1e37) : 1.0, 900.0 / next);
     floor_x = __double2float_rd(fmax(top64 - 47.0 / scale, -3.4e38));
 
     // the smallest logit whose weight, rounded to 2^-53, reaches min_p
@@ -703,53 +797,76 @@ struct Sampler {
       stay = 1;
     } else {
       if (small_k) {
-        const int n = gather(top_p < 1.0 ? bound : max(bound, least));      // (top_p is of the sum of all top_k)
+        const uint32_t from_key = top_p < 1.0 ? bound : max(bound, least);      // (top_p is of the sum of all top_k)
+        const int n = gather(from_key);
         if (n <= kList) {
-          sort_lists(n);
+          sort_lists(n, from_key);
           if (rank == 0) draw_from_list(row, min(n, top_k), top_p, 0, least);
           return;
         }
         cluster_sync();
       }
-      if (top_k < p.vocab) cut = search<false>(row_least, 0u, top_k, 0, &stay);
-      if (top_p < 1.0) {
-        const float cut_x = value_of(cut);
-        u64 sum = 0;
-        uint32_t counted = 0;
-        each([&](const float (&e)[4], int, int) {
-          if (cut == 0) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) sum += biased(e[j]);
-            counted += 4;
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (e[j] > cut_x) sum += biased(e[j]), ++counted;
+      const bool nucleus = top_p < 1.0;
+      if (top_k < p.vocab || nucleus) {
+        // Logits of no weight are never drawn.  For a nucleus alone: all logits of less than 2^z_from together are less than 1 - top_p of the sum (half of that, for
+        // what sums are rounded by), which is one or more.
+        const double z_from = top_k < p.vocab ? -46.0 : fmax(log2((1.0 - top_p) / (2.0 * p.vocab)) - 1e-6, -46.0);
+        const bool short_list = top_k == p.vocab;
+        u64 all = count_bins(z_from, row_least, nucleus, short_list);
+        int first, last;
+        bool done = !nucleus;
+        if (nucleus) {
+          __syncthreads();
+          if (threadIdx.x < ctas) st_cluster_u32(zb_mapa(zb_smem_u32(&sh.count[rank]), threadIdx.x), sh.n);
+          all = sum_all(all);
+          if (short_list) {
+            int have = 0;
+            for (int c = 0; c < ctas; ++c) have += static_cast<int>(min(sh.count[c], static_cast<uint32_t>(kList + 1)));
+            if (have <= kList) {
+              sort_lists(have, have > 256 ? key_of_bin(0) : 0u);
+              if (rank == 0) draw_from_list(row, have, top_p, all, least);
+              return;
+            }
           }
-        });
-        const u64 above = sum_all(sum - counted * kBias), at_cut = cut > 0 ? weight(cut_x) : 0, all = above + (cut > 0 ? stay * at_cut : 0), need = need_of(top_p, all);
-        cluster_sync();
-        // All logits below this weight together are less than 1 - top_p of the sum (half of that, for what sums are rounded by).
-        const double z = log2(static_cast<double>(all) / kOne * (1.0 - top_p) / (2.0 * p.vocab)) - 1e-6;
-        const uint32_t enough = max(key_of(__double2float_rd(fmax(top64 + z / scale, -3.4e38))), row_least);
-        // (a nucleus has at least need / 2^44 logits)
-        if (enough > cut && (need >> 44) < kList) {
-          const int n = gather(max(enough, least));
-          if (n <= kList) {
-            sort_lists(n);
-            if (rank == 0) draw_from_list(row, n, top_p, all, least);
+        }
+        if (top_k < p.vocab) {
+          const uint32_t n = bracket(false, top_k, &first, &last);
+          if (n > 0 && n <= kList) {
+            const uint32_t from_key = nucleus ? key_of_bin(last) : max(key_of_bin(last), least);
+            const int have = gather(from_key);
+            sort_lists(have, from_key);
+            if (rank == 0) draw_from_list(row, min(have, top_k), top_p, 0, least);
             return;
           }
-          cluster_sync();
+          if (n > 0) cut = cut_in(false, first, last, 0u, 0, &stay);
+          if (n > 0 && nucleus) {
+            const u64 at_cut = weight(value_of(cut));
+            u64 above;
+            uint32_t ties;
+            if (listed) sum_lists(cut, &above, &ties);
+            else above = sum_above(cut);
+            cluster_sync();
+            above = sum_all(lane == 0 ? above : 0);
+            all = above + stay * at_cut;
+            const u64 need = need_of(top_p, all);
+            if (above < need) stay = (need - above + at_cut - 1) / at_cut, done = true;
+            cluster_sync();
+          }
         }
-        if (above >= need) {
+        if (!done) {
+          const u64 need = need_of(top_p, all);
+          const uint32_t n = bracket(true, need, &first, &last);
+          if (n <= kList) {
+            const uint32_t from_key = max(max(key_of_bin(last), cut + 1), least);
+            const int have = gather(from_key);
+            sort_lists(have, from_key);
+            if (rank == 0) draw_from_list(row, have, top_p, all, least);
+            return;
+          }
           u64 rest;
-          const uint32_t old = cut;
-          cut = search<true>(enough, old, need, all, &rest);
+          cut = cut_in(true, first, last, cut, need, &rest);
           const u64 w = weight(value_of(cut));
           stay = (rest + w - 1) / w;
-        } else {
-          stay = (need - above + at_cut - 1) / at_cut;
         }
       }
       if (least > cut) {
@@ -771,30 +888,20 @@ struct Sampler {
 #pragma unroll
           for (int j = 0; j < 4; ++j) mass += biased(e[j]);
           counted += 4;
-        } else if (fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) >= cut_x) {
+        } else if (__any_sync(0xffffffffu, fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) >= cut_x)) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            if (e[j] > cut_x) mass += biased(e[j]), ++counted;
+            mass += biased(e[j] > cut_x ? e[j] : -INFINITY);
             ties += e[j] == cut_x ? 1 : 0;
           }
+          counted += 4;
         }
       });
       mass = warp_sum(mass - counted * kBias);
       ties = __reduce_add_sync(0xffffffffu, ties);
     };
-    if (listed) {
-      mass = 0, ties = 0;
-      for (int i = lane; i < static_cast<int>(sh.n); i += 32) {
-        const u64 c = sh.list.cand[i];
-        if (index_at(c) < from || index_at(c) >= end) continue;
-        if (key_at(c) > cut) mass += weight(value_of(key_at(c)));
-        ties += key_at(c) == cut ? 1 : 0;
-      }
-      mass = warp_sum(mass) + sh.above[warp];
-      ties = __reduce_add_sync(0xffffffffu, ties);
-    } else {
-      sum_part();
-    }
+    if (listed) sum_lists(cut, &mass, &ties);
+    else sum_part();
     if (lane == 0) sh.seg[warp] = mass, sh.seg_ties[warp] = ties;
     __syncthreads();
     if (threadIdx.x < ctas) {
