@@ -2,17 +2,21 @@
 // users' questions), bf16, head_dim 64, 128 and 256.
 //
 // A group of sequences has the same pages in front.  For the keys there, the queries of ALL members and of all heads of a key head are rows of one
-// matrix product, and the keys are read once; for the keys behind, the rows are the heads of one sequence.  Either is a list of items - (128 rows, key head, a range
-// of keys) - and one kernel walks all of them on the tensor cores (tcgen05, S and O in tensor memory, P as its A operand):
-//   S = Q K^T,  m = max S,  P = 2^(S - m),  l = sum P,  O = P V   of every item's range, and
+// matrix product, and the keys are read once; for the keys behind, the rows are the heads of one sequence.  Either way
+//   S = Q K^T,  m = max S,  P = 2^(S - m),  l = sum P,  O = P V   of a range of keys, and
 //   o = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i,  M = max m_i   over the ranges i that a row was in (zb_shared_merge_kernel).
-// What bounds it: the keys' bytes.  A tile of 64 keys of head_dim 128 is 32 KB, 1400 clocks of an SM's share of the memory rate; its products on 128
-// rows are 512 clocks whether the rows are in use or not, so that items of four rows need no other kernel.  The line of all items' tiles is cut into
-// equal pieces, one for each CTA (two on an SM up to head_dim 128: the hand-overs S -> softmax -> P of one hide under the other's), whatever the
-// lengths are; they are read from the device, so that a captured launch serves any lengths and groups.
-//   warps 0-3 : softmax and epilogue, one thread a row; they also bring in the rows' queries
-//   warp 4    : TMA producer, K and V tiles through rings that do not stop at the end of an item
-//   warp 5    : one thread issues the MMAs
+// Groups' keys: items of (128 rows, key head), tiles of 64 keys on the tensor cores (tcgen05, S and O in tensor memory, P as its A operand).
+// Sequences' own keys: items of (sequence, key head), steps of 16 keys by single warps ("walkers") with mma.sync, S^T = K Q^T and O^T = V^T P^T, where up to 8 or 16 heads are
+// the columns: 128 rows for four heads took 0.5 us a tile of an SM, and 128 sequences of their own keys twice as long.  (More than 16 heads to a key head: tiles, too.)
+// What bounds it: the keys' bytes, and of a long prefix that is shared by more than 128 rows the tiles' chain S -> softmax -> P -> O on two CTAs of an SM (tensor cores and
+// exponentials a third of the time each).  Either list of items is a line of units that is cut into equal pieces, one for each CTA (two on an SM up to head_dim 128: the
+// hand-overs of one hide under the other's) or walker, whatever the lengths are; they are read from the device, so that a captured launch serves any lengths and groups.
+//   CTAs of the groups' line     warps 0-3 : softmax and epilogue, one thread a row; they also bring in the rows' queries
+//                                warp 4    : TMA producer, K and V tiles through rings that do not stop at the end of an item
+//                                warp 5    : one thread issues the MMAs
+//   CTAs of the sequences' line  warps 0-5 : walkers, each with a ring of its own that it fills itself
+// Measured (of the bytes' floor): 8 sequences behind 2000 keys, 32 / 8 heads of 128, 18.7 us (latency: launch, plan, two kernels); 32 behind 8192, heads of 64, 27 (5.2);
+// 128 behind 4133 with 782 own keys on average, 32 / 4 heads, 71 (33); 64 behind 65536, 32 / 8 heads, 109 (47).
 // Every wait is bounded; a wait that runs out records a status and the CTA leaves through its normal exit.
 #include <cuda.h>
 
@@ -30,8 +34,12 @@ constexpr uint32_t kKernelId = 42;
 constexpr float kLazy = 8.f;                         // a row's reference moves when its maximum has grown by 2^kLazy
 constexpr int kMaxBatch = 1024;
 constexpr int kStep = 16, kWalkers = 6;
-constexpr int kSwitch = 1, kLeast = 2;
-constexpr uint32_t kTileCost = 7;                    // what a tile of a group's keys takes of a CTA's time, in steps of a sequence's own
+// What counts of a CTA's time.  A tile of a group's keys takes 1.7 - 2.8 us and the six walkers' step 1.05 - 1.7 us; an item's end and the next one's
+// beginning (its rows' parts written, other queries, an empty pipe) several of either.  With 7 and 1 instead, the CTAs that crossed items and those of the groups came in last:
+// 83 and 130 us where it is 71 and 109 (128 sequences behind 4133 keys, 64 behind 65536).
+constexpr uint32_t kTileCost = 11;                   // of a tile of a group's keys, in steps of sequences' own
+constexpr int kSwitch = 6;                           // of a change of items, in tiles or steps
+constexpr int kLeast = 3;                            // tiles of a piece, so that few pieces are none but a change
 
 struct SharedParams {
   const __nv_bfloat16* q;        // [batch, hq, HD], rows q_stride apart
