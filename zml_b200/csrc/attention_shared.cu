@@ -40,6 +40,7 @@ constexpr int kStep = 16, kWalkers = 6;
 constexpr uint32_t kTileCost = 11;                   // of a tile of a group's keys, in steps of sequences' own
 constexpr int kSwitch = 6;                           // of a change of items, in tiles or steps
 constexpr int kLeast = 3;                            // tiles of a piece, so that few pieces are none but a change
+constexpr int kLeastSteps = 8;                       // steps of a piece: three sequences of 8700 own keys in 400 parts each were merged for 40 us
 
 struct SharedParams {
   const __nv_bfloat16* q;        // [batch, hq, HD], rows q_stride apart
@@ -126,7 +127,7 @@ ZB_DEVICE Lines make_lines(int ctas, int of_groups, int of_sequences) {
   all = a + (all >> shift);
   l.of_groups = of_groups == 0 ? 0 : of_sequences == 0 ? ctas : min(max(static_cast<int>(ctas * (a >> 4) / max(all >> 4, 1u)), 1), ctas - 1);
   l.groups.cut(of_groups, min(l.of_groups, (of_groups + kLeast - 1) / kLeast));
-  l.sequences.cut(of_sequences, (ctas - l.of_groups) * (SPLIT ? kWalkers : 1));
+  l.sequences.cut(of_sequences, min((ctas - l.of_groups) * (SPLIT ? kWalkers : 1), SPLIT ? (of_sequences + kLeastSteps - 1) / kLeastSteps : of_sequences));
   return l;
 }
 
@@ -177,6 +178,8 @@ ZB_DEVICE void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+ZB_DEVICE void copy16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+ZB_DEVICE void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 ZB_DEVICE uint32_t transpose8(uint32_t x) {          // of 8 x 8 numbers of 16 bits over the warp
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -678,13 +681,18 @@ zb_shared_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     };
     const uint32_t inverse = (65536u + p.group - 1) / p.group;      // row / group of up to 128 rows is row * inverse >> 16
     const auto sequence_of = [&](const Segment& g, const Item& i, int nth) { return i.common ? plan.rows[i.first + nth] : g.entry - p.groups; };
-    const auto load_piece = [&](const Segment& g, const Item& i, int n) {
+    const auto piece_at = [&](const Segment& g, const Item& i, int n) {
       const int row = n / kPieces, nth = row * inverse >> 16, seq = max(sequence_of(g, i, nth), 0);
-      return *reinterpret_cast<const uint4*>(p.q + seq * p.q_stride + (g.head * p.group + row - nth * p.group) * HD + n % kPieces * 8);
+      return reinterpret_cast<const uint4*>(p.q + seq * p.q_stride + (g.head * p.group + row - nth * p.group) * HD + n % kPieces * 8);
     };
-    const auto store_piece = [&](int n, const uint4& x) {
+    const auto room_of = [&](int n) {
       const int row = n / kPieces, piece = n % kPieces;
-      *reinterpret_cast<uint4*>(q_s + (piece >> 3) * (kRows * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) = x;
+      return q_s + (piece >> 3) * (kRows * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
+    };
+    const auto copy_queries = [&](const Segment& g, const Item& i) {      // all on their way together
+#pragma unroll 4
+      for (int n = threadIdx.x; n < i.rows * kPieces; n += kRows) copy16(zb_smem_u32(room_of(n)), piece_at(g, i, n));
+      copies_done();
     };
     const auto publish_queries = [&]() {
       zb_fence_proxy_async_smem();
@@ -696,8 +704,7 @@ zb_shared_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     Item item;
     if (more) {
       item = item_of(seg);
-#pragma unroll 8
-      for (int n = threadIdx.x; n < item.rows * kPieces; n += kRows) store_piece(n, load_piece(seg, item, n));
+      copy_queries(seg, item);
       publish_queries();
     }
     float* owed = nullptr;                           // where the item before goes, once its O is complete
@@ -736,7 +743,7 @@ zb_shared_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         if (pieces <= kAhead * kRows) {
 #pragma unroll
           for (int i = 0; i < kAhead; ++i)
-            if (threadIdx.x + i * kRows < pieces) piece[i] = load_piece(next, after, threadIdx.x + i * kRows);
+            if (threadIdx.x + i * kRows < pieces) piece[i] = *piece_at(next, after, threadIdx.x + i * kRows);
         }
       }
       const int end = item.end, lo = item.lo;
@@ -761,10 +768,9 @@ zb_shared_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
           if (pieces <= kAhead * kRows) {
 #pragma unroll
             for (int i = 0; i < kAhead; ++i)
-              if (threadIdx.x + i * kRows < pieces) store_piece(threadIdx.x + i * kRows, piece[i]);
+              if (threadIdx.x + i * kRows < pieces) *reinterpret_cast<uint4*>(room_of(threadIdx.x + i * kRows)) = piece[i];
           } else {
-#pragma unroll 8
-            for (int n = threadIdx.x; n < pieces; n += kRows) store_piece(n, load_piece(next, after, n));
+            copy_queries(next, after);
           }
           publish_queries();
         }
@@ -897,8 +903,9 @@ zb_shared_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 }
 
 // The rows of one (sequence, key head), over all parts that the kernel above left of them.  where[seq] = {blocks of the prefix, first unit of them (of key head
-// 0), row of its parts in units of `group` (likewise), step of these to the next key head; blocks of its own, first unit of them, units of both lines}.  Of the
-// CTA's 16 warps, `warps` share a row's parts: what bounds the kernel is the chain of loads, not their number (8 sequences of 34 parts, a warp a row: 9 us).
+// 0), row of its parts in units of `group` (likewise), step of these to the next key head; blocks of its own, first unit of them, units of both lines}.  A warp
+// works on a row, or 2, 4, .. 16 on one: what bounds the kernel is the chain of loads, not their number (8 sequences of
+// 34 parts, a warp a row: 9 us; four: 18.8 us for the whole call, 16: 17.7).
 template <int HD, bool SPLIT>
 __global__ void __launch_bounds__(512)
 zb_shared_merge_kernel(const int32_t* __restrict__ where, const float* __restrict__ part_o, const float2* __restrict__ part_ml,
@@ -923,74 +930,71 @@ zb_shared_merge_kernel(const int32_t* __restrict__ where, const float* __restric
     n1 = lines.sequences.owner_of(u + back.x - 1) - c1 + 1;
   }
   const int n = n0 + n1, warps = 1 << log2_warps, share = warp & (warps - 1);
-  for (int r0 = 0; r0 < group; r0 += 16 >> log2_warps) {
-    const int r = r0 + (warp >> log2_warps);
-    float acc[kEach], top = -INFINITY, sum = 0.f;
+  const int r = blockIdx.z * (16 >> log2_warps) + (warp >> log2_warps);
+  float acc[kEach], top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) acc[j] = 0.f;
-    if (r < group) {
-      const long long row0 = (static_cast<long long>(front.z) + static_cast<long long>(head) * front.w) * group + static_cast<long long>(c0) * kRows + r;
-      const long long row1 = own_row + (static_cast<long long>(b) * hkv + head + c1) * group + r;
-      const auto place = [&](int i) {                // (a sequence that is in two groups finds a wrong row, but one that is there)
-        const long long at = i < n0 ? row0 + static_cast<long long>(i) * kRows : row1 + static_cast<long long>(i - n0) * group;
-        return at < part_rows ? at : 0ll;
-      };
-      const int mine = (n - share + warps - 1) >> log2_warps;      // parts share, share + warps, ..
-      for (int i0 = 0; i0 < mine; i0 += kOnce) {
-        float x[kOnce][kEach];
-        float2 ml = make_float2(-INFINITY, 0.f);
-        if (lane < kOnce && i0 + lane < mine) ml = part_ml[place(share + ((i0 + lane) << log2_warps))];
+  for (int j = 0; j < kEach; ++j) acc[j] = 0.f;
+  if (r < group) {
+    const long long row0 = (static_cast<long long>(front.z) + static_cast<long long>(head) * front.w) * group + static_cast<long long>(c0) * kRows + r;
+    const long long row1 = own_row + (static_cast<long long>(b) * hkv + head + c1) * group + r;
+    const auto place = [&](int i) {                // (a sequence that is in two groups finds a wrong row, but one that is there)
+      const long long at = i < n0 ? row0 + static_cast<long long>(i) * kRows : row1 + static_cast<long long>(i - n0) * group;
+      return at < part_rows ? at : 0ll;
+    };
+    const int mine = (n - share + warps - 1) >> log2_warps;      // parts share, share + warps, ..
+    for (int i0 = 0; i0 < mine; i0 += kOnce) {
+      float x[kOnce][kEach];
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (lane < kOnce && i0 + lane < mine) ml = part_ml[place(share + ((i0 + lane) << log2_warps))];
 #pragma unroll
-        for (int i = 0; i < kOnce; ++i) {
-          const float2* src = reinterpret_cast<const float2*>(part_o + place(share + (min(i0 + i, mine - 1) << log2_warps)) * HD + lane * kEach);
+      for (int i = 0; i < kOnce; ++i) {
+        const float2* src = reinterpret_cast<const float2*>(part_o + place(share + (min(i0 + i, mine - 1) << log2_warps)) * HD + lane * kEach);
 #pragma unroll
-          for (int j = 0; j < kEach / 2; ++j) {
-            const float2 y = src[j];
-            x[i][2 * j] = y.x, x[i][2 * j + 1] = y.y;
-          }
-        }
-        const float up = fmaxf(top, zb_warp_max(ml.x)), base = up == -INFINITY ? 0.f : up;
-        const float was = zb_ex2(top - base), f = zb_ex2(ml.x - base);
-        top = up;
-        sum = sum * was + zb_warp_sum(f * ml.y);
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) acc[j] *= was;
-#pragma unroll
-        for (int i = 0; i < kOnce; ++i) {
-          if (i0 + i >= mine) break;
-          const float by = __shfl_sync(0xffffffffu, f, i);
-#pragma unroll
-          for (int j = 0; j < kEach; ++j) acc[j] += by * x[i][j];
+        for (int j = 0; j < kEach / 2; ++j) {
+          const float2 y = src[j];
+          x[i][2 * j] = y.x, x[i][2 * j + 1] = y.y;
         }
       }
-    }
-    if (warps > 1) {
+      const float up = fmaxf(top, zb_warp_max(ml.x)), base = up == -INFINITY ? 0.f : up;
+      const float was = zb_ex2(top - base), f = zb_ex2(ml.x - base);
+      top = up;
+      sum = sum * was + zb_warp_sum(f * ml.y);
 #pragma unroll
-      for (int j = 0; j < kEach; ++j) sums[warp][lane * kEach + j] = acc[j];
-      if (lane == 0) stats[warp] = make_float2(top, sum);
-      __syncthreads();
-      if (share == 0 && r < group) {
-        float most = top;
-        for (int w = 1; w < warps; ++w) most = fmaxf(most, stats[warp + w].x);
-        const float base = most == -INFINITY ? 0.f : most, f = zb_ex2(top - base);
-        sum *= f;
+      for (int j = 0; j < kEach; ++j) acc[j] *= was;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) acc[j] *= f;
-        for (int w = 1; w < warps; ++w) {
-          const float g = zb_ex2(stats[warp + w].x - base);
-          sum += g * stats[warp + w].y;
+      for (int i = 0; i < kOnce; ++i) {
+        if (i0 + i >= mine) break;
+        const float by = __shfl_sync(0xffffffffu, f, i);
 #pragma unroll
-          for (int j = 0; j < kEach; ++j) acc[j] += g * sums[warp + w][lane * kEach + j];
-        }
+        for (int j = 0; j < kEach; ++j) acc[j] += by * x[i][j];
       }
     }
+  }
+  if (warps > 1) {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) sums[warp][lane * kEach + j] = acc[j];
+    if (lane == 0) stats[warp] = make_float2(top, sum);
+    __syncthreads();
     if (share == 0 && r < group) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;      // no key at all: zeros
-      __nv_bfloat16* dst = out + (static_cast<size_t>(b) * hkv * group + head * group + r) * HD + lane * kEach;
+      float most = top;
+      for (int w = 1; w < warps; ++w) most = fmaxf(most, stats[warp + w].x);
+      const float base = most == -INFINITY ? 0.f : most, f = zb_ex2(top - base);
+      sum *= f;
 #pragma unroll
-      for (int j = 0; j < kEach; j += 2) *reinterpret_cast<uint32_t*>(dst + j) = zb_pack_bf16x2(acc[j] * inv, acc[j + 1] * inv);
+      for (int j = 0; j < kEach; ++j) acc[j] *= f;
+      for (int w = 1; w < warps; ++w) {
+        const float g = zb_ex2(stats[warp + w].x - base);
+        sum += g * stats[warp + w].y;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) acc[j] += g * sums[warp + w][lane * kEach + j];
+      }
     }
-    if (warps > 1) __syncthreads();
+  }
+  if (share == 0 && r < group) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;      // no key at all: zeros
+    __nv_bfloat16* dst = out + (static_cast<size_t>(b) * hkv * group + head * group + r) * HD + lane * kEach;
+#pragma unroll
+    for (int j = 0; j < kEach; j += 2) *reinterpret_cast<uint32_t*>(dst + j) = zb_pack_bf16x2(acc[j] * inv, acc[j + 1] * inv);
   }
 }
 
@@ -1017,9 +1021,13 @@ int launch(const CUtensorMap (&maps)[4], const SharedParams& p, void* out, int r
   static bool configured[16] = {};
   if (const int rc = zb_config_smem_once(zb_shared_decode_kernel<HD, NB>, Shape<HD>::kSmem + plan_bytes(kMaxBatch, kMaxBatch), configured)) return rc;
   cudaError_t e = zb_launch(zb_shared_decode_kernel<HD, NB>, dim3(ctas), dim3(kThreads), Shape<HD>::kSmem + plan_bytes(p.batch, p.groups), s, maps[0], maps[1], maps[2], maps[3], p);
+  // as many warps a row as a CTA for a head's rows has; more where there are few rows
+  int log2_warps = p.group > 8 ? 0 : p.group > 4 ? 1 : p.group > 2 ? 2 : p.group == 2 ? 3 : 4;
+  const auto merge_ctas = [&](int log2) { return static_cast<long long>(p.batch) * p.hkv * ((p.group + (16 >> log2) - 1) / (16 >> log2)); };
+  while (log2_warps < 4 && merge_ctas(log2_warps + 1) <= 2 * zb_num_sms()) ++log2_warps;
   if (e == cudaSuccess)
-    e = zb_launch(zb_shared_merge_kernel<HD, (NB > 0)>, dim3(p.batch, p.hkv), dim3(512), 0, s, p.where, p.part_o, p.part_ml, reinterpret_cast<__nv_bfloat16*>(out),
-                  p.hkv, p.group, p.group > 8 ? 0 : p.group > 4 ? 1 : p.group > 2 ? 2 : p.group == 2 ? 3 : 4, p.own_row, rows, ctas);
+    e = zb_launch(zb_shared_merge_kernel<HD, (NB > 0)>, dim3(p.batch, p.hkv, (p.group + (16 >> log2_warps) - 1) / (16 >> log2_warps)), dim3(512), 0, s, p.where, p.part_o,
+                  p.part_ml, reinterpret_cast<__nv_bfloat16*>(out), p.hkv, p.group, log2_warps, p.own_row, rows, ctas);
   zb_count_launch(2);
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
