@@ -274,7 +274,7 @@ def long_cuts(device, dtype=torch.float32):
     few = torch.tensor([0.0, 1e-3, 2e-3, -4.0])[torch.randint(0, 4, (vocab,), generator=g)]
     rows = torch.stack([spread(1, vocab, 2.5, 1)[0][0], spread(1, vocab, 0.4, 2)[0][0], alike, few, torch.zeros(vocab), spread(1, vocab, 2.0, 3, masked=0.7)[0][0]])
     u = torch.rand(len(rows), generator=g, dtype=torch.float64)
-    for k in (0, 601, 2048, 2049, 9000, vocab - 1):
+    for k in (0, 601, 1024, 1025, 2048, 2049, 9000, vocab - 1):
         for p in (1.0, 0.9, 0.4):
             check(rows, u, {"top_k": k, "top_p": p}, device, dtype)
     check(rows, u, {"top_k": 5000, "top_p": 0.97, "min_p": 0.02, "temperature": 1.3}, device, dtype)

@@ -18,7 +18,7 @@
 // histogram over the logits after that pass, with the weights of each bin's middle, and a list tried beforehand: 256 rows with flat logits 322 us, now 257).
 // What bounds it: the logits' bytes for many rows, beside some 30 instructions of a weight where the whole row's sum is needed, some 40 with the histogram's; for few rows
 // the passes' and the cluster's barriers' latency.  Measured, with logits in L2 as a model leaves them: 1 row of 128256 with top_p 15 us, 32 rows with settings of their
-// own 39, 64 rows of 151936 without a cut 35, 128 rows of 248320 with top_k 50 and top_p 55 (127 MB: 2.3 TB/s), 256 rows of 151936 with a nucleus of 80 thousand 257.
+// own 36, 64 rows of 151936 without a cut 35, 128 rows of 248320 with top_k 50 and top_p 55 (127 MB: 2.3 TB/s), 256 rows of 151936 with a nucleus of 80 thousand 257.
 #include "common.cuh"
 #include "host_api.h"
 
@@ -27,7 +27,7 @@ namespace {
 constexpr int kMaxCtas = 8;
 constexpr int kMaxVocab = 8 * 49152;                 // (an index and a weight are one number of 19 + 45 bits)
 constexpr int kList = 2048;
-constexpr int kSmallK = 600;                        // a top_k up to this ends in a list, if all goes well
+constexpr int kSmallK = 1024;                       // a top_k up to this ends in a list, if all goes well (1.2 - 1.6 times as many logits; 32 rows of which some have 1000: 36 us, by cuts 39)
 constexpr int kBins = 2048;
 constexpr int kTable = 16;                           // 2^((j + 1/2) / 16): any 32 lanes' entries are on different banks (512 entries: 7 conflicts)
 constexpr double kOne = 17592186044416.0;            // 2^44
@@ -203,7 +203,7 @@ struct Sampler {
 
   // The k-th largest of at least k of the CTA's logits (at most 32 a warp): each warp's largest few of its lanes' largest.
   ZB_DEVICE void find_bound(uint32_t mine, int k) {
-    const int per_warp = min((k + kWarps - 1) / kWarps + 1, 32);
+    const int share = (k + kWarps - 1) / kWarps, per_warp = min(share + share / 2 + 1, 32);      // (half as many again, so that the k-th is not just the worst warp's last)
     for (int i = 0; i < per_warp; ++i) {
       const uint32_t m = __reduce_max_sync(0xffffffffu, mine);
       const uint32_t who = __ballot_sync(0xffffffffu, mine == m);

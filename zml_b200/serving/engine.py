@@ -567,7 +567,7 @@ class Engine:
         next replay)."""
         if not self.use_graphs:
             return self._decode_body(b, strategy, num_splits, max_seq_len)
-        key = (b, strategy.topk, float(strategy.temperature), float(strategy.top_p), float(strategy.min_p), num_splits, self.share_prefixes and self._groups_used)
+        key = (b, strategy.topk, float(strategy.temperature), num_splits, float(strategy.top_p), float(strategy.min_p), self.share_prefixes and self._groups_used)
         g = self._graphs.get(key)
         if g is None:
             while len(self._graphs) >= self.max_graphs:          # sampling settings come from requests: bound the cache
