@@ -9,7 +9,7 @@
 // Sequences' own keys: items of (sequence, key head), steps of 16 keys by single warps ("walkers") with mma.sync, S^T = K Q^T and O^T = V^T P^T, where up to 8 or 16 heads are
 // the columns: 128 rows for four heads took 0.5 us a tile of an SM, and 128 sequences of their own keys twice as long.  (More than 16 heads to a key head: tiles, too.)
 // What bounds it: the keys' bytes, and of a long prefix that is shared by more than 128 rows the tiles' chain S -> softmax -> P -> O on two CTAs of an SM (tensor cores and
-// exponentials a third of the time each).  Either list of items is a line of units that is cut into equal pieces, one for each CTA (two on an SM up to head_dim 128: the
+// exponentials two fifths of the time each).  Either list of items is a line of units that is cut into equal pieces, one for each CTA (two on an SM up to head_dim 128: the
 // hand-overs of one hide under the other's) or walker, whatever the lengths are; they are read from the device, so that a captured launch serves any lengths and groups.
 //   CTAs of the groups' line     warps 0-3 : softmax and epilogue, one thread a row; they also bring in the rows' queries
 //                                warp 4    : TMA producer, K and V tiles through rings that do not stop at the end of an item

@@ -31,6 +31,7 @@ constexpr int kSmallK = 1024;                       // a top_k up to this ends i
 constexpr int kBins = 2048;
 constexpr int kTable = 16;                           // 2^((j + 1/2) / 16): any 32 lanes' entries are on different banks (512 entries: 7 conflicts)
 constexpr double kOne = 17592186044416.0;            // 2^44
+constexpr double kMiddle = 1.5 * 2048.0;             // a number of less than 1024, added to it, has its 2^-41 in the last place
 constexpr unsigned long long kBias = 0x4070000000000000ull;      // 256.0: a weight added to it has its 2^-44 in the last place
 
 struct SampleParams {
@@ -139,7 +140,7 @@ struct Sampler {
 
   // The weight of a logit that is not above `top`, in 2^-44, plus kBias; a NaN's is zero.  z is held with 41 bits behind the point: 4 of them choose the table's
   // entry, and with the other 37 as r, around their middle, 2^r is a polynomial (off by 5e-16).
-  ZB_DEVICE double log2_of(float x) const { return __fma_rn(static_cast<double>(fmaxf(x, floor_x)) - top64, scale, 3072.0); }      // 1.5 * 2^11
+  ZB_DEVICE double log2_of(float x) const { return __fma_rn(static_cast<double>(fmaxf(x, floor_x)) - top64, scale, kMiddle); }
   ZB_DEVICE u64 biased(float x) const { return power(log2_of(x)); }
   ZB_DEVICE u64 power(double t) const {
     const int hi = __double2hiint(t);
@@ -450,8 +451,8 @@ struct Sampler {
   // Counts of the logits with weights of 2^z_from or more, in up to 2048 bins of equal length on the weights' logarithm (the high word of log2_of: 2^-9 or
   // more; from the row's smallest logit on).  With `list` they are listed, too, until there are too many.  Returns the thread's sum of weights.
   ZB_DEVICE u64 count_bins(double z_from, uint32_t row_least, bool sums, bool list) {
-    bin_from = max(__double2hiint(log2_of(value_of(row_least))), __double2hiint(3072.0 + z_from));
-    bin_shift = max(0, 21 - __clz(__double2hiint(3072.0) - bin_from));
+    bin_from = max(__double2hiint(log2_of(value_of(row_least))), __double2hiint(kMiddle + z_from));
+    bin_shift = max(0, 21 - __clz(__double2hiint(kMiddle) - bin_from));
     for (int i = threadIdx.x; i < kBins; i += kThreads) sh.hist[i] = 0;
     if (threadIdx.x == 0) sh.n = list ? 0 : kList + 1;
     __syncthreads();
@@ -481,7 +482,7 @@ struct Sampler {
     return sums ? sum - counted * kBias : 0;
   }
   ZB_DEVICE u64 at_edge(int bin) const {              // the weight where a bin begins
-    return power(__hiloint2double(min(bin_from + (bin << bin_shift), __double2hiint(3072.0)), 0)) - kBias;
+    return power(__hiloint2double(min(bin_from + (bin << bin_shift), __double2hiint(kMiddle)), 0)) - kBias;
   }
   // The key of the smallest logit that is in a bin or above it: 5 bits of it at a time, a lane each.
   ZB_DEVICE uint32_t key_of_bin(int bin) const {
@@ -503,13 +504,12 @@ struct Sampler {
     cluster_sync();
     constexpr int kEach = (kBins + kThreads - 1) / kThreads;      // where a row has one CTA
     const int share = kBins >> (31 - __clz(ctas)), each_bins = (share + kThreads - 1) / kThreads, top_bin = kBins - 1 - rank * share - threadIdx.x * each_bins;
-    uint32_t n[kEach], counted = 0;
+    uint32_t n[kEach] = {}, counted = 0;
     u64 up = 0, low = 0;
     const auto most_of = [&](int j) { return weights ? n[j] * (at_edge(top_bin - j + 1) + 1) : n[j]; };
     const auto least_of = [&](int j) { return weights ? n[j] * (max(at_edge(top_bin - j), 1ull) - 1) : n[j]; };
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      n[j] = 0;
       if (j < each_bins && static_cast<int>(threadIdx.x) * each_bins + j < share) {
 #pragma unroll
         for (int c = 0; c < kMaxCtas; ++c)

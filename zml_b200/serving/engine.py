@@ -21,6 +21,7 @@ schedule (SPMD), so no control traffic is needed.
 from __future__ import annotations
 
 import contextlib
+import functools
 import time
 from array import array
 from dataclasses import dataclass, field
@@ -124,6 +125,27 @@ def _bucket(n: int) -> int:
     while b < n:
         b <<= 1
     return b
+
+
+def _pages_in_common(a: list, b: list) -> int:
+    """How many pages two prompts have in front.  A page is found behind one other page only, so where two lists agree they agree up to there."""
+    lo, hi = 0, min(len(a), len(b))
+    while lo < hi:
+        mid = (lo + hi + 1) // 2
+        if a[mid - 1] == b[mid - 1]:
+            lo = mid
+        else:
+            hi = mid - 1
+    return lo
+
+
+def _order_of_pages(x, y) -> int:
+    (a, _), (b, _) = x, y
+    n = _pages_in_common(a, b)
+    return a[n] - b[n] if n < min(len(a), len(b)) else len(a) - len(b)
+
+
+_BY_PAGES = functools.cmp_to_key(_order_of_pages)
 
 
 class Engine:
@@ -313,13 +335,14 @@ class Engine:
             if len(members) < 2:
                 continue
             # in the order of their pages, whoever shares most with a request is its neighbour
-            whole = sorted((r.pages[:(len(r.prompt) - 1) // ps], row) for row, r in members)
-            lcp = [next((i for i, (x, y) in enumerate(zip(a, b)) if x != y), min(len(a), len(b))) for (a, _), (b, _) in zip(whole, whole[1:])]
+            whole = sorted(((r.pages[:(len(r.prompt) - 1) // ps], row) for row, r in members), key=_BY_PAGES)
+            lcp = [_pages_in_common(a, b) for (a, _), (b, _) in zip(whole, whole[1:])]
             split = {}
             for (w, row), n in zip(whole, map(max, lcp + [0], [0] + lcp)):
-                split.setdefault(tuple(w[:n]), []).append(row)
+                if n:
+                    split.setdefault((n, w[n - 1]), []).append(row)      # (the page tells those in front of it)
             one = [([row for _, row in whole], min(lcp))]
-            many = [(rows_, len(k)) for k, rows_ in split.items() if len(rows_) > 1 and k]
+            many = [(rows_, n) for (n, _), rows_ in split.items() if len(rows_) > 1]
             groups += max(one, many, key=lambda g: sum((len(m) - 1) * n for m, n in g))
         saved = sum((len(m) - 1) * n for m, n in groups) * ps
         if saved * self._key_bytes() < self.SHARE_BYTES:
