@@ -306,3 +306,15 @@ def test_refusals_on_the_gpu():
         call({**s, "k": flat})
     empty = call({**s, "q": s["q"][:0], "table": s["table"][:0], "lens": s["lens"][:0], "shared": ops.SharedPrefix.of([], "cuda")})
     assert empty.shape == (0, 8, 64)
+
+
+@gpu
+def test_a_sequence_that_is_listed_twice_is_where_it_is_listed_last():
+    s = make([(256, [3, 40, 5, 0, 70, 9])], (70,), 8, 2, 64, 64, device="cuda")
+    a = s["shared"].rows.tolist()
+    for groups in ([(a[:5], 256), ([a[2], a[4]], 128)], [(a[:2], 64), (a[1:], 256)], [(a[:3] + a[:2], 256)], [([a[0]] * 7, 256)]):
+        check(call({**s, "shared": ops.SharedPrefix.of(groups, "cuda")}), s)
+    s["lens"][:] = 256                                # nothing of their own
+    got = call({**s, "shared": ops.SharedPrefix.of([(a[:4], 192), ([a[3], a[1]], 64)], "cuda")})
+    check(got[a], {**s, "q": s["q"][a], "table": s["table"][a], "lens": s["lens"][a]})
+    ops.raise_on_status()

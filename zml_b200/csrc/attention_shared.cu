@@ -210,9 +210,20 @@ ZB_DEVICE Lines make_plan(const SharedParams& p, Plan<SPLIT>& plan, longlong2* s
   }
   for (int g = tid; g < g_n; g += kThreads) plan.end[g] = clamp_keys(p.lens[g], p);
   __syncthreads();
+  // a sequence that is listed twice is where it is listed last: all CTAs have to see it in the same place
   for (int i = tid; i < p.listed; i += kThreads) {
-    const int g = plan.group_of(i), b = plan.rows[i];
-    if (g >= 0 && b >= 0) plan.begin[b] = plan.end[g];
+    const int b = plan.rows[i];
+    if (b >= 0 && plan.group_of(i) >= 0) atomicMax(&plan.begin[b], i + 1);
+  }
+  __syncthreads();
+  for (int i = tid; i < p.listed; i += kThreads) {
+    const int b = plan.rows[i];
+    if (b >= 0 && plan.begin[b] != i + 1) plan.rows[i] = -1;
+  }
+  __syncthreads();
+  for (int i = tid; i < p.listed; i += kThreads) {
+    const int b = plan.rows[i];
+    if (b >= 0) plan.begin[b] = plan.end[plan.group_of(i)];
   }
   __syncthreads();
   // sums up to every entry, of both lines: a run of entries a thread, then threads, then warps

@@ -28,7 +28,8 @@ class SharedPrefix:
     """Groups of sequences with the same pages in front, as int32 tensors on the cache's device, which may change between the calls (and the
     replays of a captured one):
 
-    `rows` [n]: the members' places in the batch, group after group, none of them twice; a sequence that is in no group is not listed.
+    `rows` [n]: the members' places in the batch, group after group, each once (of two places the last one counts); a sequence that is in no group is
+    not listed.
     `starts` [groups + 1]: group g has rows[starts[g]] .. rows[starts[g + 1] - 1]; groups may be empty.
     `lens` [groups]: keys that the members of a group share, any number.  The block table's pages that hold them are the same for all members, or
     hold the same (a page that the shared keys fill in part is each member's own).
