@@ -124,7 +124,7 @@ struct Sampler {
   Shared<kThreads>& sh;
   const T* x;                    // the row
   int ctas, rank, warp, lane, from, end;              // the warp's part of the row, whole rows of 128 but for the row's end
-  int kind;                      // 1: only infinities count, as 1; 2: logits are scaled by 2^-100
+  int kind;                      // 1: only infinities count, as 1; 2: logits are scaled by 2^-64
   float top, floor_x;            // the largest logit; below floor_x weights are zero
   double top64, scale;           // log2 of a weight is (x - top) * scale
   uint32_t best;
@@ -154,7 +154,7 @@ struct Sampler {
   ZB_DEVICE u64 weight(float x) const { return biased(x) - kBias; }
 
   ZB_DEVICE float fix(float v) const {               // what counts as a logit (a NaN fails every comparison and has no weight)
-    return kind == 0 ? v : kind == 1 ? (v == INFINITY ? 1.f : -INFINITY) : v * 0x1p-100f;
+    return kind == 0 ? v : kind == 1 ? (v == INFINITY ? 1.f : -INFINITY) : v * 0x1p-64f;
   }
   // f(four logits, index of the first, distance of their indices) over the warp's part, 128 logits at a time, -inf behind the row's end.
   template <typename F>
@@ -768,16 +768,21 @@ struct Sampler {
       best = row_least = key_of(1.f);
       bound = min(bound, best);
     }
-    if (kind == 0 && t > 1e37 && (top > 1e30f || value_of(row_least) < -1e30f)) {      // so that the scale below leaves them alike
+    // Logits, and the temperature with them, are scaled by 2^-64 where the floor below would be beyond fp32: a row whose largest is as far down as the type goes
+    // (its masks' value everywhere), or one that so high a temperature makes of a few logits.  (What denormals lose of logits below 1e-19 is nothing beside such numbers.)
+    double temp = t;
+    if (kind == 0 && (fabsf(top) > 1e18f || (t > 1e30 && value_of(row_least) < -1e18f))) {
       kind = 2;
-      top *= 0x1p-100f;
-      best = key_of(top), row_least = key_of(value_of(row_least) * 0x1p-100f), bound = key_of(value_of(bound) * 0x1p-100f);
+      temp *= 0x1p-64;
+      top *= 0x1p-64f;
+      best = key_of(top), row_least = key_of(value_of(row_least) * 0x1p-64f), bound = key_of(value_of(bound) * 0x1p-64f);
     }
-    // Within bounds that change nothing: the next number below the largest has a weight of zero at 900 already, and at 1e37 all finite ones are alike.
+    // Within bounds that change nothing: the next number below the largest has a weight of zero at 900 already, and logits that are not beyond 1e20 are alike at 1e36.
+    // So the floor is below the largest logit and above -1e38, and -inf is not above it.
     top64 = top;
     const double next = best > 0x00800000u ? top64 - static_cast<double>(value_of(best - 1)) : 1.0;
-    scale = fmin(t > 0.0 ? 1.4426950408889634 / fmin(t, 1e37) : 1.0, 900.0 / next);
-    floor_x = __double2float_rd(fmax(top64 - 47.0 / scale, -3.4e38));
+    scale = fmin(t > 0.0 ? 1.4426950408889634 / fmin(temp, 1e36) : 1.0, 900.0 / next);
+    floor_x = __double2float_rd(top64 - 47.0 / scale);
 
     // the smallest logit whose weight, rounded to 2^-53, reaches min_p
     uint32_t least = 0;
