@@ -50,3 +50,16 @@ def test_no_row_is_left_without_a_token():
         out = torch.full((9,), -7, dtype=torch.int32, device="cuda")
         ops.sample(x, torch.rand(9, device="cuda"), 0.8, out=out, **settings)
         assert bool(((out >= 0) & (out < 3000)).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_largest_logit_of_zero_at_the_smallest_temperatures(device):
+    rows = [[0.0, -1.0, -1e-3, -1e-45], [-1.0, -0.0, -1e-40, -math.inf], [-5.0, 0.0, 0.0, -1e-45], [1e-45, 0.0, -1.0, -1e-45], [-1e-45, -2e-45, -1.0, -1e-40]]
+    for t in (1e-44, 1e-46, 1e-48, 1e-60, 1e-100, 1e-300, 5e-324):
+        for settings in ({}, {"top_k": 3}, {"top_p": 0.9}, {"min_p": 1e-3}, {"top_k": 3, "top_p": 0.9}):
+            for u in UNIFORMS:
+                check(rows, [u] * len(rows), {**settings, "temperature": t}, device)
+    x = -torch.rand((2, 5000), generator=torch.Generator().manual_seed(1))
+    x[:, 4321] = 0.0
+    for settings in CUTS:
+        check(x, [0.1, 0.9], {**settings, "temperature": 1e-60}, device)

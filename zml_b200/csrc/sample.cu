@@ -780,7 +780,7 @@ struct Sampler {
     // Within bounds that change nothing: the next number below the largest has a weight of zero at 900 already, and logits that are not beyond 1e20 are alike at 1e36.
     // So the floor is below the largest logit and above -1e38, and -inf is not above it.
     top64 = top;
-    const double next = best > 0x00800000u ? top64 - static_cast<double>(value_of(best - 1)) : 1.0;
+    const double next = top64 - static_cast<double>(value_of(best - (best == 0x80000000u ? 2 : 1)));      // (the key below zero's is that of no number)
     scale = fmin(t > 0.0 ? 1.4426950408889634 / fmin(temp, 1e36) : 1.0, 900.0 / next);
     floor_x = __double2float_rd(top64 - 47.0 / scale);
 
