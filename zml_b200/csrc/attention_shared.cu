@@ -216,9 +216,13 @@ ZB_DEVICE Lines make_plan(const SharedParams& p, Plan<SPLIT>& plan, longlong2* s
     if (b >= 0 && plan.group_of(i) >= 0) atomicMax(&plan.begin[b], i + 1);
   }
   __syncthreads();
+  // What a group shares ends with its shortest member, so that every member has every key of a tile: a weight of zero would not make a NaN zero that only longer
+  // members see, or nobody.  A member that has ended takes no part, its pages may be anything.
   for (int i = tid; i < p.listed; i += kThreads) {
     const int b = plan.rows[i];
-    if (b >= 0 && plan.begin[b] != i + 1) plan.rows[i] = -1;
+    if (b < 0) continue;
+    if (plan.begin[b] != i + 1 || plan.end[g_n + b] == 0) plan.rows[i] = -1;
+    else atomicMin(&plan.end[plan.group_of(i)], plan.end[g_n + b]);
   }
   __syncthreads();
   for (int i = tid; i < p.listed; i += kThreads) {
@@ -759,11 +763,7 @@ zb_shared_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
       }
       const int end = item.end, lo = item.lo;
       const bool mine = warp * 32 < item.rows, row_valid = r < item.rows;
-      int limit = end;
-      if (item.common && row_valid) {
-        const int seq = sequence_of(seg, item, r * inverse >> 16);
-        limit = seq >= 0 ? min(limit, plan.end[p.groups + seq]) : 0;
-      }
+      const int limit = item.common && row_valid && sequence_of(seg, item, r * inverse >> 16) < 0 ? 0 : end;      // (a row of no sequence sees nothing)
       const int least = __reduce_min_sync(0xffffffffu, limit);
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < seg.count; ++j, ++it) {

@@ -32,7 +32,8 @@ class SharedPrefix:
     not listed.
     `starts` [groups + 1]: group g has rows[starts[g]] .. rows[starts[g + 1] - 1]; groups may be empty.
     `lens` [groups]: keys that the members of a group share, any number.  The block table's pages that hold them are the same for all members, or
-    hold the same (a page that the shared keys fill in part is each member's own).
+    hold the same (a page that the shared keys fill in part is each member's own), as far as a member's own length goes.  As many are read together as
+    the shortest member has; one whose length is zero (a sequence that has ended) takes no part.
     """
     __slots__ = ("rows", "starts", "lens")
 
