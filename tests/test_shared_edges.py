@@ -72,3 +72,31 @@ def test_a_captured_call_whose_first_member_ends():
         check(out[live], {**s, "q": s["q"][live], "table": s["table"][live], "lens": s["lens"][live]})
         assert not out[s["lens"] == 0].any()
     ops.raise_on_status()
+
+
+@gpu
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 15, 2.0 ** 16, 2.0 ** 25, 2.0 ** 40])
+def test_scores_that_are_whole_numbers_in_fp32(size, heads):
+    """Scores of size^2, where fp32 has no fractions: all of the weight is on the largest one, which is further from the second than sums of hd
+    products are off (hd 2^-23 of their magnitudes' sum)."""
+    hq, hkv, hd = heads
+    s = make([(900, [0, 100, 300])], (65,), hq, hkv, hd, 64, seed=hd, device="cuda")
+    s["q"], s["k"] = s["q"] * size, s["k"] * size
+    got = call(s).cpu()
+    ops.raise_on_status()
+    q, k, v, table = (s[n].cpu() for n in ("q", "k", "v", "table"))
+    told = 0
+    for i, n in enumerate(s["lens"].tolist()):
+        at = table[i, :-(-n // 64)].long()
+        kk, vv = (c[at].flatten(0, 1)[:n].double().permute(1, 0, 2) for c in (k, v))
+        qq = q[i].double().unflatten(0, (hkv, -1))
+        score, mag = qq @ kk.mT, (qq.abs() @ kk.abs().mT).amax(-1)
+        top = score.topk(2, -1)
+        far = top.values[..., 0] - top.values[..., 1] > 2 * hd * 2.0 ** -23 * mag + 200 * hd ** 0.5
+        want = vv.gather(1, top.indices[..., :1].expand(-1, -1, hd)).flatten(0, 1)
+        far = far.flatten()
+        told += int(far.sum())
+        assert bool(got[i].isfinite().all())
+        assert bool(((got[i].double() - want)[far].abs() <= 2.0 ** -7 * want[far].abs()).all())
+    assert told >= 3 * hq

@@ -766,6 +766,7 @@ zb_shared_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
       const int limit = item.common && row_valid && sequence_of(seg, item, r * inverse >> 16) < 0 ? 0 : end;      // (a row of no sequence sees nothing)
       const int least = __reduce_min_sync(0xffffffffu, limit);
       float m = -INFINITY, l = 0.f;
+      bool whole = false;                            // some row's reference is so large that fp32 has whole numbers only
       for (int j = 0; j < seg.count; ++j, ++it) {
         const int b = it & 1;
         const uint32_t t_s = tmem_base + b * kKeys + lane_off;
@@ -805,12 +806,15 @@ zb_shared_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
           mx4[1] = max3(mx4[1], __uint_as_float(sr[62]), __uint_as_float(sr[63]));
           const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]) * p.scale_log2;              // in units of log2
           float alpha = 1.f;
-          if (mx > m + kLazy && row_valid) {         // also the first visible key: m = -inf
+          const bool moves = mx > m + kLazy && row_valid;      // also the first visible key: m = -inf
+          if (moves) {
             alpha = m == -INFINITY ? 1.f : zb_ex2(m - mx);
             m = mx;
             l *= alpha;
           }
-          if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+          const bool some_move = __any_sync(0xffffffffu, moves);
+          if (some_move) whole = __any_sync(0xffffffffu, fabsf(m) > 0x1p24f && m != -INFINITY);
+          if (some_move && j > 0) {
             // O += P V of the previous tile must be complete (that of the one before it is: S of this tile went behind it)
             if (!__all_sync(0xffffffffu, zb_mbar_wait(o_ready, static_cast<uint32_t>(it - 1) & 1u, abort_flag))) {
               *abort_where = 11u;
@@ -830,22 +834,43 @@ zb_shared_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
           }
           // p = 2^(s * scale - m)
           const float neg_m = m == -INFINITY ? 0.f : -m;
-          const ZbF2 nm2 = zb_pack2(neg_m, neg_m);
           ZbF2 sum[2] = {0ull, 0ull};
+          if (whole) {                               // products rounded as m is: of others the largest one's is off by half a step of m, 2^7 from 2^31 on
+#pragma unroll 1
+            for (int c = 0; c < 2; ++c) {
+              uint32_t x[32];
+              zb_tmem_ld32(t_s + 32 * c, x);
+              zb_tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t pw[16];
+              for (int i = 0; i < 32; i += 2) {
+                float e[2];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int e = 32 * c + 2 * i;
-              float x0, x1;
-              zb_unpack2(zb_fma2(zb_pack2(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1])), sc2, nm2), x0, x1);
-              x0 = zb_ex2(x0);
-              x1 = zb_ex2(x1);
-              pw[i] = zb_pack_bf16x2(x0, x1);
-              sum[i & 1] = zb_add2(sum[i & 1], zb_pack2(x0, x1));
+                for (int k = 0; k < 2; ++k) {
+                  const int key = key0 + 32 * c + i + k;
+                  e[k] = key < limit && key >= lo ? zb_ex2(__fadd_rn(__fmul_rn(__uint_as_float(x[i + k]), p.scale_log2), neg_m)) : 0.f;
+                }
+                sum[0] = zb_add2(sum[0], zb_pack2(e[0], e[1]));
+                x[i / 2] = zb_pack_bf16x2(e[0], e[1]);
+              }
+              zb_tmem_st16(t_s + 16 * c, x);         // (what these columns held has been read)
             }
-            zb_tmem_st16(t_s + 16 * c, pw);
+          } else {
+            const ZbF2 nm2 = zb_pack2(neg_m, neg_m);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              uint32_t pw[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int e = 32 * c + 2 * i;
+                float x0, x1;
+                zb_unpack2(zb_fma2(zb_pack2(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1])), sc2, nm2), x0, x1);
+                x0 = zb_ex2(x0);
+                x1 = zb_ex2(x1);
+                pw[i] = zb_pack_bf16x2(x0, x1);
+                sum[i & 1] = zb_add2(sum[i & 1], zb_pack2(x0, x1));
+              }
+              zb_tmem_st16(t_s + 16 * c, pw);
+            }
           }
           l += zb_sum2(zb_add2(sum[0], sum[1]));
         }
