@@ -1,0 +1,65 @@
+"""Who draws what a sampling strategy asks for: the tagged API, the models, the engine and the server."""
+import pytest
+import torch
+
+from zml_b200 import nn, ops
+from zml_b200.models.common import SamplingStrategy
+from zml_b200.tensor import Rng, Tensor
+
+gpu = pytest.mark.gpu
+DEVICES = ["cpu", pytest.param("cuda", marks=gpu)]
+
+
+def _draws(x, tags, opts, n=40, device="cpu"):
+    rng, out = Rng(5, device), []
+    for _ in range(n):
+        tok, rng = nn.sample_tokens(Tensor(x, None, tags), opts, rng)
+        out.append(tok.data)
+    assert tok.shape().tags == tuple(t for t in tags if t != "voc") and tok.data.dtype is torch.int32
+    return torch.stack(out)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
+def test_tagged_draws_follow_top_p_and_min_p(device, dtype):
+    x = torch.randn((3, 4, 300), generator=torch.Generator().manual_seed(0), dtype=torch.float64).to(dtype).to(device)
+    best = x.float().argmax(-1).int()
+    for tags, y in ((("b", "s", "voc"), x), (("b", "voc", "s"), x.transpose(1, 2)), (("voc", "b", "s"), x.movedim(-1, 0))):
+        for one in (SamplingStrategy(50, 1.0, 1e-4), SamplingStrategy(0, 1.0, 1.0, 1.0), SamplingStrategy(-1, 1e-4), SamplingStrategy(1, 1.0, 0.5), SamplingStrategy()):
+            assert bool((_draws(y, tags, one, 3, device) == best).all())
+        for opts in (SamplingStrategy(0, 1.0, 0.9), SamplingStrategy(-1), SamplingStrategy(40, 1.3, 0.8, 0.05), SamplingStrategy(300, 0.8, 0.7)):
+            got = _draws(y, tags, opts, 40, device)
+            assert all(len(set(got[:, i, j].tolist())) > 3 for i in range(3) for j in range(4))       # flat rows: every one draws
+            p = torch.softmax(x.double() / opts.temperature, -1)
+            order = p.sort(-1, descending=True)
+            place = torch.zeros_like(order.indices).scatter_(-1, order.indices, torch.arange(300, device=device).expand_as(order.indices))
+            place = place.gather(-1, got.movedim(0, -1).long())
+            if opts.topk > 0:
+                assert int(place.max()) < opts.topk
+            if opts.top_p < 1 and opts.topk <= 0:       # no token behind the smallest set that reaches top_p
+                most = (order.values.cumsum(-1) - order.values < opts.top_p + 1e-3).sum(-1, keepdim=True)
+                assert bool((place < most).all())
+            if opts.min_p > 0:
+                w = p.gather(-1, got.movedim(0, -1).long()) / p.amax(-1, keepdim=True)
+                assert bool((w >= opts.min_p * (1 - 1e-2)).all())
+    flat = Tensor(x[0, 0], None, ("voc",))
+    assert int(nn.sample_tokens(flat, SamplingStrategy(0, 1.0, 1e-3), Rng(1, device))[0].data) == int(best[0, 0])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_tagged_draws_are_those_of_the_operator(device):
+    x = torch.randn((6, 500), generator=torch.Generator().manual_seed(2)).to(device)
+    bits = torch.randint(0, 2 ** 53, (6,), generator=Rng(9, device).gen, device=device)
+    want = ops.sample(x, bits.double() * 2.0 ** -53, 0.7, 100, 0.95, 0.01)
+    got, _ = nn.sample_tokens(Tensor(x, None, ("b", "voc")), SamplingStrategy(100, 0.7, 0.95, 0.01), Rng(9, device))
+    assert torch.equal(got.data, want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_wide_top_k_alone_stays_with_gumbel_noise(device):
+    x = torch.randn((6, 500), generator=torch.Generator().manual_seed(2)).to(device)
+    vals, idx = torch.topk(x, 200, -1)
+    noise = Rng(9, device).gumbel(Tensor(vals, None, ("b", "topk")).shape()).data
+    want = idx.gather(1, (vals * (1 / 0.7) + noise).argmax(-1, keepdim=True))[:, 0].int()
+    got, _ = nn.sample_tokens(Tensor(x, None, ("b", "voc")), SamplingStrategy(200, 0.7), Rng(9, device))
+    assert torch.equal(got.data, want)

@@ -14,7 +14,10 @@ from ..tensor import Rng, Tensor
 def sample_tokens(activations: Tensor, opts: SamplingStrategy, rng: Rng) -> tuple[Tensor, Rng]:
     """`activations` carries a `voc` axis; returns integer ids without it.  With topk > 1 the
     k best logits are scaled by 1/temperature, Gumbel noise is added and the argmax is taken
-    (equivalent to sampling from the softmax over the k)."""
+    (equivalent to sampling from the softmax over the k).  `top_p`, `min_p` and a negative topk are drawn by
+    `ops.sample`, from numbers of `rng`."""
+    if opts.topk != 1 and (opts.top_p < 1.0 or opts.min_p > 0.0 or opts.topk < 0):
+        return _sample_cut(activations, opts, rng)
     d = activations.data
     on_kernels = (d.is_cuda and d.dtype == torch.float32 and d.dim() == 2 and activations.axis("voc") == 1 and d.stride(1) == 1
                   and opts.topk <= 128)
@@ -39,6 +42,18 @@ def sample_tokens(activations: Tensor, opts: SamplingStrategy, rng: Rng) -> tupl
     a = idx.axis("topk")
     tok = torch.gather(idx.data.long(), a, best.data.long()).squeeze(a)
     return Tensor(tok.to(torch.int32), None, tuple(t for i, t in enumerate(idx.shape().tags) if i != a)), rng
+
+
+def _sample_cut(activations: Tensor, opts: SamplingStrategy, rng: Rng) -> tuple[Tensor, Rng]:
+    from .. import ops
+    a = activations.axis("voc")
+    x = activations._gathered(a).data.movedim(a, -1)
+    rows = x.reshape(-1, x.shape[-1])
+    if rows.dtype not in (torch.float32, torch.bfloat16):
+        rows = rows.float()
+    bits = torch.randint(0, 2 ** 53, rows.shape[:1], generator=rng.gen, device=rng.device)      # (23 bits are few for a whole vocabulary)
+    tok = ops.sample(rows, (bits.double() * 2.0 ** -53).to(rows.device), opts.temperature, max(opts.topk, 0), opts.top_p, opts.min_p)
+    return Tensor(tok.reshape(x.shape[:-1]), None, tuple(t for i, t in enumerate(activations.shape().tags) if i != a)), rng
 
 
 @dataclass
