@@ -274,10 +274,13 @@ class Engine:
             raise ValueError("attention within a window does not go with shared pages")
         if getattr(m, "attn_backend", "b200") != "b200":
             raise ValueError(f"the {m.attn_backend} backend does not share pages")
-        if self.on_gpu and (m.dtype != torch.bfloat16 or c.hd not in ops.shared.HEAD_DIMS or (self.page_size not in (16, 32) and self.page_size % 64)
-                            or self.max_batch > ops.shared.MAX_BATCH):
-            raise ValueError(f"shared pages are for bfloat16 models with heads of {ops.shared.HEAD_DIMS}, pages of 16, 32 or a multiple of 64 tokens and up to "
-                             f"{ops.shared.MAX_BATCH} sequences")
+        if self.on_gpu and m.dtype != torch.bfloat16:
+            raise ValueError(f"shared pages are for bfloat16 models, got {m.dtype}")
+        if c.hd not in ops.shared.HEAD_DIMS or m.hq > ops.shared.MAX_GROUP * m.hkv or (self.page_size not in (16, 32) and self.page_size % 64) \
+                or self.max_batch > ops.shared.MAX_BATCH:
+            raise ValueError(f"shared pages are for heads of {ops.shared.HEAD_DIMS}, up to {ops.shared.MAX_GROUP} query heads to a key head, pages of 16, 32 or a "
+                             f"multiple of 64 tokens and up to {ops.shared.MAX_BATCH} sequences, got heads of {c.hd}, {m.hq} to {m.hkv}, pages of "
+                             f"{self.page_size} and {self.max_batch}")
 
     def _page_keys(self, prompt, pages):
         """((page in front, its tokens), page) of the whole pages of a prompt, without the one that has its last token: that one is always computed,
