@@ -63,3 +63,24 @@ def test_a_wide_top_k_alone_stays_with_gumbel_noise(device):
     want = idx.gather(1, (vals * (1 / 0.7) + noise).argmax(-1, keepdim=True))[:, 0].int()
     got, _ = nn.sample_tokens(Tensor(x, None, ("b", "voc")), SamplingStrategy(200, 0.7), Rng(9, device))
     assert torch.equal(got.data, want)
+
+
+class _Engine:
+    max_pages, page_size, comm = 8, 16, None
+
+
+class _Tok:
+    def decode(self, ids, *a):
+        return "x" * len(ids)
+
+
+def test_settings_next_to_their_ends_still_cut_at_the_server():
+    from zml_b200.serving.server import Server
+    greedy = Server(_Engine(), _Tok())
+    for given, top_p, min_p in (({"top_p": 0.9996}, 0.999, 0.0), ({"top_p": 0.99999999}, 0.999, 0.0), ({"top_p": 1e-9}, 0.001, 0.0), ({"top_p": 0.9994}, 0.999, 0.0),
+                                ({"min_p": 0.0004}, 1.0, 0.001), ({"min_p": 1e-9}, 1.0, 0.001), ({"min_p": 0.9999}, 1.0, 0.999), ({"top_p": 0}, 0.0, 0.0),
+                                ({"min_p": 1}, 1.0, 1.0), ({"top_p": 0.9996, "min_p": 0.0004}, 0.999, 0.001)):
+        assert greedy._sampling(given) == (0, 1.0, 0, top_p, min_p)
+        assert greedy._sampling({**given, "top_k": 500}) == (500, 1.0, 0, top_p, min_p)
+    for none in ({"top_p": 1}, {"min_p": 0}, {"top_p": 1.0, "min_p": 0.0}):
+        assert greedy._sampling(none) == (1, 1.0, 0)

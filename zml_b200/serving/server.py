@@ -132,7 +132,7 @@ class Server:
             if v is not None:
                 if isinstance(v, bool) or not isinstance(v, (int, float)) or not 0 <= v <= 1:
                     raise ValueError(f"'{name}' must be a number from 0 to 1")
-                cut[name] = round(float(v), 3)          # as the temperature below
+                cut[name] = float(v) if v in (0, 1) else min(max(round(float(v), 3), 0.001), 0.999)      # as the temperature below; what cuts still does
         cuts = cut["top_p"] < 1.0 or cut["min_p"] > 0.0
         if body.get("temperature") is not None:
             t = body["temperature"]
