@@ -84,3 +84,14 @@ def test_settings_next_to_their_ends_still_cut_at_the_server():
         assert greedy._sampling({**given, "top_k": 500}) == (500, 1.0, 0, top_p, min_p)
     for none in ({"top_p": 1}, {"min_p": 0}, {"top_p": 1.0, "min_p": 0.0}):
         assert greedy._sampling(none) == (1, 1.0, 0)
+
+
+def test_a_server_without_a_top_k_cut_keeps_it_so():
+    from zml_b200.serving.server import Server
+    every = Server(_Engine(), _Tok(), strategy=SamplingStrategy(-1, 0.9))
+    assert every._sampling({}) == (-1, 0.9, 0)
+    assert every._sampling({"temperature": 0.5}) == (-1, 0.5, 0)
+    assert every._sampling({"top_p": 1.0, "seed": 3}) == (-1, 0.9, 3)
+    assert every._sampling({"temperature": 0.5, "top_p": 0.8}) == (0, 0.5, 0, 0.8, 0.0)
+    assert every._sampling({"temperature": 0.5, "top_k": 7}) == (7, 0.5, 0)
+    assert every._sampling({"temperature": 0}) == (1, 1.0, 0)

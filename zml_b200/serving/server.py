@@ -122,7 +122,7 @@ class Server:
     def _sampling(self, body: dict) -> tuple:
         """(top-k, temperature, seed) of a request, and behind them top-p and min-p where one of these cuts.  What the body
         does not set is as in the server's strategy; `temperature: 0` is greedy; a positive temperature without `top_k`
-        draws from the server's k when that is more than 1, else from the MAX_TOP_K best tokens.  `top_p` or `min_p` that
+        draws from the server's k when that is more than 1, from all tokens when it is negative, else from the MAX_TOP_K best.  `top_p` or `min_p` that
         cut ask for a draw, too, without `top_k` or the server's k from all tokens that they leave; beside them `top_k` may
         be any number."""
         k, t = None, None
@@ -156,7 +156,8 @@ class Server:
             k = int(self.strategy.topk)
         elif k is None:
             greedy = t is None and not cuts and not self.strategy.draws
-            k = int(self.strategy.topk) if self.strategy.topk > 1 else 1 if greedy else 0 if cuts else MAX_TOP_K
+            own = int(self.strategy.topk)           # (negative: no cut)
+            k = own if own > 1 else 1 if greedy else 0 if cuts else own if own < 0 else MAX_TOP_K
         sampling = k, float(self.strategy.temperature if t is None else t), int(seed)
         return (*sampling, cut["top_p"], cut["min_p"]) if cuts and k != 1 else sampling
 
