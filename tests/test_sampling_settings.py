@@ -95,3 +95,17 @@ def test_a_server_without_a_top_k_cut_keeps_it_so():
     assert every._sampling({"temperature": 0.5, "top_p": 0.8}) == (0, 0.5, 0, 0.8, 0.0)
     assert every._sampling({"temperature": 0.5, "top_k": 7}) == (7, 0.5, 0)
     assert every._sampling({"temperature": 0}) == (1, 1.0, 0)
+
+
+def test_settings_that_cut_nothing_do_not_ask_for_a_draw():
+    from zml_b200.serving.server import Server
+    greedy = Server(_Engine(), _Tok(), strategy=SamplingStrategy(1, 1.0, 0.9))      # greedy, with a nucleus for requests that draw
+    for none in ({}, {"min_p": 0}, {"top_p": 1}, {"min_p": 0.0, "top_p": 1.0}):
+        assert greedy._sampling(none) == (1, 1.0, 0)
+    assert greedy._sampling({"temperature": 0.5, "min_p": 0}) == (0, 0.5, 0, 0.9, 0.0)
+    assert greedy._sampling({"min_p": 0.1}) == (0, 1.0, 0, 0.9, 0.1)
+    assert greedy._sampling({"top_p": 0.5}) == (0, 1.0, 0, 0.5, 0.0)
+    nucleus = Server(_Engine(), _Tok(), strategy=SamplingStrategy(0, 0.7, 0.8))
+    assert nucleus._sampling({"min_p": 0}) == (0, 0.7, 0, 0.8, 0.0) and nucleus._sampling({"top_p": 1}) == (128, 0.7, 0)
+    assert Server(_Engine(), _Tok(), strategy=SamplingStrategy(40, 0.7))._sampling({"top_p": 1}) == (40, 0.7, 0)
+    assert Server(_Engine(), _Tok(), strategy=SamplingStrategy(0))._sampling({}) == (0, 1.0, 0)

@@ -125,7 +125,7 @@ class Server:
         draws from the server's k when that is more than 1, from all tokens when it is negative, else from the MAX_TOP_K best.  `top_p` or `min_p` that
         cut ask for a draw, too, without `top_k` or the server's k from all tokens that they leave; beside them `top_k` may
         be any number."""
-        k, t = None, None
+        k, t, asks = None, None, False
         cut = {"top_p": float(self.strategy.top_p), "min_p": float(self.strategy.min_p)}
         for name in cut:
             v = body.get(name)
@@ -133,6 +133,7 @@ class Server:
                 if isinstance(v, bool) or not isinstance(v, (int, float)) or not 0 <= v <= 1:
                     raise ValueError(f"'{name}' must be a number from 0 to 1")
                 cut[name] = float(v) if v in (0, 1) else min(max(round(float(v), 3), 0.001), 0.999)      # as the temperature below; what cuts still does
+                asks = asks or v != (name == "top_p")
         cuts = cut["top_p"] < 1.0 or cut["min_p"] > 0.0
         if body.get("temperature") is not None:
             t = body["temperature"]
@@ -149,15 +150,12 @@ class Server:
             seed = 0
         if isinstance(seed, bool) or not isinstance(seed, int):
             raise ValueError("'seed' must be an integer")
-        asked = any(body.get(name) is not None for name in cut)
         if t == 0.0:
             return 1, 1.0, int(seed)
-        if t is None and k is None and not asked:
-            k = int(self.strategy.topk)
-        elif k is None:
-            greedy = t is None and not cuts and not self.strategy.draws
+        if k is None:
             own = int(self.strategy.topk)           # (negative: no cut)
-            k = own if own > 1 else 1 if greedy else 0 if cuts else own if own < 0 else MAX_TOP_K
+            draws = t is not None or asks or self.strategy.draws
+            k = own if own > 1 or not draws else 0 if cuts else own if own < 0 else MAX_TOP_K
         sampling = k, float(self.strategy.temperature if t is None else t), int(seed)
         return (*sampling, cut["top_p"], cut["min_p"]) if cuts and k != 1 else sampling
 
