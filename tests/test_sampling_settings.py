@@ -109,3 +109,31 @@ def test_settings_that_cut_nothing_do_not_ask_for_a_draw():
     assert nucleus._sampling({"min_p": 0}) == (0, 0.7, 0, 0.8, 0.0) and nucleus._sampling({"top_p": 1}) == (128, 0.7, 0)
     assert Server(_Engine(), _Tok(), strategy=SamplingStrategy(40, 0.7))._sampling({"top_p": 1}) == (40, 0.7, 0)
     assert Server(_Engine(), _Tok(), strategy=SamplingStrategy(0))._sampling({}) == (0, 1.0, 0)
+
+
+@pytest.mark.parametrize("device,vocab", [("cpu", 1000), ("cpu", 100), pytest.param("cuda", 100, marks=gpu)])
+def test_a_top_k_that_gumbel_noise_takes_keeps_it(device, vocab):
+    from zml_b200.models.decoder import DecoderModel
+    from zml_b200.parallel.comm import Comm
+    model = DecoderModel.__new__(DecoderModel)
+    model.comm = Comm.single(torch.device(device))
+    x = torch.randn((7, vocab), generator=torch.Generator().manual_seed(4)).to(device)
+    rng = torch.tensor([11, 3], device=device)
+    for k in (5, 128, 129, 200, 5000):
+        for given in (None, rng):
+            # (a counter on the CPU is the captured steps', which the CPU does not have)
+            want = ops.topk_sample(x, k, 0.8, 11, 2, rng=given if device == "cuda" else None)
+            assert torch.equal(model.sample(x, SamplingStrategy(k, 0.8), 11, 2, given), want)
+    assert torch.equal(model.sample(x, SamplingStrategy(200, 0.8, 0.9), 11, 2, rng), ops.sample(x, None, 0.8, 200, 0.9, rng=rng))
+
+
+@gpu
+def test_a_wide_top_k_of_a_model_on_the_gpu():
+    from zml_b200.models.decoder import DecoderModel
+    from zml_b200.parallel.comm import Comm
+    model = DecoderModel.__new__(DecoderModel)
+    model.comm = Comm.single(torch.device("cuda"))
+    x = torch.randn((7, 1000), generator=torch.Generator().manual_seed(4)).cuda()
+    rng = torch.tensor([11, 3], device="cuda")
+    for k in (129, 500, -1):
+        assert torch.equal(model.sample(x, SamplingStrategy(k, 0.8), 11, 2, rng), ops.sample(x, None, 0.8, max(k, 0), rng=rng))

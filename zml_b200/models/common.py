@@ -30,8 +30,8 @@ class Phase(Enum):
 
 @dataclass
 class SamplingStrategy:
-    """topk == 1 is greedy; otherwise top-k then Gumbel-max at `temperature` (zml/nn.zig:1999-2005).  With `top_p` below 1 or `min_p` above 0, with more
-    than 128 candidates, or with a negative `topk` (no such cut), the token is drawn by `ops.sample`; beside `top_p` or `min_p` topk 0 is no cut, too."""
+    """topk == 1 is greedy; otherwise top-k then Gumbel-max at `temperature` (zml/nn.zig:1999-2005).  With `top_p` below 1 or `min_p` above 0, with a negative
+    `topk` (no such cut), or on a GPU with more than 128 candidates, the token is drawn by `ops.sample`; beside `top_p` or `min_p` topk 0 is no cut, too."""
     topk: int = 1
     temperature: float = 1.0
     top_p: float = 1.0
@@ -39,7 +39,7 @@ class SamplingStrategy:
 
     @property
     def cuts(self) -> bool:
-        """Whether `ops.sample` draws."""
+        """Whether there is a cut that `ops.topk_sample` does not take (a `topk` above 128: not on a GPU)."""
         return self.topk != 1 and (self.top_p < 1.0 or self.min_p > 0.0 or self.topk < 0 or self.topk > 128)
 
     @property

@@ -124,7 +124,10 @@ class DecoderModel:
         """Token ids int32 [B] from vocab-parallel logits.  `rng`: device-side {seed, draw counter} of
         `ops.topk_sample` (the serving engine's, so that graph replays draw fresh noise)."""
         comm = self.comm
-        if strategy.cuts:
+        # A top-k alone that `topk_sample` takes (on a GPU 128 candidates, or a vocabulary of no more) keeps its Gumbel noise.
+        by_noise = strategy.topk > 1 and strategy.top_p >= 1.0 and strategy.min_p <= 0.0 and \
+            (not logits.is_cuda or min(strategy.topk, logits.shape[1] * comm.world) <= 128)
+        if strategy.cuts and not by_noise:
             # Under a split vocabulary every rank draws from the gathered logits (column j of rank r is token r * v_per + j), from the same number.
             lg = logits if comm.world == 1 else comm.all_gather(logits.contiguous(), dim=1)
             if rng is None:
