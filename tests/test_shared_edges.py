@@ -100,3 +100,35 @@ def test_scores_that_are_whole_numbers_in_fp32(size, heads):
         assert bool(got[i].isfinite().all())
         assert bool(((got[i].double() - want)[far].abs() <= 2.0 ** -7 * want[far].abs()).all())
     assert told >= 3 * hq
+
+
+@gpu
+@pytest.mark.parametrize("batch,hq,hkv,hd", [(1, 128, 1, 128), (8, 66, 1, 64), (64, 34, 2, 256), (64, 32, 8, 128), (8, 32, 2, 64)])
+def test_the_workspace_has_room_for_the_parts_and_little_else(batch, hq, hkv, hd):
+    """A row of fp32 sums and two numbers for each head of a sequence, in its prefix and behind it, and again for each piece that the keys are cut into: at most
+    two CTAs an SM of 128 rows in front, and of a key head's rows behind - six of these a CTA up to 16 heads, whose keys single warps read."""
+    lib = ops._lib.lib()
+    group, ctas = hq // hkv, 2 * lib.zb_num_sms()
+    most = 32 * batch + 4 * (hd + 2) * (2 * batch * hq + ctas * 128 + ctas * (6 if group <= 16 else 1) * group + 1)
+    assert 4 * (hd + 2) * 2 * batch * hq < lib.zb_shared_decode_workspace(batch, batch, 1, hq, hkv, hd, 64) <= most
+
+
+@gpu
+@pytest.mark.parametrize("hq,hkv,hd", [(128, 1, 128), (66, 1, 64), (34, 2, 256), (17, 1, 128)])
+def test_parts_of_many_heads_to_a_key_head_stay_in_the_workspace(hq, hkv, hd):
+    """Long keys of few and of many sequences, so that every CTA has a piece of either line; what lies behind the workspace is left as it was."""
+    for groups, alone in (([(3000, [2500, 1])], (4000,)), ([(64, [700] * 40)], ()), ([], (9000,)), ([(9000, [0])], ()), ([(130, [1] * 150)], (1,) * 50)):
+        s = make(groups, alone, hq, hkv, hd, 64, seed=hq, device="cuda")
+        guard, new_empty = [], torch.Tensor.new_empty
+
+        class Q(torch.Tensor):
+            def new_empty(self, shape, **kw):
+                if kw.get("dtype") is not torch.uint8:
+                    return new_empty(self.as_subclass(torch.Tensor), shape, **kw)
+                whole = torch.full((shape[0] + 4096,), 77, dtype=torch.uint8, device="cuda")
+                guard.append(whole[shape[0]:])
+                return whole[:shape[0]]
+        got = call({**s, "q": s["q"].as_subclass(Q)})
+        check(got, s)
+        assert len(guard) == 1 and bool((guard[0] == 77).all())
+    ops.raise_on_status()

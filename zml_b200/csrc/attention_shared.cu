@@ -1046,10 +1046,14 @@ int walk_ctas(int hd, int batch, int groups, int sms) {
   return hd == 64 ? walk_ctas<64>(batch, groups, sms) : hd == 128 ? walk_ctas<128>(batch, groups, sms) : walk_ctas<256>(batch, groups, sms);
 }
 
-// Rows of the parts: of prefixes (from row 0 on) and of the sequences' own keys.
+// Blocks of eight heads that single warps take of sequences' own keys; 0: these are tiles, too.
+int own_blocks(int group) { return group <= 8 ? 1 : group <= 16 ? 2 : 0; }
+
+// Rows of the parts: of prefixes (from row 0 on) and of the sequences' own keys, whose line is cut into pieces for warps or, as tiles, for CTAs.
 long long prefix_rows(int listed, int hq, int ctas) { return static_cast<long long>(listed) * hq + static_cast<long long>(ctas) * kRows; }
 long long part_rows(int listed, int batch, int hq, int group, int ctas) {
-  return (prefix_rows(listed, hq, ctas) + static_cast<long long>(batch) * hq + static_cast<long long>(ctas) * kWalkers * group + 1) & ~1ll;      // (16 bytes)
+  const int pieces = ctas * (own_blocks(group) > 0 ? kWalkers : 1);
+  return (prefix_rows(listed, hq, ctas) + static_cast<long long>(batch) * hq + static_cast<long long>(pieces) * group + 1) & ~1ll;      // (16 bytes)
 }
 
 template <int HD, int NB>
@@ -1069,8 +1073,11 @@ int launch(const CUtensorMap (&maps)[4], const SharedParams& p, void* out, int r
 }
 template <int HD>
 int launch(const CUtensorMap (&maps)[4], const SharedParams& p, void* out, int rows, int ctas, cudaStream_t s) {
-  if (p.group <= 8) return launch<HD, 1>(maps, p, out, rows, ctas, s);
-  return p.group <= 16 ? launch<HD, 2>(maps, p, out, rows, ctas, s) : launch<HD, 0>(maps, p, out, rows, ctas, s);
+  switch (own_blocks(p.group)) {
+    case 1: return launch<HD, 1>(maps, p, out, rows, ctas, s);
+    case 2: return launch<HD, 2>(maps, p, out, rows, ctas, s);
+    default: return launch<HD, 0>(maps, p, out, rows, ctas, s);
+  }
 }
 
 bool takes(int batch, int listed, int groups, int hq, int hkv, int hd, int page_size) {
