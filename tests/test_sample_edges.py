@@ -63,3 +63,31 @@ def test_a_largest_logit_of_zero_at_the_smallest_temperatures(device):
     x[:, 4321] = 0.0
     for settings in CUTS:
         check(x, [0.1, 0.9], {**settings, "temperature": 1e-60}, device)
+
+
+@gpu
+@pytest.mark.parametrize("vocab,longer", [(50257, 65536), (50304, 65536), (16385, 32000), (100352, 128256)])
+def test_no_length_leaves_the_list(vocab, longer):
+    """A draw with a small top_k ends in a list, for every length of a row: it does not take half as long again as that of a longer row (as it did where
+    CTAs had no logits, twice and more)."""
+    def took(n, rows):
+        x = torch.randn((rows, n), device="cuda", generator=torch.Generator(device="cuda").manual_seed(n)) * 2.5
+        u = torch.rand(rows, device="cuda")
+        ops.sample(x, u, 1.0, 50)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(20):
+                ops.sample(x, u, 1.0, 50)
+        graph.replay()
+        best = math.inf
+        for _ in range(10):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            graph.replay()
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+    for rows in (1, 32):
+        assert took(vocab, rows) < 1.5 * took(longer, rows)

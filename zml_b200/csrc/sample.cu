@@ -19,6 +19,8 @@
 // What bounds it: the logits' bytes for many rows, beside some 30 instructions of a weight where the whole row's sum is needed, some 40 with the histogram's; for few rows
 // the passes' and the cluster's barriers' latency.  Measured, with logits in L2 as a model leaves them: 1 row of 128256 with top_p 15 us, 32 rows with settings of their
 // own 36, 64 rows of 151936 without a cut 35, 128 rows of 248320 with top_k 50 and top_p 55 (127 MB: 2.3 TB/s), 256 rows of 151936 with a nucleus of 80 thousand 257.
+#include <algorithm>
+
 #include "common.cuh"
 #include "host_api.h"
 
@@ -44,7 +46,8 @@ struct SampleParams {
   const int32_t* top_k;
   long long stride;
   double temperature_all, top_p_all, min_p_all;
-  int top_k_all, vocab, slice, uniforms64, vec;  // slice: of a CTA, whole rows of 128 for each warp; vec: every row starts on four logits
+  int top_k_all, vocab, uniforms64, vec;         // vec: every row starts on four logits
+  int slice, filled;             // slice: of a CTA, whole rows of 128 for each warp; filled: CTAs of which three quarters or more have logits (at least one)
 };
 
 using u64 = unsigned long long;
@@ -721,8 +724,9 @@ struct Sampler {
     if (!(t > 0.0) || top_p <= 0.0) top_k = 1;
     if (top_k <= 0 || top_k > p.vocab) top_k = p.vocab;
     bool small_k = top_k > 1 && top_k <= kSmallK && top_k < p.vocab;
-    // If every CTA has j logits from some bound on, the row has ctas * j of them: the smallest of the CTAs' j-th largest is at most the row's.
-    const int j_th = (top_k + ctas - 1) / ctas;
+    // If each of n CTAs has j logits from some bound on, the row has n * j of them: the smallest of the CTAs' j-th largest is at most the row's.  CTAs at the row's end
+    // that have few logits or none do not count: their j-th largest says nothing (50304 logits, of which the eighth CTA has none, with a top_k of 50: 22 us, now 11).
+    const int j_th = (top_k + p.filled - 1) / p.filled;
     small_k = small_k && j_th <= kThreads;
 
     // ---- the row, its largest logit and its smallest one
@@ -748,7 +752,7 @@ struct Sampler {
       for (int w = 0; w < kWarps; ++w) b = max(b, sh.warp_best[w]), l = min(l, sh.warp_least[w]);
       st_cluster_u32(zb_mapa(zb_smem_u32(&sh.best[rank]), threadIdx.x), b);
       st_cluster_u32(zb_mapa(zb_smem_u32(&sh.least[rank]), threadIdx.x), l);
-      st_cluster_u32(zb_mapa(zb_smem_u32(&sh.bound[rank]), threadIdx.x), small_k ? sh.range[0] : ~0u);
+      st_cluster_u32(zb_mapa(zb_smem_u32(&sh.bound[rank]), threadIdx.x), small_k && rank < p.filled ? sh.range[0] : ~0u);
     }
     cluster_sync();
     uint32_t row_least = ~0u, bound = ~0u;
@@ -979,6 +983,7 @@ template <typename T, int kThreads>
 int launch(SampleParams& p, int rows, int log2, cudaStream_t s) {
   const int unit = 128 * kThreads / 32;
   p.slice = ((p.vocab + (1 << log2) - 1) / (1 << log2) + unit - 1) / unit * unit;
+  p.filled = std::max(1, (p.vocab + p.slice / 4) / p.slice);
   static bool configured[16] = {};
   if (const int rc = zb_config_smem_once(zb_sample_kernel<T, kThreads>, sizeof(Shared<kThreads>), configured)) return rc;
   const cudaError_t e = zb_launch_cluster(zb_sample_kernel<T, kThreads>, dim3(static_cast<unsigned>(rows) << log2), dim3(kThreads), sizeof(Shared<kThreads>), s, 1 << log2, p, log2);
