@@ -15,8 +15,9 @@
 //                                warp 4    : TMA producer, K and V tiles through rings that do not stop at the end of an item
 //                                warp 5    : one thread issues the MMAs
 //   CTAs of the sequences' line  warps 0-5 : walkers, each with a ring of its own that it fills itself
-// Measured (beside the bytes' floor): 8 sequences behind 2000 keys, 32 / 8 heads of 128, 17.7 us (1.4; latency: launch, plan, two kernels); 32 behind 8192, 32 / 8 heads of
-// 64, 26 (5.2); 128 behind 4133 with 782 own keys on average, 32 / 4 heads of 128, 61 (33: 3.5 TB/s); 64 behind 65536, 32 / 8 heads of 128, 103 (47: 670 TFLOP/s).
+// Measured, calls in a row on other tensors each (beside the bytes' floor): 8 sequences behind 2000 keys, 32 / 8 heads of 128, 18.9 us (1.4; latency: launch, plan, two
+// kernels); 32 behind 8192, 32 / 8 heads of 64, 27 (5.2); 128 behind 4133 with 782 own keys on average, 32 / 4 heads of 128, 62 (33: 3.4 TB/s); 64 behind 65536, 32 / 8 heads of
+// 128, 120 (47: 575 TFLOP/s; 103 where a graph of a dozen calls is all that runs); 64 behind 8192, 32 heads to one key head of 128, 31 (5.4).
 // Every wait is bounded; a wait that runs out records a status and the CTA leaves through its normal exit.
 #include <cuda.h>
 
@@ -36,7 +37,7 @@ constexpr int kMaxBatch = 1024;
 constexpr int kStep = 16, kWalkers = 6;
 // What counts of a CTA's time.  A tile of a group's keys takes 1.7 - 2.8 us and the six walkers' step 1.05 - 1.7 us; an item's end and the next one's
 // beginning (its rows' parts written, other queries, an empty pipe) several of either.  With 7 and 1 instead, the CTAs that crossed items and those of the groups came in last:
-// 83 and 130 us where it was 72 and 105 (128 sequences behind 4133 keys, 64 behind 65536).
+// 83 and 130 us where it was 72 and 105 (128 sequences behind 4133 keys, 64 behind 65536; graphs of calls, all heads with the same numbers).
 constexpr uint32_t kTileCost = 11;                   // of a tile of a group's keys, in steps of sequences' own
 constexpr int kSwitch = 6;                           // of a change of items, in tiles or steps
 constexpr int kLeast = 3;                            // tiles of a piece, so that few pieces are none but a change

@@ -4,8 +4,8 @@
 // whose predecessors' weights are less than top_p of the sum; of these, those with w_i >= min_p.  The token is the first in the vocabulary's order up to which the
 // weights that stayed sum to more than u times their sum.
 //
-// Weights are whole numbers of 2^-44.  Sums of up to 2^18 of them are exact in 64 bits and do not depend on an order; a sum is off by at most 2^-27 and
-// typically 2^-36 of the largest weight.  (A sum of fp32 weights is off by 1e-7 of the whole, and among 128 thousand flat weights each is 8e-6 of it:
+// Weights are whole numbers of 2^-44 of the largest, so that sums of a whole row are exact in 64 bits and do not depend on an order.  A weight is off by 2^-45 and, its
+// logarithm having 41 bits behind the point, by 2^-42 of itself; a sum of n by n 2^-45 and 2^-42 of itself at most.  (A sum of fp32 weights is off by 1e-7 of the whole, and among 128 thousand flat weights each is 8e-6 of it:
 // one draw in a hundred would be another token.)
 //
 // A cluster of CTAs has a row, a slice a CTA, and reads it two to four times, all but the first time from L2 (shared memory for the slices would leave two
@@ -16,9 +16,10 @@
 //     a logit at a time tell which of these is the smallest that stays and how many of its equals do, and the warp that has the drawn one looks for it.
 // The histogram has a bin for each 2^-9 .. 2^-4 of the weights' logarithm and counts logits, in the pass that sums all weights; a bin's edges bound the weights in it (a
 // histogram over the logits after that pass, with the weights of each bin's middle, and a list tried beforehand: 256 rows with flat logits 322 us, now 257).
-// What bounds it: the logits' bytes for many rows, beside some 30 instructions of a weight where the whole row's sum is needed, some 40 with the histogram's; for few rows
-// the passes' and the cluster's barriers' latency.  Measured, with logits in L2 as a model leaves them: 1 row of 128256 with top_p 15 us, 32 rows with settings of their
-// own 36, 64 rows of 151936 without a cut 35, 128 rows of 248320 with top_k 50 and top_p 55 (127 MB: 2.3 TB/s), 256 rows of 151936 with a nucleus of 80 thousand 257.
+// What bounds it: the passes over many rows, whose instructions are some 30 of a weight and some 40 with the histogram's, and some 120 an element in all for a wide nucleus;
+// for few rows the passes' and the cluster's barriers' latency.  Measured: 1 row of 128256 with top_p 15 us, 32 rows with settings of their own 32 - 43 by the settings
+// that were drawn, 64 rows of 151936 without a cut 36, 128 rows of 248320 with top_k 50 and top_p 55 (127 MB: 2.3 TB/s), 256 rows of 151936 with a nucleus of 80 thousand 259.
+// (A small top_k alone: the library's kernel for up to 128 candidates, which ranks and draws with noise, takes 10 us for a row of 128256 where this one takes 13.)
 #include <algorithm>
 
 #include "common.cuh"
@@ -29,7 +30,9 @@ namespace {
 constexpr int kMaxCtas = 8;
 constexpr int kMaxVocab = 8 * 49152;                 // (an index and a weight are one number of 19 + 45 bits)
 constexpr int kList = 2048;
-constexpr int kSmallK = 1024;                       // a top_k up to this ends in a list, if all goes well (1.2 - 1.6 times as many logits; 32 rows of which some have 1000: 36 us, by cuts 39)
+// A top_k up to this ends in a list, if all goes well.  Rows alike, top_k 1000, by lists and by cuts, us: 1 x 32000 17 / 22, 1 x 248320 24 / 36, 32 x 128256 33 / 47, 256 x 128256
+// 140 / 177; top_k 601: 14 / 21, 21 / 35, 29 / 47, 109 / 164.  Beyond it the lists of 2048 overflow: a top_k of 1500 that tries one first takes 31 / 23, 54 / 38, 68 / 48, 268 / 189.
+constexpr int kSmallK = 1024;
 constexpr int kBins = 2048;
 constexpr int kTable = 16;                           // 2^((j + 1/2) / 16): any 32 lanes' entries are on different banks (512 entries: 7 conflicts)
 constexpr double kOne = 17592186044416.0;            // 2^44

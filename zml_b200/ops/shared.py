@@ -75,7 +75,7 @@ def _workspace(index: int, *sizes: int) -> int:
 
 def paged_decode(q, k_cache, v_cache, block_table, seq_lens, shared: SharedPrefix, scale: Optional[float] = None, out=None):
     """`ops.paged_decode` with `shared`: bfloat16, heads of 64, 128 or 256, up to 128 query heads for a key head, pages of 16, 32 or a multiple of 64
-    tokens, up to 1024 sequences, a scale above zero, no window.  Sums are fp32; a weight is rounded to bf16 once (2^-9), as the product with
+    tokens, up to 1024 sequences, a scale above zero, no window.  Sums are fp32; a weight is rounded to bf16 once (2^-8), as the product with
     the values takes it."""
     if type(shared) is not SharedPrefix:
         raise TypeError(f"shared: a SharedPrefix, got {type(shared).__name__}")
